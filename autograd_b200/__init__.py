@@ -5,8 +5,9 @@ there is no CPU or library fallback, a missing library is an ImportError.
 """
 from . import _native
 from ._native import (AG_BF16, AG_CE_3XTF32, AG_CE_BF16, AG_CE_BF16X3, AG_CE_FP32, AG_CE_IGNORE_COMPAT_UNMASKED,
-                      AG_CE_IGNORE_MASKED, AG_CE_MEAN_ALL_ROWS, AG_CE_MEAN_VALID, AG_F32, AG_STATUS_BAD_INDEX,
-                      AG_STATUS_STAGE_FALLBACK, AG_STATUS_WAIT_EXPIRED, AgError)
+                      AG_CE_IGNORE_MASKED, AG_CE_MEAN_ALL_ROWS, AG_CE_MEAN_VALID, AG_DISTILL_MAX, AG_DISTILL_RENORM,
+                      AG_DISTILL_REST, AG_F32, AG_STATUS_BAD_INDEX, AG_STATUS_STAGE_FALLBACK, AG_STATUS_WAIT_EXPIRED, AG_TOP_MAX,
+                      AG_VOCAB_MAX, AgError)
 from .backend import CudaBackend
 from .context import CudaContext
 from .device import create, fuse_add_layernorm, register

@@ -20,6 +20,8 @@ AG_STATUS_BAD_INDEX, AG_STATUS_WAIT_EXPIRED, AG_STATUS_STAGE_FALLBACK = 1, 2, 4
 AG_CE_FP32, AG_CE_3XTF32, AG_CE_BF16, AG_CE_BF16X3 = 0, 1, 2, 3
 AG_CE_MEAN_ALL_ROWS, AG_CE_MEAN_VALID = 0, 1
 AG_CE_IGNORE_MASKED, AG_CE_IGNORE_COMPAT_UNMASKED = 0, 1
+AG_DISTILL_RENORM, AG_DISTILL_REST = 0, 1
+AG_VOCAB_MAX, AG_TOP_MAX, AG_DISTILL_MAX = 393216, 128, 256
 
 
 class FlceDesc(C.Structure):
@@ -94,6 +96,13 @@ SIGNATURES = {
     "ag_linear_add_scratch_bytes": (_sz, [_i64, _int, _int, _int]),
     "ag_linear_add_forward": (_int, [_ctx, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _ptr, _sz]),
     "ag_linear_add_backward": (_int, [_ctx, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _ptr, _sz]),
+    "ag_token_logprobs_forward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _f32, _int]),
+    "ag_token_logprobs_backward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _int, _f32, _int]),
+    "ag_distill_forward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _f32, _int, _int]),
+    "ag_distill_backward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _int, _int, _f32,
+                                   _int, _int]),
+    "ag_distill_forward_backward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _int,
+                                           _int, _f32, _int, _int]),
     "ag_adamw_step": (_int, [_ctx, _ptr, _ptr, _ptr, _ptr, _i64, _f64, _f64, _f64, _f64, _f64, _f64, _f64]),
     "ag_f32_to_bf16": (_int, [_ctx, _ptr, _ptr, _i64, _int]),
     "ag_bf16_to_f32": (_int, [_ctx, _ptr, _ptr, _i64]),
@@ -198,6 +207,8 @@ class _CheckedCalls:
              "ag_rope_qk", "ag_gather_forward", "ag_gather_backward", "ag_gather_backward_bf16", "ag_f32_to_bf16",
              "ag_bf16_to_f32", "ag_flce_forward", "ag_flce_backward", "ag_flce_forward_keep",
              "ag_flce_backward_kept", "ag_flce_logits_bytes", "ag_linear_add_forward", "ag_linear_add_backward",
+             "ag_token_logprobs_forward", "ag_token_logprobs_backward", "ag_distill_forward", "ag_distill_backward",
+             "ag_distill_forward_backward",
              "ag_adamw_step", "ag_adamw_step_bf16grad", "ag_event_record", "ag_graph_launch", "ag_copy_h2d",
              "ag_scatter_add_scratch_bytes", "ag_flce_scratch_bytes", "ag_linear_add_scratch_bytes")
 

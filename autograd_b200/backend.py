@@ -627,3 +627,101 @@ class CudaBackend:
         b, t, h, d = q.shape
         hkv = k.shape[2] if k is not None else 0
         _rope_qk(self._context, q, k, cos, sin, b, t, h, hkv, d, sin_sign, _ag_dtype(q.storage.dtype))
+
+    # ------------------------------------------------------------------ rows of logits
+    # What a projection onto the vocabulary puts out (ag_linear_add_forward without residual, or the caller's own product):
+    # (..., width) of fp32 or bf16 words, the first `vocab` columns of which are tokens (all of them if None; a head padded
+    # to a round width has fewer).  Formulas, limits and what -inf, NaN and empty rows give: include/autograd_b200.h.
+    @staticmethod
+    def _logits(logits, vocab):
+        n, width = _rows_cols(logits)
+        v = width if vocab is None else vocab
+        if not 0 < v <= width:
+            raise ValueError(f"{vocab} tokens in logits of {width} columns")
+        return n, width, v, _ag_dtype(logits.storage.dtype)
+
+    @staticmethod
+    def _check(name, t, count, dtype=np.float32):
+        """t, which the kernel reads or writes `count` items of; None stays None."""
+        if t is None:
+            return None
+        if t.dtype is not dtype and np.dtype(t.dtype) != np.dtype(dtype):
+            raise TypeError(f"{name} must be {np.dtype(dtype)}")
+        if _size(t) != count:
+            raise ValueError(f"{name} has {_size(t)} elements, expected {count}")
+        return t
+
+    def _gradient(self, name, t, logits, n):
+        """Row stride of a gradient of the logits."""
+        rows, width = _rows_cols(t)
+        if rows != n or _ag_dtype(t.storage.dtype) != _ag_dtype(logits.storage.dtype):
+            raise ValueError(f"{name} needs the rows and the type of the logits")
+        return width
+
+    def token_logprobs_forward(self, logits, ids, logprob, entropy=None, stats=None, top_ids=None, top_logprobs=None,
+                               temperature=1.0, vocab=None):
+        """logprob = log softmax(logits / temperature)[ids], the rows' entropies, and the top_ids.shape[-1] likeliest tokens
+        with their log-probabilities; `stats` (rows, 4) is what the backward call needs.  Outputs may be None."""
+        n, width, v, dtype = self._logits(logits, vocab)
+        check = self._check
+        top = 0
+        if top_ids is not None:
+            top = top_ids.shape[-1]
+            if top_logprobs is None:
+                raise ValueError("top_ids without top_logprobs")
+            check("top_ids", top_ids, n * top, np.int32)
+            check("top_logprobs", top_logprobs, n * top)
+        self._context.token_logprobs_forward(
+            logits, width, check("ids", ids, n, np.int32), check("logprob", logprob, n), check("entropy", entropy, n),
+            check("stats", stats, 4 * n), top_ids if top else None, top_logprobs if top else None, n, v, top, temperature, dtype)
+
+    def token_logprobs_backward(self, logits, ids, stats, dlogprob, dentropy, dlogits, dres=None, temperature=1.0, vocab=None):
+        """dlogits = (dres or 0) + local: dres=dlogits accumulates in place.  dlogprob or dentropy may be None, dlogits may be
+        the logits."""
+        n, width, v, dtype = self._logits(logits, vocab)
+        check, ld_grad = self._check, self._gradient("dlogits", dlogits, logits, n)
+        if dres is not None and self._gradient("dres", dres, logits, n) != ld_grad:
+            raise ValueError("dres and dlogits have rows of different length")
+        self._context.token_logprobs_backward(
+            logits, width, check("ids", ids, n, np.int32), check("stats", stats, 4 * n), check("dlogprob", dlogprob, n),
+            check("dentropy", dentropy, n), dres, dlogits, ld_grad, n, v, temperature, dtype)
+
+    def _teacher(self, teacher_ids, teacher_logits, row_scale, n):
+        top = teacher_ids.shape[-1]
+        self._check("teacher_ids", teacher_ids, n * top, np.int32)
+        self._check("teacher_logits", teacher_logits, n * top)
+        self._check("row_scale", row_scale, n)
+        return top
+
+    def distill_forward(self, logits, teacher_ids, teacher_logits, row_loss, loss=None, stats=None, row_scale=None,
+                        temperature=1.0, rest=False, vocab=None):
+        """Loss of each row against the teacher's distribution over its list (rows, top), and their mean, or weighted sum.
+        rest: teacher_logits are log-probabilities, and what they leave is compared too."""
+        n, width, v, dtype = self._logits(logits, vocab)
+        check, top = self._check, self._teacher(teacher_ids, teacher_logits, row_scale, n)
+        self._context.distill_forward(logits, width, teacher_ids, teacher_logits, row_scale, check("loss", loss, 1),
+                                      check("row_loss", row_loss, n), check("stats", stats, 4 * n), n, v, top, temperature,
+                                      N.AG_DISTILL_REST if rest else N.AG_DISTILL_RENORM, dtype)
+
+    def distill_backward(self, logits, teacher_ids, teacher_logits, stats, dloss, dlogits, row_scale=None, dres=None,
+                         temperature=1.0, rest=False, vocab=None):
+        """dlogits = (dres or 0) + gradient, from the stats that distill_forward left; dlogits may be the logits."""
+        n, width, v, dtype = self._logits(logits, vocab)
+        check, top = self._check, self._teacher(teacher_ids, teacher_logits, row_scale, n)
+        ld_grad = self._gradient("dlogits", dlogits, logits, n)
+        if dres is not None and self._gradient("dres", dres, logits, n) != ld_grad:
+            raise ValueError("dres and dlogits have rows of different length")
+        self._context.distill_backward(logits, width, teacher_ids, teacher_logits, row_scale, check("stats", stats, 4 * n),
+                                       check("dloss", dloss, 1), dres, dlogits, ld_grad, n, v, top, temperature,
+                                       N.AG_DISTILL_REST if rest else N.AG_DISTILL_RENORM, dtype)
+
+    def distill_forward_backward(self, logits, teacher_ids, teacher_logits, dloss, row_loss, dlogits, stats=None, loss=None,
+                                 row_scale=None, temperature=1.0, rest=False, vocab=None):
+        """Both of the above with one read of the logits, for a caller that knows the loss's gradient beforehand."""
+        n, width, v, dtype = self._logits(logits, vocab)
+        check, top = self._check, self._teacher(teacher_ids, teacher_logits, row_scale, n)
+        self._context.distill_forward_backward(
+            logits, width, teacher_ids, teacher_logits, row_scale, check("dloss", dloss, 1), check("loss", loss, 1),
+            check("row_loss", row_loss, n), check("stats", stats, 4 * n), dlogits,
+            self._gradient("dlogits", dlogits, logits, n), n, v, top, temperature,
+            N.AG_DISTILL_REST if rest else N.AG_DISTILL_RENORM, dtype)

@@ -283,6 +283,31 @@ class CudaContext:
         calls.ag_linear_add_backward(self._hi, dout, act, w, dx, dact, dw, db, N_, K_, C_, precision, scratch,
                                      scratch_bytes)
 
+    def token_logprobs_forward(self, logits, ld, ids, logprob, entropy, stats, top_ids, top_logprobs, N_, V_, top=0,
+                               temperature=1.0, dtype=N.AG_F32):
+        calls.ag_token_logprobs_forward(self._hi, logits, ld, ids, logprob, entropy, stats, top_ids, top_logprobs, N_, V_, top,
+                                        temperature, dtype)
+
+    def token_logprobs_backward(self, logits, ld, ids, stats, dlogprob, dentropy, dres, dlogits, ld_grad, N_, V_,
+                                temperature=1.0, dtype=N.AG_F32):
+        calls.ag_token_logprobs_backward(self._hi, logits, ld, ids, stats, dlogprob, dentropy, dres, dlogits, ld_grad, N_, V_,
+                                         temperature, dtype)
+
+    def distill_forward(self, logits, ld, teacher_ids, teacher_logits, row_scale, loss, row_loss, stats, N_, V_, top,
+                        temperature=1.0, mode=N.AG_DISTILL_RENORM, dtype=N.AG_F32):
+        calls.ag_distill_forward(self._hi, logits, ld, teacher_ids, teacher_logits, row_scale, loss, row_loss, stats, N_, V_,
+                                 top, temperature, mode, dtype)
+
+    def distill_backward(self, logits, ld, teacher_ids, teacher_logits, row_scale, stats, dloss, dres, dlogits, ld_grad, N_,
+                         V_, top, temperature=1.0, mode=N.AG_DISTILL_RENORM, dtype=N.AG_F32):
+        calls.ag_distill_backward(self._hi, logits, ld, teacher_ids, teacher_logits, row_scale, stats, dloss, dres, dlogits,
+                                  ld_grad, N_, V_, top, temperature, mode, dtype)
+
+    def distill_forward_backward(self, logits, ld, teacher_ids, teacher_logits, row_scale, dloss, loss, row_loss, stats,
+                                 dlogits, ld_grad, N_, V_, top, temperature=1.0, mode=N.AG_DISTILL_RENORM, dtype=N.AG_F32):
+        calls.ag_distill_forward_backward(self._hi, logits, ld, teacher_ids, teacher_logits, row_scale, dloss, loss, row_loss,
+                                          stats, dlogits, ld_grad, N_, V_, top, temperature, mode, dtype)
+
     def adamw_step(self, p, g, m, v, n, lr, lr_t, b1, b2, eps, weight_decay, grad_scale=1.0, grad_bf16=False):
         fn = calls.ag_adamw_step_bf16grad if grad_bf16 else calls.ag_adamw_step
         fn(self._hi, p, g, m, v, n, lr, lr_t, b1, b2, eps, weight_decay, grad_scale)

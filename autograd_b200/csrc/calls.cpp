@@ -463,6 +463,11 @@ PyMethodDef methods[] = {
     CALL(ag_flce_backward_kept),
     CALL(ag_linear_add_forward),
     CALL(ag_linear_add_backward),
+    CALL(ag_token_logprobs_forward),
+    CALL(ag_token_logprobs_backward),
+    CALL(ag_distill_forward),
+    CALL(ag_distill_backward),
+    CALL(ag_distill_forward_backward),
     CALL(ag_adamw_step),
     CALL(ag_adamw_step_bf16grad),
     CALL(ag_event_record),

@@ -102,6 +102,11 @@ PYBIND11_MODULE(cuda_ext, m) {
   AG_DEF(ag_linear_add_scratch_bytes);
   AG_DEF(ag_linear_add_forward);
   AG_DEF(ag_linear_add_backward);
+  AG_DEF(ag_token_logprobs_forward);
+  AG_DEF(ag_token_logprobs_backward);
+  AG_DEF(ag_distill_forward);
+  AG_DEF(ag_distill_backward);
+  AG_DEF(ag_distill_forward_backward);
   AG_DEF(ag_adamw_step);
   AG_DEF(ag_f32_to_bf16);
   AG_DEF(ag_bf16_to_f32);

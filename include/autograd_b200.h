@@ -286,6 +286,59 @@ int ag_linear_add_backward(ag_ctx* ctx, const float* dout, const float* act, con
                            float* dact, float* dw, float* db, int64_t N, int K, int C, int precision,
                            void* scratch, size_t scratch_bytes);
 
+/* ---- h1 log-probabilities of given tokens, entropy, likeliest tokens -------------------------
+ * No counterpart in the reference's fused ops; its rollout sampler takes top-k and softmax of logits
+ * (backend.py:2260-2494), its policy-gradient loss the log-probability of a token (rl_autograd.py:518-524).
+ * Rows of logits, row i at logits + i * ld elements (ld >= V; columns from V on are not read), AG_F32 or
+ * AG_BF16; V up to AG_VOCAB_MAX.  With z = x / temperature (1e-4 to 1e4), m = max x and L = ln sum exp(z - m / temperature):
+ *   logprob[i] = z_id - m / temperature - L of token ids[i]; 0 where the id is outside [0, V)
+ *   entropy[i] = - sum p ln p;  stats[i] = (m, L, entropy, 0), four floats, 16-byte aligned: what the backward call needs
+ *   top_ids[i][k], top_logprobs[i][k], k < top <= AG_TOP_MAX: the likeliest tokens, larger logits first, equal ones
+ *   by the lower index (NaN counts as largest)
+ * Every output may be NULL; ids may be NULL without logprob.  A logit of -inf is a token that cannot occur; a row of
+ * nothing else has entropy 0, log-probabilities -inf and gradient 0.  A NaN or +inf makes its row's results NaN.
+ * backward: dlogits = (dres ? dres : 0) + (a (onehot(id) - p) - b p (ln p + entropy)) / temperature with a = dlogprob[i]
+ * (0 without a token), b = dentropy[i]; either may be NULL.  A row with a = b = 0 gets gradient 0 whatever its logits are.
+ * dlogits rows (and those of dres) are ld_grad elements apart, columns from V on are not written; dlogits may be the
+ * logits themselves, or dres, with the same row stride. */
+#define AG_VOCAB_MAX 393216
+#define AG_TOP_MAX 128
+int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* ids, float* logprob,
+                              float* entropy, float* stats, int32_t* top_ids, float* top_logprobs, int64_t N, int V,
+                              int top, float temperature, int dtype);
+int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* ids, const float* stats,
+                               const float* dlogprob, const float* dentropy, const void* dres, void* dlogits,
+                               int64_t ld_grad, int64_t N, int V, float temperature, int dtype);
+
+/* ---- h2 distillation from a teacher's top logits ----------------------------------------------
+ * No counterpart in the reference.  Student's logits as above, p = softmax(x / temperature).  Row i has `top` slots
+ * (1 to AG_DISTILL_MAX): teacher_ids[i][k], negative = slot not in use, V and more = not in use and AG_STATUS_BAD_INDEX;
+ * teacher_logits[i][k] = t_k.
+ *   AG_DISTILL_RENORM: q = softmax(t / temperature) over the slots, r = 0 (t may be log-probabilities as well)
+ *   AG_DISTILL_REST:   q_k = exp(t_k), t the teacher's log-probabilities at this temperature; r = max(0, 1 - sum q), its
+ *                      mass on all other tokens, is compared with p_rest, the student's on the same tokens
+ *   row_loss[i] = sum_k q_k (ln q_k - ln p_id_k) + r (ln r - ln p_rest)
+ *   loss = sum_i row_scale[i] row_loss[i], or their mean without row_scale; rows of weight 0 take no part
+ * A row whose slots are all unused, or -inf, has loss 0 and gradient 0.  A token that is listed twice counts with both
+ * its masses.  stats[i] = (m, L, ln p_rest, 0) for the backward call, 16-byte aligned; loss and stats may be NULL.
+ * backward: dlogits = (dres ? dres : 0) + dloss[0] * weight / temperature
+ *                     * (p_j (sum q + r) - sum of q_k with id_k = j - [j not listed] r p_j / p_rest)
+ * Neither loss nor gradient has the factor temperature^2 that some training recipes put in the weight.
+ * forward_backward makes both of one read of the logits, for callers that know dloss beforehand. */
+#define AG_DISTILL_MAX 256
+enum { AG_DISTILL_RENORM = 0, AG_DISTILL_REST = 1 };
+int ag_distill_forward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* teacher_ids,
+                       const float* teacher_logits, const float* row_scale, float* loss, float* row_loss, float* stats,
+                       int64_t N, int V, int top, float temperature, int mode, int dtype);
+int ag_distill_backward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* teacher_ids,
+                        const float* teacher_logits, const float* row_scale, const float* stats, const float* dloss,
+                        const void* dres, void* dlogits, int64_t ld_grad, int64_t N, int V, int top,
+                        float temperature, int mode, int dtype);
+int ag_distill_forward_backward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* teacher_ids,
+                                const float* teacher_logits, const float* row_scale, const float* dloss, float* loss,
+                                float* row_loss, float* stats, void* dlogits, int64_t ld_grad, int64_t N, int V,
+                                int top, float temperature, int mode, int dtype);
+
 /* ---- f3 AdamW fp32 step ----------------------------------------------------------------
  * Replaces: backend.py:2013-2038 cpu_adamw_step; metal_ops.metal:10139-10227.
  * g is read as g*grad_scale. */

@@ -1,0 +1,324 @@
+"""Distillation from a teacher's top logits, against the 64-bit forms.
+
+Bounds in units u = 2^-24, as in the tests of log-probabilities: ln p is off by (300 + 8 |ln p|) u; q by 8 u and 4 u |t / temperature|
+of itself, ln q by as much; r = 1 - sum q by 8 u (1 + sum q |t|) <= 40 u of 1 and ln r by that over r; ln p_rest like ln p.  So a
+row's loss is off by 400 u of the sizes of its terms, where r's are taken whole (|ln r| + |ln p_rest| + 1 instead of r times
+them).  A gradient's terms are off by (400 + 16 |ln p|) u of themselves, r p / p_rest also by 40 u of p / p_rest (the oracle's
+`size` has a tenth of that ratio in it).  Gradients stored in bf16 add 2^-8 of their value.  The loss adds a rounding of its sum's
+size."""
+import numpy as np
+import pytest
+
+import autograd_b200 as ag
+from autograd_b200.backend import bf16_bits_to_f32, f32_to_bf16_bits
+from gpu_util import check_clean_status, down, empty, env, free, up
+from oracle import vocab_rows as R
+from test_gpu_logprobs import SENTINEL, U, fetch, near, rounded, rows_of, store, words
+
+pytestmark = pytest.mark.gpu
+
+
+def teacher_of(rng, n, v, top, rest):
+    """Lists with unused slots, repeated tokens, tokens of probability 0, rows without any."""
+    ids = np.stack([rng.permutation(v)[:top] if v >= top else rng.integers(0, v, top) for _ in range(n)]).astype(np.int32)
+    t = rng.standard_normal((n, top)).astype(np.float32) * 2
+    if rest:
+        with np.errstate(all="ignore"):
+            t = t - np.log(np.sum(np.exp(t.astype(np.float64)), 1, keepdims=True)) + np.log(rng.uniform(0.3, 0.98, (n, 1)))
+        t = t.astype(np.float32)
+    ids[2::7, top // 2:] = -1
+    if n > 3:
+        ids[3] = -5
+    if n > 5 and top > 2:
+        ids[5, 1] = ids[5, 0]
+        t[5, 2] = -np.inf
+    if n > 6:
+        t[6] = -np.inf
+    return ids, t
+
+
+def run(x, ids, t, dtype, what, row_scale=None, dloss=1.0, temperature=1.0, rest=False, ld=None, shift=0, ld_grad=None,
+        shift_grad=0, place=None, dres=None):
+    """what: "both" (forward_backward) or "apart" (forward, then backward from its statistics)."""
+    ctx, alloc, be = env()
+    n, v = x.shape
+    top = ids.shape[1]
+    d, mode = (1 if dtype == "bf16" else 0), (ag.AG_DISTILL_REST if rest else ag.AG_DISTILL_RENORM)
+    ld = v if ld is None else ld
+    tx, whole = store(x, dtype, ld, shift)
+    if place == "logits":
+        out, whole_out, ld_grad, shift_grad = tx, whole, ld, shift
+    else:
+        ld_grad = v if ld_grad is None else ld_grad
+        out, whole_out = store(np.full((n, v), SENTINEL) if place != "dres" else dres, dtype, ld_grad, shift_grad)
+    tr = whole_r = None
+    if place == "dres":
+        tr = out
+    elif dres is not None:
+        tr, whole_r = store(dres, dtype, ld_grad, shift_grad)
+    ti, tt = up(ids), up(t)
+    w = None if row_scale is None else up(np.asarray(row_scale, np.float32))
+    dl, loss = up(np.array([dloss], np.float32)), up(np.array([SENTINEL] * 2, np.float32))
+    row, st = up(np.full(n + 3, SENTINEL, np.float32)), up(np.full((n + 1, 4), SENTINEL, np.float32))
+    if what == "both":
+        ctx.distill_forward_backward(tx, ld, ti, tt, w, dl, loss, row, st, out, ld_grad, n, v, top, temperature, mode, d)
+    else:
+        ctx.distill_forward(tx, ld, ti, tt, w, loss, row, st, n, v, top, temperature, mode, d)
+        ctx.distill_backward(tx, ld, ti, tt, w, st, dl, tr, out, ld_grad, n, v, top, temperature, mode, d)
+    got = fetch(out, shift_grad + n * ld_grad, dtype)
+    rows = got[shift_grad:].reshape(n, ld_grad)
+    assert np.isnan(got[:shift_grad]).all() and np.isnan(rows[:, v:]).all(), "written beside the rows"
+    r, s, l = down(row), down(st), down(loss)
+    assert (r[n:] == SENTINEL).all() and (s[n:] == SENTINEL).all() and l[1] == SENTINEL
+    free(*{id(q): q for q in (whole, whole_out, whole_r, ti, tt, w, dl, loss, row, st) if q is not None}.values())
+    return {"row_loss": r[:n], "loss": l[0], "dlogits": rows[:, :v].copy(), "stats": s[:n]}
+
+
+def check(x, ids, t, dtype, what, dres=None, **kw):
+    got = run(x, ids, t, dtype, what, dres=dres, **kw)
+    scale = kw.get("row_scale")
+    ref = R.distill(x, ids, t, None if scale is None else np.asarray(scale, np.float32), np.float32(kw.get("dloss", 1.0)),
+                    kw.get("temperature", 1.0), kw.get("rest", False))
+    with np.errstate(all="ignore"):
+        near(got["row_loss"], ref["row_loss"], 400 * U * ref["loss_size"], "loss of a row")
+        take = ref["weight"] != 0
+        near(got["loss"], ref["loss"], U * np.sum(np.abs(ref["weight"][take]) * (400 * ref["loss_size"][take])) + U * abs(ref["loss"])
+             + 2 * U * np.sum(np.abs(ref["weight"][take] * ref["row_loss"][take])), "loss")
+        g, size = ref["dlogits"], ref["size"]
+        if dres is not None:
+            g, size = g + dres, size + np.abs(dres)
+        bound = size * (400 + 16 * np.where(np.isfinite(ref["lp"]), np.abs(ref["lp"]), 0.0)) * U + 2.0 ** -120
+        if dtype == "bf16":
+            bound = bound + np.abs(g) * 2.0 ** -8 + 2.0 ** -133
+    near(got["dlogits"], g, bound, "gradient")
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("v", [1, 2, 5, 33, 128, 640, 1001, 4099, 16384, 32768, 50257])
+def test_distill(v, rest, dtype):
+    rng = np.random.default_rng(v)
+    n, top = 24, min(v, 19)
+    x = rows_of(rng, n, v, dtype)
+    ids, t = teacher_of(rng, n, v, top, rest)
+    w = rng.random(n)
+    w[20] = 0.0
+    for what in ("both", "apart"):
+        check(x, ids, t, dtype, what, rest=rest)
+        check(x, ids, t, dtype, what, rest=rest, row_scale=w, dloss=0.37, temperature=1.7)
+        check(x, ids, t, dtype, what, rest=rest, place="logits")
+    dres = rounded(rng.standard_normal((n, v)).astype(np.float32), dtype)
+    check(x, ids, t, dtype, "apart", rest=rest, dres=dres)
+    check(x, ids, t, dtype, "apart", rest=rest, dres=dres, place="dres")
+    check_clean_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 2, 31, 32, 33, 100, 255, 256])
+def test_lengths_of_the_list(top, dtype):
+    rng = np.random.default_rng(top)
+    for n, v in ((9, 256), (40, 1000), (12, 50257)):
+        x = rounded(rng.standard_normal((n, v)).astype(np.float32) * 2, dtype)
+        for rest in (False, True):
+            ids, t = teacher_of(rng, n, v, top, rest)
+            for what in ("both", "apart"):
+                check(x, ids, t, dtype, what, rest=rest)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(1, 151936), (19, 151936), (2, 393216), (5000, 640), (700, 5000), (149, 32768), (300, 100)])
+def test_sizes(n, v, dtype):
+    rng = np.random.default_rng(n)
+    x = rounded(rng.standard_normal((n, v)).astype(np.float32) * 2, dtype)
+    for rest in (False, True):
+        ids, t = teacher_of(rng, n, v, 40, rest)
+        for what in ("both", "apart"):
+            check(x, ids, t, dtype, what, rest=rest)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1, 3, 6])
+@pytest.mark.parametrize("pad", [0, 1, 2, 8, 47])
+def test_strides_and_shifts(shift, pad, dtype):
+    rng = np.random.default_rng(shift * 50 + pad)
+    for v in (9, 641, 20001):
+        x = rounded(rng.standard_normal((6, v)).astype(np.float32) * 2, dtype)
+        ids, t = teacher_of(rng, 6, v, 7, True)
+        for what in ("both", "apart"):
+            check(x, ids, t, dtype, what, rest=True, ld=v + pad, shift=shift, ld_grad=v + pad, shift_grad=shift)
+            check(x, ids, t, dtype, what, rest=True, ld=v + pad, shift=shift, ld_grad=v + 3, shift_grad=2)
+            check(x, ids, t, dtype, what, rest=False, ld=v + pad, shift=shift, place="logits")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_small_rest_keeps_its_digits(dtype):
+    """The student gives everything but 1e-7 to the listed tokens: 1 - sum would have one digit of that left."""
+    n, v = 4, 3000
+    x = np.zeros((n, v), np.float32)
+    x[:, :4] = 24.0
+    x = rounded(x + np.linspace(-0.5, 0.5, v)[None, :], dtype)
+    ids = np.tile(np.arange(4, dtype=np.int32), (n, 1))
+    t = np.log(np.full((n, 4), 0.2475, np.float32))
+    got = check(x, ids, t, dtype, "both", rest=True)
+    ref = R.distill(x, ids, t, rest=True)
+    assert np.max(np.abs(got["stats"][:, 2] - ref["log_rest"])) < 400 * U * 20
+    check(x, ids, t, dtype, "apart", rest=True)
+
+
+def test_a_listed_token_outside_the_vocabulary_is_reported():
+    ctx, _, _ = env()
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((5, 50)).astype(np.float32)
+    ids, t = teacher_of(rng, 5, 50, 6, False)
+    ids[1, 3], ids[4, 0] = 50, 2 ** 31 - 1
+    check(x, ids, t, "f32", "both")
+    assert ctx.status() == ag.AG_STATUS_BAD_INDEX
+    check(x, ids, t, "f32", "apart")
+    assert ctx.status() == ag.AG_STATUS_BAD_INDEX
+    assert ctx.status() == 0
+
+
+def test_rows_of_weight_zero_may_hold_anything():
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((4, 64)).astype(np.float32)
+    x[1], x[2, 3] = np.nan, np.inf
+    ids, t = np.tile(np.arange(5, dtype=np.int32), (4, 1)), rng.standard_normal((4, 5)).astype(np.float32)
+    for what in ("both", "apart"):
+        got = run(x, ids, t, "f32", what, row_scale=[0.5, 0.0, 0.0, 0.5])
+        assert np.isfinite(got["loss"]) and not got["dlogits"][1:3].any() and np.isfinite(got["dlogits"]).all()
+
+
+def test_no_rows_have_loss_zero():
+    ctx, alloc, be = env()
+    loss = up(np.array([5.0], np.float32))
+    ctx.distill_forward(0, 10, 0, 0, None, loss, 0, 0, 0, 10, 3)
+    assert down(loss)[0] == 0.0
+    free(loss)
+
+
+def test_teacher_that_is_not_a_number_spoils_its_row_only():
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((4, 200)).astype(np.float32)
+    for rest in (False, True):
+        ids, t = np.tile(np.arange(5, dtype=np.int32), (4, 1)), np.log(rng.random((4, 5)).astype(np.float32) / 6)
+        t[2, 1] = np.nan
+        for what in ("both", "apart"):
+            got = run(x, ids, t, "f32", what, rest=rest)
+            assert np.isnan(got["row_loss"][2]) and np.isnan(got["dlogits"][2]).all() and np.isnan(got["loss"])
+            keep = [0, 1, 3]
+            ref = R.distill(x[keep], ids[keep], t[keep], row_scale=np.full(3, 0.25), rest=rest)
+            near(got["row_loss"][keep], ref["row_loss"], 400 * U * ref["loss_size"], "loss of a row")
+            near(got["dlogits"][keep], ref["dlogits"], ref["size"] * 600 * U + 2.0 ** -120, "gradient")
+
+
+def test_the_same_call_gives_the_same_bits():
+    rng = np.random.default_rng(9)
+    for n, v, dtype in ((3, 151936, "bf16"), (500, 5003, "f32"), (300, 32768, "f32")):
+        x = rounded(rng.standard_normal((n, v)).astype(np.float32) * 2, dtype)
+        ids, t = teacher_of(rng, n, v, 50, True)
+        for what in ("both", "apart"):
+            first = run(x, ids, t, dtype, what, rest=True)
+            for _ in range(2):
+                again = run(x, ids, t, dtype, what, rest=True)
+                assert all(np.array_equal(first[k], again[k]) for k in first)
+
+
+def test_recorded_calls_follow_their_inputs():
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(12)
+    n, v, top = 37, 5003, 9
+    tx, g, row, loss, dl = (up(np.zeros(s, np.float32)) for s in ((n, v), (n, v), (n,), (1,), (1,)))
+    ti, tt, st = up(np.zeros((n, top), np.int32)), up(np.zeros((n, top), np.float32)), up(np.zeros((n, 4), np.float32))
+
+    def apart(c):
+        c.distill_forward(tx, v, ti, tt, None, loss, row, st, n, v, top, 1.0, ag.AG_DISTILL_REST)
+        c.distill_backward(tx, v, ti, tt, None, st, dl, None, g, v, n, v, top, 1.0, ag.AG_DISTILL_REST)
+
+    def both(c):
+        c.distill_forward_backward(tx, v, ti, tt, None, dl, loss, row, None, g, v, n, v, top, 1.0, ag.AG_DISTILL_REST)
+    for f in (apart, both):
+        f(ctx)
+        ctx.synchronize()
+        graph = ctx.record(f)
+        for _ in range(2):
+            x = rng.standard_normal((n, v)).astype(np.float32)
+            ids, t = teacher_of(rng, n, v, top, True)
+            scale = float(rng.random())
+            for a, b in ((tx, x), (ti, ids), (tt, t), (dl, np.array([scale], np.float32))):
+                be.copy_from_host(a, b)
+            ctx.replay(graph)
+            ref = R.distill(x, ids, t, dloss=np.float32(scale), rest=True)
+            near(down(row), ref["row_loss"], 400 * U * ref["loss_size"], "loss of a row")
+            near(down(g), ref["dlogits"], ref["size"] * (400 + 16 * np.abs(ref["lp"])) * U + 2.0 ** -120, "gradient")
+        ctx.drop_recording(graph)
+    free(tx, g, row, loss, dl, ti, tt, st)
+
+
+def test_a_student_learns_from_its_teachers_list():
+    """The operators as a training program strings them together: the teacher's head, its likeliest tokens with their
+    log-probabilities, the student's head (a padded vocabulary), loss and gradient in the logits' place, back through the head."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(31)
+    n, c, v, width, top = 200, 128, 1001, 1008, 24
+    f32 = np.float32
+    hidden = (rng.standard_normal((n, c)) / np.sqrt(c)).astype(f32)
+    teacher_w = rng.standard_normal((c, width)).astype(f32) * 2
+    student_w = rng.standard_normal((c, width)).astype(f32) * 2
+    student_w[:, v:] = 0   # a padded column
+    th, tw, sw = up(hidden), up(teacher_w), up(student_w)
+    tz, sz = up(np.zeros((n, width), f32)), up(np.zeros((n, width), f32))
+    ids, lp = up(np.zeros((n, top), np.int32)), up(np.zeros((n, top), f32))
+    row, loss, one = up(np.zeros(n, f32)), up(np.zeros(1, f32)), up(np.ones(1, f32))
+    dh, dw = up(np.zeros((n, c), f32)), up(np.zeros((c, width), f32))
+    nbytes = ctx.linear_add_scratch_bytes(n, c, width)
+    ws = alloc.alloc((nbytes,), np.uint8)
+    for w, z in ((tw, tz), (sw, sz)):
+        ctx.linear_add_forward(None, th, w, None, z, n, c, width, ag.AG_CE_3XTF32, ws, nbytes)
+    be.token_logprobs_forward(tz, None, None, top_ids=ids, top_logprobs=lp, temperature=2.0, vocab=v)
+    be.distill_forward_backward(sz, ids, lp, one, row, sz, loss=loss, temperature=2.0, rest=True, vocab=v)
+    z = down(tz)[:, :v]
+    got_ids = down(ids)
+    assert np.array_equal(got_ids, R.top(z, top))
+    x = hidden.astype(np.float64) @ student_w.astype(np.float64)
+    grad = down(sz)
+    # what the padded columns hold is the head's output for them, 0: no gradient goes into them
+    assert not grad[:, v:].any()
+    ctx.linear_add_backward(sz, th, sw, None, dh, dw, None, n, c, width, ag.AG_CE_3XTF32, ws, nbytes)
+    ref = R.distill(x[:, :v], got_ids, down(lp), temperature=2.0, rest=True)
+    # the projection is fp32-grade: 2^-22 of the sizes of its terms per product, here 2e-6 of logits of size 2, which moves a
+    # gradient by 1e-5 of itself; 1e-4 is what the framework holds fp32 gradients to
+    assert abs(down(loss)[0] - ref["loss"]) < 1e-5 * abs(ref["loss"])
+    for got, want in ((grad[:, :v], ref["dlogits"]), (down(dh), ref["dlogits"] @ student_w[:, :v].astype(np.float64).T),
+                      (down(dw)[:, :v], hidden.astype(np.float64).T @ ref["dlogits"])):
+        assert np.max(np.abs(got - want)) < 1e-4 * np.sqrt(np.mean(want ** 2)) + 1e-4 * np.max(np.abs(want))
+    ctx.synchronize()
+    alloc.free(ws)
+    free(th, tw, sw, tz, sz, ids, lp, row, loss, one, dh, dw)
+    check_clean_status()
+
+
+def test_a_policy_step_after_a_head():
+    """Head, log-probabilities and entropy of the rollouts' tokens, their gradient onto a loss's that is there already."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(32)
+    n, c, v = 96, 64, 640
+    hidden, w = rng.standard_normal((n, c)).astype(np.float32) / 8, rng.standard_normal((c, v)).astype(np.float32)
+    th, tw, z = up(hidden), up(w), up(np.zeros((n, v), np.float32))
+    nbytes = ctx.linear_add_scratch_bytes(n, c, v)
+    ws = alloc.alloc((nbytes,), np.uint8)
+    ctx.linear_add_forward(None, th, tw, None, z, n, c, v, ag.AG_CE_3XTF32, ws, nbytes)
+    ids = rng.integers(-1, v, n)
+    tid, lp, ent, st = up(ids.astype(np.int32)), up(np.zeros(n, np.float32)), up(np.zeros(n, np.float32)), up(np.zeros((n, 4), np.float32))
+    be.token_logprobs_forward(z, tid, lp, entropy=ent, stats=st)
+    x = down(z).astype(np.float64)
+    want, h, lps, _, _ = R.token_logprobs(x, ids)
+    near(down(lp), want, (300 + 8 * np.abs(want)) * U, "log-probability")
+    a, b, there = (rng.standard_normal(s).astype(np.float32) for s in (n, n, (n, v)))
+    ta, tb, g = up(a), up(b), up(there)
+    be.token_logprobs_backward(z, tid, st, ta, tb, g, dres=g)
+    ref, size, _ = R.token_logprobs_backward(x, ids, a, b)
+    near(down(g), ref + there, (size * 1000 + np.abs(there)) * U, "gradient")
+    ctx.synchronize()
+    alloc.free(ws)
+    free(th, tw, z, tid, lp, ent, st, ta, tb, g)
