@@ -7,162 +7,383 @@
 //   d logits_j = s / temperature (p_j (Q + r) - sum_{k: id_k = j} q_k - r [j not listed] p_j / p_rest),  Q = sum q
 //
 // p_rest is summed over the unlisted logits themselves: 1 - sum_k p_id_k would keep nothing of a small rest.  A slot with a
-// negative id is not in use.  A block takes a row; a bitmap of the row's listed tokens in shared memory tells them apart.
+// negative id is not in use.
+//
+// Loss, and loss with gradient: rows cut into slices (ag_vocab.cuh), thread k has slot k.  Before the statistics are summed
+// the listed logits of the slice are replaced by -inf, so that the sum is that of the others; the listed ones are added from
+// the threads that have them, each token once.  The gradient is written from the slice, the listed tokens' entries after it.
+// Gradient alone: packets in registers, 16 KB of a row per block, which stages the listed logits among them first.
 #include "ag_vocab.cuh"
 
 namespace {
 
-constexpr int DI_THREADS = 512;
-constexpr int DI_WARPS = DI_THREADS / 32;
+constexpr int DI_THREADS = AG_ROW_THREADS, DI_WARPS = DI_THREADS / 32;
+static_assert(AG_DISTILL_MAX <= DI_THREADS, "a slot per thread");
 
 struct DistillArgs {
   const int32_t* ids;
   const float* teacher;
   const float* row_scale;  // null: 1 / N
   const float* dloss;      // null: no gradient
-  float* row_loss;         // null: no loss
+  float* row_loss;
   float4* stats;           // (m, L, ln p_rest, 0)
   int64_t N, ld, ld_grad;
   int V, top, rest;
   float inv_tau;
   int* status;
+  int S, per, buffers;
 };
 
-// The row's list in shared memory: token (-1: not in use), teacher's probability, its logarithm.
+// Part of a list, and the whole of it merged from parts: m the largest t, sum = sum exp((t - m) / temperature) (RENORM) or the
+// mass in 64 bits (REST).
+struct DistillPart {
+  float m;
+  int nan;
+  double sum;
+};
 struct DistillList {
-  int id[AG_DISTILL_MAX];
-  float q[AG_DISTILL_MAX], log_q[AG_DISTILL_MAX], x[AG_DISTILL_MAX];
-  float mass, left;  // Q and r
-  int used;
+  float m, log_sum, inv_sum;  // RENORM
+  float mass, left;           // sum q and r
+  bool used;
 };
-
-// By all threads of the block; ends with a barrier.
-__device__ void distill_list(DistillList& l, const DistillArgs& a, int64_t row) {
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    float m = -INFINITY;
-    bool nan = false;
-    for (int k = lane; k < a.top; k += 32) {
-      int id = a.ids[row * a.top + k];
-      if (id >= a.V) {
-        atomicOr(a.status, AG_STATUS_BAD_INDEX);
-        id = -1;
-      }
-      const float t = id < 0 ? -INFINITY : a.teacher[row * a.top + k];
-      l.id[k] = id;
-      l.log_q[k] = t;
-      m = fmaxf(m, t);
-      nan |= t != t;
-    }
-    m = ag_warp_max(m);
-    nan = __any_sync(0xffffffffu, nan);
-    const bool used = m > -INFINITY || nan;
-    double mass = 0.0;
-    float sum = 0.0f;
-    for (int k = lane; k < a.top; k += 32) {
-      float t = l.log_q[k];
-      if (!a.rest) t = t == -INFINITY ? t : (t - m) * a.inv_tau;
-      const float q = expf(t);
-      l.log_q[k] = t;
-      l.q[k] = q;
-      sum += q;
-      mass += q;
-    }
-    sum = ag_warp_sum(sum);
+__device__ __forceinline__ DistillPart distill_part(float t, bool rest, float inv_tau) {
+  DistillPart p;
+  p.m = ag_warp_max(t);  // ignores NaN
+  p.nan = __any_sync(0xffffffffu, t != t);
+  if (rest) {
+    p.sum = expf(t);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    if (!a.rest && used) {
-      const float log_sum = logf(sum), inv = 1.0f / sum;
-      for (int k = lane; k < a.top; k += 32) {
-        l.log_q[k] -= log_sum;
-        l.q[k] *= inv;
-      }
-    }
-    if (lane == 0) {
-      l.used = used;
-      l.mass = !used ? 0.0f : a.rest ? (float)mass : sum != sum ? sum : 1.0f;
-      l.left = a.rest && used ? (float)(1.0 - mass > 0.0 ? 1.0 - mass : mass != mass ? mass : 0.0) : 0.0f;
-    }
+    for (int o = 16; o > 0; o >>= 1) p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
+  } else {
+    p.sum = ag_warp_sum(t == -INFINITY ? 0.0f : expf((t - p.m) * inv_tau));
   }
-  __syncthreads();
+  return p;
+}
+__device__ __forceinline__ DistillList distill_list(const DistillPart* part, int n, bool rest, float inv_tau) {
+  DistillList l;
+  l.m = part[0].m;
+  int nan = part[0].nan;
+  for (int w = 1; w < n; ++w) l.m = fmaxf(l.m, part[w].m), nan |= part[w].nan;
+  l.used = l.m > -INFINITY || nan;
+  l.log_sum = 0.0f, l.inv_sum = 1.0f, l.left = 0.0f;
+  if (rest) {
+    double mass = 0.0;
+    for (int w = 0; w < n; ++w) mass += part[w].sum;
+    l.mass = (float)mass;
+    l.left = (float)(1.0 - mass > 0.0 ? 1.0 - mass : mass != mass ? mass : 0.0);
+  } else {
+    float sum = 0.0f;
+    for (int w = 0; w < n; ++w)
+      if (part[w].m != -INFINITY || part[w].nan) sum += (float)part[w].sum * expf((part[w].m - l.m) * inv_tau);
+    if (nan) sum = NAN;
+    l.log_sum = logf(sum);
+    l.inv_sum = 1.0f / sum;
+    l.mass = sum != sum ? sum : 1.0f;
+  }
+  if (!l.used) l.mass = l.left = 0.0f;
+  return l;
+}
+// ln q and q of a slot with value t
+__device__ __forceinline__ void distill_slot(const DistillList& l, float t, bool rest, float inv_tau, float& log_q, float& q) {
+  const float d = rest || t == -INFINITY ? t : (t - l.m) * inv_tau;
+  log_q = d - l.log_sum;
+  q = l.used ? expf(d) * l.inv_sum : 0.0f;
+}
+// what a listed and an unlisted token's p are multiplied with, before the row's scale
+__device__ __forceinline__ float distill_outside(const DistillList& l, float log_rest) {
+  return l.mass + l.left - (l.left != 0.0f && log_rest > -INFINITY ? l.left * expf(-log_rest) : 0.0f);
+}
+__device__ __forceinline__ float distill_scale(const DistillArgs& a, int64_t row) {
+  const float w = a.row_scale ? a.row_scale[row] : 1.0f / (float)a.N;
+  return w == 0.0f ? 0.0f : a.dloss[0] * w * a.inv_tau;
 }
 
-template <typename T>
+// Puts -inf in the place of a logit in shared memory and returns what was there.
+__device__ __forceinline__ float distill_take(float* p) { return atomicExch(p, -INFINITY); }
+__device__ __forceinline__ float distill_take(__nv_bfloat16* p) {
+  unsigned short* w = reinterpret_cast<unsigned short*>(p);
+  unsigned short old = *w, was;
+  while ((was = atomicCAS(w, old, (unsigned short)0xff80)) != old) old = was;  // only the threads of one token meet here
+  return __uint_as_float((uint32_t)old << 16);
+}
+
+size_t distill_smem(int S) {
+  return 2 * (size_t)S * DI_WARPS * 16 + 2 * DI_WARPS * sizeof(DistillPart) + 5 * AG_DISTILL_MAX * 4 + 32 * 4 + DI_WARPS * 4 + 64;
+}
+
+template <typename T, bool TRAIN>
 __global__ void __launch_bounds__(DI_THREADS)
-distill_kernel(const T* logits, const T* dres, T* dlogits, DistillArgs a, int have_stats) {
-  extern __shared__ uint32_t s_listed[];  // a bit per token
-  __shared__ DistillList l;
-  __shared__ AgStat s_stat[DI_WARPS];
+distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
+  constexpr int NV = AG_PACKET<T>;
+  extern __shared__ uint4 s_slices[];
+  const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
+  const int groups = S * DI_WARPS, parts = (a.top + 31) / 32;
+  float4* s_stat = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);      // [2][groups]
+  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_stat + 2 * groups);           // [2][DI_WARPS]
+  int* s_next_id = reinterpret_cast<int*>(s_parts + 2 * DI_WARPS);                      // a slot per thread, copied ahead
+  float* s_next_t = reinterpret_cast<float*>(s_next_id + AG_DISTILL_MAX);
+  int* s_ids = reinterpret_cast<int*>(s_next_t + AG_DISTILL_MAX);                        // [2][slots]
+  float* s_q = reinterpret_cast<float*>(s_ids + 2 * AG_DISTILL_MAX);                     // [slots]
+  float* s_edge = s_q + AG_DISTILL_MAX;                                                  // [32]
+  float* s_sum = s_edge + 32;                                                            // [DI_WARPS]
+  int* s_twice = reinterpret_cast<int*>(s_sum + DI_WARPS);                               // [2]: a token is listed twice
+  const int64_t clusters = gridDim.x / S;
+  const float c = a.inv_tau * AG_LOG2E;
+  const bool rest = a.rest;
+  auto fetch_slot = [&](int64_t row) {  // with the packets of that row, by the thread that reads it
+    if (tid < a.top) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ag_smem_u32(s_next_id + tid)), "l"(a.ids + row * a.top + tid) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ag_smem_u32(s_next_t + tid)), "l"(a.teacher + row * a.top + tid) : "memory");
+    }
+  };
+  if (tid < 2) s_twice[tid] = 0;
+  if (S > 1) ag_cluster_sync(S);  // all of them run before one stores to another
   ag_pdl_wait();
   ag_pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * a.ld;
-  const float c = a.inv_tau * AG_LOG2E;
-  for (int j = threadIdx.x; j < (a.V + 31) / 32; j += DI_THREADS) s_listed[j] = 0;
-  distill_list(l, a, row);
-  for (int k = threadIdx.x; k < a.top; k += DI_THREADS)
-    if (l.id[k] >= 0) {
-      atomicOr(&s_listed[l.id[k] >> 5], 1u << (l.id[k] & 31));
-      l.x[k] = Pack<T>::load1(x + l.id[k]);
+
+  int64_t row = blockIdx.x / S;
+  AgRow<T> r(logits + row * a.ld, a.V);
+  fetch_slot(row);
+  r.fetch(s_slices, rank, a.per);
+  int edge_index = r.edge(rank);
+  float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
+  for (int turn = 0; row < a.N; ++turn) {
+    const int now = turn & 1;
+    const bool lead = turn % S == rank, more = row + clusters < a.N;
+    uint4* slice = s_slices + (a.buffers == 2 && now ? a.per : 0);
+    const int n = r.mine(rank, a.per), at_edge = edge_index;
+    float x_edge = edge;
+    ag_fetched();
+    int id = -1;
+    float t = -INFINITY;
+    if (tid < a.top) {
+      id = s_next_id[tid];
+      if (id >= a.V) {
+        if (lead) atomicOr(a.status, AG_STATUS_BAD_INDEX);
+        id = -1;
+      }
+      if (id >= 0) t = s_next_t[tid];
+      s_ids[now * AG_DISTILL_MAX + tid] = id;
     }
-  __syncthreads();
-  float m, L, log_rest;
-  if (have_stats) {
-    const float4 st = a.stats[row];
-    m = st.x, L = st.y, log_rest = st.z;
-  } else {
-    AgStat in = ag_stat_none(), out = ag_stat_none();
-    for (int j = threadIdx.x; j < a.V; j += DI_THREADS) {
-      const float xj = Pack<T>::load1(x + j);
-      const AgStat one = {xj, xj == -INFINITY ? 0.0f : xj - xj + 1.0f, 0.0f};
-      if (s_listed[j >> 5] >> (j & 31) & 1) in = ag_stat_merge(in, one, c);
-      else out = ag_stat_merge(out, one, c);
+    const bool own = id >= 0 && r.owner(id, a.per) == rank;
+    float x_id = -INFINITY;
+    if (id >= 0 && (lead || own)) x_id = Pack<T>::load1(r.x + id);
+    const AgRow<T> next(more ? logits + (row + clusters) * a.ld : r.x, a.V);
+    if (more) {
+      fetch_slot(row + clusters);
+      if (a.buffers == 2) next.fetch(s_slices + (now ? 0 : a.per), rank, a.per);
+      edge_index = next.edge(rank);
+      edge = edge_index >= 0 ? Pack<T>::load1(next.x + edge_index) : -INFINITY;
+    }
+    if (warp < parts) {
+      const DistillPart p = distill_part(t, rest, a.inv_tau);
+      if (lane == 0) s_parts[now * DI_WARPS + warp] = p;
+    }
+    if (at_edge >= 0) s_edge[tid] = x_edge;
+    __syncthreads();  // the slice is complete, for threads other than the one that copied, too
+    bool once = own;
+    if (own) {
+      const int q = id - r.head;
+      float was;
+      if (q < 0) was = distill_take(s_edge + id);
+      else if (q >= r.body * NV) was = distill_take(s_edge + 16 + q - r.body * NV);
+      else was = distill_take(reinterpret_cast<T*>(slice) + (q - rank * a.per * NV));
+      if (was == -INFINITY) s_twice[now] = 1;  // or masked: looked at in the same way
+    }
+    __syncthreads();
+    if (tid == 0) s_twice[now ^ 1] = 0;
+    const bool twice = s_twice[now];
+    if (twice && own)
+      for (int k = 0; k < tid; ++k) once &= s_ids[now * AG_DISTILL_MAX + k] != id;
+    if (at_edge >= 0) x_edge = s_edge[tid];
+
+    const AgStat mine = ag_stat_warp(ag_slice_stat<false, T>(slice, n, x_edge, c), c);
+    AgStat in = ag_stat_none();
+    if (warp < parts) {
+      if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
+      in = ag_stat_warp(in, c);
+    }
+    {
+      const float4 out = make_float4(mine.m, mine.s, in.m, in.s);
+      float4* to = s_stat + now * groups + rank * DI_WARPS + warp;
+      if (S == 1) {
+        if (lane == 0) *to = out;
+      } else if (lane < S) {
+        ag_peer_store(ag_peer(to, lane), out);
+      }
+    }
+    ag_cluster_sync(S);
+    AgStat out = ag_stat_none();
+    in = ag_stat_none();
+    for (int g = lane; g < groups; g += 32) {
+      const float4 w = s_stat[now * groups + g];
+      out = ag_stat_merge(out, {w.x, w.y, 0.0f}, c);
+      in = ag_stat_merge(in, {w.z, w.w, 0.0f}, c);
     }
     out = ag_stat_warp(out, c);
     in = ag_stat_warp(in, c);
-    if ((threadIdx.x & 31) == 0) s_stat[threadIdx.x >> 5] = out;
-    __syncthreads();
-    out = s_stat[0];
-    for (int w = 1; w < DI_WARPS; ++w) out = ag_stat_merge(out, s_stat[w], c);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_stat[threadIdx.x >> 5] = in;
-    __syncthreads();
-    in = s_stat[0];
-    for (int w = 1; w < DI_WARPS; ++w) in = ag_stat_merge(in, s_stat[w], c);
     const AgStat all = ag_stat_merge(in, out, c);
-    m = all.m;
-    L = logf(all.s);
-    log_rest = out.m == -INFINITY && out.s == 0.0f ? -INFINITY : (out.m - m) * a.inv_tau + logf(out.s) - L;
-    if (threadIdx.x == 0 && a.stats) a.stats[row] = make_float4(m, L, a.rest ? log_rest : 0.0f, 0.0f);
-  }
-  auto log_p = [&](float xj) { return xj == -INFINITY && !(L != L) ? -INFINITY : (xj - m) * a.inv_tau - L; };
-  if (a.row_loss && threadIdx.x < 32) {
-    float sum = 0.0f;
-    for (int k = threadIdx.x; k < a.top; k += 32)
-      if (l.id[k] >= 0 && l.q[k] != 0.0f) sum += l.q[k] * (l.log_q[k] - log_p(l.x[k]));
-    sum = ag_warp_sum(sum);
-    if (l.left != 0.0f) sum += l.left * (logf(l.left) - log_rest);
-    if (threadIdx.x == 0) a.row_loss[row] = l.used ? sum : 0.0f;
-  }
-  if (!a.dloss) return;
-  const float w = a.row_scale ? a.row_scale[row] : 1.0f / (float)a.N;
-  const float s = w == 0.0f ? 0.0f : a.dloss[0] * w * a.inv_tau;
-  const bool none = s == 0.0f || !l.used || (m == -INFINITY && L == -INFINITY);
-  const float r = l.left;
-  const float outside = l.mass + r - (r != 0.0f && log_rest > -INFINITY ? r * expf(-log_rest) : 0.0f), inside = l.mass + r;
-  for (int j = threadIdx.x; j < a.V; j += DI_THREADS) {
-    const bool listed = s_listed[j >> 5] >> (j & 31) & 1;
-    float g = 0.0f;
-    if (!none) {
-      const float p = ag_ex2(((Pack<T>::load1(x + j) - m) * a.inv_tau - L) * AG_LOG2E);
-      g = p * (listed ? inside : outside);
-      if (listed)
-        for (int k = 0; k < a.top; ++k)
-          if (l.id[k] == j) g -= l.q[k];
-      g *= s;
+    const float m = all.m, L = logf(all.s);
+    const float log_rest = out.m == -INFINITY && out.s == 0.0f ? -INFINITY : (out.m - m) * a.inv_tau + logf(out.s) - L;
+    const DistillList list = distill_list(s_parts + now * DI_WARPS, parts, rest, a.inv_tau);
+    float log_q = 0.0f, q = 0.0f;
+    if (id >= 0) distill_slot(list, t, rest, a.inv_tau, log_q, q);
+    if (tid < a.top) s_q[tid] = q;
+    auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - m) * a.inv_tau - L; };
+    if (lead) {
+      if (warp < parts) {
+        const float sum = ag_warp_sum(id >= 0 && q != 0.0f ? q * (log_q - log_p(x_id)) : 0.0f);
+        if (lane == 0) s_sum[warp] = sum;
+      }
+      __syncthreads();
+      if (tid == 0) {
+        float sum = list.left != 0.0f ? list.left * (logf(list.left) - log_rest) : 0.0f;
+        for (int w = 0; w < parts; ++w) sum += s_sum[w];
+        a.row_loss[row] = list.used ? sum : 0.0f;
+        if (a.stats) a.stats[row] = make_float4(m, L, rest ? log_rest : 0.0f, 0.0f);
+      }
     }
-    if (dres) g += Pack<T>::load1(dres + row * a.ld_grad + j);
-    Pack<T>::store1(dlogits + row * a.ld_grad + j, g);
+    if (TRAIN) {
+      const float s = distill_scale(a, row);
+      const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
+      const float outside = none ? 0.0f : s * distill_outside(list, log_rest);
+      const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
+      const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
+      T* g_row = dlogits + row * a.ld_grad;
+      T* g_body = g_row + r.head + (int64_t)rank * a.per * NV;
+      const bool packets = (((uintptr_t)g_body) & 15) == 0;
+      for (int i = tid; i < n; i += DI_THREADS) {
+        float x[NV], g[NV];
+        ag_widen(slice[i], x);
+#pragma unroll
+        for (int e = 0; e < NV; e += 2) {
+          float d0, d1;
+          ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
+          g[e] = none ? 0.0f : outside * ag_ex2(d0);
+          g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
+        }
+        ag_store_packet<T>(g_body + (int64_t)i * NV, g, packets);
+      }
+      if (at_edge >= 0) Pack<T>::store1(g_row + at_edge, none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift));
+      __syncthreads();  // the entries of listed tokens are written once more
+      if (once) {
+        if (twice)
+          for (int k = tid + 1; k < a.top; ++k)
+            if (s_ids[now * AG_DISTILL_MAX + k] == id) q += s_q[k];
+        const float p = ag_ex2((x_id - m) * c + shift);
+        Pack<T>::store1(g_row + id, none ? 0.0f : s * (p * (list.mass + list.left) - q));
+      }
+    }
+    if (more && a.buffers == 1) next.fetch(s_slices, rank, a.per);
+    r = next;
+    row += clusters;
+  }
+  if (S > 1) ag_cluster_sync(S);  // nobody leaves while others may still store to its shared memory
+}
+
+// The gradient alone, from the statistics that the loss left: a block takes 16 KB of a row.
+constexpr int DB_PACKETS = 4;  // per thread
+template <typename T>
+__global__ void __launch_bounds__(DI_THREADS)
+distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const DistillArgs a, int chunks) {
+  constexpr int NV = AG_PACKET<T>, CHUNK = DI_THREADS * DB_PACKETS;
+  __shared__ DistillPart s_parts[DI_WARPS];
+  __shared__ int s_ids[AG_DISTILL_MAX];
+  __shared__ float s_q[AG_DISTILL_MAX];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = (a.top + 31) / 32;
+  ag_pdl_wait();
+  ag_pdl_trigger();
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - row * chunks);
+  const AgRow<T> r(logits + row * a.ld, a.V);
+  const int n = r.mine(chunk, CHUNK);
+  const T* x_body = r.x + r.head + (int64_t)chunk * CHUNK * NV;
+  T* g_row = dlogits + row * a.ld_grad;
+  const T* d_row = dres ? dres + row * a.ld_grad : nullptr;
+  const int64_t g_off = r.head + (int64_t)chunk * CHUNK * NV;
+  uint4 w[DB_PACKETS];
+#pragma unroll
+  for (int u = 0; u < DB_PACKETS; ++u) {
+    const int i = tid + u * DI_THREADS;
+    w[u] = i < n ? __ldcs(reinterpret_cast<const uint4*>(x_body + (int64_t)i * NV)) : make_uint4(0, 0, 0, 0);
+  }
+  const float4 st = a.stats[row];
+  const float m = st.x, L = st.y, c = a.inv_tau * AG_LOG2E;
+  int id = -1;
+  float t = -INFINITY, x_id = 0.0f, d_id = 0.0f;
+  if (tid < a.top) {
+    id = a.ids[row * a.top + tid];
+    if (id >= a.V) {
+      if (chunk == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
+      id = -1;
+    }
+    if (id >= 0) t = a.teacher[row * a.top + tid];
+    s_ids[tid] = id;
+  }
+  const int edge_index = r.edge(chunk);
+  const float x_edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : 0.0f;
+  const bool own = id >= 0 && r.owner(id, CHUNK) == chunk;
+  if (own) {
+    x_id = Pack<T>::load1(r.x + id);
+    if (d_row) d_id = Pack<T>::load1(d_row + id);
+  }
+  if (warp < parts) {
+    const DistillPart p = distill_part(t, a.rest, a.inv_tau);
+    if (lane == 0) s_parts[warp] = p;
+  }
+  __syncthreads();
+  const DistillList list = distill_list(s_parts, parts, a.rest, a.inv_tau);
+  float log_q, q = 0.0f;
+  if (id >= 0) distill_slot(list, t, a.rest, a.inv_tau, log_q, q);
+  if (tid < a.top) s_q[tid] = q;
+  const float s = distill_scale(a, row);
+  const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
+  const float outside = none ? 0.0f : s * distill_outside(list, st.z);
+  const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
+  const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
+  const bool packets = (((uintptr_t)(g_row + g_off)) & 15) == 0, d_packets = (((uintptr_t)(d_row + g_off)) & 15) == 0;
+#pragma unroll
+  for (int u = 0; u < DB_PACKETS; ++u) {
+    const int i = tid + u * DI_THREADS;
+    if (i >= n) break;
+    float x[NV], g[NV];
+    ag_widen(w[u], x);
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) {
+      float d0, d1;
+      ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
+      g[e] = none ? 0.0f : outside * ag_ex2(d0);
+      g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
+    }
+    const int64_t at = g_off + (int64_t)i * NV;
+    if (d_row) {
+      float d[NV];
+      if (d_packets) {
+        Pack<T>::load_stream(d_row + at, d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < NV; ++e) d[e] = Pack<T>::load1(d_row + at + e);
+      }
+#pragma unroll
+      for (int e = 0; e < NV; ++e) g[e] += d[e];
+    }
+    ag_store_packet<T>(g_row + at, g, packets);
+  }
+  if (edge_index >= 0) {
+    const float d = d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f;
+    Pack<T>::store1(g_row + edge_index, (none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift)) + d);
+  }
+  __syncthreads();  // the entries of listed tokens are written once more
+  if (own) {
+    bool once = true;
+    q = 0.0f;
+    for (int k = 0; k < a.top; ++k)
+      if (s_ids[k] == id) {
+        once &= k >= tid;
+        q += s_q[k];
+      }
+    const float p = ag_ex2((x_id - m) * c + shift);
+    if (once) Pack<T>::store1(g_row + id, (none ? 0.0f : s * (p * (list.mass + list.left) - q)) + d_id);
   }
 }
 
@@ -189,16 +410,24 @@ distill_loss_kernel(const float* __restrict__ row_loss, const float* __restrict_
   }
 }
 
+template <typename T, bool TRAIN>
+int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs a) {
+  static AgClusterFit fits[AG_MAX_DEVICES];
+  const AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, distill_smem);
+  a.S = p.S;
+  a.per = p.per;
+  a.buffers = p.buffers;
+  return ag_launch_rows(ctx, "distill_kernel", fits, distill_kernel<T, TRAIN>, p, a.N, (const T*)logits, (T*)dlogits, a);
+}
+
 template <typename T>
-int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, const DistillArgs& a, int have_stats) {
-  const size_t smem = (size_t)(a.V + 31) / 32 * 4;
-  static bool ready[AG_MAX_DEVICES];
-  if (!ready[ag_dev_slot(ctx)]) {
-    AG_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (AG_VOCAB_MAX + 31) / 32 * 4));
-    ready[ag_dev_slot(ctx)] = true;
-  }
-  AG_LAUNCH_PDL(ctx, "distill_kernel", distill_kernel<T>, (unsigned)a.N, DI_THREADS, smem, (const T*)logits, (const T*)dres, (T*)dlogits,
-                a, have_stats);
+int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, const DistillArgs& a, bool backward) {
+  if (!backward)
+    return a.dloss ? distill_forward<T, true>(ctx, logits, dlogits, a) : distill_forward<T, false>(ctx, logits, dlogits, a);
+  const int packets = a.V / AG_PACKET<T>, chunks = packets ? (packets + DI_THREADS * DB_PACKETS - 1) / (DI_THREADS * DB_PACKETS) : 1;
+  AG_REQUIRE(ctx, a.N * chunks < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
+  AG_LAUNCH_PDL(ctx, "distill_backward_kernel", distill_backward_kernel<T>, (unsigned)(a.N * chunks), DI_THREADS, 0, (const T*)logits,
+                (const T*)dres, (T*)dlogits, a, chunks);
   return AG_OK;
 }
 
@@ -211,10 +440,11 @@ int distill(ag_ctx* ctx, const char* who, const void* logits, int64_t ld, const 
   AG_REQUIRE(ctx, top > 0, "%s: a list of no tokens", who);
   AG_REQUIRE(ctx, (ids && teacher && (backward ? stats : row_loss) && (dloss || ld_grad < 0)) || N == 0, "%s: null pointer", who);
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
+  AG_REQUIRE(ctx, (((uintptr_t)ids | (uintptr_t)teacher) & 3) == 0, "%s: teacher's lists not aligned", who);
   if (N == 0 && !loss) return AG_OK;
   AgOnDevice on(ctx);
   const DistillArgs a = {ids, teacher, row_scale, dloss, row_loss, (float4*)stats, N, ld, ld_grad, V, top, mode == AG_DISTILL_REST,
-                         1.0f / temperature, ctx->d_status};
+                         1.0f / temperature, ctx->d_status, 0, 0, 0};
   if (int rc = N == 0 ? AG_OK
                : dtype == AG_F32 ? distill_t<float>(ctx, logits, dres, dlogits, a, backward)
                                  : distill_t<__nv_bfloat16>(ctx, logits, dres, dlogits, a, backward))

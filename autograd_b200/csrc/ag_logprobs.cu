@@ -4,88 +4,408 @@
 //   entropy H = L - sum_j p_j (x_j - m) / temperature
 //   d logits_j = (a (delta_j,id - p_j) - b p_j (log p_j + H)) / temperature,  a = dlogprob (0 without a token), b = dentropy
 //
-// A block takes a row and reads it once for the statistics, once more from L2 for each alternative.
+// Forward: rows cut into slices (ag_vocab.cuh).  The alternatives come from the slices, too:
+//   each warp hands round its J largest lane maxima along with its statistics; the top-th largest of all these is a bound that at
+//   least `top` logits reach, and few more do, since the lanes' logits lie spread over the row;
+//   the logits that reach it are collected, (order, index) as one key each, by the threads whose maximum does;
+//   one block of the cluster counts for each how many are larger, which is its place.
+// A block that collects more than twice what can be asked for (many equal logits, or the largest ones all in a few lanes)
+// searches a bound of its own first, bit by bit, and takes logits that equal it in the order of their index.
 #include "ag_vocab.cuh"
 
 namespace {
 
-constexpr int LP_THREADS = 512;
-constexpr int LP_WARPS = LP_THREADS / 32;
+constexpr int LP_THREADS = AG_ROW_THREADS, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_POOL = 256;  // lane maxima that are handed round
+
+struct LpArgs {
+  const int32_t* ids;
+  float *logprob, *entropy;
+  float4* stats;
+  int32_t* top_ids;
+  float* top_logprobs;
+  int64_t N, ld;
+  int V, top;
+  float inv_tau;
+  int S, per, buffers;
+  int J, cap;  // lane maxima per warp, keys per block
+};
+
+size_t lp_smem(int S, int J, int cap) {
+  return 2 * (size_t)S * LP_WARPS * 16 + 2 * (size_t)S * LP_WARPS * J * 4 + 2 * (size_t)cap * 8 + 128;
+}
+
+__device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
+
+// The largest bound that at least `top` of the n values in `pool` reach, or one that few more do; by one warp.
+__device__ float lp_bound(const float* pool, int n, int top) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[LP_POOL / 32];
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int i = 0; i < LP_POOL / 32; ++i) {
+    key[i] = lane + 32 * i < n ? ag_order(pool[lane + 32 * i]) : 0u;
+    if (lane + 32 * i < n) lo = min(lo, key[i]), hi = max(hi, key[i]);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);  // n >= top values reach it
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const int enough = top + (top >> 3);
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < LP_POOL / 32; ++i) count += key[i] >= mid;
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (count >= top) {
+      lo = mid;
+      if (count <= enough) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return ag_of_order(lo);
+}
+
+template <typename T>
+struct LpSlice {
+  const uint4* at;
+  int n, first;  // packets, index of the first one's first logit
+  float edge;
+  int edge_index;  // -1: none
+  // f(logit, its index) for this thread's logits
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    constexpr int NV = AG_PACKET<T>;
+    if (edge_index >= 0) f(edge, edge_index);
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+      float x[NV];
+      ag_widen(at[i], x);
+#pragma unroll
+      for (int e = 0; e < NV; ++e) f(x[e], first + i * NV + e);
+    }
+  }
+};
+
+// The block's logits whose order is `bound` or more are more than `cap`: leaves the keys of its `top` largest at least, `cap` at
+// most, in `keys` and returns how many.  By all threads of the block.  A block that has this many has more than `top` logits.
+template <typename T>
+__device__ int lp_search(const LpSlice<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
+  uint32_t hi = 0xffffffffu;
+  auto count_from = [&](uint32_t k) {
+    int c = 0;
+    sl.each([&](float x, int) { c += ag_order(x) >= k; });
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (threadIdx.x == 0) *s_count = 0;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0 && c) atomicAdd(s_count, c);
+    __syncthreads();
+    c = *s_count;
+    __syncthreads();
+    return c;
+  };
+  bool fits = false;
+  while (lo < hi && !fits) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    const int c = count_from(mid);
+    if (c >= top) lo = mid, fits = c <= cap;
+    else hi = mid - 1;
+  }
+  // fits: all that reach lo.  Otherwise lo is the top-th largest itself: all above it (fewer than top), and then equal ones.
+  if (threadIdx.x == 0) *s_count = 0;
+  __syncthreads();
+  sl.each([&](float x, int j) {
+    const uint32_t k = ag_order(x);
+    if (k > lo || (fits && k == lo)) keys[atomicAdd(s_count, 1)] = lp_key(x, j);
+  });
+  __syncthreads();
+  int have = *s_count;
+  if (fits) return have;
+  // in the order of the index: the elements before the first packet, then packets by rounds of the block, then those behind
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int s_warp[LP_WARPS];
+  constexpr int NV = AG_PACKET<T>;
+  const int rounds = (sl.n + LP_THREADS - 1) / LP_THREADS;
+  for (int r = -1; r <= rounds && have < top; ++r) {
+    float x[NV];
+    int mine = 0, first = 0;
+    const int i = r * LP_THREADS + threadIdx.x;
+    if (r < 0 || r == rounds) {
+      const bool head = sl.edge_index >= 0 && threadIdx.x < 16;
+      mine = sl.edge_index >= 0 && head == (r < 0) && ag_order(sl.edge) == lo;
+    } else if (i < sl.n) {
+      ag_widen(sl.at[i], x);
+      first = sl.first + i * NV;
+#pragma unroll
+      for (int e = 0; e < NV; ++e) mine += ag_order(x[e]) == lo;
+    }
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    if (lane == 31) s_warp[warp] = before;
+    __syncthreads();
+    int at = have + before - mine, all = 0;
+    for (int w = 0; w < LP_WARPS; ++w) {
+      if (w < warp) at += s_warp[w];
+      all += s_warp[w];
+    }
+    if (mine && at < top) {
+      if (r < 0 || r == rounds) {
+        keys[at] = lp_key(sl.edge, sl.edge_index);
+      } else {
+#pragma unroll
+        for (int e = 0; e < NV; ++e)
+          if (ag_order(x[e]) == lo && at < top) keys[at++] = lp_key(x[e], first + e);
+      }
+    }
+    have = min(have + all, top);
+    __syncthreads();
+  }
+  return have;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_THREADS)
+logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
+  extern __shared__ uint4 s_slices[];
+  const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
+  const int groups = S * LP_WARPS;
+  float4* s_stat = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);  // [2][groups]
+  unsigned long long* s_keys = reinterpret_cast<unsigned long long*>(s_stat + 2 * groups);  // [2][cap]
+  float* s_pool = reinterpret_cast<float*>(s_keys + (TOP ? 2 * a.cap : 0));                 // [2][groups * J]
+  int* s_words = reinterpret_cast<int*>(s_pool + (TOP ? 2 * groups * a.J : 0));             // [0..1] keys, [2] counter
+  float* s_bound = reinterpret_cast<float*>(s_words + 3);
+  const int64_t clusters = gridDim.x / S;
+  const float c = a.inv_tau * AG_LOG2E;
+  if (S > 1) ag_cluster_sync(S);  // all of them run before one stores to another
+  ag_pdl_wait();
+  ag_pdl_trigger();
+
+  int64_t row = blockIdx.x / S;
+  AgRow<T> r(logits + row * a.ld, a.V);
+  r.fetch(s_slices, rank, a.per);
+  int edge_index = r.edge(rank);
+  float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
+  int id = a.logprob && tid == 0 ? a.ids[row] : -1;
+  for (int turn = 0; row < a.N; ++turn) {
+    const bool lead = turn % S == rank, more = row + clusters < a.N;
+    const uint4* slice = s_slices + (a.buffers == 2 && (turn & 1) ? a.per : 0);
+    const LpSlice<T> sl = {slice, r.mine(rank, a.per), r.head + rank * a.per * AG_PACKET<T>, edge, edge_index};
+    float x_id = 0.0f;
+    const bool has = lead && id >= 0 && id < a.V;
+    if (has) x_id = Pack<T>::load1(r.x + id);
+    ag_fetched();
+    const AgRow<T> next(more ? logits + (row + clusters) * a.ld : r.x, a.V);
+    if (more) {
+      if (a.buffers == 2) next.fetch(s_slices + ((turn & 1) ? 0 : a.per), rank, a.per);
+      edge_index = next.edge(rank);
+      edge = edge_index >= 0 ? Pack<T>::load1(next.x + edge_index) : -INFINITY;
+      id = a.logprob && tid == 0 ? a.ids[row + clusters] : -1;
+    }
+
+    const AgStat own = ag_slice_stat<true, T>(slice, sl.n, sl.edge, c);
+    AgStat v = ag_stat_warp(own, c);
+    {
+      const float4 out = make_float4(v.m, v.s, v.t, 0.0f);
+      float4* to = s_stat + (turn & 1) * groups + rank * LP_WARPS + warp;
+      if (S == 1) {
+        if (lane == 0) *to = out;
+      } else if (lane < S) {
+        ag_peer_store(ag_peer(to, lane), out);
+      }
+    }
+    if (TOP) {
+      // the J largest of the lanes' maxima
+      float left = own.m, best = 0.0f;
+      for (int j = 0; j < a.J; ++j) {
+        float m;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(left));
+        const uint32_t who = __ballot_sync(0xffffffffu, left == m);
+        if (lane == j) best = m;
+        if (lane == __ffs(who) - 1) left = -INFINITY;
+      }
+      float* to = s_pool + ((turn & 1) * groups + rank * LP_WARPS + warp) * a.J;
+      if (lane < a.J) {
+        if (S == 1) to[lane] = best;
+        else
+          for (int p = 0; p < S; ++p) ag_peer_store(ag_peer(to + lane, p), best);
+      }
+    }
+    ag_cluster_sync(S);
+    v = ag_stat_none();
+    for (int g = lane; g < groups; g += 32) {
+      const float4 w = s_stat[(turn & 1) * groups + g];
+      v = ag_stat_merge(v, {w.x, w.y, w.z}, c);
+    }
+    v = ag_stat_warp(v, c);
+    const float L = logf(v.s), H = v.m == -INFINITY && v.s == 0.0f ? 0.0f : L - v.t / v.s * a.inv_tau;
+    auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - v.m) * a.inv_tau - L; };
+    if (lead && tid == 0) {
+      if (a.logprob) a.logprob[row] = has ? log_p(x_id) : 0.0f;
+      if (a.entropy) a.entropy[row] = H;
+      if (a.stats) a.stats[row] = make_float4(v.m, L, H, 0.0f);
+    }
+    if (TOP) {
+      unsigned long long* keys = s_keys + (turn & 1) * a.cap;
+      int* n_keys = s_words + (turn & 1);
+      if (warp == 0) {
+        const float b = lp_bound(s_pool + (turn & 1) * groups * a.J, groups * a.J, a.top);
+        if (lane == 0) *s_bound = b;
+      }
+      if (tid == 32) *n_keys = 0;
+      __syncthreads();
+      const float bound = *s_bound;
+      if (own.m >= bound || own.s != own.s)
+        sl.each([&](float x, int j) {
+          if (!(x < bound)) {
+            const int at = atomicAdd(n_keys, 1);
+            if (at < a.cap) keys[at] = lp_key(x, j);
+          }
+        });
+      __syncthreads();
+      if (*n_keys > a.cap) {
+        const int n = lp_search<T>(sl, ag_order(bound), a.top, a.cap, keys, s_words + 2);
+        if (tid == 0) *n_keys = n;
+      }
+      ag_cluster_sync(S);
+      if (lead) {
+        int total = 0;
+        for (int p = 0; p < S; ++p) total += S == 1 ? *n_keys : ag_peer_load_int(ag_peer(n_keys, p));
+        for (int i = tid; i < total; i += LP_THREADS) {
+          unsigned long long key = 0;
+          int place = 0;
+          for (int p = 0, at = i; p < S; ++p) {  // the i-th key of the cluster
+            const int n = S == 1 ? total : ag_peer_load_int(ag_peer(n_keys, p));
+            if (at >= 0 && at < n) key = S == 1 ? keys[at] : ag_peer_load_key(ag_peer(keys + at, p));
+            at -= n;
+          }
+          for (int p = 0; p < S; ++p) {
+            const int n = S == 1 ? total : ag_peer_load_int(ag_peer(n_keys, p));
+            for (int k = 0; k < n; ++k) place += (S == 1 ? keys[k] : ag_peer_load_key(ag_peer(keys + k, p))) > key;
+          }
+          if (place < a.top) {
+            const int64_t to = row * a.top + place;
+            a.top_ids[to] = (int32_t)~(uint32_t)key;
+            a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
+          }
+        }
+      }
+    }
+    if (more && a.buffers == 1) next.fetch(s_slices, rank, a.per);
+    r = next;
+    row += clusters;
+  }
+  if (S > 1) ag_cluster_sync(S);  // nobody leaves while another block may read its keys
+}
+
+// Gradient: a block takes 16 KB of a row, all of its loads under way before the first is used.
+constexpr int LB_PACKETS = 4;  // per thread
+struct LbArgs {
+  const int32_t* ids;
+  const float4* stats;
+  const float *dlogprob, *dentropy;
+  int64_t ld, ld_grad;
+  int V, chunks;
+  float inv_tau;
+};
 
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
-logprobs_kernel(const T* __restrict__ logits, int64_t ld, const int32_t* __restrict__ ids, float* logprob, float* entropy,
-                float4* stats, int32_t* top_ids, float* top_logprobs, int V, int top, float inv_tau) {
-  __shared__ AgStat s_stat[LP_WARPS];
-  __shared__ unsigned long long s_key[LP_WARPS];
+logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArgs p) {
+  constexpr int NV = AG_PACKET<T>, CHUNK = LP_THREADS * LB_PACKETS;
+  const int tid = threadIdx.x;
   ag_pdl_wait();
   ag_pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  const float c = inv_tau * AG_LOG2E;
-  AgStat v = ag_stat_none();
-  for (int j = threadIdx.x; j < V; j += LP_THREADS) {
-    const float xj = Pack<T>::load1(x + j);
-    v = ag_stat_merge(v, {xj, xj == -INFINITY ? 0.0f : xj - xj + 1.0f, 0.0f}, c);  // inf - inf and NaN: a NaN for the sum
+  const int64_t row = blockIdx.x / p.chunks;
+  const int chunk = (int)(blockIdx.x - row * p.chunks);
+  const AgRow<T> r(logits + row * p.ld, p.V);
+  const int n = r.mine(chunk, CHUNK), first = r.head + chunk * CHUNK * NV;
+  uint4 w[LB_PACKETS];
+#pragma unroll
+  for (int u = 0; u < LB_PACKETS; ++u) {
+    const int i = tid + u * LP_THREADS;
+    w[u] = i < n ? __ldcs(reinterpret_cast<const uint4*>(r.x + first + (int64_t)i * NV)) : make_uint4(0, 0, 0, 0);
   }
-  v = ag_stat_warp(v, c);
-  if ((threadIdx.x & 31) == 0) s_stat[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = s_stat[0];
-  for (int w = 1; w < LP_WARPS; ++w) v = ag_stat_merge(v, s_stat[w], c);
-  const float L = logf(v.s), H = v.m == -INFINITY && v.s == 0.0f ? 0.0f : L - AG_LN2 * (v.t / v.s);
-  auto log_p = [&](float xj) { return xj == -INFINITY && !(v.s != v.s) ? -INFINITY : (xj - v.m) * inv_tau - L; };
-  if (threadIdx.x == 0) {
-    if (logprob) {
-      const int id = ids[row];
-      logprob[row] = id >= 0 && id < V ? log_p(Pack<T>::load1(x + id)) : 0.0f;
+  const int edge_index = r.edge(chunk);
+  const float x_edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : 0.0f;
+  const float4 st = p.stats[row];
+  const int id = p.ids ? p.ids[row] : -1;
+  const float a = p.dlogprob && id >= 0 && id < p.V ? p.dlogprob[row] * p.inv_tau : 0.0f;
+  const float b = p.dentropy ? p.dentropy[row] * p.inv_tau : 0.0f;
+  const bool none = (a == 0.0f && b == 0.0f) || (st.x == -INFINITY && st.y == -INFINITY);
+  T* g_row = dlogits + row * p.ld_grad;
+  const T* d_row = dres ? dres + row * p.ld_grad : nullptr;
+  const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0, d_packets = (((uintptr_t)(d_row + first)) & 15) == 0;
+  // p (a + b (ln p + H)) = p (a + b H + b ln p); a logit of -inf: p = 0, and 0 times something finite
+  const float k = a + b * st.z;
+  auto local = [&](float x) {
+    const float lp = fmaxf((x - st.x) * p.inv_tau, -1e4f) - st.y;
+    return -ag_ex2(lp * AG_LOG2E) * (k + b * lp);
+  };
+#pragma unroll
+  for (int u = 0; u < LB_PACKETS; ++u) {
+    const int i = tid + u * LP_THREADS;
+    if (i >= n) break;
+    float x[NV], g[NV];
+    ag_widen(w[u], x);
+#pragma unroll
+    for (int e = 0; e < NV; ++e) g[e] = none ? 0.0f : local(x[e]);
+    const int at = first + i * NV;
+    const int hit = id - at;
+    if (hit >= 0 && hit < NV && !none) {
+#pragma unroll
+      for (int e = 0; e < NV; ++e) g[e] += e == hit ? a : 0.0f;
     }
-    if (entropy) entropy[row] = H;
-    if (stats) stats[row] = make_float4(v.m, L, H, 0.0f);
+    if (d_row) {
+      float d[NV];
+      if (d_packets) {
+        Pack<T>::load_stream(d_row + at, d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < NV; ++e) d[e] = Pack<T>::load1(d_row + at + e);
+      }
+#pragma unroll
+      for (int e = 0; e < NV; ++e) g[e] += d[e];
+    }
+    ag_store_packet<T>(g_row + at, g, packets);
   }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long best = 0;
-    for (int j = threadIdx.x; j < V; j += LP_THREADS) {
-      const unsigned long long key = (unsigned long long)ag_order(Pack<T>::load1(x + j)) << 32 | (uint32_t)(~j);
-      if (key < last && key > best) best = key;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long w = __shfl_xor_sync(0xffffffffu, best, o);
-      best = w > best ? w : best;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_key[threadIdx.x >> 5] = best;
-    __syncthreads();
-    for (int w = 0; w < LP_WARPS; ++w) best = s_key[w] > best ? s_key[w] : best;
-    if (threadIdx.x == 0) {
-      top_ids[row * top + k] = (int32_t)~(uint32_t)best;
-      top_logprobs[row * top + k] = log_p(ag_of_order((uint32_t)(best >> 32)));
-    }
-    last = best;
+  if (edge_index >= 0) {
+    const float g = none ? 0.0f : local(x_edge) + (edge_index == id ? a : 0.0f);
+    Pack<T>::store1(g_row + edge_index, g + (d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f));
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS)
-logprobs_backward_kernel(const T* logits, int64_t ld, const int32_t* __restrict__ ids, const float4* __restrict__ stats,
-                         const float* __restrict__ dlogprob, const float* __restrict__ dentropy, const T* dres, T* dlogits,
-                         int64_t ld_grad, int V, float inv_tau) {
-  ag_pdl_wait();
-  ag_pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const float4 st = stats[row];
-  const int id = ids ? ids[row] : -1;
-  const float a = dlogprob && id >= 0 && id < V ? dlogprob[row] * inv_tau : 0.0f, b = dentropy ? dentropy[row] * inv_tau : 0.0f;
-  const bool none = (a == 0.0f && b == 0.0f) || (st.x == -INFINITY && st.y == -INFINITY);
-  for (int j = threadIdx.x; j < V; j += LP_THREADS) {
-    const float xj = Pack<T>::load1(logits + row * ld + j);
-    const float lp = fmaxf((xj - st.x) * inv_tau, -1e4f) - st.y;  // -inf: p = 0, and 0 times something finite
-    const float p = ag_ex2(lp * AG_LOG2E);
-    float g = none ? 0.0f : (j == id ? a : 0.0f) - p * (a + b * (lp + st.z));
-    if (dres) g += Pack<T>::load1(dres + row * ld_grad + j);
-    Pack<T>::store1(dlogits + row * ld_grad + j, g);
-  }
+int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, LbArgs p, int64_t N) {
+  const int packets = p.V / AG_PACKET<T>;
+  p.chunks = packets ? (packets + LP_THREADS * LB_PACKETS - 1) / (LP_THREADS * LB_PACKETS) : 1;
+  AG_REQUIRE(ctx, N * p.chunks < (1ll << 31), "ag_token_logprobs_backward: too many rows for V=%d", p.V);
+  AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<T>, (unsigned)(N * p.chunks), LP_THREADS, 0,
+                (const T*)logits, (const T*)dres, (T*)dlogits, p);
+  return AG_OK;
+}
+
+// Lane maxima per warp: twice as many as are asked for of all warps together, up to LP_POOL
+int lp_lane_maxima(int S, int top) {
+  const int groups = S * LP_WARPS, want = (2 * top + groups - 1) / groups, least = (top + groups - 1) / groups;
+  const int most = LP_POOL / groups > least ? LP_POOL / groups : least;
+  return want < most ? want : most;
+}
+
+template <typename T, bool TOP>
+int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
+  static AgClusterFit fits[AG_MAX_DEVICES];
+  a.cap = TOP ? 2 * a.top + 32 : 0;
+  const AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, [&](int S) {
+    return lp_smem(S, TOP ? lp_lane_maxima(S, a.top) : 0, a.cap);
+  });
+  a.S = p.S;
+  a.per = p.per;
+  a.buffers = p.buffers;
+  a.J = TOP ? lp_lane_maxima(p.S, a.top) : 0;
+  return ag_launch_rows(ctx, "logprobs_kernel", fits, logprobs_kernel<T, TOP>, p, a.N, (const T*)logits, a);
 }
 
 }  // namespace
@@ -102,14 +422,10 @@ extern "C" int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
-  const float inv = 1.0f / temperature;
+  const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0};
   if (dtype == AG_F32)
-    AG_LAUNCH_PDL(ctx, "logprobs_kernel", logprobs_kernel<float>, (unsigned)N, LP_THREADS, 0, (const float*)logits, ld, ids, logprob,
-                  entropy, (float4*)stats, top_ids, top_logprobs, V, top, inv);
-  else
-    AG_LAUNCH_PDL(ctx, "logprobs_kernel", logprobs_kernel<__nv_bfloat16>, (unsigned)N, LP_THREADS, 0, (const __nv_bfloat16*)logits, ld,
-                  ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, V, top, inv);
-  return AG_OK;
+    return top ? logprobs<float, true>(ctx, logits, a) : logprobs<float, false>(ctx, logits, a);
+  return top ? logprobs<__nv_bfloat16, true>(ctx, logits, a) : logprobs<__nv_bfloat16, false>(ctx, logits, a);
 }
 
 extern "C" int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* ids, const float* stats,
@@ -124,13 +440,7 @@ extern "C" int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
-  const float inv = 1.0f / temperature;
-  if (dtype == AG_F32)
-    AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<float>, (unsigned)N, LP_THREADS, 0, (const float*)logits,
-                  ld, ids, (const float4*)stats, dlogprob, dentropy, (const float*)dres, (float*)dlogits, ld_grad, V, inv);
-  else
-    AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<__nv_bfloat16>, (unsigned)N, LP_THREADS, 0,
-                  (const __nv_bfloat16*)logits, ld, ids, (const float4*)stats, dlogprob, dentropy, (const __nv_bfloat16*)dres,
-                  (__nv_bfloat16*)dlogits, ld_grad, V, inv);
-  return AG_OK;
+  const LbArgs p = {ids, (const float4*)stats, dlogprob, dentropy, ld, ld_grad, V, 0, 1.0f / temperature};
+  return dtype == AG_F32 ? logprobs_backward<float>(ctx, logits, dres, dlogits, p, N)
+                         : logprobs_backward<__nv_bfloat16>(ctx, logits, dres, dlogits, p, N);
 }

@@ -1,8 +1,15 @@
-// Shared by the operators on rows of logits (ag_logprobs.cu, ag_distill.cu): argument checks, the exponential, softmax
-// statistics that can be merged.
+// Shared by the operators on rows of logits (ag_logprobs.cu, ag_distill.cu): argument checks, softmax statistics that can be
+// merged, rows that are cut into slices of shared memory.
+//
+// A row belongs to a cluster of 1 to 8 blocks, each of which holds a slice of it in shared memory, fetched with 16-byte
+// asynchronous copies while the slice of the cluster's row before is worked on.  A thread copies what it reads itself, so that the
+// copies need no barrier; one barrier of the cluster exchanges the statistics of its warps.  What comes after (the alternatives,
+// the gradient) finds the logits on chip: a row is read from memory once.
 #pragma once
 
 #include <math.h>
+
+#include <atomic>
 
 #include "ag_common.cuh"
 
@@ -64,29 +71,206 @@ __device__ __forceinline__ float ag_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float ag_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t ag_pair(float a, float b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ void ag_unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t ag_add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t ag_mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t ag_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
 
-// Statistics of a part of a row in units of log 2: m the largest logit, s = sum 2^d, t = sum 2^d d with d = (x - m) * c,
-// c = log2(e) / temperature.  Terms whose 2^d is 0 add nothing to t, however small d is.  m = -inf: nothing above -inf yet,
-// s = t = 0.  A NaN or +inf among the logits makes s NaN.
+// Statistics of a part of a row: m its largest logit, s = sum 2^(c y), t = sum 2^(c y) y with y = x - m, c = log2(e) / temperature.
+// The difference is formed before the product: x c - m c in one fma would be off by the rounding of m c, which differs between the
+// parts of a row, and overflows for rows of the lowest numbers.  Terms whose power is 0 add nothing to t, however far y is.
+// m = -inf: nothing above -inf, s = t = 0.  A NaN or +inf among the logits makes s NaN.
 struct AgStat {
   float m, s, t;
 };
 __device__ __forceinline__ AgStat ag_stat_none() { return {-INFINITY, 0.0f, 0.0f}; }
-__device__ __forceinline__ AgStat ag_stat_merge(const AgStat& a, const AgStat& b, float c) {
+// v as part of something with the largest logit m >= v.m
+__device__ __forceinline__ void ag_stat_scale(AgStat& v, float m, float c) {
+  const float y = m == -INFINITY ? 0.0f : v.m - m, e = ag_ex2(y * c);
+  v.t = e > 0.0f ? e * (v.t + v.s * y) : 0.0f;
+  v.s *= e;  // a NaN stays
+  v.m = m;
+}
+__device__ __forceinline__ AgStat ag_stat_merge(AgStat a, AgStat b, float c) {
   const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.t + b.t};
-  const float da = (a.m - m) * c, db = (b.m - m) * c;  // one of them 0, the other possibly -inf: of an empty part
-  const float ea = ag_ex2(da), eb = ag_ex2(db);
-  // s 2^d, and t 2^d + s 2^d d; NaN stays in s
-  return {m, a.s * ea + b.s * eb, (ea > 0.0f ? ea * (a.t + a.s * da) : 0.0f) + (eb > 0.0f ? eb * (b.t + b.s * db) : 0.0f)};
+  ag_stat_scale(a, m, c);
+  ag_stat_scale(b, m, c);
+  return {m, a.s + b.s, a.t + b.t};
+}
+__device__ __forceinline__ AgStat ag_stat_warp(AgStat v, float c) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
+  ag_stat_scale(v, m, c);
+  uint64_t st = ag_pair(v.s, v.t);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) st = ag_add2(st, __shfl_xor_sync(0xffffffffu, st, o));
+  ag_unpair(st, v.s, v.t);
+  return v;
 }
 
-__device__ __forceinline__ AgStat ag_stat_warp(AgStat v, float c) {
+// N logits (N even) onto v; t only if it is wanted.  A batch costs one more exponential, for what is there already.
+template <bool WITH_T, int N>
+__device__ __forceinline__ void ag_stat_add(AgStat& v, const float (&x)[N], float c) {
+  float m = v.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const AgStat w = {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.t, o)};
-    v = ag_stat_merge(v, w, c);
+  for (int i = 0; i < N; i += 2) m = ag_max3(m, x[i], x[i + 1]);
+  ag_stat_scale(v, m, c);
+  const float ref = m == -INFINITY ? 0.0f : -m;
+  const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c);
+  uint64_t s2 = ag_pair(v.s, 0.0f), t2 = ag_pair(v.t, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t y2 = ag_add2(ag_pair(x[i], x[i + 1]), ref2);
+    float d0, d1, y0, y1;
+    ag_unpair(ag_mul2(y2, c2), d0, d1);
+    const uint64_t e2 = ag_pair(ag_ex2(d0), ag_ex2(d1));
+    s2 = ag_add2(s2, e2);
+    if (!WITH_T) continue;
+    ag_unpair(y2, y0, y1);
+    t2 = ag_fma2(e2, ag_pair(fmaxf(y0, -1e30f), fmaxf(y1, -1e30f)), t2);  // 0 times -inf
   }
+  float a, b;
+  ag_unpair(s2, a, b);
+  v.s = a + b;
+  ag_unpair(t2, a, b);
+  v.t = a + b;
+}
+
+// What 16 bytes of a row hold: 4 fp32 or 8 bf16.
+template <typename T>
+constexpr int AG_PACKET = 16 / (int)sizeof(T);
+__device__ __forceinline__ void ag_widen(const uint4& w, float (&x)[4]) { Pack<float>::unpack_raw(*reinterpret_cast<const float4*>(&w), x); }
+__device__ __forceinline__ void ag_widen(const uint4& w, float (&x)[8]) { Pack<__nv_bfloat16>::unpack(w, x); }
+// 16 bytes of -inf
+template <typename T>
+__device__ __forceinline__ uint4 ag_lowest_packet() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
+
+// A packet of a gradient, whose rows may lie otherwise than the logits' with respect to 16 bytes
+template <typename T>
+__device__ __forceinline__ void ag_store_packet(T* to, const float (&g)[AG_PACKET<T>], bool whole) {
+  if (whole) {
+    Pack<T>::store_stream(to, g);
+  } else {
+#pragma unroll
+    for (int e = 0; e < AG_PACKET<T>; ++e) Pack<T>::store1(to + e, g[e]);
+  }
+}
+
+// A row as its cluster sees it: `head` elements before the first 16-byte boundary, `body` packets, `tail` elements behind them.
+// Block `rank` has the packets from rank * per; head and tail are the first block's, an element per thread (0.., 16..).
+template <typename T>
+struct AgRow {
+  const T* x;
+  int head, body, tail;
+  __device__ __forceinline__ AgRow(const T* row, int V) : x(row) {
+    constexpr int NV = AG_PACKET<T>;
+    const int past = (int)((uintptr_t)row & 15) / (int)sizeof(T);
+    head = past ? min(NV - past, V) : 0;
+    body = (V - head) / NV;
+    tail = V - head - body * NV;
+  }
+  __device__ __forceinline__ int mine(int rank, int per) const { return max(0, min(body - rank * per, per)); }
+  // index of this thread's own element of the edges, -1 without one
+  __device__ __forceinline__ int edge(int rank) const {
+    const int t = threadIdx.x;
+    return rank ? -1 : t < head ? t : t >= 16 && t < 16 + tail ? head + body * AG_PACKET<T> + t - 16 : -1;
+  }
+  __device__ __forceinline__ int owner(int id, int per) const {
+    const int q = id - head;
+    return q < 0 || q >= body * AG_PACKET<T> ? 0 : q / AG_PACKET<T> / per;
+  }
+  // asynchronous copy of this thread's packets of the slice
+  __device__ __forceinline__ void fetch(uint4* slice, int rank, int per) const {
+    const int n = mine(rank, per);
+    const T* from = x + head + (int64_t)rank * per * AG_PACKET<T>;
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ag_smem_u32(slice + i)), "l"(from + (int64_t)i * AG_PACKET<T>)
+                   : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+};
+__device__ __forceinline__ void ag_fetched() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Statistics of this thread's part of a slice: its packets, and its element of the edges (-inf without one).
+template <bool WITH_T, typename T>
+__device__ __forceinline__ AgStat ag_slice_stat(const uint4* slice, int n, float edge, float c) {
+  constexpr int NV = AG_PACKET<T>, U = 16 / NV;  // 16 logits at a time
+  AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
+  for (int i = threadIdx.x; i < n; i += U * blockDim.x) {
+    float x[16];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = i + u * blockDim.x;
+      float part[NV];
+      ag_widen(k < n ? slice[k] : ag_lowest_packet<T>(), part);
+#pragma unroll
+      for (int e = 0; e < NV; ++e) x[u * NV + e] = part[e];
+    }
+    ag_stat_add<WITH_T>(v, x, c);
+  }
+  return v;
+}
+
+// ---- clusters --------------------------------------------------------------------------
+__device__ __forceinline__ int ag_cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Every thread of every block of the cluster; S = 1: of the block.
+__device__ __forceinline__ void ag_cluster_sync(int S) {
+  if (S == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  }
+}
+// address in block `rank` of what lies at p in this one
+__device__ __forceinline__ uint32_t ag_peer(const void* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ag_smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void ag_peer_store(uint32_t a, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void ag_peer_store(uint32_t a, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
+__device__ __forceinline__ int ag_peer_load_int(uint32_t a) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long ag_peer_load_key(uint32_t a) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
 
@@ -100,4 +284,92 @@ __device__ __forceinline__ float ag_of_order(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);  // 0xfffffffe becomes a NaN again
 }
 
+
 #endif  // __CUDACC__
+
+// ---- the launch: slices, blocks per row, clusters that are resident at once --------------------------------------------------
+constexpr int AG_ROW_THREADS = 256;
+
+// How many clusters of a kernel the device holds, by blocks per cluster and shared memory; as AgOccupancy keeps its answers.
+class AgClusterFit {
+ public:
+  template <typename Query>
+  int get(int size, size_t smem, Query query) {
+    const uint64_t key = (uint64_t)smem << 36 | (uint64_t)size << 32;
+    int free = -1;
+    for (int i = 0; i < kSlots; ++i) {
+      const uint64_t word = slot_[i].load(std::memory_order_relaxed);
+      if (word >> 32 == key >> 32 && (uint32_t)word) return (int)(uint32_t)word;
+      if (!word && free < 0) free = i;
+    }
+    const int fit = query();
+    if (fit < 1) return fit;
+    if (free < 0) free = (int)((key >> 32) * 0x9E3779B97F4A7C15ull >> 60);
+    slot_[free].store(key | (uint32_t)fit, std::memory_order_relaxed);
+    return fit;
+  }
+
+ private:
+  static constexpr int kSlots = 16;
+  std::atomic<uint64_t> slot_[kSlots];
+};
+
+struct AgRowPlan {
+  int S, per, buffers;  // blocks per row, packets per block, slices in shared memory at once
+  size_t smem;
+};
+
+constexpr size_t AG_SMEM_MOST = 226 * 1024;  // and a kilobyte for what a kernel declares
+
+// `more`: what the kernel wants beside its slices, of a cluster of S
+template <typename More>
+static inline AgRowPlan ag_row_plan(const ag_ctx* ctx, int64_t N, int V, int dtype, More more) {
+  const int packets = (V * (dtype == AG_F32 ? 4 : 2) + 15) / 16;
+  AgRowPlan p;
+  p.S = 1;
+  while (p.S < 8 && (packets + p.S - 1) / p.S > 2048) p.S *= 2;
+  // few rows: more blocks for each, while they have something to do
+  while (p.S < 8 && N * p.S * 2 <= 2 * ctx->sm_count && packets / p.S >= 512) p.S *= 2;
+  p.per = (packets + p.S - 1) / p.S;
+  p.buffers = (size_t)p.per * 32 + more(p.S) <= AG_SMEM_MOST ? 2 : 1;
+  p.smem = (size_t)p.per * 16 * p.buffers + more(p.S);
+  return p;
+}
+
+// Launch on clusters of p.S blocks, at most as many as are resident at once (each takes row after row), and never more than rows.
+template <typename... P, typename... A>
+static inline int ag_launch_rows(ag_ctx* ctx, const char* name, AgClusterFit* fits, void (*kern)(P...), const AgRowPlan& p, int64_t N,
+                                 A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = AG_ROW_THREADS;
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.S;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cfg.gridDim = p.S;
+  const int fit = fits[ag_dev_slot(ctx)].get(p.S, p.smem, [&] {
+    int n = 0;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AG_SMEM_MOST);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return -(int)e;
+    }
+    return n;
+  });
+  if (fit < 1) AG_FAIL(ctx, AG_ERR_CUDA, "%s: no room for clusters of %d blocks with %zu bytes (%s)", name, p.S, p.smem,
+                       cudaGetErrorString((cudaError_t)-fit));
+  cfg.gridDim = (unsigned)((N < fit ? N : fit) * p.S);
+  cfg.numAttrs = ctx->pdl ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) AG_FAIL(ctx, AG_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e));
+  ctx->launches++;
+  ag_enqueued(ctx);
+  return AG_OK;
+}
