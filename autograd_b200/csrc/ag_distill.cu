@@ -108,7 +108,7 @@ __device__ __forceinline__ float distill_take(__nv_bfloat16* p) {
 }
 
 size_t distill_smem(int S) {
-  return 2 * (size_t)S * DI_WARPS * 16 + 2 * DI_WARPS * sizeof(DistillPart) + 5 * AG_DISTILL_MAX * 4 + 32 * 4 + DI_WARPS * 4 + 64;
+  return AgExchange::bytes(S) + 2 * DI_WARPS * sizeof(DistillPart) + 5 * AG_DISTILL_MAX * 4 + 32 * 4 + DI_WARPS * 4 + 64;
 }
 
 template <typename T, bool TRAIN>
@@ -119,7 +119,9 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * DI_WARPS, parts = (a.top + 31) / 32;
   float4* s_stat = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);      // [2][groups]
-  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_stat + 2 * groups);           // [2][DI_WARPS]
+  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_stat + 2 * groups);                   // [2]
+  const AgExchange exchange = {s_stat, s_bars, S, rank, a.status};
+  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);                     // [2][DI_WARPS]
   int* s_next_id = reinterpret_cast<int*>(s_parts + 2 * DI_WARPS);                      // a slot per thread, copied ahead
   float* s_next_t = reinterpret_cast<float*>(s_next_id + AG_DISTILL_MAX);
   int* s_ids = reinterpret_cast<int*>(s_next_t + AG_DISTILL_MAX);                        // [2][slots]
@@ -137,7 +139,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
     }
   };
   if (tid < 2) s_twice[tid] = 0;
-  if (S > 1) ag_cluster_sync(S);  // all of them run before one stores to another
+  exchange.start();
   ag_pdl_wait();
   ag_pdl_trigger();
 
@@ -203,20 +205,14 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
       if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
       in = ag_stat_warp(in, c);
     }
-    {
-      const float4 out = make_float4(mine.m, mine.s, in.m, in.s);
-      float4* to = s_stat + now * groups + rank * DI_WARPS + warp;
-      if (S == 1) {
-        if (lane == 0) *to = out;
-      } else if (lane < S) {
-        ag_peer_store(ag_peer(to, lane), out);
-      }
-    }
-    ag_cluster_sync(S);
+    // The lead's logits of other slices have arrived before its word goes out, on which those are overwritten if the gradient
+    // takes the logits' place: a store needs its operand, and instructions of a warp go in order.
+    if (TRAIN && lead && tid < a.top) reinterpret_cast<volatile float*>(s_q)[tid] = x_id;
+    const float4* told = exchange.tell(turn, make_float4(mine.m, mine.s, in.m, in.s));
     AgStat out = ag_stat_none();
     in = ag_stat_none();
     for (int g = lane; g < groups; g += 32) {
-      const float4 w = s_stat[now * groups + g];
+      const float4 w = told[g];
       out = ag_stat_merge(out, {w.x, w.y, 0.0f}, c);
       in = ag_stat_merge(in, {w.z, w.w, 0.0f}, c);
     }

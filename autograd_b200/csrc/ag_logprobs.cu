@@ -5,18 +5,17 @@
 //   d logits_j = (a (delta_j,id - p_j) - b p_j (log p_j + H)) / temperature,  a = dlogprob (0 without a token), b = dentropy
 //
 // Forward: rows cut into slices (ag_vocab.cuh).  The alternatives come from the slices, too:
-//   each warp hands round its J largest lane maxima along with its statistics; the top-th largest of all these is a bound that at
-//   least `top` logits reach, and few more do, since the lanes' logits lie spread over the row;
+//   each warp tells, along with its statistics, its J-th largest lane maximum; the (top / J)-th largest of these is a bound that at
+//   least `top` logits reach, and up to twice as many do, since the lanes' logits lie spread over the row;
 //   the logits that reach it are collected, (order, index) as one key each, by the threads whose maximum does;
 //   one block of the cluster counts for each how many are larger, which is its place.
-// A block that collects more than twice what can be asked for (many equal logits, or the largest ones all in a few lanes)
-// searches a bound of its own first, bit by bit, and takes logits that equal it in the order of their index.
+// A block that collects more than `cap` (many equal logits, or the largest ones all in a few lanes) searches a bound of its own,
+// bit by bit, and takes logits that equal it in the order of their index.
 #include "ag_vocab.cuh"
 
 namespace {
 
 constexpr int LP_THREADS = AG_ROW_THREADS, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_POOL = 256;  // lane maxima that are handed round
 
 struct LpArgs {
   const int32_t* ids;
@@ -28,35 +27,27 @@ struct LpArgs {
   int V, top;
   float inv_tau;
   int S, per, buffers;
-  int J, cap;  // lane maxima per warp, keys per block
+  int J, need, cap;  // which lane maximum of a warp, how many of these the bound has to meet, keys per block
+  int* status;
 };
 
-size_t lp_smem(int S, int J, int cap) {
-  return 2 * (size_t)S * LP_WARPS * 16 + 2 * (size_t)S * LP_WARPS * J * 4 + 2 * (size_t)cap * 8 + 128;
-}
+// the exchange, two rows' keys of a block, the keys of all blocks at the leading one, their barrier, counters
+size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (2 + S) + 64; }
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
-// The largest bound that at least `top` of the n values in `pool` reach, or one that few more do; by one warp.
-__device__ float lp_bound(const float* pool, int n, int top) {
+// The need-th largest of the n <= 64 numbers box[].w, or one that an eighth more of them reach; by one warp.
+__device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
   const int lane = threadIdx.x & 31;
-  uint32_t key[LP_POOL / 32];
-  uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll
-  for (int i = 0; i < LP_POOL / 32; ++i) {
-    key[i] = lane + 32 * i < n ? ag_order(pool[lane + 32 * i]) : 0u;
-    if (lane + 32 * i < n) lo = min(lo, key[i]), hi = max(hi, key[i]);
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);  // n >= top values reach it
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  const int enough = top + (top >> 3);
+  const bool one = lane < n, two = lane + 32 < n;
+  const uint32_t a = one ? ag_order(box[lane].w) : 0u, b = two ? ag_order(box[lane + 32].w) : 0u;
+  uint32_t lo = __reduce_min_sync(0xffffffffu, min(one ? a : 0xffffffffu, two ? b : 0xffffffffu));
+  uint32_t hi = __reduce_max_sync(0xffffffffu, max(a, b));
+  const int enough = need + (need >> 3);
   while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo + 1) / 2;
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < LP_POOL / 32; ++i) count += key[i] >= mid;
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (count >= top) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    const int count = __popc(__ballot_sync(0xffffffffu, a >= mid)) + __popc(__ballot_sync(0xffffffffu, b >= mid));
+    if (count >= need) {
       lo = mid;
       if (count <= enough) break;
     } else {
@@ -170,16 +161,23 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ uint4 s_slices[];
-  const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
+  const int S = a.S, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * LP_WARPS;
-  float4* s_stat = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);  // [2][groups]
-  unsigned long long* s_keys = reinterpret_cast<unsigned long long*>(s_stat + 2 * groups);  // [2][cap]
-  float* s_pool = reinterpret_cast<float*>(s_keys + (TOP ? 2 * a.cap : 0));                 // [2][groups * J]
-  int* s_words = reinterpret_cast<int*>(s_pool + (TOP ? 2 * groups * a.J : 0));             // [0..1] keys, [2] counter
-  float* s_bound = reinterpret_cast<float*>(s_words + 3);
+  float4* s_box = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);
+  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
+  const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
+  uint64_t* s_keys_bar = s_bars + 2;                                                        // every block has its keys
+  unsigned long long* s_keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);       // [2][cap]
+  unsigned long long* s_all = s_keys + 2 * a.cap;                                           // [S * cap], at the leading block
+  int* s_words = reinterpret_cast<int*>(s_all + S * a.cap);                                 // [0..1] keys of a row, [2] counter
   const int64_t clusters = gridDim.x / S;
   const float c = a.inv_tau * AG_LOG2E;
-  if (S > 1) ag_cluster_sync(S);  // all of them run before one stores to another
+  if (TOP && tid == 0) {
+    s_words[0] = 0;
+    ag_mbar_init(s_keys_bar, S);
+    ag_fence_mbar_init();
+  }
+  exchange.start();
   ag_pdl_wait();
   ag_pdl_trigger();
 
@@ -207,36 +205,20 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
 
     const AgStat own = ag_slice_stat<true, T>(slice, sl.n, sl.edge, c);
     AgStat v = ag_stat_warp(own, c);
-    {
-      const float4 out = make_float4(v.m, v.s, v.t, 0.0f);
-      float4* to = s_stat + (turn & 1) * groups + rank * LP_WARPS + warp;
-      if (S == 1) {
-        if (lane == 0) *to = out;
-      } else if (lane < S) {
-        ag_peer_store(ag_peer(to, lane), out);
-      }
-    }
+    float reached = 0.0f;
     if (TOP) {
-      // the J largest of the lanes' maxima
-      float left = own.m, best = 0.0f;
-      for (int j = 0; j < a.J; ++j) {
-        float m;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(left));
-        const uint32_t who = __ballot_sync(0xffffffffu, left == m);
-        if (lane == j) best = m;
+      float left = own.m;
+      reached = v.m;
+      for (int j = 1; j < a.J; ++j) {
+        const uint32_t who = __ballot_sync(0xffffffffu, left == reached);
         if (lane == __ffs(who) - 1) left = -INFINITY;
-      }
-      float* to = s_pool + ((turn & 1) * groups + rank * LP_WARPS + warp) * a.J;
-      if (lane < a.J) {
-        if (S == 1) to[lane] = best;
-        else
-          for (int p = 0; p < S; ++p) ag_peer_store(ag_peer(to + lane, p), best);
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(left));
       }
     }
-    ag_cluster_sync(S);
+    const float4* told = exchange.tell(turn, make_float4(v.m, v.s, v.t, reached));
     v = ag_stat_none();
     for (int g = lane; g < groups; g += 32) {
-      const float4 w = s_stat[(turn & 1) * groups + g];
+      const float4 w = told[g];
       v = ag_stat_merge(v, {w.x, w.y, w.z}, c);
     }
     v = ag_stat_warp(v, c);
@@ -250,13 +232,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     if (TOP) {
       unsigned long long* keys = s_keys + (turn & 1) * a.cap;
       int* n_keys = s_words + (turn & 1);
-      if (warp == 0) {
-        const float b = lp_bound(s_pool + (turn & 1) * groups * a.J, groups * a.J, a.top);
-        if (lane == 0) *s_bound = b;
-      }
-      if (tid == 32) *n_keys = 0;
-      __syncthreads();
-      const float bound = *s_bound;
+      const float bound = lp_bound(told, groups, a.need);
       if (own.m >= bound || own.s != own.s)
         sl.each([&](float x, int j) {
           if (!(x < bound)) {
@@ -268,23 +244,32 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
       if (*n_keys > a.cap) {
         const int n = lp_search<T>(sl, ag_order(bound), a.top, a.cap, keys, s_words + 2);
         if (tid == 0) *n_keys = n;
+        __syncthreads();
       }
-      ag_cluster_sync(S);
+      if (tid == 0) {
+        s_words[(turn & 1) ^ 1] = 0;  // the row after this one
+        if (S > 1) ag_peer_arrive(ag_peer(s_keys_bar, turn % S));
+      }
       if (lead) {
+        unsigned long long* all = s_all;
         int total = 0;
-        for (int p = 0; p < S; ++p) total += S == 1 ? *n_keys : ag_peer_load_int(ag_peer(n_keys, p));
-        for (int i = tid; i < total; i += LP_THREADS) {
-          unsigned long long key = 0;
-          int place = 0;
-          for (int p = 0, at = i; p < S; ++p) {  // the i-th key of the cluster
-            const int n = S == 1 ? total : ag_peer_load_int(ag_peer(n_keys, p));
-            if (at >= 0 && at < n) key = S == 1 ? keys[at] : ag_peer_load_key(ag_peer(keys + at, p));
-            at -= n;
-          }
+        if (S == 1) {
+          all = keys;
+          total = *n_keys;
+        } else {
+          ag_wait_cluster(s_keys_bar, (turn / S) & 1, a.status);
           for (int p = 0; p < S; ++p) {
-            const int n = S == 1 ? total : ag_peer_load_int(ag_peer(n_keys, p));
-            for (int k = 0; k < n; ++k) place += (S == 1 ? keys[k] : ag_peer_load_key(ag_peer(keys + k, p))) > key;
+            const int n = ag_peer_load_int(ag_peer(n_keys, p));
+            for (int k = tid; k < n; k += LP_THREADS) all[total + k] = ag_peer_load_key(ag_peer(keys + k, p));
+            total += n;
           }
+          __syncthreads();
+        }
+        for (int i = tid; i < total; i += LP_THREADS) {
+          const unsigned long long key = all[i];
+          int place = 0;
+#pragma unroll 4
+          for (int k = 0; k < total; ++k) place += all[k] > key;
           if (place < a.top) {
             const int64_t to = row * a.top + place;
             a.top_ids[to] = (int32_t)~(uint32_t)key;
@@ -297,7 +282,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     r = next;
     row += clusters;
   }
-  if (S > 1) ag_cluster_sync(S);  // nobody leaves while another block may read its keys
+  if (S > 1) ag_cluster_sync(S);  // nobody leaves while another block may read its keys or send to it
 }
 
 // Gradient: a block takes 16 KB of a row, all of its loads under way before the first is used.
@@ -387,24 +372,25 @@ int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* d
   return AG_OK;
 }
 
-// Lane maxima per warp: twice as many as are asked for of all warps together, up to LP_POOL
-int lp_lane_maxima(int S, int top) {
-  const int groups = S * LP_WARPS, want = (2 * top + groups - 1) / groups, least = (top + groups - 1) / groups;
-  const int most = LP_POOL / groups > least ? LP_POOL / groups : least;
-  return want < most ? want : most;
-}
-
 template <typename T, bool TOP>
 int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
   static AgClusterFit fits[AG_MAX_DEVICES];
-  a.cap = TOP ? 2 * a.top + 32 : 0;
-  const AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, [&](int S) {
-    return lp_smem(S, TOP ? lp_lane_maxima(S, a.top) : 0, a.cap);
-  });
+  a.cap = TOP ? 3 * a.top + 64 : 0;
+  AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, [&](int S) { return lp_smem(S, a.cap); });
+  if (p.smem > AG_SMEM_MOST) {  // the widest rows leave room for fewer keys, twice AG_TOP_MAX at least
+    a.cap -= (int)((p.smem - AG_SMEM_MOST + 8 * (2 + p.S) - 1) / (8 * (2 + p.S)));
+    p.smem = (size_t)p.per * 16 * p.buffers + lp_smem(p.S, a.cap);
+  }
   a.S = p.S;
   a.per = p.per;
   a.buffers = p.buffers;
-  a.J = TOP ? lp_lane_maxima(p.S, a.top) : 0;
+  // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
+  // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
+  const int groups = p.S * LP_WARPS;
+  a.J = (a.top + groups - 1) / groups;
+  while (TOP && a.J < 32 && (a.top + a.J - 1) / a.J * 20 > groups * 17) ++a.J;
+  a.need = TOP ? (a.top + a.J - 1) / a.J : 0;
+  a.status = ctx->d_status;
   return ag_launch_rows(ctx, "logprobs_kernel", fits, logprobs_kernel<T, TOP>, p, a.N, (const T*)logits, a);
 }
 
@@ -422,7 +408,7 @@ extern "C" int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
-  const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0};
+  const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0, 0, nullptr};
   if (dtype == AG_F32)
     return top ? logprobs<float, true>(ctx, logits, a) : logprobs<float, false>(ctx, logits, a);
   return top ? logprobs<__nv_bfloat16, true>(ctx, logits, a) : logprobs<__nv_bfloat16, false>(ctx, logits, a);

@@ -13,6 +13,7 @@
 
 #include "ag_common.cuh"
 
+constexpr int AG_ROW_THREADS = 256, AG_ROW_WARPS = AG_ROW_THREADS / 32;  // of a block of the kernels on slices
 constexpr float AG_LN2 = 0.69314718055994531f, AG_LOG2E = 1.44269504088896341f;
 
 // Launches go to the context's device, whichever is current in the calling thread.
@@ -208,10 +209,17 @@ struct AgRow {
   // asynchronous copy of this thread's packets of the slice
   __device__ __forceinline__ void fetch(uint4* slice, int rank, int per) const {
     const int n = mine(rank, per);
-    const T* from = x + head + (int64_t)rank * per * AG_PACKET<T>;
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ag_smem_u32(slice + i)), "l"(from + (int64_t)i * AG_PACKET<T>)
-                   : "memory");
+    const uint4* from = reinterpret_cast<const uint4*>(x + head) + (int64_t)rank * per + threadIdx.x;
+    uint32_t to = ag_smem_u32(slice + threadIdx.x);
+    int left = n - (int)threadIdx.x;
+    for (; left > 3 * AG_ROW_THREADS; left -= 4 * AG_ROW_THREADS, from += 4 * AG_ROW_THREADS, to += 4 * AG_ROW_THREADS * 16) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * AG_ROW_THREADS * 16), "l"(from + u * AG_ROW_THREADS)
+                     : "memory");
+    }
+    for (; left > 0; left -= AG_ROW_THREADS, from += AG_ROW_THREADS, to += AG_ROW_THREADS * 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 };
@@ -222,16 +230,22 @@ template <bool WITH_T, typename T>
 __device__ __forceinline__ AgStat ag_slice_stat(const uint4* slice, int n, float edge, float c) {
   constexpr int NV = AG_PACKET<T>, U = 16 / NV;  // 16 logits at a time
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
-  for (int i = threadIdx.x; i < n; i += U * blockDim.x) {
+  const uint4* p = slice + threadIdx.x;
+  int left = n - (int)threadIdx.x;
+  for (; left > (U - 1) * AG_ROW_THREADS; left -= U * AG_ROW_THREADS, p += U * AG_ROW_THREADS) {
     float x[16];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = i + u * blockDim.x;
       float part[NV];
-      ag_widen(k < n ? slice[k] : ag_lowest_packet<T>(), part);
+      ag_widen(p[u * AG_ROW_THREADS], part);
 #pragma unroll
       for (int e = 0; e < NV; ++e) x[u * NV + e] = part[e];
     }
+    ag_stat_add<WITH_T>(v, x, c);
+  }
+  for (; left > 0; left -= AG_ROW_THREADS, p += AG_ROW_THREADS) {
+    float x[NV];
+    ag_widen(*p, x);
     ag_stat_add<WITH_T>(v, x, c);
   }
   return v;
@@ -257,12 +271,67 @@ __device__ __forceinline__ uint32_t ag_peer(const void* p, int rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ag_smem_u32(p)), "r"(rank));
   return a;
 }
-__device__ __forceinline__ void ag_peer_store(uint32_t a, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+// Stores to a block of the cluster that count themselves at a barrier of that block when they are there: no thread waits for them,
+// and there is no fence, which a barrier of the whole cluster would have (16384 x 32768 fp32, 4 blocks per row: a fifth of the time).
+__device__ __forceinline__ void ag_send(uint32_t to, float4 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar)
+               : "memory");
 }
-__device__ __forceinline__ void ag_peer_store(uint32_t a, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+__device__ __forceinline__ bool ag_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(ag_smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
+__device__ __forceinline__ void ag_wait_cluster(uint64_t* bar, uint32_t parity, int* status) {
+  for (uint32_t i = 0; i < 1u << 20; ++i) {
+    if (ag_try_wait_cluster(bar, parity)) return;
+    if (i > 64) __nanosleep(32);
+  }
+  atomicOr(status, AG_STATUS_WAIT_EXPIRED);
+}
+
+// What each warp of a cluster tells all others about its part of a row: one float4 per warp, in turn at two places.  A block can be
+// one row ahead of another, never two: for the row between it waits for what all warps of the other have to tell, and they tell it
+// when they have read what came before.
+struct AgExchange {
+  float4* box;      // [2][S * AG_ROW_WARPS]
+  uint64_t* bar;    // [2]
+  int S, rank;
+  int* status;
+  __device__ __forceinline__ void start() const {
+    if (S == 1) return;
+    if (threadIdx.x == 0) {
+      ag_mbar_init(bar, 1);
+      ag_mbar_init(bar + 1, 1);
+      ag_fence_mbar_init();
+    }
+    ag_cluster_sync(S);  // all of them run, with barriers set up, before one sends
+  }
+  // by whole warps, every lane with the same v; the box is returned, in which all entries are then
+  __device__ __forceinline__ const float4* tell(int turn, float4 v) const {
+    const int now = turn & 1, lane = threadIdx.x & 31;
+    float4* all = box + now * S * AG_ROW_WARPS;
+    float4* to = all + rank * AG_ROW_WARPS + (threadIdx.x >> 5);
+    if (S == 1) {
+      if (lane == 0) *to = v;
+      __syncthreads();
+    } else {
+      if (lane < S) ag_send(ag_peer(to, lane), v, ag_peer(bar + now, lane));
+      if (threadIdx.x == 0) ag_mbar_expect_tx(bar + now, S * AG_ROW_WARPS * 16);
+      ag_wait_cluster(bar + now, (turn >> 1) & 1, status);
+    }
+    return all;
+  }
+  static constexpr size_t bytes(int S) { return 2 * (size_t)S * AG_ROW_WARPS * 16 + 16; }
+};
+
 __device__ __forceinline__ int ag_peer_load_int(uint32_t a) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -272,6 +341,10 @@ __device__ __forceinline__ unsigned long long ag_peer_load_key(uint32_t a) {
   unsigned long long v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
+}
+// one arrival at a barrier of another block, after everything that this thread has seen done
+__device__ __forceinline__ void ag_peer_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // The order of the alternatives: larger logits first (NaN before all, -0 beside +0), equal ones by the lower index.
@@ -288,7 +361,6 @@ __device__ __forceinline__ float ag_of_order(uint32_t k) {
 #endif  // __CUDACC__
 
 // ---- the launch: slices, blocks per row, clusters that are resident at once --------------------------------------------------
-constexpr int AG_ROW_THREADS = 256;
 
 // How many clusters of a kernel the device holds, by blocks per cluster and shared memory; as AgOccupancy keeps its answers.
 class AgClusterFit {
