@@ -199,7 +199,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
       for (int k = 0; k < tid; ++k) once &= s_ids[now * AG_DISTILL_MAX + k] != id;
     if (at_edge >= 0) x_edge = s_edge[tid];
 
-    const AgStat mine = ag_stat_warp(ag_slice_stat<false, T>(slice, n, x_edge, c), c);
+    const AgStat mine = ag_stat_warp(ag_part_stat<false, T, 4>(slice, n, x_edge, c), c);
     AgStat in = ag_stat_none();
     if (warp < parts) {
       if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};

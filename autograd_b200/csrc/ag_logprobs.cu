@@ -4,7 +4,8 @@
 //   entropy H = L - sum_j p_j (x_j - m) / temperature
 //   d logits_j = (a (delta_j,id - p_j) - b p_j (log p_j + H)) / temperature,  a = dlogprob (0 without a token), b = dentropy
 //
-// Forward: rows cut into slices (ag_vocab.cuh).  The alternatives come from the slices, too:
+// Forward: a block, or for few rows a cluster of 2 to 8, streams a row through registers.  The alternatives come from a second look
+// at the row, which L2 still holds:
 //   each warp tells, along with its statistics, its J-th largest lane maximum; the (top / J)-th largest of these is a bound that at
 //   least `top` logits reach, and up to twice as many do, since the lanes' logits lie spread over the row;
 //   the logits that reach it are collected, (order, index) as one key each, by the threads whose maximum does;
@@ -26,13 +27,13 @@ struct LpArgs {
   int64_t N, ld;
   int V, top;
   float inv_tau;
-  int S, per, buffers;
+  int S, per;  // blocks per row, packets per block
   int J, need, cap;  // which lane maximum of a warp, how many of these the bound has to meet, keys per block
   int* status;
 };
 
-// the exchange, two rows' keys of a block, the keys of all blocks at the leading one, their barrier, counters
-size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (2 + S) + 64; }
+// the exchange, a barrier, a block's keys, the keys of all blocks at block 0, counters
+size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (S == 1 ? 1 : 1 + S) + 32; }
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
@@ -58,7 +59,7 @@ __device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
 }
 
 template <typename T>
-struct LpSlice {
+struct LpPart {
   const uint4* at;
   int n, first;  // packets, index of the first one's first logit
   float edge;
@@ -80,7 +81,7 @@ struct LpSlice {
 // The block's logits whose order is `bound` or more are more than `cap`: leaves the keys of its `top` largest at least, `cap` at
 // most, in `keys` and returns how many.  By all threads of the block.  A block that has this many has more than `top` logits.
 template <typename T>
-__device__ int lp_search(const LpSlice<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
+__device__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
   uint32_t hi = 0xffffffffu;
   auto count_from = [&](uint32_t k) {
     int c = 0;
@@ -158,22 +159,20 @@ __device__ int lp_search(const LpSlice<T>& sl, uint32_t lo, int top, int cap, un
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS)
+__global__ void __launch_bounds__(LP_THREADS, TOP ? 4 : 6)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
-  extern __shared__ uint4 s_slices[];
+  extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * LP_WARPS;
-  float4* s_box = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
   const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
-  uint64_t* s_keys_bar = s_bars + 2;                                                        // every block has its keys
-  unsigned long long* s_keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);       // [2][cap]
-  unsigned long long* s_all = s_keys + 2 * a.cap;                                           // [S * cap], at the leading block
-  int* s_words = reinterpret_cast<int*>(s_all + S * a.cap);                                 // [0..1] keys of a row, [2] counter
-  const int64_t clusters = gridDim.x / S;
+  uint64_t* s_keys_bar = s_bars + 2;                                                   // every block has its keys
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);    // [cap]
+  unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
+  int* n_keys = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);           // and a counter behind it
   const float c = a.inv_tau * AG_LOG2E;
   if (TOP && tid == 0) {
-    s_words[0] = 0;
+    *n_keys = 0;
     ag_mbar_init(s_keys_bar, S);
     ag_fence_mbar_init();
   }
@@ -181,108 +180,86 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   ag_pdl_wait();
   ag_pdl_trigger();
 
-  int64_t row = blockIdx.x / S;
-  AgRow<T> r(logits + row * a.ld, a.V);
-  r.fetch(s_slices, rank, a.per);
-  int edge_index = r.edge(rank);
-  float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
-  int id = a.logprob && tid == 0 ? a.ids[row] : -1;
-  for (int turn = 0; row < a.N; ++turn) {
-    const bool lead = turn % S == rank, more = row + clusters < a.N;
-    const uint4* slice = s_slices + (a.buffers == 2 && (turn & 1) ? a.per : 0);
-    const LpSlice<T> sl = {slice, r.mine(rank, a.per), r.head + rank * a.per * AG_PACKET<T>, edge, edge_index};
-    float x_id = 0.0f;
-    const bool has = lead && id >= 0 && id < a.V;
+  const int64_t row = blockIdx.x / S;
+  const AgRow<T> r(logits + row * a.ld, a.V);
+  const int edge_index = r.edge(rank);
+  const float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
+  const int n = r.mine(rank, a.per), first = r.head + rank * a.per * AG_PACKET<T>;
+  const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
+  float x_id = 0.0f;
+  bool has = false;
+  if (tid == 0 && rank == 0 && a.logprob) {
+    const int id = a.ids[row];
+    has = id >= 0 && id < a.V;
     if (has) x_id = Pack<T>::load1(r.x + id);
-    ag_fetched();
-    const AgRow<T> next(more ? logits + (row + clusters) * a.ld : r.x, a.V);
-    if (more) {
-      if (a.buffers == 2) next.fetch(s_slices + ((turn & 1) ? 0 : a.per), rank, a.per);
-      edge_index = next.edge(rank);
-      edge = edge_index >= 0 ? Pack<T>::load1(next.x + edge_index) : -INFINITY;
-      id = a.logprob && tid == 0 ? a.ids[row + clusters] : -1;
-    }
-
-    const AgStat own = ag_slice_stat<true, T>(slice, sl.n, sl.edge, c);
-    AgStat v = ag_stat_warp(own, c);
-    float reached = 0.0f;
-    if (TOP) {
-      float left = own.m;
-      reached = v.m;
-      for (int j = 1; j < a.J; ++j) {
-        const uint32_t who = __ballot_sync(0xffffffffu, left == reached);
-        if (lane == __ffs(who) - 1) left = -INFINITY;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(left));
-      }
-    }
-    const float4* told = exchange.tell(turn, make_float4(v.m, v.s, v.t, reached));
-    v = ag_stat_none();
-    for (int g = lane; g < groups; g += 32) {
-      const float4 w = told[g];
-      v = ag_stat_merge(v, {w.x, w.y, w.z}, c);
-    }
-    v = ag_stat_warp(v, c);
-    const float L = logf(v.s), H = v.m == -INFINITY && v.s == 0.0f ? 0.0f : L - v.t / v.s * a.inv_tau;
-    auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - v.m) * a.inv_tau - L; };
-    if (lead && tid == 0) {
-      if (a.logprob) a.logprob[row] = has ? log_p(x_id) : 0.0f;
-      if (a.entropy) a.entropy[row] = H;
-      if (a.stats) a.stats[row] = make_float4(v.m, L, H, 0.0f);
-    }
-    if (TOP) {
-      unsigned long long* keys = s_keys + (turn & 1) * a.cap;
-      int* n_keys = s_words + (turn & 1);
-      const float bound = lp_bound(told, groups, a.need);
-      if (own.m >= bound || own.s != own.s)
-        sl.each([&](float x, int j) {
-          if (!(x < bound)) {
-            const int at = atomicAdd(n_keys, 1);
-            if (at < a.cap) keys[at] = lp_key(x, j);
-          }
-        });
-      __syncthreads();
-      if (*n_keys > a.cap) {
-        const int n = lp_search<T>(sl, ag_order(bound), a.top, a.cap, keys, s_words + 2);
-        if (tid == 0) *n_keys = n;
-        __syncthreads();
-      }
-      if (tid == 0) {
-        s_words[(turn & 1) ^ 1] = 0;  // the row after this one
-        if (S > 1) ag_peer_arrive(ag_peer(s_keys_bar, turn % S));
-      }
-      if (lead) {
-        unsigned long long* all = s_all;
-        int total = 0;
-        if (S == 1) {
-          all = keys;
-          total = *n_keys;
-        } else {
-          ag_wait_cluster(s_keys_bar, (turn / S) & 1, a.status);
-          for (int p = 0; p < S; ++p) {
-            const int n = ag_peer_load_int(ag_peer(n_keys, p));
-            for (int k = tid; k < n; k += LP_THREADS) all[total + k] = ag_peer_load_key(ag_peer(keys + k, p));
-            total += n;
-          }
-          __syncthreads();
-        }
-        for (int i = tid; i < total; i += LP_THREADS) {
-          const unsigned long long key = all[i];
-          int place = 0;
-#pragma unroll 4
-          for (int k = 0; k < total; ++k) place += all[k] > key;
-          if (place < a.top) {
-            const int64_t to = row * a.top + place;
-            a.top_ids[to] = (int32_t)~(uint32_t)key;
-            a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
-          }
-        }
-      }
-    }
-    if (more && a.buffers == 1) next.fetch(s_slices, rank, a.per);
-    r = next;
-    row += clusters;
   }
-  if (S > 1) ag_cluster_sync(S);  // nobody leaves while another block may read its keys or send to it
+  const AgStat own = ag_part_stat<true, T, 4>(at, n, edge, c);
+  AgStat v = ag_stat_warp(own, c);
+  float reached = v.m;
+  if (TOP) {
+    float left = own.m;
+    for (int j = 1; j < a.J; ++j) {
+      const uint32_t who = __ballot_sync(0xffffffffu, left == reached);
+      if (lane == __ffs(who) - 1) left = -INFINITY;
+      asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(left));
+    }
+  }
+  const float4 word = make_float4(v.m, v.s, v.t, reached);
+  const float4* told = TOP ? exchange.tell(0, word) : exchange.tell_first(word);
+  if (!TOP && (rank || tid >= 32)) return;
+  v = lane < groups ? AgStat{told[lane].x, told[lane].y, told[lane].z} : ag_stat_none();
+  if (lane + 32 < groups) v = ag_stat_merge(v, {told[lane + 32].x, told[lane + 32].y, told[lane + 32].z}, c);
+  v = ag_stat_warp(v, c);
+  const float L = logf(v.s);
+  auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - v.m) * a.inv_tau - L; };
+  if (rank == 0 && tid == 0) {
+    const float H = v.m == -INFINITY && v.s == 0.0f ? 0.0f : L - v.t / v.s * a.inv_tau;
+    if (a.logprob) a.logprob[row] = has ? log_p(x_id) : 0.0f;
+    if (a.entropy) a.entropy[row] = H;
+    if (a.stats) a.stats[row] = make_float4(v.m, L, H, 0.0f);
+  }
+  if (!TOP) return;
+  const float bound = lp_bound(told, groups, a.need);
+  const LpPart<T> part = {at, n, first, edge, edge_index};
+  if (own.m >= bound || own.s != own.s)
+    part.each([&](float x, int j) {
+      if (!(x < bound)) {
+        const int k = atomicAdd(n_keys, 1);
+        if (k < a.cap) keys[k] = lp_key(x, j);
+      }
+    });
+  __syncthreads();
+  if (*n_keys > a.cap) {
+    const int found = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 1);
+    if (tid == 0) *n_keys = found;
+    __syncthreads();
+  }
+  int total = *n_keys;
+  if (S > 1) {
+    if (tid == 0) ag_peer_arrive(ag_peer(s_keys_bar, 0));
+    if (rank == 0) {
+      ag_wait_cluster(s_keys_bar, 0, a.status);
+      total = 0;
+      for (int p = 0; p < S; ++p) {
+        const int m = ag_peer_load_int(ag_peer(n_keys, p));
+        for (int k = tid; k < m; k += LP_THREADS) all[total + k] = ag_peer_load_key(ag_peer(keys + k, p));
+        total += m;
+      }
+    }
+    ag_cluster_sync(S);  // nobody leaves while block 0 reads its keys
+    if (rank) return;
+  }
+  for (int i = tid; i < total; i += LP_THREADS) {
+    const unsigned long long key = all[i];
+    int place = 0;
+#pragma unroll 4
+    for (int k = 0; k < total; ++k) place += all[k] > key;
+    if (place < a.top) {
+      const int64_t to = row * a.top + place;
+      a.top_ids[to] = (int32_t)~(uint32_t)key;
+      a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
+    }
+  }
 }
 
 // Gradient: a block takes 16 KB of a row, all of its loads under way before the first is used.
@@ -374,24 +351,20 @@ int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* d
 
 template <typename T, bool TOP>
 int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
-  static AgClusterFit fits[AG_MAX_DEVICES];
+  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
+  a.S = 1;
+  while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
+  a.per = (packets + a.S - 1) / a.S;
   a.cap = TOP ? 3 * a.top + 64 : 0;
-  AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, [&](int S) { return lp_smem(S, a.cap); });
-  if (p.smem > AG_SMEM_MOST) {  // the widest rows leave room for fewer keys, twice AG_TOP_MAX at least
-    a.cap -= (int)((p.smem - AG_SMEM_MOST + 8 * (2 + p.S) - 1) / (8 * (2 + p.S)));
-    p.smem = (size_t)p.per * 16 * p.buffers + lp_smem(p.S, a.cap);
-  }
-  a.S = p.S;
-  a.per = p.per;
-  a.buffers = p.buffers;
   // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
   // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
-  const int groups = p.S * LP_WARPS;
+  const int groups = a.S * LP_WARPS;
   a.J = (a.top + groups - 1) / groups;
   while (TOP && a.J < 32 && (a.top + a.J - 1) / a.J * 20 > groups * 17) ++a.J;
   a.need = TOP ? (a.top + a.J - 1) / a.J : 0;
   a.status = ctx->d_status;
-  return ag_launch_rows(ctx, "logprobs_kernel", fits, logprobs_kernel<T, TOP>, p, a.N, (const T*)logits, a);
+  AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_token_logprobs_forward: too many rows");
+  return ag_launch_clusters(ctx, "logprobs_kernel", logprobs_kernel<T, TOP>, a.S, lp_smem(a.S, a.cap), a.N, (const T*)logits, a);
 }
 
 }  // namespace
@@ -408,7 +381,7 @@ extern "C" int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
-  const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0, 0, nullptr};
+  const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0, nullptr};
   if (dtype == AG_F32)
     return top ? logprobs<float, true>(ctx, logits, a) : logprobs<float, false>(ctx, logits, a);
   return top ? logprobs<__nv_bfloat16, true>(ctx, logits, a) : logprobs<__nv_bfloat16, false>(ctx, logits, a);

@@ -132,34 +132,6 @@ __device__ __forceinline__ AgStat ag_stat_warp(AgStat v, float c) {
   return v;
 }
 
-// N logits (N even) onto v; t only if it is wanted.  A batch costs one more exponential, for what is there already.
-template <bool WITH_T, int N>
-__device__ __forceinline__ void ag_stat_add(AgStat& v, const float (&x)[N], float c) {
-  float m = v.m;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) m = ag_max3(m, x[i], x[i + 1]);
-  ag_stat_scale(v, m, c);
-  const float ref = m == -INFINITY ? 0.0f : -m;
-  const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c);
-  uint64_t s2 = ag_pair(v.s, 0.0f), t2 = ag_pair(v.t, 0.0f);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const uint64_t y2 = ag_add2(ag_pair(x[i], x[i + 1]), ref2);
-    float d0, d1, y0, y1;
-    ag_unpair(ag_mul2(y2, c2), d0, d1);
-    const uint64_t e2 = ag_pair(ag_ex2(d0), ag_ex2(d1));
-    s2 = ag_add2(s2, e2);
-    if (!WITH_T) continue;
-    ag_unpair(y2, y0, y1);
-    t2 = ag_fma2(e2, ag_pair(fmaxf(y0, -1e30f), fmaxf(y1, -1e30f)), t2);  // 0 times -inf
-  }
-  float a, b;
-  ag_unpair(s2, a, b);
-  v.s = a + b;
-  ag_unpair(t2, a, b);
-  v.t = a + b;
-}
-
 // What 16 bytes of a row hold: 4 fp32 or 8 bf16.
 template <typename T>
 constexpr int AG_PACKET = 16 / (int)sizeof(T);
@@ -170,6 +142,63 @@ template <typename T>
 __device__ __forceinline__ uint4 ag_lowest_packet() {
   const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
   return make_uint4(w, w, w, w);
+}
+
+// The largest logit of packets as they lie in memory (NaN ignored).
+template <int U>
+__device__ __forceinline__ float ag_largest(const uint4 (&w)[U], float) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    m = ag_max3(m, __uint_as_float(w[u].x), __uint_as_float(w[u].y));
+    m = ag_max3(m, __uint_as_float(w[u].z), __uint_as_float(w[u].w));
+  }
+  return m;
+}
+__device__ __forceinline__ uint32_t ag_max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+template <int U>
+__device__ __forceinline__ float ag_largest(const uint4 (&w)[U], __nv_bfloat16) {
+  uint32_t m = 0xff80ff80u;
+#pragma unroll
+  for (int u = 0; u < U; ++u) m = ag_max_bf16x2(m, ag_max_bf16x2(ag_max_bf16x2(w[u].x, w[u].y), ag_max_bf16x2(w[u].z, w[u].w)));
+  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+
+// U packets onto v; t only if it is wanted.  A batch costs one more exponential, for what is there already.
+template <bool WITH_T, typename T, int U>
+__device__ __forceinline__ void ag_stat_add(AgStat& v, const uint4 (&w)[U], float c) {
+  constexpr int NV = AG_PACKET<T>;
+  const float m = fmaxf(v.m, ag_largest(w, T()));
+  ag_stat_scale(v, m, c);
+  const float ref = m == -INFINITY ? 0.0f : -m;
+  const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c);
+  uint64_t s2 = ag_pair(v.s, 0.0f), t2 = ag_pair(v.t, 0.0f);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float x[NV];
+    ag_widen(w[u], x);
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) {
+      const uint64_t y2 = ag_add2(ag_pair(x[i], x[i + 1]), ref2);
+      float d0, d1, y0, y1;
+      ag_unpair(ag_mul2(y2, c2), d0, d1);
+      const uint64_t e2 = ag_pair(ag_ex2(d0), ag_ex2(d1));
+      s2 = ag_add2(s2, e2);
+      if (!WITH_T) continue;
+      ag_unpair(y2, y0, y1);
+      t2 = ag_fma2(e2, ag_pair(fmaxf(y0, -1e30f), fmaxf(y1, -1e30f)), t2);  // 0 times -inf
+    }
+  }
+  float a, b;
+  ag_unpair(s2, a, b);
+  v.s = a + b;
+  if (!WITH_T) return;
+  ag_unpair(t2, a, b);
+  v.t = a + b;
 }
 
 // A packet of a gradient, whose rows may lie otherwise than the logits' with respect to 16 bytes
@@ -225,28 +254,22 @@ struct AgRow {
 };
 __device__ __forceinline__ void ag_fetched() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Statistics of this thread's part of a slice: its packets, and its element of the edges (-inf without one).
-template <bool WITH_T, typename T>
-__device__ __forceinline__ AgStat ag_slice_stat(const uint4* slice, int n, float edge, float c) {
-  constexpr int NV = AG_PACKET<T>, U = 16 / NV;  // 16 logits at a time
+// Statistics of this thread's part of n packets (in shared or global memory), U at a time, and of its element of the edges (-inf
+// without one).
+template <bool WITH_T, typename T, int U>
+__device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c) {
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
-  const uint4* p = slice + threadIdx.x;
+  const uint4* p = at + threadIdx.x;
   int left = n - (int)threadIdx.x;
   for (; left > (U - 1) * AG_ROW_THREADS; left -= U * AG_ROW_THREADS, p += U * AG_ROW_THREADS) {
-    float x[16];
+    uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float part[NV];
-      ag_widen(p[u * AG_ROW_THREADS], part);
-#pragma unroll
-      for (int e = 0; e < NV; ++e) x[u * NV + e] = part[e];
-    }
-    ag_stat_add<WITH_T>(v, x, c);
+    for (int u = 0; u < U; ++u) w[u] = p[u * AG_ROW_THREADS];
+    ag_stat_add<WITH_T, T>(v, w, c);
   }
   for (; left > 0; left -= AG_ROW_THREADS, p += AG_ROW_THREADS) {
-    float x[NV];
-    ag_widen(*p, x);
-    ag_stat_add<WITH_T>(v, x, c);
+    const uint4 w[1] = {*p};
+    ag_stat_add<WITH_T, T>(v, w, c);
   }
   return v;
 }
@@ -313,6 +336,20 @@ struct AgExchange {
       ag_fence_mbar_init();
     }
     ag_cluster_sync(S);  // all of them run, with barriers set up, before one sends
+  }
+  // to block 0 only, whose warps all get the box; the others get null and have no more to do here
+  __device__ __forceinline__ const float4* tell_first(float4 v) const {
+    const int lane = threadIdx.x & 31, at = rank * AG_ROW_WARPS + (threadIdx.x >> 5);
+    if (S == 1) {
+      if (lane == 0) box[at] = v;
+      __syncthreads();
+      return box;
+    }
+    if (lane == 0) ag_send(ag_peer(box + at, 0), v, ag_peer(bar, 0));
+    if (rank) return nullptr;
+    if (threadIdx.x == 0) ag_mbar_expect_tx(bar, S * AG_ROW_WARPS * 16);
+    ag_wait_cluster(bar, 0, status);
+    return box;
   }
   // by whole warps, every lane with the same v; the box is returned, in which all entries are then
   __device__ __forceinline__ const float4* tell(int turn, float4 v) const {
@@ -408,6 +445,29 @@ static inline AgRowPlan ag_row_plan(const ag_ctx* ctx, int64_t N, int V, int dty
   return p;
 }
 
+// Launch of n clusters of S blocks.
+template <typename... P, typename... A>
+static inline int ag_launch_clusters(ag_ctx* ctx, const char* name, void (*kern)(P...), int S, size_t smem, int64_t n, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = (unsigned)(n * S);
+  cfg.blockDim = AG_ROW_THREADS;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = ctx->pdl;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = S;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) AG_FAIL(ctx, AG_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e));
+  ctx->launches++;
+  ag_enqueued(ctx);
+  return AG_OK;
+}
+
 // Launch on clusters of p.S blocks, at most as many as are resident at once (each takes row after row), and never more than rows.
 template <typename... P, typename... A>
 static inline int ag_launch_rows(ag_ctx* ctx, const char* name, AgClusterFit* fits, void (*kern)(P...), const AgRowPlan& p, int64_t N,
@@ -435,7 +495,8 @@ static inline int ag_launch_rows(ag_ctx* ctx, const char* name, AgClusterFit* fi
     }
     return n;
   });
-  if (fit < 1) AG_FAIL(ctx, AG_ERR_CUDA, "%s: no room for clusters of %d blocks with %zu bytes (%s)", name, p.S, p.smem,
+  if (fit < 1)
+    AG_FAIL(ctx, AG_ERR_CUDA, "%s: no room for clusters of %d blocks with %zu bytes (%s)", name, p.S, p.smem,
                        cudaGetErrorString((cudaError_t)-fit));
   cfg.gridDim = (unsigned)((N < fit ? N : fit) * p.S);
   cfg.numAttrs = ctx->pdl ? 2 : 1;
