@@ -9,15 +9,16 @@
 // p_rest is summed over the unlisted logits themselves: 1 - sum_k p_id_k would keep nothing of a small rest.  A slot with a
 // negative id is not in use.
 //
-// Loss, and loss with gradient: rows cut into slices (ag_vocab.cuh), thread k has slot k.  Before the statistics are summed
-// the listed logits of the slice are replaced by -inf, so that the sum is that of the others; the listed ones are added from
-// the threads that have them, each token once.  The gradient is written from the slice, the listed tokens' entries after it.
+// Loss, and loss with gradient: a block, or a cluster of 2 to 8, streams a row through registers, thread k has slot k.  A bit per
+// token tells what is listed: in the sum over the others those logits count as -inf, and the listed ones are added from the threads
+// that have them, each token once.  The gradient comes from a second look at the row, which L2 still holds: rows under way take
+// up to DI_IN_FLIGHT bytes, more blocks per row where they would take more.  The listed tokens' entries are written after it.
 // Gradient alone: packets in registers, 16 KB of a row per block, which stages the listed logits among them first.
 #include "ag_vocab.cuh"
 
 namespace {
 
-constexpr int DI_THREADS = AG_ROW_THREADS, DI_WARPS = DI_THREADS / 32;
+constexpr int DI_THREADS = AG_ROW_THREADS, DI_WARPS = DI_THREADS / 32, DI_BLOCKS = 4;
 static_assert(AG_DISTILL_MAX <= DI_THREADS, "a slot per thread");
 
 struct DistillArgs {
@@ -29,9 +30,9 @@ struct DistillArgs {
   float4* stats;           // (m, L, ln p_rest, 0)
   int64_t N, ld, ld_grad;
   int V, top, rest;
-  float inv_tau;
+  float inv_tau, inv_n;
   int* status;
-  int S, per, buffers;
+  int S, per;  // blocks per row, packets per block
 };
 
 // Part of a list, and the whole of it merged from parts: m the largest t, sum = sum exp((t - m) / temperature) (RENORM) or the
@@ -59,22 +60,24 @@ __device__ __forceinline__ DistillPart distill_part(float t, bool rest, float in
   }
   return p;
 }
+// by whole warps; n <= 8 parts
 __device__ __forceinline__ DistillList distill_list(const DistillPart* part, int n, bool rest, float inv_tau) {
+  const int lane = threadIdx.x & 31;
+  const DistillPart p = lane < n ? part[lane] : DistillPart{-INFINITY, 0, 0.0};
   DistillList l;
-  l.m = part[0].m;
-  int nan = part[0].nan;
-  for (int w = 1; w < n; ++w) l.m = fmaxf(l.m, part[w].m), nan |= part[w].nan;
+  l.m = ag_warp_max(p.m);
+  const bool nan = __any_sync(0xffffffffu, p.nan);
   l.used = l.m > -INFINITY || nan;
   l.log_sum = 0.0f, l.inv_sum = 1.0f, l.left = 0.0f;
   if (rest) {
-    double mass = 0.0;
-    for (int w = 0; w < n; ++w) mass += part[w].sum;
+    double mass = p.sum;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    mass = __shfl_sync(0xffffffffu, mass, 0);
     l.mass = (float)mass;
     l.left = (float)(1.0 - mass > 0.0 ? 1.0 - mass : mass != mass ? mass : 0.0);
   } else {
-    float sum = 0.0f;
-    for (int w = 0; w < n; ++w)
-      if (part[w].m != -INFINITY || part[w].nan) sum += (float)part[w].sum * expf((part[w].m - l.m) * inv_tau);
+    float sum = ag_warp_sum(p.m == -INFINITY ? 0.0f : (float)p.sum * expf((p.m - l.m) * inv_tau));
     if (nan) sum = NAN;
     l.log_sum = logf(sum);
     l.inv_sum = 1.0f / sum;
@@ -94,187 +97,205 @@ __device__ __forceinline__ float distill_outside(const DistillList& l, float log
   return l.mass + l.left - (l.left != 0.0f && log_rest > -INFINITY ? l.left * expf(-log_rest) : 0.0f);
 }
 __device__ __forceinline__ float distill_scale(const DistillArgs& a, int64_t row) {
-  const float w = a.row_scale ? a.row_scale[row] : 1.0f / (float)a.N;
+  const float w = a.row_scale ? a.row_scale[row] : a.inv_n;
   return w == 0.0f ? 0.0f : a.dloss[0] * w * a.inv_tau;
 }
 
-// Puts -inf in the place of a logit in shared memory and returns what was there.
-__device__ __forceinline__ float distill_take(float* p) { return atomicExch(p, -INFINITY); }
-__device__ __forceinline__ float distill_take(__nv_bfloat16* p) {
-  unsigned short* w = reinterpret_cast<unsigned short*>(p);
-  unsigned short old = *w, was;
-  while ((was = atomicCAS(w, old, (unsigned short)0xff80)) != old) old = was;  // only the threads of one token meet here
-  return __uint_as_float((uint32_t)old << 16);
+// -inf in the places of a packet whose bits are set
+__device__ __forceinline__ void distill_mask(uint4& w, uint32_t bits, float) {
+  if (bits & 1) w.x = 0xff800000u;
+  if (bits & 2) w.y = 0xff800000u;
+  if (bits & 4) w.z = 0xff800000u;
+  if (bits & 8) w.w = 0xff800000u;
+}
+__device__ __forceinline__ void distill_mask(uint4& w, uint32_t bits, __nv_bfloat16) {
+  uint32_t* v = &w.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (bits >> (2 * i) & 1) v[i] = (v[i] & 0xffff0000u) | 0xff80u;
+    if (bits >> (2 * i) & 2) v[i] = (v[i] & 0xffffu) | 0xff800000u;
+  }
 }
 
-size_t distill_smem(int S) {
-  return AgExchange::bytes(S) + 2 * DI_WARPS * sizeof(DistillPart) + 5 * AG_DISTILL_MAX * 4 + 32 * 4 + DI_WARPS * 4 + 64;
+// Statistics of the unlisted logits of this thread's part; as ag_part_stat.  map: a byte per packet.
+template <typename T>
+__device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8_t* map, int n, float edge, float c) {
+  constexpr int U = 4;
+  AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};
+  const uint4* p = at + threadIdx.x;
+  const uint8_t* b = map + threadIdx.x;
+  int left = n - (int)threadIdx.x;
+  for (; left > (U - 1) * DI_THREADS; left -= U * DI_THREADS, p += U * DI_THREADS, b += U * DI_THREADS) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = p[u * DI_THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (const uint32_t bits = b[u * DI_THREADS]) distill_mask(w[u], bits, T());
+    ag_stat_add<false, T>(v, w, c);
+  }
+  for (; left > 0; left -= DI_THREADS, p += DI_THREADS, b += DI_THREADS) {
+    uint4 w[1] = {*p};
+    distill_mask(w[0], *b, T());
+    ag_stat_add<false, T>(v, w, c);
+  }
+  return v;
 }
 
-template <typename T, bool TRAIN>
-__global__ void __launch_bounds__(DI_THREADS)
+// exchange, parts of the list, slots' tokens and masses, loss per warp, bits of the edges, bits of the packets
+size_t distill_smem(int S, int per, bool map) {
+  return AgExchange::bytes(S) + DI_WARPS * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + DI_WARPS * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
+}
+
+template <typename T, bool TRAIN, bool REST>
+__global__ void __launch_bounds__(DI_THREADS, DI_BLOCKS)
 distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   constexpr int NV = AG_PACKET<T>;
-  extern __shared__ uint4 s_slices[];
+  extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * DI_WARPS, parts = (a.top + 31) / 32;
-  float4* s_stat = reinterpret_cast<float4*>(s_slices + (size_t)a.per * a.buffers);      // [2][groups]
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_stat + 2 * groups);                   // [2]
-  const AgExchange exchange = {s_stat, s_bars, S, rank, a.status};
-  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);                     // [2][DI_WARPS]
-  int* s_next_id = reinterpret_cast<int*>(s_parts + 2 * DI_WARPS);                      // a slot per thread, copied ahead
-  float* s_next_t = reinterpret_cast<float*>(s_next_id + AG_DISTILL_MAX);
-  int* s_ids = reinterpret_cast<int*>(s_next_t + AG_DISTILL_MAX);                        // [2][slots]
-  float* s_q = reinterpret_cast<float*>(s_ids + 2 * AG_DISTILL_MAX);                     // [slots]
-  float* s_edge = s_q + AG_DISTILL_MAX;                                                  // [32]
-  float* s_sum = s_edge + 32;                                                            // [DI_WARPS]
-  int* s_twice = reinterpret_cast<int*>(s_sum + DI_WARPS);                               // [2]: a token is listed twice
-  const int64_t clusters = gridDim.x / S;
+  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
+  const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
+  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);
+  int* s_ids = reinterpret_cast<int*>(s_parts + DI_WARPS);
+  float* s_q = reinterpret_cast<float*>(s_ids + AG_DISTILL_MAX);
+  float* s_sum = s_q + AG_DISTILL_MAX;
+  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_sum + DI_WARPS);  // [0] edges, [1] a token is listed twice, [4..] packets
+  uint8_t* s_map = reinterpret_cast<uint8_t*>(s_marks + 4);
   const float c = a.inv_tau * AG_LOG2E;
-  const bool rest = a.rest;
-  auto fetch_slot = [&](int64_t row) {  // with the packets of that row, by the thread that reads it
-    if (tid < a.top) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ag_smem_u32(s_next_id + tid)), "l"(a.ids + row * a.top + tid) : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ag_smem_u32(s_next_t + tid)), "l"(a.teacher + row * a.top + tid) : "memory");
-    }
-  };
-  if (tid < 2) s_twice[tid] = 0;
   exchange.start();
   ag_pdl_wait();
   ag_pdl_trigger();
 
-  int64_t row = blockIdx.x / S;
-  AgRow<T> r(logits + row * a.ld, a.V);
-  fetch_slot(row);
-  r.fetch(s_slices, rank, a.per);
-  int edge_index = r.edge(rank);
+  const int64_t row = blockIdx.x / S;
+  const AgRow<T> r(logits + row * a.ld, a.V);
+  const int n = r.mine(rank, a.per), first = r.head + rank * a.per * NV;
+  const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
+  int id = tid < a.top ? a.ids[row * a.top + tid] : -1;
+  float t = tid < a.top ? a.teacher[row * a.top + tid] : -INFINITY;
+  const float s = TRAIN ? distill_scale(a, row) : 0.0f;
+  const int edge_index = r.edge(rank);
   float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
-  for (int turn = 0; row < a.N; ++turn) {
-    const int now = turn & 1;
-    const bool lead = turn % S == rank, more = row + clusters < a.N;
-    uint4* slice = s_slices + (a.buffers == 2 && now ? a.per : 0);
-    const int n = r.mine(rank, a.per), at_edge = edge_index;
-    float x_edge = edge;
-    ag_fetched();
-    int id = -1;
-    float t = -INFINITY;
-    if (tid < a.top) {
-      id = s_next_id[tid];
-      if (id >= a.V) {
-        if (lead) atomicOr(a.status, AG_STATUS_BAD_INDEX);
-        id = -1;
-      }
-      if (id >= 0) t = s_next_t[tid];
-      s_ids[now * AG_DISTILL_MAX + tid] = id;
-    }
-    const bool own = id >= 0 && r.owner(id, a.per) == rank;
-    float x_id = -INFINITY;
-    if (id >= 0 && (lead || own)) x_id = Pack<T>::load1(r.x + id);
-    const AgRow<T> next(more ? logits + (row + clusters) * a.ld : r.x, a.V);
-    if (more) {
-      fetch_slot(row + clusters);
-      if (a.buffers == 2) next.fetch(s_slices + (now ? 0 : a.per), rank, a.per);
-      edge_index = next.edge(rank);
-      edge = edge_index >= 0 ? Pack<T>::load1(next.x + edge_index) : -INFINITY;
-    }
-    if (warp < parts) {
-      const DistillPart p = distill_part(t, rest, a.inv_tau);
-      if (lane == 0) s_parts[now * DI_WARPS + warp] = p;
-    }
-    if (at_edge >= 0) s_edge[tid] = x_edge;
-    __syncthreads();  // the slice is complete, for threads other than the one that copied, too
-    bool once = own;
-    if (own) {
-      const int q = id - r.head;
-      float was;
-      if (q < 0) was = distill_take(s_edge + id);
-      else if (q >= r.body * NV) was = distill_take(s_edge + 16 + q - r.body * NV);
-      else was = distill_take(reinterpret_cast<T*>(slice) + (q - rank * a.per * NV));
-      if (was == -INFINITY) s_twice[now] = 1;  // or masked: looked at in the same way
-    }
+  if (TRAIN || REST) {
+    for (int i = tid; i < (a.per + 15) / 16 + 1; i += DI_THREADS) reinterpret_cast<uint4*>(s_marks)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (tid == 0) s_twice[now ^ 1] = 0;
-    const bool twice = s_twice[now];
-    if (twice && own)
-      for (int k = 0; k < tid; ++k) once &= s_ids[now * AG_DISTILL_MAX + k] != id;
-    if (at_edge >= 0) x_edge = s_edge[tid];
-
-    const AgStat mine = ag_stat_warp(ag_part_stat<false, T, 4>(slice, n, x_edge, c), c);
-    AgStat in = ag_stat_none();
-    if (warp < parts) {
-      if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
-      in = ag_stat_warp(in, c);
-    }
-    // The lead's logits of other slices have arrived before its word goes out, on which those are overwritten if the gradient
-    // takes the logits' place: a store needs its operand, and instructions of a warp go in order.
-    if (TRAIN && lead && tid < a.top) reinterpret_cast<volatile float*>(s_q)[tid] = x_id;
-    const float4* told = exchange.tell(turn, make_float4(mine.m, mine.s, in.m, in.s));
-    AgStat out = ag_stat_none();
-    in = ag_stat_none();
-    for (int g = lane; g < groups; g += 32) {
-      const float4 w = told[g];
-      out = ag_stat_merge(out, {w.x, w.y, 0.0f}, c);
-      in = ag_stat_merge(in, {w.z, w.w, 0.0f}, c);
-    }
-    out = ag_stat_warp(out, c);
-    in = ag_stat_warp(in, c);
-    const AgStat all = ag_stat_merge(in, out, c);
-    const float m = all.m, L = logf(all.s);
-    const float log_rest = out.m == -INFINITY && out.s == 0.0f ? -INFINITY : (out.m - m) * a.inv_tau + logf(out.s) - L;
-    const DistillList list = distill_list(s_parts + now * DI_WARPS, parts, rest, a.inv_tau);
-    float log_q = 0.0f, q = 0.0f;
-    if (id >= 0) distill_slot(list, t, rest, a.inv_tau, log_q, q);
-    if (tid < a.top) s_q[tid] = q;
-    auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - m) * a.inv_tau - L; };
-    if (lead) {
-      if (warp < parts) {
-        const float sum = ag_warp_sum(id >= 0 && q != 0.0f ? q * (log_q - log_p(x_id)) : 0.0f);
-        if (lane == 0) s_sum[warp] = sum;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        float sum = list.left != 0.0f ? list.left * (logf(list.left) - log_rest) : 0.0f;
-        for (int w = 0; w < parts; ++w) sum += s_sum[w];
-        a.row_loss[row] = list.used ? sum : 0.0f;
-        if (a.stats) a.stats[row] = make_float4(m, L, rest ? log_rest : 0.0f, 0.0f);
-      }
-    }
-    if (TRAIN) {
-      const float s = distill_scale(a, row);
-      const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
-      const float outside = none ? 0.0f : s * distill_outside(list, log_rest);
-      const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
-      const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
-      T* g_row = dlogits + row * a.ld_grad;
-      T* g_body = g_row + r.head + (int64_t)rank * a.per * NV;
-      const bool packets = (((uintptr_t)g_body) & 15) == 0;
-      for (int i = tid; i < n; i += DI_THREADS) {
-        float x[NV], g[NV];
-        ag_widen(slice[i], x);
-#pragma unroll
-        for (int e = 0; e < NV; e += 2) {
-          float d0, d1;
-          ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
-          g[e] = none ? 0.0f : outside * ag_ex2(d0);
-          g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
-        }
-        ag_store_packet<T>(g_body + (int64_t)i * NV, g, packets);
-      }
-      if (at_edge >= 0) Pack<T>::store1(g_row + at_edge, none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift));
-      __syncthreads();  // the entries of listed tokens are written once more
-      if (once) {
-        if (twice)
-          for (int k = tid + 1; k < a.top; ++k)
-            if (s_ids[now * AG_DISTILL_MAX + k] == id) q += s_q[k];
-        const float p = ag_ex2((x_id - m) * c + shift);
-        Pack<T>::store1(g_row + id, none ? 0.0f : s * (p * (list.mass + list.left) - q));
-      }
-    }
-    if (more && a.buffers == 1) next.fetch(s_slices, rank, a.per);
-    r = next;
-    row += clusters;
   }
-  if (S > 1) ag_cluster_sync(S);  // nobody leaves while others may still store to its shared memory
+  if (id >= a.V) {
+    if (rank == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
+    id = -1;
+  }
+  if (id < 0) t = -INFINITY;
+  const bool own = id >= 0 && r.owner(id, a.per) == rank;
+  float x_id = -INFINITY;
+  if (id >= 0 && (rank == 0 || own)) x_id = Pack<T>::load1(r.x + id);
+  if ((TRAIN || REST) && own) {
+    const int q = id - first;  // among this block's packets, or in the edges: 0.. before them, 16.. behind them
+    const bool body = id >= r.head && id < r.head + r.body * NV;
+    const int edge_bit = id < r.head ? id : 16 + id - r.head - r.body * NV;
+    const uint32_t bit = body ? 1u << ((q / NV & 3) * 8 + q % NV) : 1u << edge_bit;
+    if (atomicOr(body ? s_marks + 4 + q / NV / 4 : s_marks, bit) & bit) s_marks[1] = 1;
+  }
+  if (tid < a.top) s_ids[tid] = id;
+  if (warp < parts) {
+    const DistillPart p = distill_part(t, REST, a.inv_tau);
+    if (lane == 0) s_parts[warp] = p;
+  }
+  __syncthreads();
+  bool once = own;
+  if ((TRAIN || REST) && s_marks[1] && own)
+    for (int k = 0; k < tid; ++k) once &= s_ids[k] != id;
+  const float x_edge = edge;
+  if (REST && edge_index >= 0 && s_marks[0] >> tid & 1) edge = -INFINITY;
+
+  const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T>(at, s_map, n, edge, c) : ag_part_stat<false, T, 4>(at, n, edge, c), c);
+  AgStat in = ag_stat_none();
+  if (REST && warp < parts) {
+    if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
+    in = ag_stat_warp(in, c);
+  }
+  // The first block's logits of other blocks' parts have arrived before its word goes out, on which those are overwritten if the
+  // gradient takes the logits' place: a store needs its operand, and instructions of a warp go in order.
+  if (TRAIN && rank == 0 && tid < a.top) reinterpret_cast<volatile float*>(s_q)[tid] = x_id;
+  const float4 word = make_float4(mine.m, mine.s, in.m, in.s);
+  const float4* told = TRAIN ? exchange.tell(0, word) : exchange.tell_first(word);
+  if (!TRAIN && rank) return;
+  AgStat out = ag_stat_none();
+  in = ag_stat_none();
+  if (lane < groups) {
+    const float4 w = told[lane];
+    out = {w.x, w.y, 0.0f};
+    if (REST) in = {w.z, w.w, 0.0f};
+  }
+  if (lane + 32 < groups) {
+    const float4 w = told[lane + 32];
+    out = ag_stat_merge(out, {w.x, w.y, 0.0f}, c);
+    if (REST) in = ag_stat_merge(in, {w.z, w.w, 0.0f}, c);
+  }
+  out = ag_stat_warp(out, c);
+  AgStat all = out;
+  float log_rest = 0.0f;
+  if (REST) {
+    all = ag_stat_merge(ag_stat_warp(in, c), out, c);
+    log_rest = out.m == -INFINITY && out.s == 0.0f ? -INFINITY : (out.m - all.m) * a.inv_tau + logf(out.s) - logf(all.s);
+  }
+  const float m = all.m, L = logf(all.s);
+  const DistillList list = distill_list(s_parts, parts, REST, a.inv_tau);
+  auto log_p = [&](float x) { return x == -INFINITY && !(L != L) ? -INFINITY : (x - m) * a.inv_tau - L; };
+  float q = 0.0f;
+  if (warp < parts) {
+    float log_q = 0.0f;
+    if (id >= 0) distill_slot(list, t, REST, a.inv_tau, log_q, q);
+    if (TRAIN && tid < a.top) s_q[tid] = q;
+    if (rank == 0) {
+      const float sum = ag_warp_sum(id >= 0 && q != 0.0f ? q * (log_q - log_p(x_id)) : 0.0f);
+      if (lane == 0) s_sum[warp] = sum;
+    }
+  }
+  const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
+  const float shift = none ? 0.0f : -L * AG_LOG2E;
+  T* g_row = dlogits + row * a.ld_grad;
+  if (TRAIN) {
+    const float outside = none ? 0.0f : s * distill_outside(list, log_rest), ref = none ? 0.0f : -m;
+    const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
+    const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0;
+    auto put = [&](const uint4& w, int i) {
+      float x[NV], g[NV];
+      ag_widen(w, x);
+#pragma unroll
+      for (int e = 0; e < NV; e += 2) {
+        float d0, d1;
+        ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
+        g[e] = none ? 0.0f : outside * ag_ex2(d0);
+        g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
+      }
+      ag_store_packet<T>(g_row + first + (int64_t)i * NV, g, packets);
+    };
+    constexpr int U = 4;
+    int i = tid;
+    for (; i + (U - 1) * DI_THREADS < n; i += U * DI_THREADS) {
+      uint4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = at[i + u * DI_THREADS];
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(w[u], i + u * DI_THREADS);
+    }
+    for (; i < n; i += DI_THREADS) put(at[i], i);
+    if (edge_index >= 0) Pack<T>::store1(g_row + edge_index, none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift));
+  }
+  __syncthreads();  // the loss of each warp is there; the entries of listed tokens are written once more
+  if (rank == 0 && tid == 0) {
+    float sum = list.left != 0.0f ? list.left * (logf(list.left) - log_rest) : 0.0f;
+    for (int w = 0; w < parts; ++w) sum += s_sum[w];
+    a.row_loss[row] = list.used ? sum : 0.0f;
+    if (a.stats) a.stats[row] = make_float4(m, L, log_rest, 0.0f);
+  }
+  if (TRAIN && once) {
+    if (s_marks[1])
+      for (int k = tid + 1; k < a.top; ++k)
+        if (s_ids[k] == id) q += s_q[k];
+    const float p = ag_ex2((x_id - m) * c + shift);
+    Pack<T>::store1(g_row + id, none ? 0.0f : s * (p * (list.mass + list.left) - q));
+  }
 }
 
 // The gradient alone, from the statistics that the loss left: a block takes 16 KB of a row.
@@ -406,20 +427,32 @@ distill_loss_kernel(const float* __restrict__ row_loss, const float* __restrict_
   }
 }
 
-template <typename T, bool TRAIN>
+constexpr int64_t DI_IN_FLIGHT = 48 << 20;
+template <typename T, bool TRAIN, bool REST>
 int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs a) {
-  static AgClusterFit fits[AG_MAX_DEVICES];
-  const AgRowPlan p = ag_row_plan(ctx, a.N, a.V, sizeof(T) == 4 ? AG_F32 : AG_BF16, distill_smem);
-  a.S = p.S;
-  a.per = p.per;
-  a.buffers = p.buffers;
-  return ag_launch_rows(ctx, "distill_kernel", fits, distill_kernel<T, TRAIN>, p, a.N, (const T*)logits, (T*)dlogits, a);
+  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
+  a.S = 1;
+  while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
+  if (TRAIN)
+    while (a.S < 8 && (int64_t)packets * 16 * ctx->sm_count * DI_BLOCKS > DI_IN_FLIGHT * a.S && packets / a.S >= 512) a.S *= 2;
+  a.per = (packets + a.S - 1) / a.S;
+  AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "distillation: too many rows");
+  static std::atomic<bool> ready[AG_MAX_DEVICES];
+  const size_t smem = distill_smem(a.S, a.per, TRAIN || REST);
+  if (smem > 48 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
+    AG_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<T, TRAIN, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)distill_smem(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
+    ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
+  }
+  return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST>, a.S, smem, a.N, (const T*)logits, (T*)dlogits, a);
 }
 
 template <typename T>
 int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, const DistillArgs& a, bool backward) {
-  if (!backward)
-    return a.dloss ? distill_forward<T, true>(ctx, logits, dlogits, a) : distill_forward<T, false>(ctx, logits, dlogits, a);
+  if (!backward) {
+    if (a.dloss) return a.rest ? distill_forward<T, true, true>(ctx, logits, dlogits, a) : distill_forward<T, true, false>(ctx, logits, dlogits, a);
+    return a.rest ? distill_forward<T, false, true>(ctx, logits, dlogits, a) : distill_forward<T, false, false>(ctx, logits, dlogits, a);
+  }
   const int packets = a.V / AG_PACKET<T>, chunks = packets ? (packets + DI_THREADS * DB_PACKETS - 1) / (DI_THREADS * DB_PACKETS) : 1;
   AG_REQUIRE(ctx, a.N * chunks < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
   AG_LAUNCH_PDL(ctx, "distill_backward_kernel", distill_backward_kernel<T>, (unsigned)(a.N * chunks), DI_THREADS, 0, (const T*)logits,
@@ -440,7 +473,7 @@ int distill(ag_ctx* ctx, const char* who, const void* logits, int64_t ld, const 
   if (N == 0 && !loss) return AG_OK;
   AgOnDevice on(ctx);
   const DistillArgs a = {ids, teacher, row_scale, dloss, row_loss, (float4*)stats, N, ld, ld_grad, V, top, mode == AG_DISTILL_REST,
-                         1.0f / temperature, ctx->d_status, 0, 0, 0};
+                         1.0f / temperature, N ? (float)(1.0 / (double)N) : 0.0f, ctx->d_status, 0, 0};
   if (int rc = N == 0 ? AG_OK
                : dtype == AG_F32 ? distill_t<float>(ctx, logits, dres, dlogits, a, backward)
                                  : distill_t<__nv_bfloat16>(ctx, logits, dres, dlogits, a, backward))

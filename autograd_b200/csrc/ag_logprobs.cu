@@ -32,8 +32,8 @@ struct LpArgs {
   int* status;
 };
 
-// the exchange, a barrier, a block's keys, the keys of all blocks at block 0, counters
-size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (S == 1 ? 1 : 1 + S) + 32; }
+// the exchange, a barrier, a block's keys, the keys of all blocks at block 0, a list of packets, counters
+size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (S == 1 ? 1 : 1 + S) + (size_t)cap * 4 + 32; }
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
@@ -44,7 +44,7 @@ __device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
   const uint32_t a = one ? ag_order(box[lane].w) : 0u, b = two ? ag_order(box[lane + 32].w) : 0u;
   uint32_t lo = __reduce_min_sync(0xffffffffu, min(one ? a : 0xffffffffu, two ? b : 0xffffffffu));
   uint32_t hi = __reduce_max_sync(0xffffffffu, max(a, b));
-  const int enough = need + (need >> 3);
+  const int enough = need + max(1, need >> 3);
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo) / 2 + 1;
     const int count = __popc(__ballot_sync(0xffffffffu, a >= mid)) + __popc(__ballot_sync(0xffffffffu, b >= mid));
@@ -81,7 +81,7 @@ struct LpPart {
 // The block's logits whose order is `bound` or more are more than `cap`: leaves the keys of its `top` largest at least, `cap` at
 // most, in `keys` and returns how many.  By all threads of the block.  A block that has this many has more than `top` logits.
 template <typename T>
-__device__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
+__device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
   uint32_t hi = 0xffffffffu;
   auto count_from = [&](uint32_t k) {
     int c = 0;
@@ -159,7 +159,7 @@ __device__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top, int cap, uns
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, TOP ? 4 : 6)
+__global__ void __launch_bounds__(LP_THREADS, TOP ? 5 : 6)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
@@ -169,10 +169,11 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   uint64_t* s_keys_bar = s_bars + 2;                                                   // every block has its keys
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);    // [cap]
   unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
-  int* n_keys = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);           // and a counter behind it
+  int* packets = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);          // [cap]
+  int* n_keys = packets + a.cap;                                                       // keys, packets, a counter
   const float c = a.inv_tau * AG_LOG2E;
   if (TOP && tid == 0) {
-    *n_keys = 0;
+    n_keys[0] = n_keys[1] = 0;
     ag_mbar_init(s_keys_bar, S);
     ag_fence_mbar_init();
   }
@@ -221,16 +222,30 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   if (!TOP) return;
   const float bound = lp_bound(told, groups, a.need);
   const LpPart<T> part = {at, n, first, edge, edge_index};
-  if (own.m >= bound || own.s != own.s)
-    part.each([&](float x, int j) {
-      if (!(x < bound)) {
-        const int k = atomicAdd(n_keys, 1);
-        if (k < a.cap) keys[k] = lp_key(x, j);
-      }
-    });
+  // Packets with something in them go on a list first, and are taken apart by all threads: with a logit in every third packet
+  // that a warp looks at, taking it apart on the spot has the other lanes wait (64 alternatives of 32768 bf16: half of all
+  // instructions).
+  if (own.m >= bound || own.s != own.s) {
+    if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
+    for (int i = tid; i < n; i += LP_THREADS) {
+      const uint4 w[1] = {at[i]};
+      if (ag_largest(w, T()) < bound && own.s == own.s) continue;  // nothing here, and NaN nowhere
+      const int k = atomicAdd(n_keys + 1, 1);
+      if (k < a.cap) packets[k] = i;
+    }
+  }
   __syncthreads();
-  if (*n_keys > a.cap) {
-    const int found = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 1);
+  const int listed = min(n_keys[1], a.cap);
+  for (int k = tid; k < listed * AG_PACKET<T>; k += LP_THREADS) {
+    const int index = packets[k / AG_PACKET<T>] * AG_PACKET<T> + k % AG_PACKET<T>;
+    const float x = Pack<T>::load1(r.x + first + index);
+    if (x < bound) continue;
+    const int to = atomicAdd(n_keys, 1);
+    if (to < a.cap) keys[to] = lp_key(x, first + index);
+  }
+  __syncthreads();
+  if (n_keys[0] > a.cap || n_keys[1] > a.cap) {
+    const int found = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 2);
     if (tid == 0) *n_keys = found;
     __syncthreads();
   }
@@ -249,16 +264,30 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     ag_cluster_sync(S);  // nobody leaves while block 0 reads its keys
     if (rank) return;
   }
-  for (int i = tid; i < total; i += LP_THREADS) {
-    const unsigned long long key = all[i];
+  // a key's place is the number of larger ones; where there are threads for it, several count for each key
+  auto put = [&](unsigned long long key, int place) {
+    if (place >= a.top) return;
+    const int64_t to = row * a.top + place;
+    a.top_ids[to] = (int32_t)~(uint32_t)key;
+    a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
+  };
+  auto larger = [&](unsigned long long key, int from, int step) {
     int place = 0;
 #pragma unroll 4
-    for (int k = 0; k < total; ++k) place += all[k] > key;
-    if (place < a.top) {
-      const int64_t to = row * a.top + place;
-      a.top_ids[to] = (int32_t)~(uint32_t)key;
-      a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
-    }
+    for (int k = from; k < total; k += step) place += all[k] > key;
+    return place;
+  };
+  __shared__ int s_place[LP_THREADS / 2];
+  if (S > 1) __syncthreads();  // the keys are here
+  if (total <= LP_THREADS / 2) {
+    const int lanes = (total + 31) & ~31, parts = LP_THREADS / lanes, i = tid % lanes;
+    if (tid < lanes) s_place[i] = 0;
+    __syncthreads();
+    if (i < total && tid < parts * lanes) atomicAdd(&s_place[i], larger(all[i], tid / lanes, parts));
+    __syncthreads();
+    if (tid < total) put(all[tid], s_place[tid]);
+  } else {
+    for (int i = tid; i < total; i += LP_THREADS) put(all[i], larger(all[i], 0, 1));
   }
 }
 
