@@ -13,7 +13,7 @@
 // token tells what is listed: in the sum over the others those logits count as -inf, and the listed ones are added from the threads
 // that have them, each token once.  The gradient comes from a second look at the row, which L2 still holds: rows under way take
 // up to DI_IN_FLIGHT bytes, more blocks per row where they would take more.  The listed tokens' entries are written after it.
-// Gradient alone: packets in registers, 16 KB of a row per block, which stages the listed logits among them first.
+// Gradient alone: the same, without the first look.
 #include "ag_vocab.cuh"
 
 namespace {
@@ -298,73 +298,65 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   }
 }
 
-// The gradient alone, from the statistics that the loss left: a block takes 16 KB of a row.
-constexpr int DB_PACKETS = 4;  // per thread
-template <typename T>
-__global__ void __launch_bounds__(DI_THREADS)
-distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const DistillArgs a, int chunks) {
-  constexpr int NV = AG_PACKET<T>, CHUNK = DI_THREADS * DB_PACKETS;
+// The gradient alone, from the statistics that the loss left: a block takes `per` packets of a row.
+template <typename T, bool REST>
+__global__ void __launch_bounds__(DI_THREADS, DI_BLOCKS)
+distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const DistillArgs a) {
+  constexpr int NV = AG_PACKET<T>, U = 4;
   __shared__ DistillPart s_parts[DI_WARPS];
   __shared__ int s_ids[AG_DISTILL_MAX];
   __shared__ float s_q[AG_DISTILL_MAX];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = (a.top + 31) / 32;
   ag_pdl_wait();
   ag_pdl_trigger();
-  const int64_t row = blockIdx.x / chunks;
-  const int chunk = (int)(blockIdx.x - row * chunks);
+  const int64_t row = blockIdx.x / a.S;
+  const int rank = (int)(blockIdx.x - row * a.S);
   const AgRow<T> r(logits + row * a.ld, a.V);
-  const int n = r.mine(chunk, CHUNK);
-  const T* x_body = r.x + r.head + (int64_t)chunk * CHUNK * NV;
+  const int n = r.mine(rank, a.per), first = r.head + rank * a.per * NV;
+  const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
   T* g_row = dlogits + row * a.ld_grad;
   const T* d_row = dres ? dres + row * a.ld_grad : nullptr;
-  const int64_t g_off = r.head + (int64_t)chunk * CHUNK * NV;
-  uint4 w[DB_PACKETS];
-#pragma unroll
-  for (int u = 0; u < DB_PACKETS; ++u) {
-    const int i = tid + u * DI_THREADS;
-    w[u] = i < n ? __ldcs(reinterpret_cast<const uint4*>(x_body + (int64_t)i * NV)) : make_uint4(0, 0, 0, 0);
-  }
   const float4 st = a.stats[row];
   const float m = st.x, L = st.y, c = a.inv_tau * AG_LOG2E;
   int id = -1;
   float t = -INFINITY, x_id = 0.0f, d_id = 0.0f;
   if (tid < a.top) {
     id = a.ids[row * a.top + tid];
+    t = a.teacher[row * a.top + tid];
     if (id >= a.V) {
-      if (chunk == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
+      if (rank == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
       id = -1;
     }
-    if (id >= 0) t = a.teacher[row * a.top + tid];
+    if (id < 0) t = -INFINITY;
     s_ids[tid] = id;
   }
-  const int edge_index = r.edge(chunk);
+  const float s = distill_scale(a, row);
+  const int edge_index = r.edge(rank);
   const float x_edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : 0.0f;
-  const bool own = id >= 0 && r.owner(id, CHUNK) == chunk;
+  const bool own = id >= 0 && r.owner(id, a.per) == rank;
   if (own) {
     x_id = Pack<T>::load1(r.x + id);
     if (d_row) d_id = Pack<T>::load1(d_row + id);
   }
   if (warp < parts) {
-    const DistillPart p = distill_part(t, a.rest, a.inv_tau);
+    const DistillPart p = distill_part(t, REST, a.inv_tau);
     if (lane == 0) s_parts[warp] = p;
   }
   __syncthreads();
-  const DistillList list = distill_list(s_parts, parts, a.rest, a.inv_tau);
-  float log_q, q = 0.0f;
-  if (id >= 0) distill_slot(list, t, a.rest, a.inv_tau, log_q, q);
-  if (tid < a.top) s_q[tid] = q;
-  const float s = distill_scale(a, row);
+  const DistillList list = distill_list(s_parts, parts, REST, a.inv_tau);
+  if (tid < a.top) {
+    float log_q, q = 0.0f;
+    if (id >= 0) distill_slot(list, t, REST, a.inv_tau, log_q, q);
+    s_q[tid] = q;
+  }
   const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
   const float outside = none ? 0.0f : s * distill_outside(list, st.z);
   const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
   const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
-  const bool packets = (((uintptr_t)(g_row + g_off)) & 15) == 0, d_packets = (((uintptr_t)(d_row + g_off)) & 15) == 0;
-#pragma unroll
-  for (int u = 0; u < DB_PACKETS; ++u) {
-    const int i = tid + u * DI_THREADS;
-    if (i >= n) break;
+  const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0, d_packets = (((uintptr_t)(d_row + first)) & 15) == 0;
+  auto put = [&](const uint4& w, int i) {
     float x[NV], g[NV];
-    ag_widen(w[u], x);
+    ag_widen(w, x);
 #pragma unroll
     for (int e = 0; e < NV; e += 2) {
       float d0, d1;
@@ -372,20 +364,24 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
       g[e] = none ? 0.0f : outside * ag_ex2(d0);
       g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
     }
-    const int64_t at = g_off + (int64_t)i * NV;
+    const int to = first + i * NV;
     if (d_row) {
       float d[NV];
-      if (d_packets) {
-        Pack<T>::load_stream(d_row + at, d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < NV; ++e) d[e] = Pack<T>::load1(d_row + at + e);
-      }
+      ag_load_packet<T>(d_row + to, d, d_packets);
 #pragma unroll
       for (int e = 0; e < NV; ++e) g[e] += d[e];
     }
-    ag_store_packet<T>(g_row + at, g, packets);
+    ag_store_packet<T>(g_row + to, g, packets);
+  };
+  int i = tid;
+  for (; i + (U - 1) * DI_THREADS < n; i += U * DI_THREADS) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * DI_THREADS);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(w[u], i + u * DI_THREADS);
   }
+  for (; i < n; i += DI_THREADS) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
     const float d = d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f;
     Pack<T>::store1(g_row + edge_index, (none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift)) + d);
@@ -393,7 +389,7 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
   __syncthreads();  // the entries of listed tokens are written once more
   if (own) {
     bool once = true;
-    q = 0.0f;
+    float q = 0.0f;
     for (int k = 0; k < a.top; ++k)
       if (s_ids[k] == id) {
         once &= k >= tid;
@@ -448,15 +444,20 @@ int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs 
 }
 
 template <typename T>
-int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, const DistillArgs& a, bool backward) {
+int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, DistillArgs a, bool backward) {
   if (!backward) {
     if (a.dloss) return a.rest ? distill_forward<T, true, true>(ctx, logits, dlogits, a) : distill_forward<T, true, false>(ctx, logits, dlogits, a);
     return a.rest ? distill_forward<T, false, true>(ctx, logits, dlogits, a) : distill_forward<T, false, false>(ctx, logits, dlogits, a);
   }
-  const int packets = a.V / AG_PACKET<T>, chunks = packets ? (packets + DI_THREADS * DB_PACKETS - 1) / (DI_THREADS * DB_PACKETS) : 1;
-  AG_REQUIRE(ctx, a.N * chunks < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
-  AG_LAUNCH_PDL(ctx, "distill_backward_kernel", distill_backward_kernel<T>, (unsigned)(a.N * chunks), DI_THREADS, 0, (const T*)logits,
-                (const T*)dres, (T*)dlogits, a, chunks);
+  a.S = ag_row_parts(ctx, a.N, a.V / AG_PACKET<T>);
+  a.per = (a.V / AG_PACKET<T> + a.S - 1) / a.S;
+  AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
+  if (a.rest)
+    AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, true>), (unsigned)(a.N * a.S), DI_THREADS, 0,
+                  (const T*)logits, (const T*)dres, (T*)dlogits, a);
+  else
+    AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, false>), (unsigned)(a.N * a.S), DI_THREADS, 0,
+                  (const T*)logits, (const T*)dres, (T*)dlogits, a);
   return AG_OK;
 }
 

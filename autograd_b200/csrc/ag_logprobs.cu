@@ -291,35 +291,29 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   }
 }
 
-// Gradient: a block takes 16 KB of a row, all of its loads under way before the first is used.
-constexpr int LB_PACKETS = 4;  // per thread
+// Gradient: a block takes `per` packets of a row.
 struct LbArgs {
   const int32_t* ids;
   const float4* stats;
   const float *dlogprob, *dentropy;
   int64_t ld, ld_grad;
-  int V, chunks;
+  int V, S, per;
   float inv_tau;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS)
+__global__ void __launch_bounds__(LP_THREADS, 4)
 logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArgs p) {
-  constexpr int NV = AG_PACKET<T>, CHUNK = LP_THREADS * LB_PACKETS;
+  constexpr int NV = AG_PACKET<T>, U = 4;
   const int tid = threadIdx.x;
   ag_pdl_wait();
   ag_pdl_trigger();
-  const int64_t row = blockIdx.x / p.chunks;
-  const int chunk = (int)(blockIdx.x - row * p.chunks);
+  const int64_t row = blockIdx.x / p.S;
+  const int rank = (int)(blockIdx.x - row * p.S);
   const AgRow<T> r(logits + row * p.ld, p.V);
-  const int n = r.mine(chunk, CHUNK), first = r.head + chunk * CHUNK * NV;
-  uint4 w[LB_PACKETS];
-#pragma unroll
-  for (int u = 0; u < LB_PACKETS; ++u) {
-    const int i = tid + u * LP_THREADS;
-    w[u] = i < n ? __ldcs(reinterpret_cast<const uint4*>(r.x + first + (int64_t)i * NV)) : make_uint4(0, 0, 0, 0);
-  }
-  const int edge_index = r.edge(chunk);
+  const int n = r.mine(rank, p.per), first = r.head + rank * p.per * NV;
+  const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
+  const int edge_index = r.edge(rank);
   const float x_edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : 0.0f;
   const float4 st = p.stats[row];
   const int id = p.ids ? p.ids[row] : -1;
@@ -335,33 +329,33 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
     const float lp = fmaxf((x - st.x) * p.inv_tau, -1e4f) - st.y;
     return -ag_ex2(lp * AG_LOG2E) * (k + b * lp);
   };
-#pragma unroll
-  for (int u = 0; u < LB_PACKETS; ++u) {
-    const int i = tid + u * LP_THREADS;
-    if (i >= n) break;
+  auto put = [&](const uint4& w, int i) {
     float x[NV], g[NV];
-    ag_widen(w[u], x);
+    ag_widen(w, x);
 #pragma unroll
     for (int e = 0; e < NV; ++e) g[e] = none ? 0.0f : local(x[e]);
-    const int at = first + i * NV;
-    const int hit = id - at;
+    const int to = first + i * NV, hit = id - to;
     if (hit >= 0 && hit < NV && !none) {
 #pragma unroll
       for (int e = 0; e < NV; ++e) g[e] += e == hit ? a : 0.0f;
     }
     if (d_row) {
       float d[NV];
-      if (d_packets) {
-        Pack<T>::load_stream(d_row + at, d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < NV; ++e) d[e] = Pack<T>::load1(d_row + at + e);
-      }
+      ag_load_packet<T>(d_row + to, d, d_packets);
 #pragma unroll
       for (int e = 0; e < NV; ++e) g[e] += d[e];
     }
-    ag_store_packet<T>(g_row + at, g, packets);
+    ag_store_packet<T>(g_row + to, g, packets);
+  };
+  int i = tid;
+  for (; i + (U - 1) * LP_THREADS < n; i += U * LP_THREADS) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * LP_THREADS);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(w[u], i + u * LP_THREADS);
   }
+  for (; i < n; i += LP_THREADS) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
     const float g = none ? 0.0f : local(x_edge) + (edge_index == id ? a : 0.0f);
     Pack<T>::store1(g_row + edge_index, g + (d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f));
@@ -370,11 +364,11 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
 
 template <typename T>
 int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, LbArgs p, int64_t N) {
-  const int packets = p.V / AG_PACKET<T>;
-  p.chunks = packets ? (packets + LP_THREADS * LB_PACKETS - 1) / (LP_THREADS * LB_PACKETS) : 1;
-  AG_REQUIRE(ctx, N * p.chunks < (1ll << 31), "ag_token_logprobs_backward: too many rows for V=%d", p.V);
-  AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<T>, (unsigned)(N * p.chunks), LP_THREADS, 0,
-                (const T*)logits, (const T*)dres, (T*)dlogits, p);
+  p.S = ag_row_parts(ctx, N, p.V / AG_PACKET<T>);
+  p.per = (p.V / AG_PACKET<T> + p.S - 1) / p.S;
+  AG_REQUIRE(ctx, N * p.S < (1ll << 31), "ag_token_logprobs_backward: too many rows for V=%d", p.V);
+  AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<T>, (unsigned)(N * p.S), LP_THREADS, 0, (const T*)logits,
+                (const T*)dres, (T*)dlogits, p);
   return AG_OK;
 }
 
@@ -428,7 +422,7 @@ extern "C" int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
-  const LbArgs p = {ids, (const float4*)stats, dlogprob, dentropy, ld, ld_grad, V, 0, 1.0f / temperature};
+  const LbArgs p = {ids, (const float4*)stats, dlogprob, dentropy, ld, ld_grad, V, 0, 0, 1.0f / temperature};
   return dtype == AG_F32 ? logprobs_backward<float>(ctx, logits, dres, dlogits, p, N)
                          : logprobs_backward<__nv_bfloat16>(ctx, logits, dres, dlogits, p, N);
 }

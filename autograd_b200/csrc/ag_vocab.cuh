@@ -1,10 +1,5 @@
 // Shared by the operators on rows of logits (ag_logprobs.cu, ag_distill.cu): argument checks, softmax statistics that can be
-// merged, rows that are cut into slices of shared memory.
-//
-// A row belongs to a cluster of 1 to 8 blocks, each of which holds a slice of it in shared memory, fetched with 16-byte
-// asynchronous copies while the slice of the cluster's row before is worked on.  A thread copies what it reads itself, so that the
-// copies need no barrier; one barrier of the cluster exchanges the statistics of its warps.  What comes after (the alternatives,
-// the gradient) finds the logits on chip: a row is read from memory once.
+// merged, rows in 16-byte packets, what the blocks of a row tell one another.
 #pragma once
 
 #include <math.h>
@@ -13,7 +8,7 @@
 
 #include "ag_common.cuh"
 
-constexpr int AG_ROW_THREADS = 256, AG_ROW_WARPS = AG_ROW_THREADS / 32;  // of a block of the kernels on slices
+constexpr int AG_ROW_THREADS = 256, AG_ROW_WARPS = AG_ROW_THREADS / 32;  // of a block
 constexpr float AG_LN2 = 0.69314718055994531f, AG_LOG2E = 1.44269504088896341f;
 
 // Launches go to the context's device, whichever is current in the calling thread.
@@ -212,6 +207,16 @@ __device__ __forceinline__ void ag_store_packet(T* to, const float (&g)[AG_PACKE
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void ag_load_packet(const T* from, float (&d)[AG_PACKET<T>], bool whole) {
+  if (whole) {
+    Pack<T>::load_stream(from, d);
+  } else {
+#pragma unroll
+    for (int e = 0; e < AG_PACKET<T>; ++e) d[e] = Pack<T>::load1(from + e);
+  }
+}
+
 // A row as its cluster sees it: `head` elements before the first 16-byte boundary, `body` packets, `tail` elements behind them.
 // Block `rank` has the packets from rank * per; head and tail are the first block's, an element per thread (0.., 16..).
 template <typename T>
@@ -235,24 +240,7 @@ struct AgRow {
     const int q = id - head;
     return q < 0 || q >= body * AG_PACKET<T> ? 0 : q / AG_PACKET<T> / per;
   }
-  // asynchronous copy of this thread's packets of the slice
-  __device__ __forceinline__ void fetch(uint4* slice, int rank, int per) const {
-    const int n = mine(rank, per);
-    const uint4* from = reinterpret_cast<const uint4*>(x + head) + (int64_t)rank * per + threadIdx.x;
-    uint32_t to = ag_smem_u32(slice + threadIdx.x);
-    int left = n - (int)threadIdx.x;
-    for (; left > 3 * AG_ROW_THREADS; left -= 4 * AG_ROW_THREADS, from += 4 * AG_ROW_THREADS, to += 4 * AG_ROW_THREADS * 16) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * AG_ROW_THREADS * 16), "l"(from + u * AG_ROW_THREADS)
-                     : "memory");
-    }
-    for (; left > 0; left -= AG_ROW_THREADS, from += AG_ROW_THREADS, to += AG_ROW_THREADS * 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
 };
-__device__ __forceinline__ void ag_fetched() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // Statistics of this thread's part of n packets (in shared or global memory), U at a time, and of its element of the edges (-inf
 // without one).
@@ -397,52 +385,12 @@ __device__ __forceinline__ float ag_of_order(uint32_t k) {
 
 #endif  // __CUDACC__
 
-// ---- the launch: slices, blocks per row, clusters that are resident at once --------------------------------------------------
-
-// How many clusters of a kernel the device holds, by blocks per cluster and shared memory; as AgOccupancy keeps its answers.
-class AgClusterFit {
- public:
-  template <typename Query>
-  int get(int size, size_t smem, Query query) {
-    const uint64_t key = (uint64_t)smem << 36 | (uint64_t)size << 32;
-    int free = -1;
-    for (int i = 0; i < kSlots; ++i) {
-      const uint64_t word = slot_[i].load(std::memory_order_relaxed);
-      if (word >> 32 == key >> 32 && (uint32_t)word) return (int)(uint32_t)word;
-      if (!word && free < 0) free = i;
-    }
-    const int fit = query();
-    if (fit < 1) return fit;
-    if (free < 0) free = (int)((key >> 32) * 0x9E3779B97F4A7C15ull >> 60);
-    slot_[free].store(key | (uint32_t)fit, std::memory_order_relaxed);
-    return fit;
-  }
-
- private:
-  static constexpr int kSlots = 16;
-  std::atomic<uint64_t> slot_[kSlots];
-};
-
-struct AgRowPlan {
-  int S, per, buffers;  // blocks per row, packets per block, slices in shared memory at once
-  size_t smem;
-};
-
-constexpr size_t AG_SMEM_MOST = 226 * 1024;  // and a kilobyte for what a kernel declares
-
-// `more`: what the kernel wants beside its slices, of a cluster of S
-template <typename More>
-static inline AgRowPlan ag_row_plan(const ag_ctx* ctx, int64_t N, int V, int dtype, More more) {
-  const int packets = (V * (dtype == AG_F32 ? 4 : 2) + 15) / 16;
-  AgRowPlan p;
-  p.S = 1;
-  while (p.S < 8 && (packets + p.S - 1) / p.S > 2048) p.S *= 2;
-  // few rows: more blocks for each, while they have something to do
-  while (p.S < 8 && N * p.S * 2 <= 2 * ctx->sm_count && packets / p.S >= 512) p.S *= 2;
-  p.per = (packets + p.S - 1) / p.S;
-  p.buffers = (size_t)p.per * 32 + more(p.S) <= AG_SMEM_MOST ? 2 : 1;
-  p.smem = (size_t)p.per * 16 * p.buffers + more(p.S);
-  return p;
+// ---- launches ---------------------------------------------------------------------------
+// Blocks per row of a kernel whose blocks need nothing of one another: one, unless that leaves SMs without work.
+static inline int ag_row_parts(const ag_ctx* ctx, int64_t N, int packets) {
+  int S = 1;
+  while (N * S < 4 * ctx->sm_count && packets / S >= 1024) S *= 2;
+  return S;
 }
 
 // Launch of n clusters of S blocks.
@@ -468,41 +416,3 @@ static inline int ag_launch_clusters(ag_ctx* ctx, const char* name, void (*kern)
   return AG_OK;
 }
 
-// Launch on clusters of p.S blocks, at most as many as are resident at once (each takes row after row), and never more than rows.
-template <typename... P, typename... A>
-static inline int ag_launch_rows(ag_ctx* ctx, const char* name, AgClusterFit* fits, void (*kern)(P...), const AgRowPlan& p, int64_t N,
-                                 A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = AG_ROW_THREADS;
-  cfg.dynamicSmemBytes = p.smem;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.S;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cfg.gridDim = p.S;
-  const int fit = fits[ag_dev_slot(ctx)].get(p.S, p.smem, [&] {
-    int n = 0;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AG_SMEM_MOST);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return -(int)e;
-    }
-    return n;
-  });
-  if (fit < 1)
-    AG_FAIL(ctx, AG_ERR_CUDA, "%s: no room for clusters of %d blocks with %zu bytes (%s)", name, p.S, p.smem,
-                       cudaGetErrorString((cudaError_t)-fit));
-  cfg.gridDim = (unsigned)((N < fit ? N : fit) * p.S);
-  cfg.numAttrs = ctx->pdl ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  if (e != cudaSuccess) AG_FAIL(ctx, AG_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e));
-  ctx->launches++;
-  ag_enqueued(ctx);
-  return AG_OK;
-}
