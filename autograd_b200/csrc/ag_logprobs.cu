@@ -17,6 +17,7 @@
 namespace {
 
 constexpr int LP_THREADS = AG_ROW_THREADS, LP_WARPS = LP_THREADS / 32;
+static_assert(3 * AG_TOP_MAX + 64 <= 2 * LP_THREADS, "two keys per thread are moved");
 
 struct LpArgs {
   const int32_t* ids;
@@ -32,8 +33,9 @@ struct LpArgs {
   int* status;
 };
 
-// the exchange, a barrier, a block's keys, the keys of all blocks at block 0, a list of packets, counters
-size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * 8 * (S == 1 ? 1 : 1 + S) + (size_t)cap * 4 + 32; }
+// the exchange, packets with a logit that passes, a barrier, a block's keys, those of all blocks at block 0, where the packets are
+// from, counters
+size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * (16 + 8 * (S == 1 ? 1 : 1 + S) + 4) + 64; }
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
@@ -166,11 +168,13 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   const int groups = S * LP_WARPS;
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
   const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
-  uint64_t* s_keys_bar = s_bars + 2;                                                   // every block has its keys
+  uint4* packets = reinterpret_cast<uint4*>(s_bars + 2);                               // [cap]
+  uint64_t* s_keys_bar = reinterpret_cast<uint64_t*>(packets + a.cap);                 // every block's keys are at block 0
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);    // [cap]
   unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
-  int* packets = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);          // [cap]
-  int* n_keys = packets + a.cap;                                                       // keys, packets, a counter
+  int* places = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);           // [cap]
+  int* counts = places + a.cap;                                                        // [8]
+  int* n_keys = counts + 8;                                                            // keys, packets, a counter
   const float c = a.inv_tau * AG_LOG2E;
   if (TOP && tid == 0) {
     n_keys[0] = n_keys[1] = 0;
@@ -187,14 +191,10 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   const float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
   const int n = r.mine(rank, a.per), first = r.head + rank * a.per * AG_PACKET<T>;
   const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
-  float x_id = 0.0f;
-  bool has = false;
-  if (tid == 0 && rank == 0 && a.logprob) {
-    const int id = a.ids[row];
-    has = id >= 0 && id < a.V;
-    if (has) x_id = Pack<T>::load1(r.x + id);
-  }
+  const int id = tid == 0 && rank == 0 && a.logprob ? a.ids[row] : -1;
   const AgStat own = ag_part_stat<true, T, 4>(at, n, edge, c);
+  const bool has = id >= 0 && id < a.V;
+  const float x_id = has ? Pack<T>::load1(r.x + id) : 0.0f;  // not before: the warp's packets would wait for the id
   AgStat v = ag_stat_warp(own, c);
   float reached = v.m;
   if (TOP) {
@@ -227,42 +227,48 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   // instructions).
   if (own.m >= bound || own.s != own.s) {
     if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
+#pragma unroll 2
     for (int i = tid; i < n; i += LP_THREADS) {
       const uint4 w[1] = {at[i]};
       if (ag_largest(w, T()) < bound && own.s == own.s) continue;  // nothing here, and NaN nowhere
       const int k = atomicAdd(n_keys + 1, 1);
-      if (k < a.cap) packets[k] = i;
+      if (k < a.cap) packets[k] = w[0], places[k] = first + i * AG_PACKET<T>;
     }
   }
   __syncthreads();
   const int listed = min(n_keys[1], a.cap);
   for (int k = tid; k < listed * AG_PACKET<T>; k += LP_THREADS) {
-    const int index = packets[k / AG_PACKET<T>] * AG_PACKET<T> + k % AG_PACKET<T>;
-    const float x = Pack<T>::load1(r.x + first + index);
+    const int e = k % AG_PACKET<T>;
+    const float x = Pack<T>::load1(reinterpret_cast<const T*>(packets) + k);
     if (x < bound) continue;
     const int to = atomicAdd(n_keys, 1);
-    if (to < a.cap) keys[to] = lp_key(x, first + index);
+    if (to < a.cap) keys[to] = lp_key(x, places[k / AG_PACKET<T>] + e);
   }
   __syncthreads();
-  if (n_keys[0] > a.cap || n_keys[1] > a.cap) {
-    const int found = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 2);
-    if (tid == 0) *n_keys = found;
-    __syncthreads();
-  }
-  int total = *n_keys;
+  int total = n_keys[0];
+  if (total > a.cap || n_keys[1] > a.cap) total = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 2);
   if (S > 1) {
+    // to block 0, each to its own place there
+    const uint32_t to = ag_peer(all + (size_t)rank * a.cap, 0);
+    for (int k = tid; k < total; k += LP_THREADS) ag_peer_store(to + k * 8, keys[k]);
+    if (tid == 0) ag_peer_store(ag_peer(counts + rank, 0), total);
+    __syncthreads();
     if (tid == 0) ag_peer_arrive(ag_peer(s_keys_bar, 0));
-    if (rank == 0) {
-      ag_wait_cluster(s_keys_bar, 0, a.status);
-      total = 0;
-      for (int p = 0; p < S; ++p) {
-        const int m = ag_peer_load_int(ag_peer(n_keys, p));
-        for (int k = tid; k < m; k += LP_THREADS) all[total + k] = ag_peer_load_key(ag_peer(keys + k, p));
-        total += m;
-      }
-    }
-    ag_cluster_sync(S);  // nobody leaves while block 0 reads its keys
     if (rank) return;
+    ag_wait_cluster(s_keys_bar, 0, a.status);
+    // side by side
+    total = counts[0];
+    for (int p = 1; p < S; ++p) {
+      const int more = counts[p];
+      unsigned long long mine[2];  // cap <= 2 * LP_THREADS, and what is moved down may lie over what is not yet
+      for (int k = 0; k < 2; ++k)
+        if (tid + k * LP_THREADS < more) mine[k] = all[(size_t)p * a.cap + tid + k * LP_THREADS];
+      __syncthreads();
+      for (int k = 0; k < 2; ++k)
+        if (tid + k * LP_THREADS < more) all[total + tid + k * LP_THREADS] = mine[k];
+      total += more;
+    }
+    __syncthreads();
   }
   // a key's place is the number of larger ones; where there are threads for it, several count for each key
   auto put = [&](unsigned long long key, int place) {
@@ -278,7 +284,6 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     return place;
   };
   __shared__ int s_place[LP_THREADS / 2];
-  if (S > 1) __syncthreads();  // the keys are here
   if (total <= LP_THREADS / 2) {
     const int lanes = (total + 31) & ~31, parts = LP_THREADS / lanes, i = tid % lanes;
     if (tid < lanes) s_place[i] = 0;

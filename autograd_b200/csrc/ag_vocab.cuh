@@ -357,15 +357,11 @@ struct AgExchange {
   static constexpr size_t bytes(int S) { return 2 * (size_t)S * AG_ROW_WARPS * 16 + 16; }
 };
 
-__device__ __forceinline__ int ag_peer_load_int(uint32_t a) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void ag_peer_store(uint32_t to, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
 }
-__device__ __forceinline__ unsigned long long ag_peer_load_key(uint32_t a) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void ag_peer_store(uint32_t to, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(v) : "memory");
 }
 // one arrival at a barrier of another block, after everything that this thread has seen done
 __device__ __forceinline__ void ag_peer_arrive(uint32_t bar) {
