@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int LP_THREADS = AG_ROW_THREADS, LP_WARPS = LP_THREADS / 32;
-static_assert(3 * AG_TOP_MAX + 64 <= 2 * LP_THREADS, "two keys per thread are moved");
+static_assert(3 * AG_TOP_MAX + 64 + 1 <= 2 * LP_THREADS, "two keys per thread are moved");
 
 struct LpArgs {
   const int32_t* ids;
@@ -42,6 +42,15 @@ __device__ __forceinline__ unsigned long long lp_key(float x, int index) { retur
 // The need-th largest of the n <= 64 numbers box[].w, or one that an eighth more of them reach; by one warp.
 __device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
   const int lane = threadIdx.x & 31;
+  if (n <= 16) {  // a lane each, which counts the larger ones: the bisection takes some 20 steps
+    const float mine = lane < n ? box[lane].w : -INFINITY;
+    int place = 0;
+    for (int g = 0; g < n; ++g) {
+      const float w = box[g].w;
+      place += w > mine || (w == mine && g < lane);
+    }
+    return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, lane < n && place == need - 1)) - 1);
+  }
   const bool one = lane < n, two = lane + 32 < n;
   const uint32_t a = one ? ag_order(box[lane].w) : 0u, b = two ? ag_order(box[lane + 32].w) : 0u;
   uint32_t lo = __reduce_min_sync(0xffffffffu, min(one ? a : 0xffffffffu, two ? b : 0xffffffffu));
@@ -170,7 +179,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
   uint4* packets = reinterpret_cast<uint4*>(s_bars + 2);                               // [cap]
   uint64_t* s_keys_bar = reinterpret_cast<uint64_t*>(packets + a.cap);                 // every block's keys are at block 0
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 1);    // [cap]
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], cap even
   unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
   int* places = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);           // [cap]
   int* counts = places + a.cap;                                                        // [8]
@@ -277,18 +286,25 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     a.top_ids[to] = (int32_t)~(uint32_t)key;
     a.top_logprobs[to] = log_p(ag_of_order((uint32_t)(key >> 32)));
   };
-  auto larger = [&](unsigned long long key, int from, int step) {
+  auto larger = [&](unsigned long long key, int from, int step) {  // pairs of keys from, from + step, ...; the last one may stand alone
     int place = 0;
 #pragma unroll 4
-    for (int k = from; k < total; k += step) place += all[k] > key;
-    return place;
+    for (int k = 2 * from; k < total - 1; k += 2 * step) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(all + k);
+      place += two.x > key;
+      place += two.y > key;
+    }
+    return place + ((total & 1) && from == 0 && all[total - 1] > key);
   };
   __shared__ int s_place[LP_THREADS / 2];
   if (total <= LP_THREADS / 2) {
     const int lanes = (total + 31) & ~31, parts = LP_THREADS / lanes, i = tid % lanes;
     if (tid < lanes) s_place[i] = 0;
     __syncthreads();
-    if (i < total && tid < parts * lanes) atomicAdd(&s_place[i], larger(all[i], tid / lanes, parts));
+    if (i < total && tid < parts * lanes) {
+      const int place = larger(all[i], tid / lanes, parts);
+      if (place) atomicAdd(&s_place[i], place);
+    }
     __syncthreads();
     if (tid < total) put(all[tid], s_place[tid]);
   } else {
@@ -383,7 +399,7 @@ int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
   a.S = 1;
   while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
   a.per = (packets + a.S - 1) / a.S;
-  a.cap = TOP ? 3 * a.top + 64 : 0;
+  a.cap = TOP ? 3 * a.top + 64 + (a.top & 1) : 0;
   // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
   // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
   const int groups = a.S * LP_WARPS;
