@@ -132,12 +132,12 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (const uint32_t bits = b[u * DI_THREADS]) distill_mask(w[u], bits, T());
-    ag_stat_add<false, T>(v, w, c);
+    ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
   }
   for (; left > 0; left -= DI_THREADS, p += DI_THREADS, b += DI_THREADS) {
     uint4 w[1] = {*p};
     distill_mask(w[0], *b, T());
-    ag_stat_add<false, T>(v, w, c);
+    ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
   }
   return v;
 }

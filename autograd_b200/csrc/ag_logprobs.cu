@@ -33,9 +33,21 @@ struct LpArgs {
   int* status;
 };
 
-// the exchange, packets with a logit that passes, a barrier, a block's keys, those of all blocks at block 0, where the packets are
-// from, counters
-size_t lp_smem(int S, int cap) { return AgExchange::bytes(S) + (size_t)cap * (16 + 8 * (S == 1 ? 1 : 1 + S) + 4) + 64; }
+constexpr int LP_BATCH = 4;  // packets
+// whole batches of a thread before which (and at which) `left` packets of the block lie, and packets behind them
+__host__ __device__ constexpr int lp_whole(int left) {
+  return left > (LP_BATCH - 1) * LP_THREADS ? (left - (LP_BATCH - 1) * LP_THREADS - 1) / (LP_BATCH * LP_THREADS) + 1 : 0;
+}
+__host__ __device__ constexpr int lp_rest(int left) {
+  return left > lp_whole(left) * LP_BATCH * LP_THREADS ? (left - lp_whole(left) * LP_BATCH * LP_THREADS - 1) / LP_THREADS + 1 : 0;
+}
+
+// the exchange, a barrier, a block's keys, those of all blocks at block 0, batches with a logit that passes, counters, the batches'
+// largest logits
+size_t lp_smem(int S, int cap, int per) {
+  return AgExchange::bytes(S) + 16 + (size_t)cap * (8 * (S == 1 ? 1 : 1 + S) + 8) + 48 +
+         (cap ? (size_t)(lp_whole(per) + LP_BATCH - 1) * LP_THREADS * 4 : 0);
+}
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
@@ -170,23 +182,25 @@ __device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top,
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, TOP ? 5 : 6)
+__global__ void __launch_bounds__(LP_THREADS, 6)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * LP_WARPS;
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
   const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
-  uint4* packets = reinterpret_cast<uint4*>(s_bars + 2);                               // [cap]
-  uint64_t* s_keys_bar = reinterpret_cast<uint64_t*>(packets + a.cap);                 // every block's keys are at block 0
+  uint64_t* s_keys_bar = s_bars + 2;                                                   // every block's keys are at block 0
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], cap even
   unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
-  int* places = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);           // [cap]
-  int* counts = places + a.cap;                                                        // [8]
-  int* n_keys = counts + 8;                                                            // keys, packets, a counter
+  int* batches = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);          // [cap]
+  float* list_most = reinterpret_cast<float*>(batches + a.cap);                        // [cap]
+  int* counts = reinterpret_cast<int*>(list_most + a.cap);                             // [8]
+  int* n_keys = counts + 8;                                                            // keys, batches, a counter, a bound
+  uint32_t* s_bound = reinterpret_cast<uint32_t*>(n_keys + 3);
+  float* most = reinterpret_cast<float*>(n_keys + 4);                                  // [batches and packets of a thread][threads]
   const float c = a.inv_tau * AG_LOG2E;
   if (TOP && tid == 0) {
-    n_keys[0] = n_keys[1] = 0;
+    n_keys[0] = n_keys[1] = n_keys[3] = 0;
     ag_mbar_init(s_keys_bar, S);
     ag_fence_mbar_init();
   }
@@ -201,7 +215,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   const int n = r.mine(rank, a.per), first = r.head + rank * a.per * AG_PACKET<T>;
   const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
   const int id = tid == 0 && rank == 0 && a.logprob ? a.ids[row] : -1;
-  const AgStat own = ag_part_stat<true, T, 4>(at, n, edge, c);
+  const AgStat own = ag_part_stat<true, T, LP_BATCH>(at, n, edge, c, TOP ? most + tid - LP_THREADS : nullptr);
   const bool has = id >= 0 && id < a.V;
   const float x_id = has ? Pack<T>::load1(r.x + id) : 0.0f;  // not before: the warp's packets would wait for the id
   AgStat v = ag_stat_warp(own, c);
@@ -229,29 +243,49 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     if (a.stats) a.stats[row] = make_float4(v.m, L, H, 0.0f);
   }
   if (!TOP) return;
-  const float bound = lp_bound(told, groups, a.need);
+  float bound = lp_bound(told, groups, a.need);
+  const bool nan = L != L;  // NaN may lie in any batch, whatever its largest number is
   const LpPart<T> part = {at, n, first, edge, edge_index};
-  // Packets with something in them go on a list first, and are taken apart by all threads: with a logit in every third packet
-  // that a warp looks at, taking it apart on the spot has the other lanes wait (64 alternatives of 32768 bf16: half of all
-  // instructions).
+  // Batches with something in them go on a list, whose packets all threads then fetch from L2 and take apart.
   if (own.m >= bound || own.s != own.s) {
-    if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
-#pragma unroll 2
-    for (int i = tid; i < n; i += LP_THREADS) {
-      const uint4 w[1] = {at[i]};
-      if (ag_largest(w, T()) < bound && own.s == own.s) continue;  // nothing here, and NaN nowhere
+    const int entries = lp_whole(n - tid) + lp_rest(n - tid);
+    for (int b = 0; b < entries; ++b) {
+      const float m = most[b * LP_THREADS + tid];
+      if (m < bound && own.s == own.s) continue;
       const int k = atomicAdd(n_keys + 1, 1);
-      if (k < a.cap) packets[k] = w[0], places[k] = first + i * AG_PACKET<T>;
+      if (k < a.cap) batches[k] = b * LP_THREADS + tid, list_most[k] = m;
     }
   }
   __syncthreads();
   const int listed = min(n_keys[1], a.cap);
-  for (int k = tid; k < listed * AG_PACKET<T>; k += LP_THREADS) {
-    const int e = k % AG_PACKET<T>;
-    const float x = Pack<T>::load1(reinterpret_cast<const T*>(packets) + k);
-    if (x < bound) continue;
-    const int to = atomicAdd(n_keys, 1);
-    if (to < a.cap) keys[to] = lp_key(x, places[k / AG_PACKET<T>] + e);
+  // With `top` batches and more, the top-th largest of their maxima is a bound that hardly more than `top` logits reach; what it
+  // leaves out need not be fetched, or counted against all others.
+  if (listed > a.top && !nan) {
+    for (int k = tid; k < listed; k += LP_THREADS) {
+      const float m = list_most[k];
+      int place = 0;
+#pragma unroll 4
+      for (int g = 0; g < listed; ++g) place += list_most[g] > m;
+      if (place < a.top) atomicMax(s_bound, ag_order(m) ^ 0xffffffffu);
+    }
+    __syncthreads();
+    bound = fmaxf(bound, ag_of_order(*s_bound ^ 0xffffffffu));
+  }
+  if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
+  for (int k = tid; k < listed * LP_BATCH; k += LP_THREADS) {
+    if (list_most[k / LP_BATCH] < bound && !nan) continue;
+    const int b = batches[k / LP_BATCH] / LP_THREADS, of = batches[k / LP_BATCH] % LP_THREADS, whole = lp_whole(n - of);
+    if (b >= whole && k % LP_BATCH) continue;  // a packet by itself
+    const int i = (b < whole ? b * LP_BATCH + k % LP_BATCH : whole * LP_BATCH + b - whole) * LP_THREADS + of;
+    float x[AG_PACKET<T>];
+    ag_widen(at[i], x);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int e = 0; e < AG_PACKET<T>; ++e) hits |= x[e] < bound ? 0u : 1u << e;
+    for (; hits; hits &= hits - 1) {
+      const int index = first + i * AG_PACKET<T> + __ffs(hits) - 1, to = atomicAdd(n_keys, 1);
+      if (to < a.cap) keys[to] = lp_key(Pack<T>::load1(r.x + index), index);
+    }
   }
   __syncthreads();
   int total = n_keys[0];
@@ -408,7 +442,15 @@ int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
   a.need = TOP ? (a.top + a.J - 1) / a.J : 0;
   a.status = ctx->d_status;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_token_logprobs_forward: too many rows");
-  return ag_launch_clusters(ctx, "logprobs_kernel", logprobs_kernel<T, TOP>, a.S, lp_smem(a.S, a.cap), a.N, (const T*)logits, a);
+  const size_t smem = lp_smem(a.S, a.cap, a.per);
+  if (smem > 47 * 1024) {
+    static std::atomic<bool> ready[AG_MAX_DEVICES];
+    if (!ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
+      AG_CUDA(ctx, cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+      ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
+    }
+  }
+  return ag_launch_clusters(ctx, "logprobs_kernel", logprobs_kernel<T, TOP>, a.S, smem, a.N, (const T*)logits, a);
 }
 
 }  // namespace

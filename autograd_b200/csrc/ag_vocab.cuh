@@ -163,11 +163,12 @@ __device__ __forceinline__ float ag_largest(const uint4 (&w)[U], __nv_bfloat16) 
   return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
 }
 
-// U packets onto v; t only if it is wanted.  A batch costs one more exponential, for what is there already.
+// U packets, the largest of which is `most`, onto v; t only if it is wanted.  A batch costs one more exponential, for what is there
+// already.
 template <bool WITH_T, typename T, int U>
-__device__ __forceinline__ void ag_stat_add(AgStat& v, const uint4 (&w)[U], float c) {
+__device__ __forceinline__ void ag_stat_add(AgStat& v, const uint4 (&w)[U], float most, float c) {
   constexpr int NV = AG_PACKET<T>;
-  const float m = fmaxf(v.m, ag_largest(w, T()));
+  const float m = fmaxf(v.m, most);
   ag_stat_scale(v, m, c);
   const float ref = m == -INFINITY ? 0.0f : -m;
   const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c);
@@ -242,10 +243,11 @@ struct AgRow {
   }
 };
 
-// Statistics of this thread's part of n packets (in shared or global memory), U at a time, and of its element of the edges (-inf
-// without one).
+// Statistics of this thread's part of n packets, U at a time, and of its element of the edges (-inf without one).  `most` (null: not
+// wanted): the largest logit of each batch, and of each packet that is left behind the last whole batch, this thread's
+// AG_ROW_THREADS apart, the first one that far behind `most`.
 template <bool WITH_T, typename T, int U>
-__device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c) {
+__device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c, float* most = nullptr) {
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
   const uint4* p = at + threadIdx.x;
   int left = n - (int)threadIdx.x;
@@ -253,11 +255,15 @@ __device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edg
     uint4 w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = p[u * AG_ROW_THREADS];
-    ag_stat_add<WITH_T, T>(v, w, c);
+    const float m = ag_largest(w, T());
+    if (most) *(most += AG_ROW_THREADS) = m;
+    ag_stat_add<WITH_T, T>(v, w, m, c);
   }
   for (; left > 0; left -= AG_ROW_THREADS, p += AG_ROW_THREADS) {
     const uint4 w[1] = {*p};
-    ag_stat_add<WITH_T, T>(v, w, c);
+    const float m = ag_largest(w, T());
+    if (most) *(most += AG_ROW_THREADS) = m;
+    ag_stat_add<WITH_T, T>(v, w, m, c);
   }
   return v;
 }
