@@ -144,7 +144,7 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
 
 // exchange, parts of the list, slots' tokens and masses, loss per warp, bits of the edges, bits of the packets
 size_t distill_smem(int S, int per, bool map) {
-  return AgExchange::bytes(S) + DI_WARPS * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + DI_WARPS * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
+  return AgExchange<>::bytes(S) + DI_WARPS * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + DI_WARPS * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
 }
 
 template <typename T, bool TRAIN, bool REST>
@@ -155,7 +155,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * DI_WARPS, parts = (a.top + 31) / 32;
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
-  const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
+  const AgExchange<> exchange = {s_box, s_bars, S, rank, a.status};
   DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);
   int* s_ids = reinterpret_cast<int*>(s_parts + DI_WARPS);
   float* s_q = reinterpret_cast<float*>(s_ids + AG_DISTILL_MAX);
@@ -440,7 +440,7 @@ int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs 
                                       (int)distill_smem(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
     ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
   }
-  return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST>, a.S, smem, a.N, (const T*)logits, (T*)dlogits, a);
+  return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST>, a.S, DI_THREADS, smem, a.N, (const T*)logits, (T*)dlogits, a);
 }
 
 template <typename T>

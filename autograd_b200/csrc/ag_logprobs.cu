@@ -4,20 +4,22 @@
 //   entropy H = L - sum_j p_j (x_j - m) / temperature
 //   d logits_j = (a (delta_j,id - p_j) - b p_j (log p_j + H)) / temperature,  a = dlogprob (0 without a token), b = dentropy
 //
-// Forward: a block, or for few rows a cluster of 2 to 8, streams a row through registers.  The alternatives come from a second look
-// at the row, which L2 still holds:
-//   each warp tells, along with its statistics, its J-th largest lane maximum; the (top / J)-th largest of these is a bound that at
-//   least `top` logits reach, and up to twice as many do, since the lanes' logits lie spread over the row;
-//   the logits that reach it are collected, (order, index) as one key each, by the threads whose maximum does;
-//   one block of the cluster counts for each how many are larger, which is its place.
-// A block that collects more than `cap` (many equal logits, or the largest ones all in a few lanes) searches a bound of its own,
-// bit by bit, and takes logits that equal it in the order of their index.
+// Forward: a block, or for few rows a cluster of 2 to 8, streams a row through registers.  For the alternatives it notes the largest
+// logit of every batch of packets that a thread reads at a time:
+//   a block with a row to itself takes the top-th largest of these (or a little less: lp_threshold) as a bound, which `top` logits
+//   at least reach, and hardly more do;
+//   the blocks of a cluster, which would find a bound each, tell one another their warps' J-th largest lane maxima instead, and take
+//   the (top / J)-th largest of these, which up to twice as many reach (8 rows of 151936 bf16, 20 alternatives: 10.4 / 7.7 us);
+//   the batches that reach it, still in L2, are fetched again and their logits that do collected, (order, index) as one key each;
+//   the first block of the cluster counts for each how many are larger, which is its place.
+// A block that collects more than `cap` (many equal logits, many in one batch) searches a bound among the logits themselves, bit by
+// bit, and takes those that equal it in the order of their index.
 #include "ag_vocab.cuh"
 
 namespace {
 
-constexpr int LP_THREADS = AG_ROW_THREADS, LP_WARPS = LP_THREADS / 32;
-static_assert(3 * AG_TOP_MAX + 64 + 1 <= 2 * LP_THREADS, "two keys per thread are moved");
+constexpr int LP_THREADS = AG_ROW_THREADS, LP_FEW = 128;  // threads of a block
+constexpr int LP_FEW_PACKETS = 8191;
 
 struct LpArgs {
   const int32_t* ids;
@@ -35,34 +37,78 @@ struct LpArgs {
 
 constexpr int LP_BATCH = 4;  // packets
 // whole batches of a thread before which (and at which) `left` packets of the block lie, and packets behind them
+template <int TH>
 __host__ __device__ constexpr int lp_whole(int left) {
-  return left > (LP_BATCH - 1) * LP_THREADS ? (left - (LP_BATCH - 1) * LP_THREADS - 1) / (LP_BATCH * LP_THREADS) + 1 : 0;
+  return left > (LP_BATCH - 1) * TH ? (left - (LP_BATCH - 1) * TH - 1) / (LP_BATCH * TH) + 1 : 0;
 }
+template <int TH>
 __host__ __device__ constexpr int lp_rest(int left) {
-  return left > lp_whole(left) * LP_BATCH * LP_THREADS ? (left - lp_whole(left) * LP_BATCH * LP_THREADS - 1) / LP_THREADS + 1 : 0;
+  return left > lp_whole<TH>(left) * LP_BATCH * TH ? (left - lp_whole<TH>(left) * LP_BATCH * TH - 1) / TH + 1 : 0;
 }
 
-// the exchange, a barrier, a block's keys, those of all blocks at block 0, batches with a logit that passes, counters, the batches'
-// largest logits
+// the exchange, a barrier, a block's keys, those of all blocks at block 0, batches with a logit that passes, counters, a histogram,
+// the batches' largest logits
+template <int TH>
 size_t lp_smem(int S, int cap, int per) {
-  return AgExchange::bytes(S) + 16 + (size_t)cap * (8 * (S == 1 ? 1 : 1 + S) + 8) + 48 +
-         (cap ? (size_t)(lp_whole(per) + LP_BATCH - 1) * LP_THREADS * 4 : 0);
+  return AgExchange<TH>::bytes(S) + 16 + (size_t)cap * (8 * (S == 1 ? 1 : 1 + S) + 4) + 48 +
+         (cap ? 1024 + (size_t)(lp_whole<TH>(per) + LP_BATCH - 1) * TH * 4 : 0);
 }
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
-// The need-th largest of the n <= 64 numbers box[].w, or one that an eighth more of them reach; by one warp.
-__device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
-  const int lane = threadIdx.x & 31;
-  if (n <= 16) {  // a lane each, which counts the larger ones: the bisection takes some 20 steps
-    const float mine = lane < n ? box[lane].w : -INFINITY;
-    int place = 0;
-    for (int g = 0; g < n; ++g) {
-      const float w = box[g].w;
-      place += w > mine || (w == mine && g < lane);
+// An order that at least `need` of the block's values reach and, unless many are equal, `enough` at most; 0 if there are fewer than
+// `need` from lo on.  each(f) calls f(order) for this thread's values; lo <= the need-th largest if it exists, hi >= all.  hist: 256
+// zeros, which it does not leave.  A histogram of the range finds the 256th of it where the need-th lies, until that is narrow
+// enough; from the smallest of the lanes' largest logits on the first one usually is.  By all threads of the block.
+template <int TH, typename F>
+__device__ __forceinline__ uint32_t lp_threshold(F each, uint32_t lo, uint32_t hi, int need, int enough, uint32_t* hist) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (;;) {
+    const int shift = max(0, 24 - __clz(hi - lo));
+    each([&](uint32_t k) {
+      if (k >= lo && k <= hi) atomicAdd(hist + ((k - lo) >> shift), 1u);
+    });
+    __syncthreads();
+    // every warp: bins 8 * lane .. 8 * lane + 7, and how many values lie in those of the lanes above
+    uint32_t bin[8];
+    *reinterpret_cast<uint4*>(bin) = *reinterpret_cast<const uint4*>(hist + 8 * lane);
+    *reinterpret_cast<uint4*>(bin + 4) = *reinterpret_cast<const uint4*>(hist + 8 * lane + 4);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine += bin[i];
+    int upto = mine;  // of this lane and those above
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_down_sync(0xffffffffu, upto, o);
+      if (lane + o < 32) upto += w;
     }
-    return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, lane < n && place == need - 1)) - 1);
+    const uint32_t who = __ballot_sync(0xffffffffu, upto >= need);
+    if (!who) return 0;  // too few values
+    int above = upto - mine, at = 0, reach = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      if (!found && above + (int)bin[i] >= need) found = true, at = 8 * lane + i, reach = above + bin[i];
+      if (!found) above += bin[i];
+    }
+    const int from = 31 - __clz(who);  // the highest lane that gets there
+    at = __shfl_sync(0xffffffffu, at, from);
+    above = __shfl_sync(0xffffffffu, above, from);
+    reach = __shfl_sync(0xffffffffu, reach, from);
+    lo += (uint32_t)at << shift;
+    if (reach <= enough || shift == 0) return lo;
+    need -= above;
+    enough -= above;
+    hi = min(hi, lo + (1u << shift) - 1);
+    __syncthreads();
+    for (int b = tid; b < 256; b += TH) hist[b] = 0;
+    __syncthreads();
   }
+}
+
+// The order of the need-th largest of the n <= 64 numbers box[].w, or of one that an eighth more of them reach; by one warp.
+__device__ __forceinline__ uint32_t lp_bound(const float4* box, int n, int need) {
+  const int lane = threadIdx.x & 31;
   const bool one = lane < n, two = lane + 32 < n;
   const uint32_t a = one ? ag_order(box[lane].w) : 0u, b = two ? ag_order(box[lane + 32].w) : 0u;
   uint32_t lo = __reduce_min_sync(0xffffffffu, min(one ? a : 0xffffffffu, two ? b : 0xffffffffu));
@@ -78,10 +124,10 @@ __device__ __forceinline__ float lp_bound(const float4* box, int n, int need) {
       hi = mid - 1;
     }
   }
-  return ag_of_order(lo);
+  return lo;
 }
 
-template <typename T>
+template <typename T, int TH>
 struct LpPart {
   const uint4* at;
   int n, first;  // packets, index of the first one's first logit
@@ -92,7 +138,7 @@ struct LpPart {
   __device__ __forceinline__ void each(F f) const {
     constexpr int NV = AG_PACKET<T>;
     if (edge_index >= 0) f(edge, edge_index);
-    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+    for (int i = threadIdx.x; i < n; i += TH) {
       float x[NV];
       ag_widen(at[i], x);
 #pragma unroll
@@ -103,8 +149,8 @@ struct LpPart {
 
 // The block's logits whose order is `bound` or more are more than `cap`: leaves the keys of its `top` largest at least, `cap` at
 // most, in `keys` and returns how many.  By all threads of the block.  A block that has this many has more than `top` logits.
-template <typename T>
-__device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
+template <typename T, int TH>
+__device__ __noinline__ int lp_search(const LpPart<T, TH>& sl, uint32_t lo, int top, int cap, unsigned long long* keys, int* s_count) {
   uint32_t hi = 0xffffffffu;
   auto count_from = [&](uint32_t k) {
     int c = 0;
@@ -137,13 +183,13 @@ __device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top,
   if (fits) return have;
   // in the order of the index: the elements before the first packet, then packets by rounds of the block, then those behind
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __shared__ int s_warp[LP_WARPS];
+  __shared__ int s_warp[(TH / 32)];
   constexpr int NV = AG_PACKET<T>;
-  const int rounds = (sl.n + LP_THREADS - 1) / LP_THREADS;
+  const int rounds = (sl.n + TH - 1) / TH;
   for (int r = -1; r <= rounds && have < top; ++r) {
     float x[NV];
     int mine = 0, first = 0;
-    const int i = r * LP_THREADS + threadIdx.x;
+    const int i = r * TH + threadIdx.x;
     if (r < 0 || r == rounds) {
       const bool head = sl.edge_index >= 0 && threadIdx.x < 16;
       mine = sl.edge_index >= 0 && head == (r < 0) && ag_order(sl.edge) == lo;
@@ -162,7 +208,7 @@ __device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top,
     if (lane == 31) s_warp[warp] = before;
     __syncthreads();
     int at = have + before - mine, all = 0;
-    for (int w = 0; w < LP_WARPS; ++w) {
+    for (int w = 0; w < (TH / 32); ++w) {
       if (w < warp) at += s_warp[w];
       all += s_warp[w];
     }
@@ -181,26 +227,26 @@ __device__ __noinline__ int lp_search(const LpPart<T>& sl, uint32_t lo, int top,
   return have;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 6)
+template <typename T, bool TOP, int TH, bool MANY>
+__global__ void __launch_bounds__(TH, (TOP && sizeof(T) == 4 ? 5 : 6) * 256 / TH)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ float4 s_box[];
-  const int S = a.S, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
-  const int groups = S * LP_WARPS;
+  const int S = MANY || !TOP ? a.S : 1, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
+  const int groups = S * (TH / 32);
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
-  const AgExchange exchange = {s_box, s_bars, S, rank, a.status};
+  const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
   uint64_t* s_keys_bar = s_bars + 2;                                                   // every block's keys are at block 0
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], cap even
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], a multiple of four
   unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
   int* batches = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);          // [cap]
-  float* list_most = reinterpret_cast<float*>(batches + a.cap);                        // [cap]
-  int* counts = reinterpret_cast<int*>(list_most + a.cap);                             // [8]
-  int* n_keys = counts + 8;                                                            // keys, batches, a counter, a bound
-  uint32_t* s_bound = reinterpret_cast<uint32_t*>(n_keys + 3);
-  float* most = reinterpret_cast<float*>(n_keys + 4);                                  // [batches and packets of a thread][threads]
+  int* counts = batches + a.cap;                                                       // [8]
+  int* n_keys = counts + 8;                                                            // keys, batches, a counter
+  uint32_t* hist = reinterpret_cast<uint32_t*>(n_keys + 4);                            // [256]
+  float* most = reinterpret_cast<float*>(hist + 256);                                  // [batches and packets of a thread][threads]
   const float c = a.inv_tau * AG_LOG2E;
+  for (int b = tid; TOP && !MANY && b < 256; b += TH) hist[b] = 0;
   if (TOP && tid == 0) {
-    n_keys[0] = n_keys[1] = n_keys[3] = 0;
+    n_keys[0] = n_keys[1] = 0;
     ag_mbar_init(s_keys_bar, S);
     ag_fence_mbar_init();
   }
@@ -215,18 +261,20 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   const int n = r.mine(rank, a.per), first = r.head + rank * a.per * AG_PACKET<T>;
   const uint4* at = reinterpret_cast<const uint4*>(r.x + first);
   const int id = tid == 0 && rank == 0 && a.logprob ? a.ids[row] : -1;
-  const AgStat own = ag_part_stat<true, T, LP_BATCH>(at, n, edge, c, TOP ? most + tid - LP_THREADS : nullptr);
+  const AgStat own = ag_part_stat<true, T, LP_BATCH, TH>(at, n, edge, c, TOP ? most + tid - TH : nullptr);
   const bool has = id >= 0 && id < a.V;
   const float x_id = has ? Pack<T>::load1(r.x + id) : 0.0f;  // not before: the warp's packets would wait for the id
   AgStat v = ag_stat_warp(own, c);
   float reached = v.m;
-  if (TOP) {
+  if (TOP && MANY) {  // the J-th largest of the lanes' maxima
     float left = own.m;
     for (int j = 1; j < a.J; ++j) {
       const uint32_t who = __ballot_sync(0xffffffffu, left == reached);
       if (lane == __ffs(who) - 1) left = -INFINITY;
       asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(left));
     }
+  } else if (TOP) {  // the smallest
+    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(own.m));
   }
   const float4 word = make_float4(v.m, v.s, v.t, reached);
   const float4* told = TOP ? exchange.tell(0, word) : exchange.tell_first(word);
@@ -243,40 +291,31 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     if (a.stats) a.stats[row] = make_float4(v.m, L, H, 0.0f);
   }
   if (!TOP) return;
-  float bound = lp_bound(told, groups, a.need);
-  const bool nan = L != L;  // NaN may lie in any batch, whatever its largest number is
-  const LpPart<T> part = {at, n, first, edge, edge_index};
-  // Batches with something in them go on a list, whose packets all threads then fetch from L2 and take apart.
-  if (own.m >= bound || own.s != own.s) {
-    const int entries = lp_whole(n - tid) + lp_rest(n - tid);
-    for (int b = 0; b < entries; ++b) {
-      const float m = most[b * LP_THREADS + tid];
-      if (m < bound && own.s == own.s) continue;
-      const int k = atomicAdd(n_keys + 1, 1);
-      if (k < a.cap) batches[k] = b * LP_THREADS + tid, list_most[k] = m;
-    }
+  const int entries = lp_whole<TH>(n - tid) + lp_rest<TH>(n - tid);
+  uint32_t least = 0;  // the order of a NaN, which nothing is below
+  if (MANY) {
+    if (L == L) least = lp_bound(told, groups, a.need);
+  } else if (L == L) {  // with NaN or +inf in the row the batches' largest logits say little
+    reached = lane < groups ? told[lane].w : INFINITY;
+    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(reached));
+    auto each = [&](auto f) {
+      for (int b = 0; b < entries; ++b) f(ag_order(most[b * TH + tid]));
+    };
+    least = lp_threshold<TH>(each, ag_order(reached), ag_order(v.m), a.top, a.top + (a.top >> 1) + 16, hist);
+  }
+  const float bound = ag_of_order(least);
+  for (int b = 0; b < entries; ++b) {
+    if (most[b * TH + tid] < bound) continue;
+    const int k = atomicAdd(n_keys + 1, 1);
+    if (k < a.cap) batches[k] = b * TH + tid;
   }
   __syncthreads();
   const int listed = min(n_keys[1], a.cap);
-  // With `top` batches and more, the top-th largest of their maxima is a bound that hardly more than `top` logits reach; what it
-  // leaves out need not be fetched, or counted against all others.
-  if (listed > a.top && !nan) {
-    for (int k = tid; k < listed; k += LP_THREADS) {
-      const float m = list_most[k];
-      int place = 0;
-#pragma unroll 4
-      for (int g = 0; g < listed; ++g) place += list_most[g] > m;
-      if (place < a.top) atomicMax(s_bound, ag_order(m) ^ 0xffffffffu);
-    }
-    __syncthreads();
-    bound = fmaxf(bound, ag_of_order(*s_bound ^ 0xffffffffu));
-  }
   if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
-  for (int k = tid; k < listed * LP_BATCH; k += LP_THREADS) {
-    if (list_most[k / LP_BATCH] < bound && !nan) continue;
-    const int b = batches[k / LP_BATCH] / LP_THREADS, of = batches[k / LP_BATCH] % LP_THREADS, whole = lp_whole(n - of);
+  for (int k = tid; k < listed * LP_BATCH; k += TH) {
+    const int b = batches[k / LP_BATCH] / TH, of = batches[k / LP_BATCH] % TH, whole = lp_whole<TH>(n - of);
     if (b >= whole && k % LP_BATCH) continue;  // a packet by itself
-    const int i = (b < whole ? b * LP_BATCH + k % LP_BATCH : whole * LP_BATCH + b - whole) * LP_THREADS + of;
+    const int i = (b < whole ? b * LP_BATCH + k % LP_BATCH : whole * LP_BATCH + b - whole) * TH + of;
     float x[AG_PACKET<T>];
     ag_widen(at[i], x);
     uint32_t hits = 0;
@@ -289,26 +328,30 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   }
   __syncthreads();
   int total = n_keys[0];
-  if (total > a.cap || n_keys[1] > a.cap) total = lp_search<T>(part, ag_order(bound), a.top, a.cap, keys, n_keys + 2);
-  if (S > 1) {
+  if (total > a.cap || n_keys[1] > a.cap) {
+    const LpPart<T, TH> part = {at, n, first, edge, edge_index};
+    total = lp_search<T, TH>(part, least, a.top, a.cap, keys, n_keys + 2);
+  }
+  if (MANY) {
     // to block 0, each to its own place there
     const uint32_t to = ag_peer(all + (size_t)rank * a.cap, 0);
-    for (int k = tid; k < total; k += LP_THREADS) ag_peer_store(to + k * 8, keys[k]);
+    for (int k = tid; k < total; k += TH) ag_peer_store(to + k * 8, keys[k]);
     if (tid == 0) ag_peer_store(ag_peer(counts + rank, 0), total);
     __syncthreads();
     if (tid == 0) ag_peer_arrive(ag_peer(s_keys_bar, 0));
     if (rank) return;
     ag_wait_cluster(s_keys_bar, 0, a.status);
     // side by side
+    constexpr int MOVE = (3 * AG_TOP_MAX + 64 + TH - 1) / TH;  // keys of a block per thread, at most
     total = counts[0];
     for (int p = 1; p < S; ++p) {
       const int more = counts[p];
-      unsigned long long mine[2];  // cap <= 2 * LP_THREADS, and what is moved down may lie over what is not yet
-      for (int k = 0; k < 2; ++k)
-        if (tid + k * LP_THREADS < more) mine[k] = all[(size_t)p * a.cap + tid + k * LP_THREADS];
+      unsigned long long mine[MOVE];  // what is moved down may lie over what is not yet
+      for (int k = 0; k < MOVE; ++k)
+        if (tid + k * TH < more) mine[k] = all[(size_t)p * a.cap + tid + k * TH];
       __syncthreads();
-      for (int k = 0; k < 2; ++k)
-        if (tid + k * LP_THREADS < more) all[total + tid + k * LP_THREADS] = mine[k];
+      for (int k = 0; k < MOVE; ++k)
+        if (tid + k * TH < more) all[total + tid + k * TH] = mine[k];
       total += more;
     }
     __syncthreads();
@@ -330,9 +373,9 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     }
     return place + ((total & 1) && from == 0 && all[total - 1] > key);
   };
-  __shared__ int s_place[LP_THREADS / 2];
-  if (total <= LP_THREADS / 2) {
-    const int lanes = (total + 31) & ~31, parts = LP_THREADS / lanes, i = tid % lanes;
+  __shared__ int s_place[TH / 2];
+  if (total <= TH / 2) {
+    const int lanes = (total + 31) & ~31, parts = TH / lanes, i = tid % lanes;
     if (tid < lanes) s_place[i] = 0;
     __syncthreads();
     if (i < total && tid < parts * lanes) {
@@ -342,7 +385,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     __syncthreads();
     if (tid < total) put(all[tid], s_place[tid]);
   } else {
-    for (int i = tid; i < total; i += LP_THREADS) put(all[i], larger(all[i], 0, 1));
+    for (int i = tid; i < total; i += TH) put(all[i], larger(all[i], 0, 1));
   }
 }
 
@@ -427,30 +470,41 @@ int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* d
   return AG_OK;
 }
 
-template <typename T, bool TOP>
-int logprobs(ag_ctx* ctx, const void* logits, LpArgs a) {
+template <typename T, bool TOP, int TH, bool MANY>
+int logprobs_launch(ag_ctx* ctx, const T* logits, const LpArgs& a) {
+  const size_t smem = lp_smem<TH>(a.S, a.cap, a.per);
+  static std::atomic<bool> ready[AG_MAX_DEVICES];
+  if (smem > 47 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
+    AG_CUDA(ctx, cudaFuncSetAttribute(logprobs_kernel<T, TOP, TH, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
+  }
+  return ag_launch_clusters(ctx, "logprobs_kernel", logprobs_kernel<T, TOP, TH, MANY>, a.S, TH, smem, a.N, logits, a);
+}
+
+template <typename T>
+int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
+  const T* logits = static_cast<const T*>(x);
   const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
   a.S = 1;
   while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
   a.per = (packets + a.S - 1) / a.S;
-  a.cap = TOP ? 3 * a.top + 64 + (a.top & 1) : 0;
-  // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
-  // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
-  const int groups = a.S * LP_WARPS;
-  a.J = (a.top + groups - 1) / groups;
-  while (TOP && a.J < 32 && (a.top + a.J - 1) / a.J * 20 > groups * 17) ++a.J;
-  a.need = TOP ? (a.top + a.J - 1) / a.J : 0;
   a.status = ctx->d_status;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_token_logprobs_forward: too many rows");
-  const size_t smem = lp_smem(a.S, a.cap, a.per);
-  if (smem > 47 * 1024) {
-    static std::atomic<bool> ready[AG_MAX_DEVICES];
-    if (!ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
-      AG_CUDA(ctx, cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-      ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
-    }
+  if (a.top == 0) return logprobs_launch<T, false, LP_THREADS, true>(ctx, logits, a);
+  a.cap = (3 * a.top + 64 + 3) & ~3;  // a multiple of four: what follows in shared memory is read 16 bytes at a time
+  if (a.S > 1) {
+    // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
+    // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
+    const int groups = a.S * (LP_THREADS / 32);
+    a.J = (a.top + groups - 1) / groups;
+    while (a.J < 32 && (a.top + a.J - 1) / a.J * 20 > groups * 17) ++a.J;
+    a.need = (a.top + a.J - 1) / a.J;
+    return logprobs_launch<T, true, LP_THREADS, true>(ctx, logits, a);
   }
-  return ag_launch_clusters(ctx, "logprobs_kernel", logprobs_kernel<T, TOP>, a.S, smem, a.N, (const T*)logits, a);
+  // Short rows: what each warp does once per row weighs more than what more threads read at a time.  128 / 256 threads, us:
+  // 8192 x 32768 bf16, 64 alternatives 128 / 146, fp32 207 / 200; 2048 x 151936 bf16, 20 alternatives 145 / 128.
+  if (packets <= LP_FEW_PACKETS) return logprobs_launch<T, true, LP_FEW, false>(ctx, logits, a);
+  return logprobs_launch<T, true, LP_THREADS, false>(ctx, logits, a);
 }
 
 }  // namespace
@@ -468,9 +522,7 @@ extern "C" int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
   const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0, nullptr};
-  if (dtype == AG_F32)
-    return top ? logprobs<float, true>(ctx, logits, a) : logprobs<float, false>(ctx, logits, a);
-  return top ? logprobs<__nv_bfloat16, true>(ctx, logits, a) : logprobs<__nv_bfloat16, false>(ctx, logits, a);
+  return dtype == AG_F32 ? logprobs<float>(ctx, logits, a) : logprobs<__nv_bfloat16>(ctx, logits, a);
 }
 
 extern "C" int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, const int32_t* ids, const float* stats,

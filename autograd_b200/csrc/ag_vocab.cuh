@@ -8,7 +8,7 @@
 
 #include "ag_common.cuh"
 
-constexpr int AG_ROW_THREADS = 256, AG_ROW_WARPS = AG_ROW_THREADS / 32;  // of a block
+constexpr int AG_ROW_THREADS = 256;  // of a block, where it is not said otherwise
 constexpr float AG_LN2 = 0.69314718055994531f, AG_LOG2E = 1.44269504088896341f;
 
 // Launches go to the context's device, whichever is current in the calling thread.
@@ -245,24 +245,24 @@ struct AgRow {
 
 // Statistics of this thread's part of n packets, U at a time, and of its element of the edges (-inf without one).  `most` (null: not
 // wanted): the largest logit of each batch, and of each packet that is left behind the last whole batch, this thread's
-// AG_ROW_THREADS apart, the first one that far behind `most`.
-template <bool WITH_T, typename T, int U>
+// TH (the threads of the block) apart, the first one that far behind `most`.
+template <bool WITH_T, typename T, int U, int TH = AG_ROW_THREADS>
 __device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c, float* most = nullptr) {
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
   const uint4* p = at + threadIdx.x;
   int left = n - (int)threadIdx.x;
-  for (; left > (U - 1) * AG_ROW_THREADS; left -= U * AG_ROW_THREADS, p += U * AG_ROW_THREADS) {
+  for (; left > (U - 1) * TH; left -= U * TH, p += U * TH) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = p[u * AG_ROW_THREADS];
+    for (int u = 0; u < U; ++u) w[u] = p[u * TH];
     const float m = ag_largest(w, T());
-    if (most) *(most += AG_ROW_THREADS) = m;
+    if (most) *(most += TH) = m;
     ag_stat_add<WITH_T, T>(v, w, m, c);
   }
-  for (; left > 0; left -= AG_ROW_THREADS, p += AG_ROW_THREADS) {
+  for (; left > 0; left -= TH, p += TH) {
     const uint4 w[1] = {*p};
     const float m = ag_largest(w, T());
-    if (most) *(most += AG_ROW_THREADS) = m;
+    if (most) *(most += TH) = m;
     ag_stat_add<WITH_T, T>(v, w, m, c);
   }
   return v;
@@ -317,8 +317,9 @@ __device__ __forceinline__ void ag_wait_cluster(uint64_t* bar, uint32_t parity, 
 // What each warp of a cluster tells all others about its part of a row: one float4 per warp, in turn at two places.  A block can be
 // one row ahead of another, never two: for the row between it waits for what all warps of the other have to tell, and they tell it
 // when they have read what came before.
+template <int TH = AG_ROW_THREADS>
 struct AgExchange {
-  float4* box;      // [2][S * AG_ROW_WARPS]
+  float4* box;      // [2][S * warps of a block]
   uint64_t* bar;    // [2]
   int S, rank;
   int* status;
@@ -333,7 +334,7 @@ struct AgExchange {
   }
   // to block 0 only, whose warps all get the box; the others get null and have no more to do here
   __device__ __forceinline__ const float4* tell_first(float4 v) const {
-    const int lane = threadIdx.x & 31, at = rank * AG_ROW_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, at = rank * (TH / 32) + (threadIdx.x >> 5);
     if (S == 1) {
       if (lane == 0) box[at] = v;
       __syncthreads();
@@ -341,26 +342,26 @@ struct AgExchange {
     }
     if (lane == 0) ag_send(ag_peer(box + at, 0), v, ag_peer(bar, 0));
     if (rank) return nullptr;
-    if (threadIdx.x == 0) ag_mbar_expect_tx(bar, S * AG_ROW_WARPS * 16);
+    if (threadIdx.x == 0) ag_mbar_expect_tx(bar, S * (TH / 32) * 16);
     ag_wait_cluster(bar, 0, status);
     return box;
   }
   // by whole warps, every lane with the same v; the box is returned, in which all entries are then
   __device__ __forceinline__ const float4* tell(int turn, float4 v) const {
     const int now = turn & 1, lane = threadIdx.x & 31;
-    float4* all = box + now * S * AG_ROW_WARPS;
-    float4* to = all + rank * AG_ROW_WARPS + (threadIdx.x >> 5);
+    float4* all = box + now * S * (TH / 32);
+    float4* to = all + rank * (TH / 32) + (threadIdx.x >> 5);
     if (S == 1) {
       if (lane == 0) *to = v;
       __syncthreads();
     } else {
       if (lane < S) ag_send(ag_peer(to, lane), v, ag_peer(bar + now, lane));
-      if (threadIdx.x == 0) ag_mbar_expect_tx(bar + now, S * AG_ROW_WARPS * 16);
+      if (threadIdx.x == 0) ag_mbar_expect_tx(bar + now, S * (TH / 32) * 16);
       ag_wait_cluster(bar + now, (turn >> 1) & 1, status);
     }
     return all;
   }
-  static constexpr size_t bytes(int S) { return 2 * (size_t)S * AG_ROW_WARPS * 16 + 16; }
+  static constexpr size_t bytes(int S) { return 2 * (size_t)S * (TH / 32) * 16 + 16; }
 };
 
 __device__ __forceinline__ void ag_peer_store(uint32_t to, int v) {
@@ -397,10 +398,11 @@ static inline int ag_row_parts(const ag_ctx* ctx, int64_t N, int packets) {
 
 // Launch of n clusters of S blocks.
 template <typename... P, typename... A>
-static inline int ag_launch_clusters(ag_ctx* ctx, const char* name, void (*kern)(P...), int S, size_t smem, int64_t n, A... args) {
+static inline int ag_launch_clusters(ag_ctx* ctx, const char* name, void (*kern)(P...), int S, int threads, size_t smem, int64_t n,
+                                     A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = (unsigned)(n * S);
-  cfg.blockDim = AG_ROW_THREADS;
+  cfg.blockDim = threads;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[2];
