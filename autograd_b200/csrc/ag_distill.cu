@@ -18,8 +18,10 @@
 
 namespace {
 
-constexpr int DI_THREADS = AG_ROW_THREADS, DI_WARPS = DI_THREADS / 32, DI_BLOCKS = 4;
-static_assert(AG_DISTILL_MAX <= DI_THREADS, "a slot per thread");
+constexpr int DI_BLOCKS = 4;  // of 256 threads per SM
+constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;  // of a row, up to which a block has 64 or 128 threads
+constexpr int64_t DI_IN_FLIGHT = 48 << 20;
+static_assert(AG_DISTILL_MAX <= 256, "a slot per thread");
 
 struct DistillArgs {
   const int32_t* ids;
@@ -118,23 +120,23 @@ __device__ __forceinline__ void distill_mask(uint4& w, uint32_t bits, __nv_bfloa
 }
 
 // Statistics of the unlisted logits of this thread's part; as ag_part_stat.  map: a byte per packet.
-template <typename T>
+template <typename T, int TH>
 __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8_t* map, int n, float edge, float c) {
   constexpr int U = 4;
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};
   const uint4* p = at + threadIdx.x;
   const uint8_t* b = map + threadIdx.x;
   int left = n - (int)threadIdx.x;
-  for (; left > (U - 1) * DI_THREADS; left -= U * DI_THREADS, p += U * DI_THREADS, b += U * DI_THREADS) {
+  for (; left > (U - 1) * TH; left -= U * TH, p += U * TH, b += U * TH) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = p[u * DI_THREADS];
+    for (int u = 0; u < U; ++u) w[u] = p[u * TH];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (const uint32_t bits = b[u * DI_THREADS]) distill_mask(w[u], bits, T());
+      if (const uint32_t bits = b[u * TH]) distill_mask(w[u], bits, T());
     ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
   }
-  for (; left > 0; left -= DI_THREADS, p += DI_THREADS, b += DI_THREADS) {
+  for (; left > 0; left -= TH, p += TH, b += TH) {
     uint4 w[1] = {*p};
     distill_mask(w[0], *b, T());
     ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
@@ -143,24 +145,25 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
 }
 
 // exchange, parts of the list, slots' tokens and masses, loss per warp, bits of the edges, bits of the packets
+template <int TH>
 size_t distill_smem(int S, int per, bool map) {
-  return AgExchange<>::bytes(S) + DI_WARPS * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + DI_WARPS * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
+  return AgExchange<TH>::bytes(S) + (TH / 32) * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + 8 * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
 }
 
-template <typename T, bool TRAIN, bool REST>
-__global__ void __launch_bounds__(DI_THREADS, DI_BLOCKS)
+template <typename T, bool TRAIN, bool REST, int TH>
+__global__ void __launch_bounds__(TH, DI_BLOCKS * 256 / TH)
 distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   constexpr int NV = AG_PACKET<T>;
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
-  const int groups = S * DI_WARPS, parts = (a.top + 31) / 32;
+  const int groups = S * (TH / 32), parts = (a.top + 31) / 32;
   uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
-  const AgExchange<> exchange = {s_box, s_bars, S, rank, a.status};
+  const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
   DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);
-  int* s_ids = reinterpret_cast<int*>(s_parts + DI_WARPS);
+  int* s_ids = reinterpret_cast<int*>(s_parts + (TH / 32));
   float* s_q = reinterpret_cast<float*>(s_ids + AG_DISTILL_MAX);
   float* s_sum = s_q + AG_DISTILL_MAX;
-  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_sum + DI_WARPS);  // [0] edges, [1] a token is listed twice, [4..] packets
+  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_sum + 8);  // [0] edges, [1] a token is listed twice, [4..] packets
   uint8_t* s_map = reinterpret_cast<uint8_t*>(s_marks + 4);
   const float c = a.inv_tau * AG_LOG2E;
   exchange.start();
@@ -177,7 +180,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   const int edge_index = r.edge(rank);
   float edge = edge_index >= 0 ? Pack<T>::load1(r.x + edge_index) : -INFINITY;
   if (TRAIN || REST) {
-    for (int i = tid; i < (a.per + 15) / 16 + 1; i += DI_THREADS) reinterpret_cast<uint4*>(s_marks)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < (a.per + 15) / 16 + 1; i += TH) reinterpret_cast<uint4*>(s_marks)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   if (id >= a.V) {
@@ -207,7 +210,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   const float x_edge = edge;
   if (REST && edge_index >= 0 && s_marks[0] >> tid & 1) edge = -INFINITY;
 
-  const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T>(at, s_map, n, edge, c) : ag_part_stat<false, T, 4>(at, n, edge, c), c);
+  const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T, TH>(at, s_map, n, edge, c) : ag_part_stat<false, T, 4, TH>(at, n, edge, c), c);
   AgStat in = ag_stat_none();
   if (REST && warp < parts) {
     if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
@@ -272,14 +275,14 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
     };
     constexpr int U = 4;
     int i = tid;
-    for (; i + (U - 1) * DI_THREADS < n; i += U * DI_THREADS) {
+    for (; i + (U - 1) * TH < n; i += U * TH) {
       uint4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = at[i + u * DI_THREADS];
+      for (int u = 0; u < U; ++u) w[u] = at[i + u * TH];
 #pragma unroll
-      for (int u = 0; u < U; ++u) put(w[u], i + u * DI_THREADS);
+      for (int u = 0; u < U; ++u) put(w[u], i + u * TH);
     }
-    for (; i < n; i += DI_THREADS) put(at[i], i);
+    for (; i < n; i += TH) put(at[i], i);
     if (edge_index >= 0) Pack<T>::store1(g_row + edge_index, none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift));
   }
   __syncthreads();  // the loss of each warp is there; the entries of listed tokens are written once more
@@ -299,11 +302,11 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
 }
 
 // The gradient alone, from the statistics that the loss left: a block takes `per` packets of a row.
-template <typename T, bool REST>
-__global__ void __launch_bounds__(DI_THREADS, DI_BLOCKS)
+template <typename T, bool REST, int TH>
+__global__ void __launch_bounds__(TH, DI_BLOCKS * 256 / TH)
 distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const DistillArgs a) {
   constexpr int NV = AG_PACKET<T>, U = 4;
-  __shared__ DistillPart s_parts[DI_WARPS];
+  __shared__ DistillPart s_parts[(TH / 32)];
   __shared__ int s_ids[AG_DISTILL_MAX];
   __shared__ float s_q[AG_DISTILL_MAX];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = (a.top + 31) / 32;
@@ -374,14 +377,14 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
     ag_store_packet<T>(g_row + to, g, packets);
   };
   int i = tid;
-  for (; i + (U - 1) * DI_THREADS < n; i += U * DI_THREADS) {
+  for (; i + (U - 1) * TH < n; i += U * TH) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * DI_THREADS);
+    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * TH);
 #pragma unroll
-    for (int u = 0; u < U; ++u) put(w[u], i + u * DI_THREADS);
+    for (int u = 0; u < U; ++u) put(w[u], i + u * TH);
   }
-  for (; i < n; i += DI_THREADS) put(__ldcs(at + i), i);
+  for (; i < n; i += TH) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
     const float d = d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f;
     Pack<T>::store1(g_row + edge_index, (none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift)) + d);
@@ -423,7 +426,24 @@ distill_loss_kernel(const float* __restrict__ row_loss, const float* __restrict_
   }
 }
 
-constexpr int64_t DI_IN_FLIGHT = 48 << 20;
+// Threads of a block: short rows leave most of 256 idle, but a slot of the list needs one.
+int distill_threads(int packets, int top) {
+  const int th = packets <= DI_PACKETS_64 ? 64 : packets <= DI_PACKETS_128 ? 128 : 256;
+  return th >= top ? th : top <= 128 ? 128 : 256;
+}
+
+template <typename T, bool TRAIN, bool REST, int TH>
+int distill_launch(ag_ctx* ctx, const T* logits, T* dlogits, const DistillArgs& a) {
+  static std::atomic<bool> ready[AG_MAX_DEVICES];
+  const size_t smem = distill_smem<TH>(a.S, a.per, TRAIN || REST);
+  if (smem > 48 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
+    AG_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<T, TRAIN, REST, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)distill_smem<TH>(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
+    ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
+  }
+  return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST, TH>, a.S, TH, smem, a.N, logits, dlogits, a);
+}
+
 template <typename T, bool TRAIN, bool REST>
 int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs a) {
   const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
@@ -433,32 +453,34 @@ int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs 
     while (a.S < 8 && (int64_t)packets * 16 * ctx->sm_count * DI_BLOCKS > DI_IN_FLIGHT * a.S && packets / a.S >= 512) a.S *= 2;
   a.per = (packets + a.S - 1) / a.S;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "distillation: too many rows");
-  static std::atomic<bool> ready[AG_MAX_DEVICES];
-  const size_t smem = distill_smem(a.S, a.per, TRAIN || REST);
-  if (smem > 48 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
-    AG_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<T, TRAIN, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)distill_smem(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
-    ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
-  }
-  return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST>, a.S, DI_THREADS, smem, a.N, (const T*)logits, (T*)dlogits, a);
+  const T* x = static_cast<const T*>(logits);
+  T* g = static_cast<T*>(dlogits);
+  const int th = a.S > 1 ? 256 : distill_threads(packets, a.top);
+  return th == 64 ? distill_launch<T, TRAIN, REST, 64>(ctx, x, g, a) : th == 128 ? distill_launch<T, TRAIN, REST, 128>(ctx, x, g, a)
+                                                                               : distill_launch<T, TRAIN, REST, 256>(ctx, x, g, a);
+}
+
+template <typename T, bool REST>
+int distill_backward(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, DistillArgs a) {
+  const int packets = a.V / AG_PACKET<T>;
+  a.S = ag_row_parts(ctx, a.N, packets);
+  a.per = (packets + a.S - 1) / a.S;
+  AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
+  const T *x = static_cast<const T*>(logits), *d = static_cast<const T*>(dres);
+  T* g = static_cast<T*>(dlogits);
+  const unsigned grid = (unsigned)(a.N * a.S);
+  const int th = a.S > 1 ? 256 : distill_threads(packets, a.top);
+  if (th == 64) AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, REST, 64>), grid, 64, 0, x, d, g, a);
+  else if (th == 128) AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, REST, 128>), grid, 128, 0, x, d, g, a);
+  else AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, REST, 256>), grid, 256, 0, x, d, g, a);
+  return AG_OK;
 }
 
 template <typename T>
-int distill_t(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, DistillArgs a, bool backward) {
-  if (!backward) {
-    if (a.dloss) return a.rest ? distill_forward<T, true, true>(ctx, logits, dlogits, a) : distill_forward<T, true, false>(ctx, logits, dlogits, a);
-    return a.rest ? distill_forward<T, false, true>(ctx, logits, dlogits, a) : distill_forward<T, false, false>(ctx, logits, dlogits, a);
-  }
-  a.S = ag_row_parts(ctx, a.N, a.V / AG_PACKET<T>);
-  a.per = (a.V / AG_PACKET<T> + a.S - 1) / a.S;
-  AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_distill_backward: too many rows for V=%d", a.V);
-  if (a.rest)
-    AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, true>), (unsigned)(a.N * a.S), DI_THREADS, 0,
-                  (const T*)logits, (const T*)dres, (T*)dlogits, a);
-  else
-    AG_LAUNCH_PDL(ctx, "distill_backward_kernel", (distill_backward_kernel<T, false>), (unsigned)(a.N * a.S), DI_THREADS, 0,
-                  (const T*)logits, (const T*)dres, (T*)dlogits, a);
-  return AG_OK;
+int distill_t(ag_ctx* ctx, const void* x, const void* d, void* g, const DistillArgs& a, bool backward) {
+  if (backward) return a.rest ? distill_backward<T, true>(ctx, x, d, g, a) : distill_backward<T, false>(ctx, x, d, g, a);
+  if (a.dloss) return a.rest ? distill_forward<T, true, true>(ctx, x, g, a) : distill_forward<T, true, false>(ctx, x, g, a);
+  return a.rest ? distill_forward<T, false, true>(ctx, x, g, a) : distill_forward<T, false, false>(ctx, x, g, a);
 }
 
 int distill(ag_ctx* ctx, const char* who, const void* logits, int64_t ld, const int32_t* ids, const float* teacher,

@@ -18,8 +18,8 @@
 
 namespace {
 
-constexpr int LP_THREADS = AG_ROW_THREADS, LP_FEW = 128;  // threads of a block
-constexpr int LP_FEW_PACKETS = 8191;
+// packets of a row up to which a block has 64 or 128 threads: without alternatives, with them, for the gradient
+constexpr int LP_PACKETS_64 = 1300, LP_PACKETS_128 = 2560, LP_TOP_64 = 2500, LP_TOP_128 = 8191, LB_PACKETS_64 = 800, LB_PACKETS_128 = 2560;
 
 struct LpArgs {
   const int32_t* ids;
@@ -399,8 +399,8 @@ struct LbArgs {
   float inv_tau;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 4)
+template <typename T, int TH>
+__global__ void __launch_bounds__(TH, 4 * 256 / TH)
 logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArgs p) {
   constexpr int NV = AG_PACKET<T>, U = 4;
   const int tid = threadIdx.x;
@@ -446,14 +446,14 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
     ag_store_packet<T>(g_row + to, g, packets);
   };
   int i = tid;
-  for (; i + (U - 1) * LP_THREADS < n; i += U * LP_THREADS) {
+  for (; i + (U - 1) * TH < n; i += U * TH) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * LP_THREADS);
+    for (int u = 0; u < U; ++u) w[u] = __ldcs(at + i + u * TH);
 #pragma unroll
-    for (int u = 0; u < U; ++u) put(w[u], i + u * LP_THREADS);
+    for (int u = 0; u < U; ++u) put(w[u], i + u * TH);
   }
-  for (; i < n; i += LP_THREADS) put(__ldcs(at + i), i);
+  for (; i < n; i += TH) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
     const float g = none ? 0.0f : local(x_edge) + (edge_index == id ? a : 0.0f);
     Pack<T>::store1(g_row + edge_index, g + (d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f));
@@ -462,11 +462,17 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
 
 template <typename T>
 int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* dlogits, LbArgs p, int64_t N) {
-  p.S = ag_row_parts(ctx, N, p.V / AG_PACKET<T>);
-  p.per = (p.V / AG_PACKET<T> + p.S - 1) / p.S;
+  const int packets = p.V / AG_PACKET<T>;
+  p.S = ag_row_parts(ctx, N, packets);
+  p.per = (packets + p.S - 1) / p.S;
   AG_REQUIRE(ctx, N * p.S < (1ll << 31), "ag_token_logprobs_backward: too many rows for V=%d", p.V);
-  AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", logprobs_backward_kernel<T>, (unsigned)(N * p.S), LP_THREADS, 0, (const T*)logits,
-                (const T*)dres, (T*)dlogits, p);
+  const T *x = static_cast<const T*>(logits), *d = static_cast<const T*>(dres);
+  T* g = static_cast<T*>(dlogits);
+  const unsigned grid = (unsigned)(N * p.S);
+  const int th = p.S > 1 ? 256 : packets <= LB_PACKETS_64 ? 64 : packets <= LB_PACKETS_128 ? 128 : 256;
+  if (th == 64) AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 64>), grid, 64, 0, x, d, g, p);
+  else if (th == 128) AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 128>), grid, 128, 0, x, d, g, p);
+  else AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 256>), grid, 256, 0, x, d, g, p);
   return AG_OK;
 }
 
@@ -490,21 +496,26 @@ int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
   a.per = (packets + a.S - 1) / a.S;
   a.status = ctx->d_status;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_token_logprobs_forward: too many rows");
-  if (a.top == 0) return logprobs_launch<T, false, LP_THREADS, true>(ctx, logits, a);
+  if (a.top == 0) {
+    if (a.S > 1 || packets > LP_PACKETS_128) return logprobs_launch<T, false, 256, true>(ctx, logits, a);
+    return packets > LP_PACKETS_64 ? logprobs_launch<T, false, 128, true>(ctx, logits, a)
+                                   : logprobs_launch<T, false, 64, true>(ctx, logits, a);
+  }
   a.cap = (3 * a.top + 64 + 3) & ~3;  // a multiple of four: what follows in shared memory is read 16 bytes at a time
   if (a.S > 1) {
     // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
     // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.
-    const int groups = a.S * (LP_THREADS / 32);
+    const int groups = a.S * 8;
     a.J = (a.top + groups - 1) / groups;
     while (a.J < 32 && (a.top + a.J - 1) / a.J * 20 > groups * 17) ++a.J;
     a.need = (a.top + a.J - 1) / a.J;
-    return logprobs_launch<T, true, LP_THREADS, true>(ctx, logits, a);
+    return logprobs_launch<T, true, 256, true>(ctx, logits, a);
   }
   // Short rows: what each warp does once per row weighs more than what more threads read at a time.  128 / 256 threads, us:
-  // 8192 x 32768 bf16, 64 alternatives 128 / 146, fp32 207 / 200; 2048 x 151936 bf16, 20 alternatives 145 / 128.
-  if (packets <= LP_FEW_PACKETS) return logprobs_launch<T, true, LP_FEW, false>(ctx, logits, a);
-  return logprobs_launch<T, true, LP_THREADS, false>(ctx, logits, a);
+  // 8192 x 32768 bf16, 64 alternatives 125 / 141, fp32 206 / 197; 2048 x 151936 bf16, 20 alternatives 147 / 126.
+  if (packets <= LP_TOP_64) return logprobs_launch<T, true, 64, false>(ctx, logits, a);
+  if (packets <= LP_TOP_128) return logprobs_launch<T, true, 128, false>(ctx, logits, a);
+  return logprobs_launch<T, true, 256, false>(ctx, logits, a);
 }
 
 }  // namespace

@@ -8,7 +8,6 @@
 
 #include "ag_common.cuh"
 
-constexpr int AG_ROW_THREADS = 256;  // of a block, where it is not said otherwise
 constexpr float AG_LN2 = 0.69314718055994531f, AG_LOG2E = 1.44269504088896341f;
 
 // Launches go to the context's device, whichever is current in the calling thread.
@@ -246,7 +245,7 @@ struct AgRow {
 // Statistics of this thread's part of n packets, U at a time, and of its element of the edges (-inf without one).  `most` (null: not
 // wanted): the largest logit of each batch, and of each packet that is left behind the last whole batch, this thread's
 // TH (the threads of the block) apart, the first one that far behind `most`.
-template <bool WITH_T, typename T, int U, int TH = AG_ROW_THREADS>
+template <bool WITH_T, typename T, int U, int TH>
 __device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c, float* most = nullptr) {
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
   const uint4* p = at + threadIdx.x;
@@ -317,7 +316,7 @@ __device__ __forceinline__ void ag_wait_cluster(uint64_t* bar, uint32_t parity, 
 // What each warp of a cluster tells all others about its part of a row: one float4 per warp, in turn at two places.  A block can be
 // one row ahead of another, never two: for the row between it waits for what all warps of the other have to tell, and they tell it
 // when they have read what came before.
-template <int TH = AG_ROW_THREADS>
+template <int TH>
 struct AgExchange {
   float4* box;      // [2][S * warps of a block]
   uint64_t* bar;    // [2]
