@@ -18,9 +18,9 @@
 
 namespace {
 
-constexpr int DI_BLOCKS = 4;  // of 256 threads per SM
+constexpr int DI_BLOCKS = 5, DI_BLOCKS_REST = 4;  // of 256 threads per SM
 constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;  // of a row, up to which a block has 64 or 128 threads
-constexpr int64_t DI_IN_FLIGHT = 48 << 20;
+constexpr int64_t DI_IN_FLIGHT = 64 << 20;
 static_assert(AG_DISTILL_MAX <= 256, "a slot per thread");
 
 struct DistillArgs {
@@ -151,7 +151,7 @@ size_t distill_smem(int S, int per, bool map) {
 }
 
 template <typename T, bool TRAIN, bool REST, int TH>
-__global__ void __launch_bounds__(TH, DI_BLOCKS * 256 / TH)
+__global__ void __launch_bounds__(TH, (REST ? DI_BLOCKS_REST : DI_BLOCKS) * 256 / TH)
 distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   constexpr int NV = AG_PACKET<T>;
   extern __shared__ float4 s_box[];
@@ -303,7 +303,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
 
 // The gradient alone, from the statistics that the loss left: a block takes `per` packets of a row.
 template <typename T, bool REST, int TH>
-__global__ void __launch_bounds__(TH, DI_BLOCKS * 256 / TH)
+__global__ void __launch_bounds__(TH, 4 * 256 / TH)
 distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const DistillArgs a) {
   constexpr int NV = AG_PACKET<T>, U = 4;
   __shared__ DistillPart s_parts[(TH / 32)];
@@ -446,16 +446,16 @@ int distill_launch(ag_ctx* ctx, const T* logits, T* dlogits, const DistillArgs& 
 
 template <typename T, bool TRAIN, bool REST>
 int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs a) {
-  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
+  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>, blocks = REST ? DI_BLOCKS_REST : DI_BLOCKS;
   a.S = 1;
   while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
   if (TRAIN)
-    while (a.S < 8 && (int64_t)packets * 16 * ctx->sm_count * DI_BLOCKS > DI_IN_FLIGHT * a.S && packets / a.S >= 512) a.S *= 2;
+    while (a.S < 8 && (int64_t)packets * 16 * ctx->sm_count * blocks > DI_IN_FLIGHT * a.S && packets / a.S >= 512) a.S *= 2;
   a.per = (packets + a.S - 1) / a.S;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "distillation: too many rows");
   const T* x = static_cast<const T*>(logits);
   T* g = static_cast<T*>(dlogits);
-  const int th = a.S > 1 ? 256 : distill_threads(packets, a.top);
+  const int th = a.S > 1 || (TRAIN && packets > DI_PACKETS_64) ? 256 : distill_threads(packets, a.top);
   return th == 64 ? distill_launch<T, TRAIN, REST, 64>(ctx, x, g, a) : th == 128 ? distill_launch<T, TRAIN, REST, 128>(ctx, x, g, a)
                                                                                : distill_launch<T, TRAIN, REST, 256>(ctx, x, g, a);
 }
