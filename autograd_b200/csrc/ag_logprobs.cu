@@ -389,7 +389,8 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   }
 }
 
-// Gradient: a block takes `per` packets of a row.
+// Gradient: a block takes `per` packets of a row.  fp32 gains by twice as many under way (8192 x 32768 334 / 328 us), bf16 by more
+// blocks (179 / 171, which is nearer to what its exponentials take).
 struct LbArgs {
   const int32_t* ids;
   const float4* stats;
@@ -400,9 +401,9 @@ struct LbArgs {
 };
 
 template <typename T, int TH>
-__global__ void __launch_bounds__(TH, 4 * 256 / TH)
+__global__ void __launch_bounds__(TH, (sizeof(T) == 4 ? 4 : 5) * 256 / TH)
 logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArgs p) {
-  constexpr int NV = AG_PACKET<T>, U = 4;
+  constexpr int NV = AG_PACKET<T>, U = sizeof(T) == 4 ? 8 : 4;
   const int tid = threadIdx.x;
   ag_pdl_wait();
   ag_pdl_trigger();
@@ -469,7 +470,7 @@ int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* d
   const T *x = static_cast<const T*>(logits), *d = static_cast<const T*>(dres);
   T* g = static_cast<T*>(dlogits);
   const unsigned grid = (unsigned)(N * p.S);
-  const int th = p.S > 1 ? 256 : packets <= LB_PACKETS_64 ? 64 : packets <= LB_PACKETS_128 ? 128 : 256;
+  const int th = p.S > 1 ? 256 : ag_row_threads(ctx, N, packets, LB_PACKETS_64, LB_PACKETS_128);
   if (th == 64) AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 64>), grid, 64, 0, x, d, g, p);
   else if (th == 128) AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 128>), grid, 128, 0, x, d, g, p);
   else AG_LAUNCH_PDL(ctx, "logprobs_backward_kernel", (logprobs_backward_kernel<T, 256>), grid, 256, 0, x, d, g, p);
@@ -491,15 +492,15 @@ template <typename T>
 int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
   const T* logits = static_cast<const T*>(x);
   const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>;
-  a.S = 1;
-  while (a.S < 8 && a.N * a.S * 2 <= 2 * ctx->sm_count && packets / a.S >= 512) a.S *= 2;
+  a.S = ag_cluster_parts(ctx, a.N, packets);
   a.per = (packets + a.S - 1) / a.S;
   a.status = ctx->d_status;
   AG_REQUIRE(ctx, a.N * a.S < (1ll << 31), "ag_token_logprobs_forward: too many rows");
   if (a.top == 0) {
-    if (a.S > 1 || packets > LP_PACKETS_128) return logprobs_launch<T, false, 256, true>(ctx, logits, a);
-    return packets > LP_PACKETS_64 ? logprobs_launch<T, false, 128, true>(ctx, logits, a)
-                                   : logprobs_launch<T, false, 64, true>(ctx, logits, a);
+    const int th = a.S > 1 ? 256 : ag_row_threads(ctx, a.N, packets, LP_PACKETS_64, LP_PACKETS_128);
+    return th == 64    ? logprobs_launch<T, false, 64, true>(ctx, logits, a)
+           : th == 128 ? logprobs_launch<T, false, 128, true>(ctx, logits, a)
+                       : logprobs_launch<T, false, 256, true>(ctx, logits, a);
   }
   a.cap = (3 * a.top + 64 + 3) & ~3;  // a multiple of four: what follows in shared memory is read 16 bytes at a time
   if (a.S > 1) {
@@ -513,9 +514,10 @@ int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
   }
   // Short rows: what each warp does once per row weighs more than what more threads read at a time.  128 / 256 threads, us:
   // 8192 x 32768 bf16, 64 alternatives 125 / 141, fp32 206 / 197; 2048 x 151936 bf16, 20 alternatives 147 / 126.
-  if (packets <= LP_TOP_64) return logprobs_launch<T, true, 64, false>(ctx, logits, a);
-  if (packets <= LP_TOP_128) return logprobs_launch<T, true, 128, false>(ctx, logits, a);
-  return logprobs_launch<T, true, 256, false>(ctx, logits, a);
+  const int th = ag_row_threads(ctx, a.N, packets, LP_TOP_64, LP_TOP_128);
+  return th == 64    ? logprobs_launch<T, true, 64, false>(ctx, logits, a)
+         : th == 128 ? logprobs_launch<T, true, 128, false>(ctx, logits, a)
+                     : logprobs_launch<T, true, 256, false>(ctx, logits, a);
 }
 
 }  // namespace

@@ -395,6 +395,20 @@ static inline int ag_row_parts(const ag_ctx* ctx, int64_t N, int packets) {
   return S;
 }
 
+// Blocks of a cluster that share a row, where they have something to tell one another: more while the SMs have about one block each,
+// and the blocks at least two packets per thread.  Us, by 1.0 / 1.4 / 2.8 blocks per SM up to which they are doubled: 200 rows of
+// 32768 bf16, 20 alternatives 10.4 / 9.3 / 9.3; 64 rows 7.1 / 7.1 / 10.4; distillation loss of 200 rows fp32 9.6 / 9.0 / 9.0.
+static inline int ag_cluster_parts(const ag_ctx* ctx, int64_t N, int packets) {
+  int S = 1;
+  while (S < 8 && N * S * 5 <= 7 * ctx->sm_count && packets / S >= 512) S *= 2;
+  return S;
+}
+
+// Threads of a block with a row to itself: up to p64 packets 64, up to p128 128; not 64 for a few rows, which wait for their own loads.
+static inline int ag_row_threads(const ag_ctx* ctx, int64_t N, int packets, int p64, int p128) {
+  return packets > p128 ? 256 : packets > p64 || N < 4 * ctx->sm_count ? 128 : 64;
+}
+
 // Launch of n clusters of S blocks.
 template <typename... P, typename... A>
 static inline int ag_launch_clusters(ag_ctx* ctx, const char* name, void (*kern)(P...), int S, int threads, size_t smem, int64_t n,
