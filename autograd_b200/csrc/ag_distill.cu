@@ -19,7 +19,11 @@
 
 namespace {
 
-constexpr int DI_BLOCKS = 5, DI_BLOCKS_REST = 4;  // of 256 threads per SM
+// Blocks of 256 threads per SM, packets per thread under way in the first look.  Without a gradient and with the map more packets
+// gain what more blocks do otherwise: us, 4 packets and 5 blocks (REST 4) / 8 packets and 4 blocks: loss of 512 x 32768 fp32 RENORM
+// 17.0 / 15.2, REST 17.5 / 16.5, gradient REST of 8192 x 50257 bf16 349 / 332, 16384 x 32768 fp32 822 / 777, RENORM 725 / 829.
+constexpr int distill_blocks(bool train, bool rest) { return train && !rest ? 5 : 4; }
+constexpr int distill_batch(bool train, bool rest) { return train && !rest ? 4 : 8; }
 constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;  // of a row, up to which a block has 64 or 128 threads
 constexpr int64_t DI_IN_FLIGHT = 64 << 20;
 static_assert(AG_DISTILL_MAX <= 256, "a slot per thread");
@@ -121,9 +125,8 @@ __device__ __forceinline__ void distill_mask(uint4& w, uint32_t bits, __nv_bfloa
 }
 
 // Statistics of the unlisted logits of this thread's part; as ag_part_stat.  map: a byte per packet.
-template <typename T, int TH>
+template <typename T, int U, int TH>
 __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8_t* map, int n, float edge, float c) {
-  constexpr int U = 4;
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};
   const uint4* p = at + threadIdx.x;
   const uint8_t* b = map + threadIdx.x;
@@ -145,6 +148,21 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
   return v;
 }
 
+// outside * p of a packet's logits, log2 p = (x + ref) c + shift
+template <typename T>
+__device__ __forceinline__ void distill_dense(const uint4& w, uint64_t ref2, uint64_t c2, uint64_t shift2, float outside,
+                                              float (&g)[AG_PACKET<T>]) {
+  float x[AG_PACKET<T>];
+  ag_widen(w, x);
+#pragma unroll
+  for (int e = 0; e < AG_PACKET<T>; e += 2) {
+    float d0, d1;
+    ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
+    g[e] = outside * ag_ex2(d0);  // not as a pair: 16384 x 32768 fp32 took 776 us that way, 727 this way
+    g[e + 1] = outside * ag_ex2(d1);
+  }
+}
+
 // exchange, parts of the list, slots' tokens and masses, loss per warp, bits of the edges, bits of the packets
 template <int TH>
 size_t distill_smem(int S, int per, bool map) {
@@ -152,9 +170,9 @@ size_t distill_smem(int S, int per, bool map) {
 }
 
 template <typename T, bool TRAIN, bool REST, int TH>
-__global__ void __launch_bounds__(TH, (REST ? DI_BLOCKS_REST : DI_BLOCKS) * 256 / TH)
+__global__ void __launch_bounds__(TH, distill_blocks(TRAIN, REST) * 256 / TH)
 distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
-  constexpr int NV = AG_PACKET<T>;
+  constexpr int NV = AG_PACKET<T>, BATCH = distill_batch(TRAIN, REST);
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * (TH / 32), parts = (a.top + 31) / 32;
@@ -211,7 +229,8 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   const float x_edge = edge;
   if (REST && edge_index >= 0 && s_marks[0] >> tid & 1) edge = -INFINITY;
 
-  const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T, TH>(at, s_map, n, edge, c) : ag_part_stat<false, T, 4, TH>(at, n, edge, c), c);
+  const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T, BATCH, TH>(at, s_map, n, edge, c)
+                                          : ag_part_stat<false, T, BATCH, TH>(at, n, edge, c), c);
   AgStat in = ag_stat_none();
   if (REST && warp < parts) {
     if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};
@@ -263,19 +282,16 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
     const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
     const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0;
     auto put = [&](const uint4& w, int i) {
-      float x[NV], g[NV];
-      ag_widen(w, x);
-#pragma unroll
-      for (int e = 0; e < NV; e += 2) {
-        float d0, d1;
-        ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
-        g[e] = none ? 0.0f : outside * ag_ex2(d0);
-        g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
-      }
+      float g[NV];
+      distill_dense<T>(w, ref2, c2, shift2, outside, g);
       ag_store_packet<T>(g_row + first + (int64_t)i * NV, g, packets);
     };
     constexpr int U = 4;
     int i = tid;
+    if (none) {  // 0, whatever the logits are
+      const float g[NV] = {};
+      for (; i < n; i += TH) ag_store_packet<T>(g_row + first + (int64_t)i * NV, g, packets);
+    }
     for (; i + (U - 1) * TH < n; i += U * TH) {
       uint4 w[U];
 #pragma unroll
@@ -358,16 +374,7 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
   const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
   const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
   const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0, d_packets = (((uintptr_t)(d_row + first)) & 15) == 0;
-  auto put = [&](const uint4& w, int i) {
-    float x[NV], g[NV];
-    ag_widen(w, x);
-#pragma unroll
-    for (int e = 0; e < NV; e += 2) {
-      float d0, d1;
-      ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
-      g[e] = none ? 0.0f : outside * ag_ex2(d0);
-      g[e + 1] = none ? 0.0f : outside * ag_ex2(d1);
-    }
+  auto add = [&](float (&g)[NV], int i) {
     const int to = first + i * NV;
     if (d_row) {
       float d[NV];
@@ -377,7 +384,17 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
     }
     ag_store_packet<T>(g_row + to, g, packets);
   };
+  auto put = [&](const uint4& w, int i) {
+    float g[NV];
+    distill_dense<T>(w, ref2, c2, shift2, outside, g);
+    add(g, i);
+  };
   int i = tid;
+  if (none)  // 0, whatever the logits are
+    for (; i < n; i += TH) {
+      float g[NV] = {};
+      add(g, i);
+    }
   for (; i + (U - 1) * TH < n; i += U * TH) {
     uint4 w[U];
 #pragma unroll
@@ -447,7 +464,7 @@ int distill_launch(ag_ctx* ctx, const T* logits, T* dlogits, const DistillArgs& 
 
 template <typename T, bool TRAIN, bool REST>
 int distill_forward(ag_ctx* ctx, const void* logits, void* dlogits, DistillArgs a) {
-  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>, blocks = REST ? DI_BLOCKS_REST : DI_BLOCKS;
+  const int packets = (a.V + AG_PACKET<T> - 1) / AG_PACKET<T>, blocks = distill_blocks(TRAIN, REST);
   a.S = ag_cluster_parts(ctx, a.N, packets);
   if (TRAIN)
     while (a.S < 8 && (int64_t)packets * 16 * ctx->sm_count * blocks > DI_IN_FLIGHT * a.S && packets / a.S >= 512) a.S *= 2;

@@ -422,17 +422,19 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
   T* g_row = dlogits + row * p.ld_grad;
   const T* d_row = dres ? dres + row * p.ld_grad : nullptr;
   const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0, d_packets = (((uintptr_t)(d_row + first)) & 15) == 0;
-  // p (a + b (ln p + H)) = p (a + b H + b ln p); a logit of -inf: p = 0, and 0 times something finite
-  const float k = a + b * st.z;
-  auto local = [&](float x) {
-    const float lp = fmaxf((x - st.x) * p.inv_tau, -1e4f) - st.y;
-    return -ag_ex2(lp * AG_LOG2E) * (k + b * lp);
+  // p (a + b (ln p + H)) = p (k + b ln p) with ln p = d ln 2, p = 2^d.  A logit of -inf: p = 0, and 0 times something finite; a NaN
+  // has to stay one.
+  const float c = p.inv_tau * AG_LOG2E, shift = -st.y * AG_LOG2E, k = -(a + b * st.z), bd = -b * AG_LN2;
+  const uint64_t ref2 = ag_pair(-st.x, -st.x), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift), k2 = ag_pair(k, k),
+                 bd2 = ag_pair(bd, bd);
+  auto local = [&](float x0, float x1, float& g0, float& g1) {
+    float d0, d1;
+    ag_unpair(ag_fma2(ag_add2(ag_pair(x0, x1), ref2), c2, shift2), d0, d1);
+    d0 = ag_max_nan(d0, -1e4f);
+    d1 = ag_max_nan(d1, -1e4f);
+    ag_unpair(ag_mul2(ag_pair(ag_ex2(d0), ag_ex2(d1)), ag_fma2(bd2, ag_pair(d0, d1), k2)), g0, g1);
   };
-  auto put = [&](const uint4& w, int i) {
-    float x[NV], g[NV];
-    ag_widen(w, x);
-#pragma unroll
-    for (int e = 0; e < NV; ++e) g[e] = none ? 0.0f : local(x[e]);
+  auto add = [&](float (&g)[NV], int i) {
     const int to = first + i * NV, hit = id - to;
     if (hit >= 0 && hit < NV && !none) {
 #pragma unroll
@@ -446,7 +448,19 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
     }
     ag_store_packet<T>(g_row + to, g, packets);
   };
+  auto put = [&](const uint4& w, int i) {
+    float x[NV], g[NV];
+    ag_widen(w, x);
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) local(x[e], x[e + 1], g[e], g[e + 1]);
+    add(g, i);
+  };
   int i = tid;
+  if (none)  // 0, whatever the logits are
+    for (; i < n; i += TH) {
+      float g[NV] = {};
+      add(g, i);
+    }
   for (; i + (U - 1) * TH < n; i += U * TH) {
     uint4 w[U];
 #pragma unroll
@@ -456,7 +470,9 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
   }
   for (; i < n; i += TH) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
-    const float g = none ? 0.0f : local(x_edge) + (edge_index == id ? a : 0.0f);
+    float g = 0.0f, other;
+    if (!none) local(x_edge, x_edge, g, other);
+    if (!none && edge_index == id) g += a;
     Pack<T>::store1(g_row + edge_index, g + (d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f));
   }
 }

@@ -71,6 +71,11 @@ __device__ __forceinline__ float ag_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+__device__ __forceinline__ float ag_max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // pairs of fp32 in one instruction
 __device__ __forceinline__ uint64_t ag_pair(float a, float b) {
   uint64_t y;
