@@ -509,7 +509,7 @@ int distill(ag_ctx* ctx, const char* who, const void* logits, int64_t ld, const 
   AG_REQUIRE(ctx, top > 0, "%s: a list of no tokens", who);
   AG_REQUIRE(ctx, (ids && teacher && (backward ? stats : row_loss) && (dloss || ld_grad < 0)) || N == 0, "%s: null pointer", who);
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
-  AG_REQUIRE(ctx, (((uintptr_t)ids | (uintptr_t)teacher) & 3) == 0, "%s: teacher's lists not aligned", who);
+  AG_REQUIRE(ctx, ag_aligned4(ids, teacher, row_scale, dloss, loss, row_loss), "%s: pointer not aligned to its type", who);
   if (N == 0 && !loss) return AG_OK;
   AgOnDevice on(ctx);
   const DistillArgs a = {ids, teacher, row_scale, dloss, row_loss, (float4*)stats, N, ld, ld_grad, V, top, mode == AG_DISTILL_REST,

@@ -176,10 +176,13 @@ __device__ __noinline__ int lp_search(const LpPart<T, TH>& sl, uint32_t lo, int 
   __syncthreads();
   sl.each([&](float x, int j) {
     const uint32_t k = ag_order(x);
-    if (k > lo || (fits && k == lo)) keys[atomicAdd(s_count, 1)] = lp_key(x, j);
+    if (k > lo || (fits && k == lo)) {
+      const int to = atomicAdd(s_count, 1);
+      if (to < cap) keys[to] = lp_key(x, j);  // always, unless the logits change under way
+    }
   });
   __syncthreads();
-  int have = *s_count;
+  int have = min(*s_count, cap);
   if (fits) return have;
   // in the order of the index: the elements before the first packet, then packets by rounds of the block, then those behind
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -343,9 +346,10 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     ag_wait_cluster(s_keys_bar, 0, a.status);
     // side by side
     constexpr int MOVE = (3 * AG_TOP_MAX + 64 + TH - 1) / TH;  // keys of a block per thread, at most
-    total = counts[0];
+    // (a count may be anything if the wait has expired)
+    total = max(0, min(counts[0], a.cap));
     for (int p = 1; p < S; ++p) {
-      const int more = counts[p];
+      const int more = max(0, min(counts[p], a.cap));
       unsigned long long mine[MOVE];  // what is moved down may lie over what is not yet
       for (int k = 0; k < MOVE; ++k)
         if (tid + k * TH < more) mine[k] = all[(size_t)p * a.cap + tid + k * TH];
@@ -375,7 +379,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   };
   __shared__ int s_place[TH / 2];
   if (total <= TH / 2) {
-    const int lanes = (total + 31) & ~31, parts = TH / lanes, i = tid % lanes;
+    const int lanes = max(32, (total + 31) & ~31), parts = TH / lanes, i = tid % lanes;
     if (tid < lanes) s_place[i] = 0;
     __syncthreads();
     if (i < total && tid < parts * lanes) {
@@ -545,9 +549,11 @@ extern "C" int ag_token_logprobs_forward(ag_ctx* ctx, const void* logits, int64_
   const char* who = "ag_token_logprobs_forward";
   if (int rc = ag_vocab_check(ctx, who, {N, ld, -1, V, top, dtype, temperature}, AG_VOCAB_MAX, AG_TOP_MAX, logits, nullptr, nullptr))
     return rc;
+  AG_REQUIRE(ctx, top <= V, "%s: %d of %d tokens", who, top, V);
   AG_REQUIRE(ctx, !logprob || ids, "%s: log-probabilities of no tokens", who);
   AG_REQUIRE(ctx, top == 0 || (top_ids && top_logprobs) || N == 0, "%s: null pointer", who);
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
+  AG_REQUIRE(ctx, ag_aligned4(ids, logprob, entropy, top_ids, top_logprobs), "%s: pointer not aligned to its type", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
   const LpArgs a = {ids, logprob, entropy, (float4*)stats, top_ids, top_logprobs, N, ld, V, top, 1.0f / temperature, 0, 0, 0, 0, 0, nullptr};
@@ -564,6 +570,7 @@ extern "C" int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64
   AG_REQUIRE(ctx, !dlogprob || ids, "%s: a gradient of log-probabilities of no tokens", who);
   AG_REQUIRE(ctx, stats || N == 0, "%s: null stats", who);
   AG_REQUIRE(ctx, ag_aligned16(stats), "%s: stats not 16-byte aligned", who);
+  AG_REQUIRE(ctx, ag_aligned4(ids, dlogprob, dentropy), "%s: pointer not aligned to its type", who);
   if (N == 0) return AG_OK;
   AgOnDevice on(ctx);
   const LbArgs p = {ids, (const float4*)stats, dlogprob, dentropy, ld, ld_grad, V, 0, 0, 1.0f / temperature};

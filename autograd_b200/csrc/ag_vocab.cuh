@@ -22,6 +22,12 @@ struct AgOnDevice {
   }
 };
 
+// Pointers to 32-bit numbers, or null
+template <typename... P>
+static inline bool ag_aligned4(const P*... p) {
+  return ((((uintptr_t)p & 3) == 0) && ...);
+}
+
 struct AgVocabShape {
   int64_t N, ld, ld_grad;
   int V, top, dtype;
@@ -35,7 +41,7 @@ static inline int ag_vocab_check(ag_ctx* ctx, const char* who, const AgVocabShap
              (long long)s.N, s.V, max_v);
   AG_REQUIRE(ctx, s.dtype == AG_F32 || s.dtype == AG_BF16, "%s: unknown dtype %d", who, s.dtype);
   AG_REQUIRE(ctx, s.temperature >= 1e-4f && s.temperature <= 1e4f, "%s: temperature %g outside 1e-4 to 1e4", who, s.temperature);
-  AG_REQUIRE(ctx, s.top >= 0 && s.top <= max_top && s.top <= s.V, "%s: %d tokens per row, up to %d and V", who, s.top, max_top);
+  AG_REQUIRE(ctx, s.top >= 0 && s.top <= max_top, "%s: %d tokens per row, up to %d", who, s.top, max_top);
   // beyond 2^40 elements the products below would overflow before they could be compared with anything
   AG_REQUIRE(ctx, s.ld >= s.V && s.ld < (1ll << 31), "%s: row stride %lld smaller than V=%d, or too large", who, (long long)s.ld, s.V);
   AG_REQUIRE(ctx, logits || s.N == 0, "%s: null logits", who);

@@ -322,3 +322,67 @@ def test_a_policy_step_after_a_head():
     ctx.synchronize()
     alloc.free(ws)
     free(th, tw, z, tid, lp, ent, st, ta, tb, g)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(1, 4097), (2, 32768), (3, 151937), (40, 50257), (100, 20001), (200, 32768)])
+def test_gradients_in_the_place_of_few_wide_logits(n, v, dtype):
+    """Rows that several blocks share: one reads the listed logits of all others before those are written over."""
+    rng = np.random.default_rng(v)
+    x = rounded(rng.standard_normal((n, v)).astype(np.float32) * 2, dtype)
+    for rest in (False, True):
+        ids, t = teacher_of(rng, n, v, 200, rest)
+        for what in ("both", "apart"):
+            check(x, ids, t, dtype, what, rest=rest, place="logits", temperature=0.8)
+            check(x, ids, t, dtype, what, rest=rest, place="logits", ld=v + 3, shift=1)
+
+
+def test_tokens_that_are_listed_many_times():
+    rng = np.random.default_rng(7)
+    for n, v, top in ((5, 40, 64), (600, 700, 60), (3, 33000, 256)):
+        x = rng.standard_normal((n, v)).astype(np.float32)
+        x[:, 5] = -np.inf
+        ids = rng.choice([0, 5, 7, v - 1, -1], (n, top)).astype(np.int32)
+        for rest in (False, True):
+            t = np.log(rng.random((n, top)) / top).astype(np.float32)
+            t[ids == 5] = -np.inf
+            for what in ("both", "apart"):
+                check(x, ids, t, "f32", what, rest=rest)
+
+
+def test_two_streams_at_once():
+    """The same calls from two threads, each with a device context of its own, on logits of its own."""
+    import threading
+
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(17)
+    n, v, top = 24, 40000, 30
+    work = []
+    for _ in range(2):
+        x = rng.standard_normal((n, v)).astype(np.float32)
+        ids, t = teacher_of(rng, n, v, top, True)
+        c = ag.CudaContext(0)
+        dev = [up(a) for a in (x, ids, t, np.ones(1, np.float32), np.zeros(1, np.float32), np.zeros(n, np.float32),
+                               np.zeros((n, v), np.float32), np.zeros((n, top), np.int32), np.zeros((n, top), np.float32))]
+        work.append((x, ids, t, c, dev))
+    ctx.synchronize()
+
+    def run_on(c, dev):
+        tx, ti, tt, dl, loss, row, g, oi, ol = dev
+        for _ in range(50):
+            c.token_logprobs_forward(tx, v, None, None, None, None, oi, ol, n, v, top)
+            c.distill_forward_backward(tx, v, ti, tt, None, dl, loss, row, None, g, v, n, v, top, 1.0, ag.AG_DISTILL_REST)
+    threads = [threading.Thread(target=run_on, args=(w[3], w[4])) for w in work]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for x, ids, t, c, dev in work:
+        c.synchronize()
+        assert c.status() == 0
+        ref = R.distill(x, ids, t, rest=True)
+        assert np.array_equal(down(dev[7]), R.top(x, top))
+        near(down(dev[5]), ref["row_loss"], 400 * U * ref["loss_size"], "loss of a row")
+        near(down(dev[6]), ref["dlogits"], ref["size"] * (400 + 16 * np.abs(ref["lp"])) * U + 2.0 ** -120, "gradient")
+        c.close()
+        free(*dev)

@@ -98,6 +98,10 @@ REFUSED = (
     [(n, c) for n in DISTILL for c in (
         dict(top=0), dict(top=-1), dict(top=N.AG_DISTILL_MAX + 1, V=1000, ld=1000, ld_grad=1000), dict(mode=2), dict(mode=-1),
         dict(ids=0), dict(top_logprobs=0))] +
+    [("ag_token_logprobs_forward", {k: BASE + 2}) for k in ("ids", "logprob", "entropy", "top_ids", "top_logprobs")] +
+    [("ag_token_logprobs_backward", {k: BASE + 1}) for k in ("ids", "dlogprob", "dentropy")] +
+    [(n, {k: BASE + 2}) for n in DISTILL for k in ("ids", "top_logprobs", "row_scale")] +
+    [(n, {k: BASE + 2}) for n in DISTILL if "forward" in n for k in ("loss", "row_loss")] +
     [(n, dict(row_loss=0)) for n in DISTILL if "forward" in n] + [(n, dict(dloss=0)) for n in DISTILL if "backward" in n] +
     [("ag_distill_backward", dict(stats=0))])
 
