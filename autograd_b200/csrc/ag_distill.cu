@@ -24,9 +24,14 @@ namespace {
 // 17.0 / 15.2, REST 17.5 / 16.5, gradient REST of 8192 x 50257 bf16 349 / 332, 16384 x 32768 fp32 822 / 777, RENORM 725 / 829.
 constexpr int distill_blocks(bool train, bool rest) { return train && !rest ? 5 : 4; }
 constexpr int distill_batch(bool train, bool rest) { return train && !rest ? 4 : 8; }
-constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;  // of a row, up to which a block has 64 or 128 threads
+// Packets of a row up to which a block has 64 or 128 threads.  16384 rows (of 32768: 8192), lists of 20 to 64, 64 / 128 / 256 threads,
+// us: loss 640 fp32 34 / 48 / 85, 5003 73 / 84 / 122; with gradient 640 fp32 39 / 56 / 96, 5003 131 / 138 / 172, 10007 bf16
+// 161 / 180 / 242; gradient alone 5003 bf16 51 / 54 / 91, 10007 85 / 84 / 106, 32768 224 / 205 / 209.
+constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;
+// Bytes of the rows that are under way at a time, above which more blocks share a row: what is written then pushes out of L2 what is
+// to be read again.  Us: 16384 x 32768 fp32, 1 / 2 / 4 blocks per row (97, 48, 24 MB) 940 / 727 / 933; 8192 x 50257 bf16, 1 / 2 (60,
+// 30 MB) 344 / 406; 4096 x 151936 bf16, 2 / 4 (90, 45 MB) 305 / 284.
 constexpr int64_t DI_IN_FLIGHT = 64 << 20;
-static_assert(AG_DISTILL_MAX <= 256, "a slot per thread");
 
 struct DistillArgs {
   const int32_t* ids;

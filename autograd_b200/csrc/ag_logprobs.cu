@@ -18,7 +18,10 @@
 
 namespace {
 
-// packets of a row up to which a block has 64 or 128 threads: without alternatives, with them, for the gradient
+// Packets of a row up to which a block has 64 or 128 threads: without alternatives, with them, for the gradient.  16384 rows (of
+// 32768: 8192), 64 / 128 / 256 threads, us: none 640 bf16 18 / 19 / 30, 5003 fp32 55 / 57 / 68, 32768 bf16 93 / 89 / 87; 20 alternatives
+// 5003 bf16 69 / 86 / 156, 10007 fp32 144 / 148 / 203; 64 of 32768 bf16 - / 125 / 141, fp32 - / 206 / 197; gradient 640 fp32
+// 24 / 27 / 40, 5003 bf16 67 / 68 / 108, 5003 fp32 116 / 111 / 121, 32768 bf16 193 / 182 / 178.
 constexpr int LP_PACKETS_64 = 1300, LP_PACKETS_128 = 2560, LP_TOP_64 = 2500, LP_TOP_128 = 8191, LB_PACKETS_64 = 800, LB_PACKETS_128 = 2560;
 
 struct LpArgs {
@@ -230,6 +233,8 @@ __device__ __noinline__ int lp_search(const LpPart<T, TH>& sl, uint32_t lo, int 
   return have;
 }
 
+// MANY: the blocks of a cluster may share a row.  Six blocks of 256 threads per SM (40 registers), with alternatives of fp32 five:
+// 64 of 8192 x 32768, at 6 / 5 of 256 threads: bf16 170 / 176 us, fp32 237 / 223.
 template <typename T, bool TOP, int TH, bool MANY>
 __global__ void __launch_bounds__(TH, (TOP && sizeof(T) == 4 ? 5 : 6) * 256 / TH)
 logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
@@ -532,8 +537,7 @@ int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
     a.need = (a.top + a.J - 1) / a.J;
     return logprobs_launch<T, true, 256, true>(ctx, logits, a);
   }
-  // Short rows: what each warp does once per row weighs more than what more threads read at a time.  128 / 256 threads, us:
-  // 8192 x 32768 bf16, 64 alternatives 125 / 141, fp32 206 / 197; 2048 x 151936 bf16, 20 alternatives 147 / 126.
+  // Short rows: what each warp does once per row weighs more than what more threads read at a time.
   const int th = ag_row_threads(ctx, a.N, packets, LP_TOP_64, LP_TOP_128);
   return th == 64    ? logprobs_launch<T, true, 64, false>(ctx, logits, a)
          : th == 128 ? logprobs_launch<T, true, 128, false>(ctx, logits, a)

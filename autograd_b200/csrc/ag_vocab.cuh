@@ -299,7 +299,7 @@ __device__ __forceinline__ uint32_t ag_peer(const void* p, int rank) {
   return a;
 }
 // Stores to a block of the cluster that count themselves at a barrier of that block when they are there: no thread waits for them,
-// and there is no fence, which a barrier of the whole cluster would have (16384 x 32768 fp32, 4 blocks per row: a fifth of the time).
+// and there is no fence, which a barrier of the whole cluster would have (a sixth of the stalls of 4 blocks per row of 32768 fp32).
 __device__ __forceinline__ void ag_send(uint32_t to, float4 v, uint32_t bar) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
                "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar)

@@ -386,3 +386,24 @@ def test_two_streams_at_once():
         near(down(dev[6]), ref["dlogits"], ref["size"] * (400 + 16 * np.abs(ref["lp"])) * U + 2.0 ** -120, "gradient")
         c.close()
         free(*dev)
+
+
+def test_logits_of_weights_stored_by_token():
+    """Weights (V, C), as the CE head has them: the logits are the projection's backward product, dact += dout . w^T."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(33)
+    n, c, v = 70, 64, 500
+    hidden, w = (rng.standard_normal((n, c)) / 8).astype(np.float32), rng.standard_normal((v, c)).astype(np.float32)
+    th, tw, z = up(hidden), up(w), up(np.zeros((n, v), np.float32))
+    nbytes = ctx.linear_add_scratch_bytes(n, v, c)
+    ws = alloc.alloc((nbytes,), np.uint8)
+    ctx.linear_add_backward(th, None, tw, None, z, None, None, n, v, c, ag.AG_CE_3XTF32, ws, nbytes)
+    lp, ids = up(np.zeros(n, np.float32)), rng.integers(0, v, n)
+    tid = up(ids.astype(np.int32))
+    be.token_logprobs_forward(z, tid, lp)
+    want = R.token_logprobs(hidden.astype(np.float64) @ w.astype(np.float64).T, ids)[0]
+    # fp32-grade logits of size 1: 64 terms of at most 1/2, each product off by 2^-22 of its terms; twice that in a difference
+    near(down(lp), want, 2 * 64 * 2.0 ** -23 + (300 + 8 * np.abs(want)) * U, "log-probability")
+    ctx.synchronize()
+    alloc.free(ws)
+    free(th, tw, z, lp, tid)
