@@ -186,3 +186,16 @@ def test_tensors_that_do_not_fit_are_refused():
         with pytest.raises(TypeError):
             bad()
     assert not ctx.calls
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("name", ALL)
+def test_both_bindings_take_the_arguments(name, compiled):
+    """Tensors, integers, None and numbers in their places; a context that is null fails every call after that."""
+    calls = N.calls if compiled else N._CheckedCalls(N.lib)
+    values = {N._ptr: [_tensor((4, 64)), BASE, None, np.int64(BASE)], N._i64: [64], N._int: [4, np.int32(4)], N._f32: [1, 0.5]}
+    args = [values[t][i % len(values[t])] for i, t in enumerate(N.SIGNATURES[name][1][1:])]
+    with pytest.raises(N.AgError):
+        getattr(calls, name)(0, *args)
+    with pytest.raises((TypeError, ValueError)):
+        getattr(calls, name)(0, *args[:-1])
