@@ -145,10 +145,17 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
       if (const uint32_t bits = b[u * TH]) distill_mask(w[u], bits, T());
     ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
   }
-  for (; left > 0; left -= TH, p += TH, b += TH) {
-    uint4 w[1] = {*p};
-    distill_mask(w[0], *b, T());
-    ag_stat_add<false, T>(v, w, ag_largest(w, T()), c);
+  for (; left > 0; left -= 4 * TH, p += 4 * TH, b += 4 * TH) {
+    uint4 w[4][1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (left > u * TH) w[u][0] = p[u * TH];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (left > u * TH) {
+        distill_mask(w[u][0], b[u * TH], T());
+        ag_stat_add<false, T>(v, w[u], ag_largest(w[u], T()), c);
+      }
   }
   return v;
 }
@@ -235,7 +242,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   if (REST && edge_index >= 0 && s_marks[0] >> tid & 1) edge = -INFINITY;
 
   const AgStat mine = ag_stat_warp(REST ? distill_part_stat<T, BATCH, TH>(at, s_map, n, edge, c)
-                                          : ag_part_stat<false, T, BATCH, TH>(at, n, edge, c), c);
+                                          : ag_part_stat<false, T, BATCH, TH, !TRAIN>(at, n, edge, c), c);
   AgStat in = ag_stat_none();
   if (REST && warp < parts) {
     if (once) in = {x_id == x_id ? x_id : -INFINITY, x_id == -INFINITY ? 0.0f : x_id - x_id + 1.0f, 0.0f};

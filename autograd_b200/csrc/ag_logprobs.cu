@@ -477,7 +477,15 @@ logprobs_backward_kernel(const T* logits, const T* dres, T* dlogits, const LbArg
 #pragma unroll
     for (int u = 0; u < U; ++u) put(w[u], i + u * TH);
   }
-  for (; i < n; i += TH) put(__ldcs(at + i), i);
+  for (; i < n; i += 4 * TH) {  // what is left of a batch
+    uint4 w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * TH < n) w[u] = __ldcs(at + i + u * TH);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * TH < n) put(w[u], i + u * TH);
+  }
   if (edge_index >= 0) {
     float g = 0.0f, other;
     if (!none) local(x_edge, x_edge, g, other);

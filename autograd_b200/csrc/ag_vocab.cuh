@@ -256,7 +256,7 @@ struct AgRow {
 // Statistics of this thread's part of n packets, U at a time, and of its element of the edges (-inf without one).  `most` (null: not
 // wanted): the largest logit of each batch, and of each packet that is left behind the last whole batch, this thread's
 // TH (the threads of the block) apart, the first one that far behind `most`.
-template <bool WITH_T, typename T, int U, int TH>
+template <bool WITH_T, typename T, int U, int TH, bool AHEAD = true>
 __device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edge, float c, float* most = nullptr) {
   AgStat v = {edge == edge ? edge : -INFINITY, edge == -INFINITY ? 0.0f : edge - edge + 1.0f, 0.0f};  // NaN and inf - inf: a NaN for the sum
   const uint4* p = at + threadIdx.x;
@@ -269,11 +269,20 @@ __device__ __forceinline__ AgStat ag_part_stat(const uint4* at, int n, float edg
     if (most) *(most += TH) = m;
     ag_stat_add<WITH_T, T>(v, w, m, c);
   }
-  for (; left > 0; left -= TH, p += TH) {
-    const uint4 w[1] = {*p};
-    const float m = ag_largest(w, T());
-    if (most) *(most += TH) = m;
-    ag_stat_add<WITH_T, T>(v, w, m, c);
+  // what is left of a batch: all loads under way before the first is used, where there are registers for it (AHEAD)
+  constexpr int R = AHEAD ? 4 : 1;
+  for (; left > 0; left -= R * TH, p += R * TH) {
+    uint4 w[R][1];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+      if (left > u * TH) w[u][0] = p[u * TH];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+      if (left > u * TH) {
+        const float m = ag_largest(w[u], T());
+        if (most) *(most += TH) = m;
+        ag_stat_add<WITH_T, T>(v, w[u], m, c);
+      }
   }
   return v;
 }
