@@ -188,7 +188,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * (TH / 32), parts = (a.top + 31) / 32;
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
+  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + groups);
   const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
   DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);
   int* s_ids = reinterpret_cast<int*>(s_parts + (TH / 32));
@@ -252,7 +252,7 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   // gradient takes the logits' place: a store needs its operand, and instructions of a warp go in order.
   if (TRAIN && rank == 0 && tid < a.top) reinterpret_cast<volatile float*>(s_q)[tid] = x_id;
   const float4 word = make_float4(mine.m, mine.s, in.m, in.s);
-  const float4* told = TRAIN ? exchange.tell(0, word) : exchange.tell_first(word);
+  const float4* told = exchange.template tell<TRAIN>(word);
   if (!TRAIN && rank) return;
   AgStat out = ag_stat_none();
   in = ag_stat_none();

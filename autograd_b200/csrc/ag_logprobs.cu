@@ -241,7 +241,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ float4 s_box[];
   const int S = MANY || !TOP ? a.S : 1, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * (TH / 32);
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + 2 * groups);
+  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + groups);
   const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
   uint64_t* s_keys_bar = s_bars + 2;                                                   // every block's keys are at block 0
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], a multiple of four
@@ -285,7 +285,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(reached) : "f"(own.m));
   }
   const float4 word = make_float4(v.m, v.s, v.t, reached);
-  const float4* told = TOP ? exchange.tell(0, word) : exchange.tell_first(word);
+  const float4* told = exchange.template tell<TOP>(word);
   if (!TOP && (rank || tid >= 32)) return;
   v = lane < groups ? AgStat{told[lane].x, told[lane].y, told[lane].z} : ag_stat_none();
   if (lane + 32 < groups) v = ag_stat_merge(v, {told[lane + 32].x, told[lane + 32].y, told[lane + 32].z}, c);

@@ -42,7 +42,7 @@ static inline int ag_vocab_check(ag_ctx* ctx, const char* who, const AgVocabShap
   AG_REQUIRE(ctx, s.dtype == AG_F32 || s.dtype == AG_BF16, "%s: unknown dtype %d", who, s.dtype);
   AG_REQUIRE(ctx, s.temperature >= 1e-4f && s.temperature <= 1e4f, "%s: temperature %g outside 1e-4 to 1e4", who, s.temperature);
   AG_REQUIRE(ctx, s.top >= 0 && s.top <= max_top, "%s: %d tokens per row, up to %d", who, s.top, max_top);
-  // beyond 2^40 elements the products below would overflow before they could be compared with anything
+  // strides below 2^31: the products below stay below 2^64
   AG_REQUIRE(ctx, s.ld >= s.V && s.ld < (1ll << 31), "%s: row stride %lld smaller than V=%d, or too large", who, (long long)s.ld, s.V);
   AG_REQUIRE(ctx, logits || s.N == 0, "%s: null logits", who);
   const uintptr_t mask = s.size() - 1;
@@ -293,13 +293,9 @@ __device__ __forceinline__ int ag_cluster_rank() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// Every thread of every block of the cluster; S = 1: of the block.
-__device__ __forceinline__ void ag_cluster_sync(int S) {
-  if (S == 1) {
-    __syncthreads();
-  } else {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-  }
+// Every thread of every block of the cluster.
+__device__ __forceinline__ void ag_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 // address in block `rank` of what lies at p in this one
 __device__ __forceinline__ uint32_t ag_peer(const void* p, int rank) {
@@ -333,54 +329,39 @@ __device__ __forceinline__ void ag_wait_cluster(uint64_t* bar, uint32_t parity, 
   atomicOr(status, AG_STATUS_WAIT_EXPIRED);
 }
 
-// What each warp of a cluster tells all others about its part of a row: one float4 per warp, in turn at two places.  A block can be
-// one row ahead of another, never two: for the row between it waits for what all warps of the other have to tell, and they tell it
-// when they have read what came before.
+// What each warp of a cluster tells the others about its part of a row, once: one float4 per warp.  S = 1: a block by itself.
 template <int TH>
 struct AgExchange {
-  float4* box;      // [2][S * warps of a block]
-  uint64_t* bar;    // [2]
+  float4* box;    // [S * warps of a block]
+  uint64_t* bar;
   int S, rank;
   int* status;
   __device__ __forceinline__ void start() const {
     if (S == 1) return;
     if (threadIdx.x == 0) {
       ag_mbar_init(bar, 1);
-      ag_mbar_init(bar + 1, 1);
       ag_fence_mbar_init();
     }
-    ag_cluster_sync(S);  // all of them run, with barriers set up, before one sends
+    ag_cluster_sync();  // all of them run, with barriers set up, before one sends
   }
-  // to block 0 only, whose warps all get the box; the others get null and have no more to do here
-  __device__ __forceinline__ const float4* tell_first(float4 v) const {
-    const int lane = threadIdx.x & 31, at = rank * (TH / 32) + (threadIdx.x >> 5);
+  // To block 0 only, or to all; by whole warps, every lane with the same v.  The box is returned, in which all entries are then; null
+  // where nothing was sent to, which has no more to do here.
+  template <bool ALL>
+  __device__ __forceinline__ const float4* tell(float4 v) const {
+    const int lane = threadIdx.x & 31;
+    float4* to = box + rank * (TH / 32) + (threadIdx.x >> 5);
     if (S == 1) {
-      if (lane == 0) box[at] = v;
+      if (lane == 0) *to = v;
       __syncthreads();
       return box;
     }
-    if (lane == 0) ag_send(ag_peer(box + at, 0), v, ag_peer(bar, 0));
-    if (rank) return nullptr;
+    if (lane < (ALL ? S : 1)) ag_send(ag_peer(to, lane), v, ag_peer(bar, lane));
+    if (!ALL && rank) return nullptr;
     if (threadIdx.x == 0) ag_mbar_expect_tx(bar, S * (TH / 32) * 16);
     ag_wait_cluster(bar, 0, status);
     return box;
   }
-  // by whole warps, every lane with the same v; the box is returned, in which all entries are then
-  __device__ __forceinline__ const float4* tell(int turn, float4 v) const {
-    const int now = turn & 1, lane = threadIdx.x & 31;
-    float4* all = box + now * S * (TH / 32);
-    float4* to = all + rank * (TH / 32) + (threadIdx.x >> 5);
-    if (S == 1) {
-      if (lane == 0) *to = v;
-      __syncthreads();
-    } else {
-      if (lane < S) ag_send(ag_peer(to, lane), v, ag_peer(bar + now, lane));
-      if (threadIdx.x == 0) ag_mbar_expect_tx(bar + now, S * (TH / 32) * 16);
-      ag_wait_cluster(bar + now, (turn >> 1) & 1, status);
-    }
-    return all;
-  }
-  static constexpr size_t bytes(int S) { return 2 * (size_t)S * (TH / 32) * 16 + 16; }
+  static constexpr size_t bytes(int S) { return (size_t)S * (TH / 32) * 16 + 16; }
 };
 
 __device__ __forceinline__ void ag_peer_store(uint32_t to, int v) {
@@ -403,7 +384,6 @@ __device__ __forceinline__ uint32_t ag_order(float x) {
 __device__ __forceinline__ float ag_of_order(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);  // 0xfffffffe becomes a NaN again
 }
-
 
 #endif  // __CUDACC__
 
