@@ -141,6 +141,7 @@ struct LpPart {
   __device__ __forceinline__ void each(F f) const {
     constexpr int NV = AG_PACKET<T>;
     if (edge_index >= 0) f(edge, edge_index);
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += TH) {
       float x[NV];
       ag_widen(at[i], x);
@@ -168,11 +169,14 @@ __device__ __noinline__ int lp_search(const LpPart<T, TH>& sl, uint32_t lo, int 
     return c;
   };
   bool fits = false;
-  while (lo < hi && !fits) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+  lo = max(lo, ag_order(-INFINITY));
+  // first whether the logits that equal lo make up the number: rows where fewer than `top` tokens are allowed, and all others are
+  // masked with one value
+  for (bool first = true; lo < hi && !fits; first = false) {
+    const uint32_t mid = first ? lo + 1 : lo + (hi - lo) / 2 + 1;
     const int c = count_from(mid);
     if (c >= top) lo = mid, fits = c <= cap;
-    else hi = mid - 1;
+    else hi = mid - 1;  // the first time lo itself
   }
   // fits: all that reach lo.  Otherwise lo is the top-th largest itself: all above it (fewer than top), and then equal ones.
   if (threadIdx.x == 0) *s_count = 0;

@@ -290,8 +290,9 @@ int ag_linear_add_backward(ag_ctx* ctx, const float* dout, const float* act, con
  * No counterpart in the reference's fused ops; its rollout sampler takes top-k and softmax of logits
  * (backend.py:2260-2494), its policy-gradient loss the log-probability of a token (rl_autograd.py:518-524).
  * Rows of logits, row i at logits + i * ld elements (ld >= V; columns from V on are not read), AG_F32 or
- * AG_BF16; V up to AG_VOCAB_MAX.  With z = x / temperature (1e-4 to 1e4), m = max x and L = ln sum exp(z - m / temperature):
- *   logprob[i] = z_id - m / temperature - L of token ids[i]; 0 where the id is outside [0, V)
+ * AG_BF16; V up to AG_VOCAB_MAX.  With temperature 1e-4 to 1e4, m = max x and
+ * L = ln sum exp((x - m) / temperature):
+ *   logprob[i] = (x_id - m) / temperature - L of token ids[i]; 0 where the id is outside [0, V)
  *   entropy[i] = - sum p ln p;  stats[i] = (m, L, entropy, 0), four floats, 16-byte aligned: what the backward call needs
  *   top_ids[i][k], top_logprobs[i][k], k < top <= AG_TOP_MAX: the likeliest tokens, larger logits first, equal ones
  *   by the lower index (NaN counts as largest)

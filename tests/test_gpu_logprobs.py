@@ -202,6 +202,21 @@ def test_alternatives_of_rows_with_many_equal_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("mask", [-np.inf, -1e9, None])
+def test_alternatives_where_few_tokens_are_allowed(mask, dtype):
+    """Fewer than are asked for, or hardly more; the others masked with -inf, a large number, the lowest one."""
+    rng = np.random.default_rng(6)
+    mask = LOWEST[dtype] if mask is None else mask
+    for n, v in ((600, 5003), (40, 32768), (3, 50257)):
+        x = np.full((n, v), mask, np.float32)
+        for r in range(n):
+            x[r, rng.permutation(v)[:(0, 1, 5, 19, 20, 21, 60)[r % 7]]] = rng.standard_normal((0, 1, 5, 19, 20, 21, 60)[r % 7])
+        x = rounded(x, dtype)
+        for top in (20, 128):
+            check_forward(x, np.zeros(n, np.int64), forward(x, np.zeros(n), dtype, top), top, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows", [1, 2, 9, 64, 147, 148, 149, 300, 1200, 5000])
 def test_forward_row_counts(rows, dtype):
     rng = np.random.default_rng(rows)
