@@ -316,6 +316,11 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     least = lp_threshold<TH>(each, ag_order(reached), ag_order(v.m), a.top, a.top + (a.top >> 1) + 16, hist);
   }
   const float bound = ag_of_order(least);
+  // Counted even where there is no room: warps are at different places here, so that any of them may come behind `cap` others.
+  auto take = [&](float x, int index) {
+    const int to = atomicAdd(n_keys, 1);
+    if (to < a.cap) keys[to] = lp_key(x, index);
+  };
   for (int b = 0; b < entries; ++b) {
     if (most[b * TH + tid] < bound) continue;
     const int k = atomicAdd(n_keys + 1, 1);
@@ -323,7 +328,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   }
   __syncthreads();
   const int listed = min(n_keys[1], a.cap);
-  if (edge_index >= 0 && !(edge < bound)) keys[atomicAdd(n_keys, 1)] = lp_key(edge, edge_index);
+  if (edge_index >= 0 && !(edge < bound)) take(edge, edge_index);
   for (int k = tid; k < listed * LP_BATCH; k += TH) {
     const int b = batches[k / LP_BATCH] / TH, of = batches[k / LP_BATCH] % TH, whole = lp_whole<TH>(n - of);
     if (b >= whole && k % LP_BATCH) continue;  // a packet by itself
@@ -334,8 +339,8 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
 #pragma unroll
     for (int e = 0; e < AG_PACKET<T>; ++e) hits |= x[e] < bound ? 0u : 1u << e;
     for (; hits; hits &= hits - 1) {
-      const int index = first + i * AG_PACKET<T> + __ffs(hits) - 1, to = atomicAdd(n_keys, 1);
-      if (to < a.cap) keys[to] = lp_key(Pack<T>::load1(r.x + index), index);
+      const int index = first + i * AG_PACKET<T> + __ffs(hits) - 1;
+      take(Pack<T>::load1(r.x + index), index);
     }
   }
   __syncthreads();

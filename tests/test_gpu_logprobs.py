@@ -414,3 +414,19 @@ def test_recorded_calls_follow_their_inputs():
         ctx.drop_recording(g)
     free(*t, *grad, tid, a, *(w for o in out for w in o.values()))
     check_clean_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(700, 1003), (700, 9003), (700, 20003), (300, 33003), (24, 33003), (3, 50257)])
+def test_edges_of_rows_whose_logits_all_reach_the_bound(n, v, dtype):
+    """Rows that start and end between two 16-byte boundaries, where far more logits pass than there is room for: what lies beside
+    the packets finds the list full, whichever warp comes first.  With 64, 128, 256 threads per row and with blocks that share one."""
+    rng = np.random.default_rng(v)
+    x = np.zeros((n, v), np.float32)
+    x[1::3] = 2.5
+    x[2::3] = rng.integers(0, 2, (len(x[2::3]), v))
+    x = rounded(x, dtype)
+    for top in (1, 2, 20, 128):
+        for shift, pad in ((1, 0), (3, 1), (0, 2)):
+            check_forward(x, np.zeros(n, np.int64), forward(x, np.zeros(n), dtype, top, 1.0, v + pad, shift), top, 1.0)
+    check_clean_status()
