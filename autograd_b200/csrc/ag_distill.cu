@@ -8,6 +8,9 @@
 //
 // p_rest is summed over the unlisted logits themselves: 1 - sum_k p_id_k would keep nothing of a small rest.  A slot with a
 // negative id is not in use.
+// p_j / p_rest of an unlisted token is at most 1, but neither p_j nor 1 / p_rest need be a number of 32 bits: where ln p_rest is
+// below DI_FAR it is one power, 2^((x_j - m') c - log2 sum') with the largest logit m' and the sum of the unlisted tokens alone,
+// and p_j (Q + r) lies below its rounding (2^-46 against r / 2^24).
 //
 // Loss, and loss with gradient: a block, or a cluster of 2 to 8, streams a row through registers, thread k has slot k.  A bit per
 // token tells what is listed: in the sum over the others those logits count as -inf, and the listed ones are added from the threads
@@ -32,6 +35,7 @@ constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;
 // to be read again.  Us: 16384 x 32768 fp32, 1 / 2 / 4 blocks per row (97, 48, 24 MB) 940 / 727 / 933; 8192 x 50257 bf16, 1 / 2 (60,
 // 30 MB) 344 / 406; 4096 x 151936 bf16, 2 / 4 (90, 45 MB) 305 / 284.
 constexpr int64_t DI_IN_FLIGHT = 64 << 20;
+constexpr float DI_FAR = -32.0f;  // ln p_rest
 
 struct DistillArgs {
   const int32_t* ids;
@@ -39,7 +43,7 @@ struct DistillArgs {
   const float* row_scale;  // null: 1 / N
   const float* dloss;      // null: no gradient
   float* row_loss;
-  float4* stats;           // (m, L, ln p_rest, 0)
+  float4* stats;           // (m, L, ln p_rest, 0), of a far rest (m, L, 1 + ln sum', m')
   int64_t N, ld, ld_grad;
   int V, top, rest;
   float inv_tau, inv_n;
@@ -104,9 +108,17 @@ __device__ __forceinline__ void distill_slot(const DistillList& l, float t, bool
   log_q = d - l.log_sum;
   q = l.used ? expf(d) * l.inv_sum : 0.0f;
 }
-// what a listed and an unlisted token's p are multiplied with, before the row's scale
-__device__ __forceinline__ float distill_outside(const DistillList& l, float log_rest) {
-  return l.mass + l.left - (l.left != 0.0f && log_rest > -INFINITY ? l.left * expf(-log_rest) : 0.0f);
+// The gradient of the unlisted tokens as scale * 2^((x + ref) c + shift).  The listed ones, whose place it takes for a while, may
+// be anything.  log_rest = ln p_rest; far: p / p_rest = 2^((x - m_out) c - log_out * log2(e)).  Nothing is left of p_rest = 0.
+struct DistillDense {
+  float scale, ref, shift;
+};
+__device__ __forceinline__ bool distill_far(float log_rest) { return log_rest < DI_FAR && log_rest > -INFINITY; }
+__device__ __forceinline__ DistillDense distill_unlisted(const DistillList& l, float s, float m, float L, bool far, float log_rest,
+                                                         float m_out, float log_out) {
+  if (far && l.left != 0.0f) return {-s * l.left, -m_out, -log_out * AG_LOG2E};
+  const float rest = l.left != 0.0f && log_rest > -INFINITY ? l.left * expf(-log_rest) : 0.0f;
+  return {s * (l.mass + l.left - rest), -m, -L * AG_LOG2E};
 }
 __device__ __forceinline__ float distill_scale(const DistillArgs& a, int64_t row) {
   const float w = a.row_scale ? a.row_scale[row] : a.inv_n;
@@ -160,9 +172,9 @@ __device__ __forceinline__ AgStat distill_part_stat(const uint4* at, const uint8
   return v;
 }
 
-// outside * p of a packet's logits, log2 p = (x + ref) c + shift
+// scale * 2^((x + ref) c + shift) of a packet's logits
 template <typename T>
-__device__ __forceinline__ void distill_dense(const uint4& w, uint64_t ref2, uint64_t c2, uint64_t shift2, float outside,
+__device__ __forceinline__ void distill_dense(const uint4& w, uint64_t ref2, uint64_t c2, uint64_t shift2, float scale,
                                               float (&g)[AG_PACKET<T>]) {
   float x[AG_PACKET<T>];
   ag_widen(w, x);
@@ -170,8 +182,8 @@ __device__ __forceinline__ void distill_dense(const uint4& w, uint64_t ref2, uin
   for (int e = 0; e < AG_PACKET<T>; e += 2) {
     float d0, d1;
     ag_unpair(ag_fma2(ag_add2(ag_pair(x[e], x[e + 1]), ref2), c2, shift2), d0, d1);
-    g[e] = outside * ag_ex2(d0);  // not as a pair: 16384 x 32768 fp32 took 776 us that way, 727 this way
-    g[e + 1] = outside * ag_ex2(d1);
+    g[e] = scale * ag_ex2(d0);  // not as a pair: 16384 x 32768 fp32 took 776 us that way, 727 this way
+    g[e + 1] = scale * ag_ex2(d1);
   }
 }
 
@@ -287,15 +299,15 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
     }
   }
   const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
-  const float shift = none ? 0.0f : -L * AG_LOG2E;
+  const bool far = REST && distill_far(log_rest);
   T* g_row = dlogits + row * a.ld_grad;
   if (TRAIN) {
-    const float outside = none ? 0.0f : s * distill_outside(list, log_rest), ref = none ? 0.0f : -m;
-    const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
+    const DistillDense u = distill_unlisted(list, s, m, L, far, log_rest, out.m, logf(out.s));
+    const uint64_t ref2 = ag_pair(u.ref, u.ref), c2 = ag_pair(c, c), shift2 = ag_pair(u.shift, u.shift);
     const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0;
     auto put = [&](const uint4& w, int i) {
       float g[NV];
-      distill_dense<T>(w, ref2, c2, shift2, outside, g);
+      distill_dense<T>(w, ref2, c2, shift2, u.scale, g);
       ag_store_packet<T>(g_row + first + (int64_t)i * NV, g, packets);
     };
     constexpr int U = 4;
@@ -312,20 +324,20 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
       for (int u = 0; u < U; ++u) put(w[u], i + u * TH);
     }
     for (; i < n; i += TH) put(at[i], i);
-    if (edge_index >= 0) Pack<T>::store1(g_row + edge_index, none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift));
+    if (edge_index >= 0) Pack<T>::store1(g_row + edge_index, none ? 0.0f : u.scale * ag_ex2((x_edge + u.ref) * c + u.shift));
   }
   __syncthreads();  // the loss of each warp is there; the entries of listed tokens are written once more
   if (rank == 0 && tid == 0) {
     float sum = list.left != 0.0f ? list.left * (logf(list.left) - log_rest) : 0.0f;
     for (int w = 0; w < parts; ++w) sum += s_sum[w];
     a.row_loss[row] = list.used ? sum : 0.0f;
-    if (a.stats) a.stats[row] = make_float4(m, L, log_rest, 0.0f);
+    if (a.stats) a.stats[row] = far ? make_float4(m, L, 1.0f + logf(out.s), out.m) : make_float4(m, L, log_rest, 0.0f);
   }
   if (TRAIN && once) {
     if (s_marks[1])
       for (int k = tid + 1; k < a.top; ++k)
         if (s_ids[k] == id) q += s_q[k];
-    const float p = ag_ex2((x_id - m) * c + shift);
+    const float p = ag_ex2((x_id - m) * c - L * AG_LOG2E);
     Pack<T>::store1(g_row + id, none ? 0.0f : s * (p * (list.mass + list.left) - q));
   }
 }
@@ -382,9 +394,10 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
     s_q[tid] = q;
   }
   const bool none = s == 0.0f || !list.used || (m == -INFINITY && L == -INFINITY);
-  const float outside = none ? 0.0f : s * distill_outside(list, st.z);
-  const float ref = none ? 0.0f : -m, shift = none ? 0.0f : -L * AG_LOG2E;
-  const uint64_t ref2 = ag_pair(ref, ref), c2 = ag_pair(c, c), shift2 = ag_pair(shift, shift);
+  // A far rest as the loss leaves it; ln p_rest that comes from elsewhere serves as well, to 2^-22 |ln p_rest| of the result.
+  const bool left = REST && st.z >= 0.5f, far = REST && (left || distill_far(st.z));
+  const DistillDense v = distill_unlisted(list, s, m, L, far, st.z, left ? st.w : m, left ? st.z - 1.0f : L + st.z);
+  const uint64_t ref2 = ag_pair(v.ref, v.ref), c2 = ag_pair(c, c), shift2 = ag_pair(v.shift, v.shift);
   const bool packets = (((uintptr_t)(g_row + first)) & 15) == 0, d_packets = (((uintptr_t)(d_row + first)) & 15) == 0;
   auto add = [&](float (&g)[NV], int i) {
     const int to = first + i * NV;
@@ -398,7 +411,7 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
   };
   auto put = [&](const uint4& w, int i) {
     float g[NV];
-    distill_dense<T>(w, ref2, c2, shift2, outside, g);
+    distill_dense<T>(w, ref2, c2, shift2, v.scale, g);
     add(g, i);
   };
   int i = tid;
@@ -417,7 +430,7 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
   for (; i < n; i += TH) put(__ldcs(at + i), i);
   if (edge_index >= 0) {
     const float d = d_row ? Pack<T>::load1(d_row + edge_index) : 0.0f;
-    Pack<T>::store1(g_row + edge_index, (none ? 0.0f : outside * ag_ex2((x_edge - m) * c + shift)) + d);
+    Pack<T>::store1(g_row + edge_index, (none ? 0.0f : v.scale * ag_ex2((x_edge + v.ref) * c + v.shift)) + d);
   }
   __syncthreads();  // the entries of listed tokens are written once more
   if (own) {
@@ -428,7 +441,7 @@ distill_backward_kernel(const T* logits, const T* dres, T* dlogits, const Distil
         once &= k >= tid;
         q += s_q[k];
       }
-    const float p = ag_ex2((x_id - m) * c + shift);
+    const float p = ag_ex2((x_id - m) * c - L * AG_LOG2E);
     if (once) Pack<T>::store1(g_row + id, (none ? 0.0f : s * (p * (list.mass + list.left) - q)) + d_id);
   }
 }

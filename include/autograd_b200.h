@@ -321,7 +321,12 @@ int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, cons
  *   row_loss[i] = sum_k q_k (ln q_k - ln p_id_k) + r (ln r - ln p_rest)
  *   loss = sum_i row_scale[i] row_loss[i], or their mean without row_scale; rows of weight 0 take no part
  * A row whose slots are all unused, or -inf, has loss 0 and gradient 0.  A token that is listed twice counts with both
- * its masses.  stats[i] = (m, L, ln p_rest, 0) for the backward call, 16-byte aligned; loss and stats may be NULL.
+ * its masses.  stats[i] for the backward call, 16-byte aligned: (m, L, ln p_rest, 0), or where ln p_rest is below -32
+ * (m, L, 1 + ln sum exp((x - m') / temperature), m') with the sum over the tokens not listed and m' their largest logit,
+ * from which p_j / p_rest keeps its digits however small p_rest is (ln p_rest itself is taken there too, and costs
+ * 2^-22 |ln p_rest| of them).  loss and stats may be NULL.
+ * p_rest = 0 (all tokens not listed at -inf, or ln p_rest beyond the largest 32-bit number) with r > 0: the row's loss
+ * is +inf, its gradient has no term of the rest.
  * backward: dlogits = (dres ? dres : 0) + dloss[0] * weight / temperature
  *                     * (p_j (sum q + r) - sum of q_k with id_k = j - [j not listed] r p_j / p_rest)
  * Neither loss nor gradient has the factor temperature^2 that some training recipes put in the weight.

@@ -86,9 +86,11 @@ def teacher(ids, t, vocab, temperature=1.0, rest=False):
 
 
 def distill(x, ids, t, row_scale=None, dloss=1.0, temperature=1.0, rest=False):
-    """loss, row_loss, d logits, and for bounds of their errors: the sizes of the terms of both, ln p, ln p_rest."""
+    """loss, row_loss, d logits, and for bounds of their errors: the sizes of the terms of both, ln p, ln p_rest, and `share`, the
+    logarithm of an unlisted token's part of p_rest.  p_rest may be no number of 64 bits: its logarithm and the shares are formed
+    from the unlisted logits alone."""
     n, v = x.shape
-    lp, m, _ = log_softmax(x, temperature)
+    lp, m, total = log_softmax(x, temperature)
     used, q, log_q, left, row = teacher(ids, t, v, temperature, rest)
     at = np.where(used, ids, 0).astype(np.int64)
     with np.errstate(all="ignore"):
@@ -97,25 +99,26 @@ def distill(x, ids, t, row_scale=None, dloss=1.0, temperature=1.0, rest=False):
         rows = np.arange(n)[:, None].repeat(ids.shape[1], 1)
         np.add.at(mass, (rows[used], at[used]), q[used])
         listed[rows[used], at[used]] = True
-        outside = np.where(listed, 0.0, p).sum(1)
+        share, m_out, total_out = log_softmax(np.where(listed, -np.inf, np.asarray(x, F64)), temperature)
+        log_rest = np.where(m_out == -np.inf, -np.inf, (m_out - m) / temperature + total_out - total)
+        part = np.exp(share)
         some = used & (q > 0)
         slot_lp = np.take_along_axis(lp, at, 1)
         row_loss = np.where(some, q * (log_q - slot_lp), 0.0).sum(1)
         size = np.where(some, q * (np.abs(log_q) + np.abs(slot_lp)), 0.0).sum(1) + 1.0
         has = left > 0
-        row_loss = row_loss + np.where(has, left * (np.log(left) - np.log(outside)), 0.0)
-        size = size + np.where(has, np.abs(np.log(left)) + np.abs(np.log(outside)), 0.0)
+        row_loss = row_loss + np.where(has, left * (np.log(left) - log_rest), 0.0)
+        size = size + np.where(has, np.abs(np.log(left)) + np.abs(log_rest), 0.0)
         row_loss = np.where(row, row_loss, 0.0)
         weight = np.full(n, 1.0 / n) if row_scale is None else np.asarray(row_scale, F64)
         take = weight != 0
         loss = np.sum(weight[take] * row_loss[take])
         full = (q.sum(1) + left)[:, None]
-        ratio = np.where(has & (outside > 0), left / outside, 0.0)[:, None]
+        has = (has & (m_out != -np.inf))[:, None]
         s = (dloss * weight / temperature)[:, None]
-        away = np.where(listed, 0.0, p)
-        g = s * (p * full - mass - ratio * away)
-        gsize = np.abs(s) * (p * full + mass + (ratio + np.where(has & (outside > 0), 0.1 / outside, 0.0)[:, None]) * away)
+        g = s * (p * full - mass - np.where(has, left[:, None] * part, 0.0))
+        gsize = np.abs(s) * (p * full + mass + np.where(has, (left[:, None] + 0.1) * part, 0.0))
     still = (~take | ~row | (np.asarray(x) == -np.inf).all(1) | (s[:, 0] == 0))[:, None]
     return {"loss": loss, "row_loss": row_loss, "loss_size": size, "dlogits": np.where(still, 0.0, g),
-            "size": np.where(still, 0.0, gsize), "lp": lp, "log_rest": np.log(outside, where=outside > 0, out=np.full(n, -np.inf)),
+            "size": np.where(still, 0.0, gsize), "lp": lp, "log_rest": log_rest, "share": share,
             "weight": weight}

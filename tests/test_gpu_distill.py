@@ -13,7 +13,7 @@ import autograd_b200 as ag
 from autograd_b200.backend import bf16_bits_to_f32, f32_to_bf16_bits
 from gpu_util import check_clean_status, down, empty, env, free, up
 from oracle import vocab_rows as R
-from test_gpu_logprobs import SENTINEL, U, fetch, near, rounded, rows_of, store, words
+from test_gpu_logprobs import LOWEST, SENTINEL, U, fetch, near, rounded, rows_of, store, words
 
 pytestmark = pytest.mark.gpu
 
@@ -407,3 +407,92 @@ def test_logits_of_weights_stored_by_token():
     ctx.synchronize()
     alloc.free(ws)
     free(th, tw, z, lp, tid)
+
+
+GAPS = [5.0, 20.0, 30.0, 34.0, 60.0, 80.0, 90.0, 95.0, 110.0, 200.0, 1e3, 3e4]
+
+
+def far_rests(rng, n, v, top, dtype, temperature):
+    """Rows whose unlisted tokens together have e^-5 to e^-30000 of the student's mass, the last four of every sixteen with those
+    masked by a finite number; lists of `top` tokens (at most half) that leave 0.01 to 0.5 of the teacher's mass."""
+    ids = np.stack([rng.permutation(v)[:top] for _ in range(n)]).astype(np.int32)
+    x = rng.standard_normal((n, v))
+    masks = [-1e4, -1e9, -1e30 if temperature < 1 else LOWEST[dtype], -65504.0]
+    for i in range(n):
+        k = i % 16
+        listed = x[i, ids[i]].copy()
+        x[i] = x[i] * temperature - (GAPS[k] + np.log(v)) * temperature if k < 12 else masks[k - 12]
+        x[i, ids[i]] = listed * temperature
+    t = rng.standard_normal((n, top))
+    t = t - np.log(np.exp(t).sum(1, keepdims=True)) + np.log(rng.uniform(0.5, 0.99, (n, 1)))
+    return rounded(x.astype(np.float32), dtype), ids, t.astype(np.float32)
+
+
+def check_far(x, ids, t, dtype, temperature, got, dres=None, made=False, row_scale=None, dloss=1.0):
+    """An unlisted token's p is off by (400 + 16 |ln p|) u of itself, its part of p_rest by that with its own logarithm for ln p: it is
+    one power, from the unlisted tokens' statistics.  Down to ln p_rest = -32 it comes from p and p_rest instead, where ln p_rest
+    adds to the logarithm and what is flushed below 2^-126 is multiplied by r / p_rest; with statistics made from ln p_rest at any."""
+    ref = R.distill(x, ids, t, row_scale, np.float32(dloss), temperature, True)
+    near(got["row_loss"], ref["row_loss"], 400 * U * ref["loss_size"], "loss of a row")
+    _, q, _, left, _ = R.teacher(ids, t, x.shape[1], temperature, True)
+    with np.errstate(all="ignore"):
+        p, part = np.exp(ref["lp"]), np.exp(ref["share"])
+        rest = np.abs(ref["log_rest"])[:, None]
+        s = np.abs(dloss * ref["weight"] / temperature)[:, None]
+        mass = np.zeros(x.shape)
+        np.add.at(mass, (np.arange(len(x))[:, None], ids), q)
+        full = (q.sum(1) + left)[:, None]
+        by = np.where(np.isfinite(ref["share"]), np.abs(ref["share"]), 0.0) + np.where(made | (rest < 33), rest, 0.0)
+        bound = s * U * ((p * full + mass) * (400 + 16 * np.where(p > 0, np.abs(ref["lp"]), 0.0)) + (left[:, None] + 0.1) * part * (400 + 16 * by))
+        bound = bound + s * 2.0 ** -125 * np.where(rest < 33, 1 + np.exp(np.minimum(rest, 33)), 1.0) + 2.0 ** -120
+    g = ref["dlogits"]
+    if dres is not None:
+        g, bound = g + dres, bound + 2 * U * (np.abs(dres) + np.abs(g))
+    if dtype == "bf16":
+        bound = bound + np.abs(g) * 2.0 ** -8 + 2.0 ** -133
+    near(got["dlogits"], g, bound, "gradient")
+    return ref
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [1.0, 0.1, 3.0])
+@pytest.mark.parametrize("n,v,top", [(16, 61, 9), (32, 1003, 40), (700, 641, 19), (300, 20003, 64), (16, 50257, 256), (1, 32768, 20)])
+def test_a_rest_that_the_student_gives_almost_nothing(n, v, top, temperature, dtype):
+    """The gradient into the unlisted tokens sums to r whatever p_rest is: neither p nor 1 / p_rest has to be a number for that."""
+    rng = np.random.default_rng(n + v)
+    x, ids, t = far_rests(rng, n, v, top, dtype, temperature)
+    if n == 1:
+        x[0, np.setdiff1d(np.arange(v), ids[0])] = -1e3 * temperature
+        x = rounded(x, dtype)
+    kw = dict(temperature=temperature, rest=True)
+    for what in ("both", "apart"):
+        got = run(x, ids, t, dtype, what, **kw)
+        ref = check_far(x, ids, t, dtype, temperature, got)
+        check_far(x, ids, t, dtype, temperature, run(x, ids, t, dtype, what, place="logits", ld=v + 3, shift=1, **kw))
+        far = ref["log_rest"] < -32
+        assert far.any() and np.isfinite(got["dlogits"]).all()
+    w = rng.random(n)
+    dres = rounded(rng.standard_normal((n, v)).astype(np.float32), dtype)
+    got = run(x, ids, t, dtype, "apart", dres=dres, row_scale=w, dloss=0.6, **kw)
+    check_far(x, ids, t, dtype, temperature, got, dres, row_scale=w.astype(np.float32), dloss=0.6)
+    check_clean_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradient_from_the_logarithm_of_a_small_rest(dtype):
+    """Statistics (m, L, ln p_rest, 0) that a program has worked out itself, also where the loss leaves others."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(21)
+    n, v, top = 32, 1003, 40
+    x, ids, t = far_rests(rng, n, v, top, dtype, 1.0)
+    keep = np.arange(n) % 16 < 11  # down to e^-1000
+    x, ids, t = x[keep], ids[keep], t[keep]
+    n = len(x)
+    ref = R.distill(x, ids, t, rest=True)
+    _, m, total = R.log_softmax(x)
+    st = np.stack([m, total, ref["log_rest"], np.zeros(n)], 1).astype(np.float32)
+    tx, ti, tt, ts, one, g = up(words(x, dtype)), up(ids), up(t), up(st), up(np.ones(1, np.float32)), up(words(np.zeros((n, v), np.float32), dtype))
+    ctx.distill_backward(tx, v, ti, tt, None, ts, one, None, g, v, n, v, top, 1.0, ag.AG_DISTILL_REST, 1 if dtype == "bf16" else 0)
+    got = fetch(g, n * v, dtype).reshape(n, v)
+    check_far(x, ids, t, dtype, 1.0, {"row_loss": ref["row_loss"], "dlogits": got}, made=True)
+    free(tx, ti, tt, ts, one, g)

@@ -52,6 +52,25 @@ def test_gradient_of_distillation_is_its_derivative(temperature, rest):
     assert got["row_loss"][3] == 0 and not got["dlogits"][3].any()
 
 
+@pytest.mark.parametrize("gap", [10.0, 100.0, 1000.0])
+def test_gradient_of_a_small_rest_is_its_derivative(gap):
+    """The unlisted tokens have e^-gap of the student's mass: no number of 64 bits in the last case."""
+    rng = RNG(5)
+    x = rng.standard_normal((3, 11))
+    ids = np.array([[1, 4, 10], [2, 0, 3], [5, 5, 0]])
+    t = np.log(rng.random((3, 3)) * 0.3)
+    listed = np.zeros(x.shape, bool)
+    np.put_along_axis(listed, ids, True, 1)
+    x = np.where(listed, x, x - gap)
+    got = R.distill(x, ids, t, rest=True)
+    diff = _differences(lambda z: R.distill(z, ids, t, rest=True)["loss"], x, 1e-4)
+    # rounding 1e-16 gap / step = 1e-9, third derivative times step^2 / 6 = 2e-9
+    assert np.max(np.abs(got["dlogits"] - diff)) < 1e-8
+    left = 1 - np.exp(t).sum(1)
+    # what flows into them is p_rest (Q + r) - r, a third of which is the mean's
+    assert np.allclose(np.where(listed, 0.0, got["dlogits"]).sum(1) * 3, np.exp(got["log_rest"]) - left, rtol=1e-9, atol=0)
+
+
 # ---------------------------------------------------------------------------- refusals of the C interface
 # A context of zeros is enough for calls that are refused before they reach a device; one that is not refused fails to launch
 # with another code.
