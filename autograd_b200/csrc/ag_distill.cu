@@ -2,7 +2,7 @@
 // gradient.  With p = softmax(x / temperature) over the V tokens, slots k of the row's list with token id_k and value t_k:
 //
 //   RENORM  q = softmax(t / temperature) over the slots, r = 0
-//   REST    q_k = exp(t_k), r = max(0, 1 - sum q): t are log-probabilities, r what they leave to all other tokens together
+//   REST    q_k = exp(t_k), r = 1 - sum q, none up to DI_LEAST: t are log-probabilities, r what they leave to all other tokens together
 //   row_loss = sum_k q_k (ln q_k - ln p_id_k) + r (ln r - ln p_rest),  p_rest = sum of p over the tokens not listed
 //   d logits_j = s / temperature (p_j (Q + r) - sum_{k: id_k = j} q_k - r [j not listed] p_j / p_rest),  Q = sum q
 //
@@ -36,6 +36,11 @@ constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;
 // 30 MB) 344 / 406; 4096 x 151936 bf16, 2 / 4 (90, 45 MB) 305 / 284.
 constexpr int64_t DI_IN_FLIGHT = 64 << 20;
 constexpr float DI_FAR = -32.0f;  // ln p_rest
+// What 1 - sum q may be of a list that leaves nothing: of log-probabilities t in 32 bits, each within 7 u |t| and together with exp
+// 25 u (u = 2^-24: differences from the largest logit, their product, the logarithm of the sum, its roundings, t's own, exp), of a
+// distribution over 256 tokens at most, sum q |t| <= ln 256: 7 * 5.6 + 25 = 64 u.  Against a p_rest of 0, or of forbidden tokens,
+// such an r would count without limit.
+constexpr double DI_LEAST = 64.0 / (1 << 24);
 
 struct DistillArgs {
   const int32_t* ids;
@@ -91,7 +96,7 @@ __device__ __forceinline__ DistillList distill_list(const DistillPart* part, int
     for (int o = 4; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
     mass = __shfl_sync(0xffffffffu, mass, 0);
     l.mass = (float)mass;
-    l.left = (float)(1.0 - mass > 0.0 ? 1.0 - mass : mass != mass ? mass : 0.0);
+    l.left = (float)(1.0 - mass > DI_LEAST ? 1.0 - mass : mass != mass ? mass : 0.0);
   } else {
     float sum = ag_warp_sum(p.m == -INFINITY ? 0.0f : (float)p.sum * expf((p.m - l.m) * inv_tau));
     if (nan) sum = NAN;

@@ -316,8 +316,9 @@ int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, cons
  * (1 to AG_DISTILL_MAX): teacher_ids[i][k], negative = slot not in use, V and more = not in use and AG_STATUS_BAD_INDEX;
  * teacher_logits[i][k] = t_k.
  *   AG_DISTILL_RENORM: q = softmax(t / temperature) over the slots, r = 0 (t may be log-probabilities as well)
- *   AG_DISTILL_REST:   q_k = exp(t_k), t the teacher's log-probabilities at this temperature; r = max(0, 1 - sum q), its
- *                      mass on all other tokens, is compared with p_rest, the student's on the same tokens
+ *   AG_DISTILL_REST:   q_k = exp(t_k), t the teacher's log-probabilities at this temperature; r = 1 - sum q, its
+ *                      mass on all other tokens, is compared with p_rest, the student's on the same tokens.  Up to
+ *                      2^-18 r counts as 0: that is what roundings leave of a list of all the tokens there are
  *   row_loss[i] = sum_k q_k (ln q_k - ln p_id_k) + r (ln r - ln p_rest)
  *   loss = sum_i row_scale[i] row_loss[i], or their mean without row_scale; rows of weight 0 take no part
  * A row whose slots are all unused, or -inf, has loss 0 and gradient 0.  A token that is listed twice counts with both

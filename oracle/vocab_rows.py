@@ -8,6 +8,7 @@ from __future__ import annotations
 import numpy as np
 
 F64 = np.float64
+LEAST_REST = 2.0 ** -18   # what the roundings of a list in 32 bits can leave of a distribution
 
 
 def log_softmax(x, temperature=1.0):
@@ -68,7 +69,7 @@ def token_logprobs_backward(x, ids, dlogprob, dentropy, temperature=1.0):
 
 
 def teacher(ids, t, vocab, temperature=1.0, rest=False):
-    """(in use, q, ln q, r, row takes part)"""
+    """(in use, q, ln q, r, row takes part); r of LEAST_REST and less is none."""
     used = (ids >= 0) & (ids < vocab)
     with np.errstate(all="ignore"):
         t = np.where(used, np.asarray(t, F64), -np.inf)
@@ -81,7 +82,8 @@ def teacher(ids, t, vocab, temperature=1.0, rest=False):
             log_q = d - np.log(np.sum(np.exp(d), axis=1, keepdims=True))
             log_q = np.where(t == -np.inf, -np.inf, log_q)
         q = np.where(row[:, None], np.exp(log_q), 0.0)
-        left = np.where(row, np.maximum(0.0, 1.0 - q.sum(1)), 0.0) if rest else np.zeros(len(t))
+        left = 1.0 - q.sum(1)
+        left = np.where(row & ~(left <= LEAST_REST), left, 0.0) if rest else np.zeros(len(t))
     return used, q, log_q, left, row
 
 

@@ -496,3 +496,47 @@ def test_gradient_from_the_logarithm_of_a_small_rest(dtype):
     got = fetch(g, n * v, dtype).reshape(n, v)
     check_far(x, ids, t, dtype, 1.0, {"row_loss": ref["row_loss"], "dlogits": got}, made=True)
     free(tx, ti, tt, ts, one, g)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("mask", [-np.inf, -1e9])
+@pytest.mark.parametrize("n,v,temperature", [(40, 1003, 1.0), (700, 5003, 0.7), (300, 20003, 2.0), (9, 50257, 1.0)])
+def test_lists_of_all_the_tokens_that_are_allowed(n, v, temperature, mask, dtype):
+    """A teacher's likeliest tokens under a grammar that allows fewer than are asked for, its student under the same: what the list
+    leaves is rounding, and no rest that the forbidden tokens, of which the student thinks nothing, could have."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(n)
+    d = 1 if dtype == "bf16" else 0
+    for top in (20, 128):
+        teacher, student = np.full((n, v), mask, np.float32), np.full((n, v), mask, np.float32)
+        for r in range(n):
+            at = rng.permutation(v)[:(1, 2, 5, 13, 19, 20)[r % 6] * (1 if top == 20 else 6)]
+            teacher[r, at], student[r, at] = rng.standard_normal(len(at)) * 3, rng.standard_normal(len(at)) * 2
+        teacher, student = rounded(teacher, dtype), rounded(student, dtype)
+        tz, ti, tl = up(words(teacher, dtype)), up(np.zeros((n, top), np.int32)), up(np.zeros((n, top), np.float32))
+        ctx.token_logprobs_forward(tz, v, None, None, None, None, ti, tl, n, v, top, temperature, d)
+        ids, t = down(ti), down(tl)
+        free(tz, ti, tl)
+        # 25 u and 7 u for each |t|, of at most ln 120 on average: what counts as no rest is 64 u
+        assert np.all(np.abs(1 - np.exp(t.astype(np.float64)).sum(1)) < 60 * U)
+        for what in ("both", "apart"):
+            got = check(student, ids, t, dtype, what, rest=True, temperature=temperature)
+            assert np.isfinite(got["row_loss"]).all() and np.isfinite(got["loss"])
+            assert not got["dlogits"][student < -1e8].any()
+    check_clean_status()
+
+
+@pytest.mark.parametrize("rest", [2.0 ** -16, 2.0 ** -12])
+def test_a_rest_above_what_roundings_leave_counts(rest):
+    """64 tokens of (1 - rest) / 64 each: t = -4.2 is off by 2^-22 at most, the sum as much of itself."""
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((20, 500)).astype(np.float32)
+    ids = np.stack([rng.permutation(500)[:64] for _ in range(20)]).astype(np.int32)
+    t = np.full((20, 64), np.log((1 - rest) / 64), np.float32)
+    ref = R.distill(x, ids, t, rest=True)
+    size = np.abs(np.log(rest)) + np.abs(ref["log_rest"])
+    for what in ("both", "apart"):
+        got = check(x, ids, t, "f32", what, rest=True)
+        without = R.distill(x, ids, t + np.float32(2 * rest), rest=True)   # nothing left
+        # the rest is worth rest * (ln rest - ln p_rest), which 32 bits of the sum show
+        assert np.all(np.abs(got["row_loss"] - without["row_loss"]) > rest * (size.min() / 4))

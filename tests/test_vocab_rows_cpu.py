@@ -71,6 +71,26 @@ def test_gradient_of_a_small_rest_is_its_derivative(gap):
     assert np.allclose(np.where(listed, 0.0, got["dlogits"]).sum(1) * 3, np.exp(got["log_rest"]) - left, rtol=1e-9, atol=0)
 
 
+def test_what_roundings_leave_of_a_list_is_no_rest():
+    """Lists of all tokens that can occur, as log-probabilities in 32 bits: the others have p_rest = 0, or e^-1e9."""
+    rng = RNG(6)
+    z = rng.standard_normal((400, 20)) * 2
+    t = (z - np.log(np.exp(z).sum(1, keepdims=True))).astype(np.float32)
+    assert np.any(np.exp(t.astype(np.float64)).sum(1) < 1)
+    ids = np.tile(np.arange(20), (400, 1))
+    for mask in (-np.inf, -1e9):
+        x = np.full((400, 30), mask)
+        x[:, :20] = rng.standard_normal((400, 20))
+        got = R.distill(x, ids, t, rest=True)
+        lp = x[:, :20] - np.log(np.exp(x[:, :20]).sum(1, keepdims=True))
+        q = np.exp(t.astype(np.float64))
+        assert np.allclose(got["row_loss"], (q * (t - lp)).sum(1), rtol=1e-12)
+        assert not got["dlogits"][:, 20:].any()
+    # eight times that is one
+    got = R.distill(x, ids, np.log(np.exp(t.astype(np.float64)) * (1 - 2.0 ** -15)), rest=True)
+    assert np.all(got["row_loss"] > 1e4)
+
+
 # ---------------------------------------------------------------------------- refusals of the C interface
 # A context of zeros is enough for calls that are refused before they reach a device; one that is not refused fails to launch
 # with another code.
