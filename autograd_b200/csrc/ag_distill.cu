@@ -475,6 +475,7 @@ distill_loss_kernel(const float* __restrict__ row_loss, const float* __restrict_
 }
 
 // Threads of a block: short rows leave most of 256 idle, but a slot of the list needs one.
+static_assert(AG_DISTILL_MAX <= 256, "a slot per thread, and eight warps' parts of the list and of the loss");
 int distill_threads(const ag_ctx* ctx, int64_t N, int packets, int top) {
   const int th = ag_row_threads(ctx, N, packets, DI_PACKETS_64, DI_PACKETS_128);
   return th >= top ? th : top <= 128 ? 128 : 256;
