@@ -297,6 +297,11 @@ __device__ __forceinline__ int ag_cluster_rank() {
 __device__ __forceinline__ void ag_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// What the lanes of this warp have read and written comes before what any of them sends afterwards.
+__device__ __forceinline__ void ag_cluster_fence() {
+  __syncwarp();
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
 // address in block `rank` of what lies at p in this one
 __device__ __forceinline__ uint32_t ag_peer(const void* p, int rank) {
   uint32_t a;

@@ -540,3 +540,14 @@ def test_a_rest_above_what_roundings_leave_counts(rest):
         without = R.distill(x, ids, t + np.float32(2 * rest), rest=True)   # nothing left
         # the rest is worth rest * (ln rest - ln p_rest), which 32 bits of the sum show
         assert np.all(np.abs(got["row_loss"] - without["row_loss"]) > rest * (size.min() / 4))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(250, 40001), (209, 100003)])
+def test_gradients_in_the_place_of_many_wide_logits(n, v, dtype):
+    """Blocks share a row for what L2 holds, with a list that lies in the parts of all of them and is long enough for all warps."""
+    rng = np.random.default_rng(v)
+    x = rounded(rng.standard_normal((n, v)).astype(np.float32) * 2, dtype)
+    ids, t = teacher_of(rng, n, v, 256, True)
+    for rest in (False, True):
+        check(x, ids, t, dtype, "both", rest=rest, place="logits")
