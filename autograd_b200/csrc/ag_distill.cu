@@ -192,11 +192,30 @@ __device__ __forceinline__ void distill_dense(const uint4& w, uint64_t ref2, uin
   }
 }
 
-// exchange, parts of the list, slots' tokens and masses, loss per warp, bits of the edges, bits of the packets
+// Shared memory from the exchange's box on, for the kernel and for the launch that counts it.  All lengths are multiples of 16 bytes.
+static_assert(sizeof(DistillPart) == 16 && AG_DISTILL_MAX % 4 == 0, "marks are cleared 16 bytes at a time");
 template <int TH>
-size_t distill_smem(int S, int per, bool map) {
-  return AgExchange<TH>::bytes(S) + (TH / 32) * sizeof(DistillPart) + 2 * AG_DISTILL_MAX * 4 + 8 * 4 + 48 + (map ? (per + 15) / 16 * 16 : 0);
-}
+struct DistillShared {
+  uint64_t* bars;      // [2] one of the exchange
+  DistillPart* parts;  // [warps of a block] of the list
+  int* ids;            // [AG_DISTILL_MAX] slots' tokens
+  float* q;            // [AG_DISTILL_MAX] and masses
+  float* sum;          // [8] loss per warp
+  uint32_t* marks;     // [4] bits of the edges, whether a token is listed twice
+  uint8_t* map;        // a byte per packet
+  __host__ __device__ __forceinline__ DistillShared(float4* box, int S) {
+    bars = reinterpret_cast<uint64_t*>(box + S * (TH / 32));
+    parts = reinterpret_cast<DistillPart*>(bars + 2);
+    ids = reinterpret_cast<int*>(parts + (TH / 32));
+    q = reinterpret_cast<float*>(ids + AG_DISTILL_MAX);
+    sum = q + AG_DISTILL_MAX;
+    marks = reinterpret_cast<uint32_t*>(sum + 8);
+    map = reinterpret_cast<uint8_t*>(marks + 4);
+  }
+  static size_t bytes(int S, int per, bool map) {
+    return ag_counted_bytes(DistillShared(ag_counted_shared(), S).map + (map ? (per + 15) / 16 * 16 : 0));
+  }
+};
 
 template <typename T, bool TRAIN, bool REST, int TH>
 __global__ void __launch_bounds__(TH, distill_blocks(TRAIN, REST) * 256 / TH)
@@ -205,14 +224,13 @@ distill_kernel(const T* logits, T* dlogits, const DistillArgs a) {
   extern __shared__ float4 s_box[];
   const int S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * (TH / 32), parts = (a.top + 31) / 32;
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + groups);
-  const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
-  DistillPart* s_parts = reinterpret_cast<DistillPart*>(s_bars + 2);
-  int* s_ids = reinterpret_cast<int*>(s_parts + (TH / 32));
-  float* s_q = reinterpret_cast<float*>(s_ids + AG_DISTILL_MAX);
-  float* s_sum = s_q + AG_DISTILL_MAX;
-  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_sum + 8);  // [0] edges, [1] a token is listed twice, [4..] packets
-  uint8_t* s_map = reinterpret_cast<uint8_t*>(s_marks + 4);
+  const DistillShared<TH> shared(s_box, S);
+  const AgExchange<TH> exchange = {s_box, shared.bars, S, rank, a.status};
+  DistillPart* s_parts = shared.parts;
+  int* s_ids = shared.ids;
+  float *s_q = shared.q, *s_sum = shared.sum;
+  uint32_t* s_marks = shared.marks;  // [0] edges, [1] a token is listed twice, [4..] packets
+  uint8_t* s_map = shared.map;
   const float c = a.inv_tau * AG_LOG2E;
   exchange.start();
   ag_pdl_wait();
@@ -484,10 +502,10 @@ int distill_threads(const ag_ctx* ctx, int64_t N, int packets, int top) {
 template <typename T, bool TRAIN, bool REST, int TH>
 int distill_launch(ag_ctx* ctx, const T* logits, T* dlogits, const DistillArgs& a) {
   static std::atomic<bool> ready[AG_MAX_DEVICES];
-  const size_t smem = distill_smem<TH>(a.S, a.per, TRAIN || REST);
+  const size_t smem = DistillShared<TH>::bytes(a.S, a.per, TRAIN || REST);
   if (smem > 48 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
     AG_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<T, TRAIN, REST, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)distill_smem<TH>(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
+                                      (int)DistillShared<TH>::bytes(8, AG_VOCAB_MAX / AG_PACKET<T> + 1, true)));
     ready[ag_dev_slot(ctx)].store(true, std::memory_order_release);
   }
   return ag_launch_clusters(ctx, "distill_kernel", distill_kernel<T, TRAIN, REST, TH>, a.S, TH, smem, a.N, logits, dlogits, a);

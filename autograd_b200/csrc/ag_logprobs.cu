@@ -49,13 +49,45 @@ __host__ __device__ constexpr int lp_rest(int left) {
   return left > lp_whole<TH>(left) * LP_BATCH * TH ? (left - lp_whole<TH>(left) * LP_BATCH * TH - 1) / TH + 1 : 0;
 }
 
-// the exchange, a barrier, a block's keys, those of all blocks at block 0, batches with a logit that passes, counters, a histogram,
-// the batches' largest logits
+// Keys that a block has room for.  A multiple of four: keys are read in pairs, the histogram behind them 16 bytes at a time.
+constexpr int lp_cap(int top) { return top ? (3 * top + 64 + 3) & ~3 : 0; }
+
+// Shared memory from the exchange's box on, for the kernel and for the launch that counts it.  All lengths before `most` are
+// multiples of 16 bytes.
 template <int TH>
-size_t lp_smem(int S, int cap, int per) {
-  return AgExchange<TH>::bytes(S) + 16 + (size_t)cap * (8 * (S == 1 ? 1 : 1 + S) + 4) + 48 +
-         (cap ? 1024 + (size_t)(lp_whole<TH>(per) + LP_BATCH - 1) * TH * 4 : 0);
+struct LpShared {
+  uint64_t* bars;            // [2] one of the exchange
+  uint64_t* keys_bar;        // [2] every block's keys are at block 0
+  unsigned long long* keys;  // [cap]
+  unsigned long long* all;   // [S * cap], of block 0; a block with a row to itself has only those
+  int* batches;              // [cap] with a logit that passes
+  int* counts;               // [8]
+  int* n_keys;               // [4] keys, batches, a counter
+  uint32_t* hist;            // [256]
+  float* most;               // [batches and packets of a thread][threads] their largest logits
+  __host__ __device__ __forceinline__ LpShared(float4* box, int S, int cap) {
+    bars = reinterpret_cast<uint64_t*>(box + S * (TH / 32));
+    keys_bar = bars + 2;
+    keys = reinterpret_cast<unsigned long long*>(keys_bar + 2);
+    all = S == 1 ? keys : keys + cap;
+    batches = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * cap);
+    counts = batches + cap;
+    n_keys = counts + 8;
+    hist = reinterpret_cast<uint32_t*>(n_keys + 4);
+    most = reinterpret_cast<float*>(hist + 256);
+  }
+  static size_t bytes(int S, int cap, int per) {
+    const LpShared at(ag_counted_shared(), S, cap);
+    return ag_counted_bytes(cap ? reinterpret_cast<char*>(at.most + (lp_whole<TH>(per) + LP_BATCH - 1) * TH)
+                                : reinterpret_cast<char*>(at.keys_bar));
+  }
+};
+constexpr bool lp_lengths() {
+  for (int top = 1; top <= AG_TOP_MAX; ++top)
+    if (lp_cap(top) % 4 || lp_cap(top) < 3 * top + 64) return false;
+  return true;
 }
+static_assert(lp_lengths(), "keys, batches and what lies behind them start at multiples of 16 bytes");
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int index) { return (unsigned long long)ag_order(x) << 32 | (uint32_t)~index; }
 
@@ -245,16 +277,13 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
   extern __shared__ float4 s_box[];
   const int S = MANY || !TOP ? a.S : 1, tid = threadIdx.x, lane = tid & 31, rank = S > 1 ? ag_cluster_rank() : 0;
   const int groups = S * (TH / 32);
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_box + groups);
-  const AgExchange<TH> exchange = {s_box, s_bars, S, rank, a.status};
-  uint64_t* s_keys_bar = s_bars + 2;                                                   // every block's keys are at block 0
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(s_keys_bar + 2);    // [cap], a multiple of four
-  unsigned long long* all = S == 1 ? keys : keys + a.cap;                              // [S * cap], of block 0
-  int* batches = reinterpret_cast<int*>(keys + (S == 1 ? 1 : 1 + S) * a.cap);          // [cap]
-  int* counts = batches + a.cap;                                                       // [8]
-  int* n_keys = counts + 8;                                                            // keys, batches, a counter
-  uint32_t* hist = reinterpret_cast<uint32_t*>(n_keys + 4);                            // [256]
-  float* most = reinterpret_cast<float*>(hist + 256);                                  // [batches and packets of a thread][threads]
+  const LpShared<TH> s(s_box, S, a.cap);
+  const AgExchange<TH> exchange = {s_box, s.bars, S, rank, a.status};
+  uint64_t* s_keys_bar = s.keys_bar;
+  unsigned long long *keys = s.keys, *all = s.all;
+  int *batches = s.batches, *counts = s.counts, *n_keys = s.n_keys;
+  uint32_t* hist = s.hist;
+  float* most = s.most;
   const float c = a.inv_tau * AG_LOG2E;
   for (int b = tid; TOP && !MANY && b < 256; b += TH) hist[b] = 0;
   if (TOP && tid == 0) {
@@ -359,7 +388,7 @@ logprobs_kernel(const T* __restrict__ logits, const LpArgs a) {
     if (rank) return;
     ag_wait_cluster(s_keys_bar, 0, a.status);
     // side by side
-    constexpr int MOVE = (3 * AG_TOP_MAX + 64 + TH - 1) / TH;  // keys of a block per thread, at most
+    constexpr int MOVE = (lp_cap(AG_TOP_MAX) + TH - 1) / TH;  // keys of a block per thread, at most
     // (a count may be anything if the wait has expired)
     total = max(0, min(counts[0], a.cap));
     for (int p = 1; p < S; ++p) {
@@ -521,7 +550,7 @@ int logprobs_backward(ag_ctx* ctx, const void* logits, const void* dres, void* d
 
 template <typename T, bool TOP, int TH, bool MANY>
 int logprobs_launch(ag_ctx* ctx, const T* logits, const LpArgs& a) {
-  const size_t smem = lp_smem<TH>(a.S, a.cap, a.per);
+  const size_t smem = LpShared<TH>::bytes(a.S, a.cap, a.per);
   static std::atomic<bool> ready[AG_MAX_DEVICES];
   if (smem > 47 * 1024 && !ready[ag_dev_slot(ctx)].load(std::memory_order_acquire)) {
     AG_CUDA(ctx, cudaFuncSetAttribute(logprobs_kernel<T, TOP, TH, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
@@ -544,7 +573,7 @@ int logprobs(ag_ctx* ctx, const void* x, LpArgs a) {
            : th == 128 ? logprobs_launch<T, false, 128, true>(ctx, logits, a)
                        : logprobs_launch<T, false, 256, true>(ctx, logits, a);
   }
-  a.cap = (3 * a.top + 64 + 3) & ~3;  // a multiple of four: what follows in shared memory is read 16 bytes at a time
+  a.cap = lp_cap(a.top);
   if (a.S > 1) {
     // Lane maxima: where nearly all warps have to meet the bound, the one with the smallest logits decides, and many more than
     // `top` pass.  33 of 32 warps: the smallest of the second ones is passed by 200, the 17th of them by 55.

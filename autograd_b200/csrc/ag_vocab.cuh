@@ -366,8 +366,11 @@ struct AgExchange {
     ag_wait_cluster(bar, 0, status);
     return box;
   }
-  static constexpr size_t bytes(int S) { return (size_t)S * (TH / 32) * 16 + 16; }
 };
+// Where the launch counts what a block's pointers into shared memory span: aligned as the real ones are.
+static inline float4* ag_counted_shared() { return reinterpret_cast<float4*>((uintptr_t)1 << 20); }
+template <typename T>
+static inline size_t ag_counted_bytes(const T* end) { return (size_t)((uintptr_t)end - ((uintptr_t)1 << 20)); }
 
 __device__ __forceinline__ void ag_peer_store(uint32_t to, int v) {
   asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
