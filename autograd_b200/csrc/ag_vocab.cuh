@@ -142,12 +142,6 @@ template <typename T>
 constexpr int AG_PACKET = 16 / (int)sizeof(T);
 __device__ __forceinline__ void ag_widen(const uint4& w, float (&x)[4]) { Pack<float>::unpack_raw(*reinterpret_cast<const float4*>(&w), x); }
 __device__ __forceinline__ void ag_widen(const uint4& w, float (&x)[8]) { Pack<__nv_bfloat16>::unpack(w, x); }
-// 16 bytes of -inf
-template <typename T>
-__device__ __forceinline__ uint4 ag_lowest_packet() {
-  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-  return make_uint4(w, w, w, w);
-}
 
 // The largest logit of packets as they lie in memory (NaN ignored).
 template <int U>
