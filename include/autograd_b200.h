@@ -315,7 +315,8 @@ int ag_token_logprobs_backward(ag_ctx* ctx, const void* logits, int64_t ld, cons
  * No counterpart in the reference.  Student's logits as above, p = softmax(x / temperature).  Row i has `top` slots
  * (1 to AG_DISTILL_MAX): teacher_ids[i][k], negative = slot not in use, V and more = not in use and AG_STATUS_BAD_INDEX;
  * teacher_logits[i][k] = t_k.
- *   AG_DISTILL_RENORM: q = softmax(t / temperature) over the slots, r = 0 (t may be log-probabilities as well)
+ *   AG_DISTILL_RENORM: q = softmax(t / temperature) over the slots, r = 0 (t may be log-probabilities at temperature 1 as
+ *                      well; those made at this temperature would be tempered twice)
  *   AG_DISTILL_REST:   q_k = exp(t_k), t the teacher's log-probabilities at this temperature; r = 1 - sum q, its
  *                      mass on all other tokens, is compared with p_rest, the student's on the same tokens.  Up to
  *                      2^-18 r counts as 0: that is what roundings leave of a list of all the tokens there are
