@@ -665,10 +665,10 @@ class CudaBackend:
         n, width, v, dtype = self._logits(logits, vocab)
         check = self._check
         top = 0
+        if (top_ids is None) != (top_logprobs is None):
+            raise ValueError("top_ids and top_logprobs come together")
         if top_ids is not None:
             top = top_ids.shape[-1]
-            if top_logprobs is None:
-                raise ValueError("top_ids without top_logprobs")
             check("top_ids", top_ids, n * top, np.int32)
             check("top_logprobs", top_logprobs, n * top)
         self._context.token_logprobs_forward(

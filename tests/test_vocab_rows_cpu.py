@@ -238,3 +238,13 @@ def test_both_bindings_take_the_arguments(name, compiled):
         getattr(calls, name)(0, *args)
     with pytest.raises((TypeError, ValueError)):
         getattr(calls, name)(0, *args[:-1])
+
+
+def test_alternatives_are_asked_for_with_both_outputs():
+    """One of the two by itself would be left as it was."""
+    ctx, be = _backend()
+    x, k_ids, k = _tensor((6, 64)), _tensor((6, 5), np.int32), _tensor((6, 5))
+    for half in (dict(top_ids=k_ids), dict(top_logprobs=k)):
+        with pytest.raises(ValueError):
+            be.token_logprobs_forward(x, None, None, **half)
+    assert not ctx.calls
