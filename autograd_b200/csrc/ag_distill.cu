@@ -24,16 +24,16 @@ namespace {
 
 // Blocks of 256 threads per SM, packets per thread under way in the first look.  Without a gradient and with the map more packets
 // gain what more blocks do otherwise: us, 4 packets and 5 blocks (REST 4) / 8 packets and 4 blocks: loss of 512 x 32768 fp32 RENORM
-// 17.0 / 15.2, REST 17.5 / 16.5, gradient REST of 8192 x 50257 bf16 349 / 332, 16384 x 32768 fp32 822 / 777, RENORM 725 / 829.
+// 17.0 / 15.2, REST 17.5 / 16.5, gradient REST of 8192 x 50257 bf16 341 / 322, 16384 x 32768 fp32 800 / 758, RENORM 734 / 827.
 constexpr int distill_blocks(bool train, bool rest) { return train && !rest ? 5 : 4; }
 constexpr int distill_batch(bool train, bool rest) { return train && !rest ? 4 : 8; }
 // Packets of a row up to which a block has 64 or 128 threads.  16384 rows (of 32768: 8192), lists of 20 to 64, 64 / 128 / 256 threads,
-// us: loss 640 fp32 34 / 48 / 85, 5003 73 / 84 / 122; with gradient 640 fp32 39 / 56 / 96, 5003 131 / 138 / 172, 10007 bf16
-// 161 / 180 / 242; gradient alone 5003 bf16 51 / 54 / 91, 10007 85 / 84 / 106, 32768 224 / 205 / 209.
+// us: loss REST 640 fp32 34 / 53 / 98, 5003 66 / 85 / 143; with gradient RENORM 640 fp32 36 / 50 / 86, 5003 130 / 129 / 155, REST 10007
+// bf16 156 / 179 / 256; gradient alone 5003 bf16 51 / 54 / 91, 10007 85 / 84 / 106, 32768 224 / 205 / 209.
 constexpr int DI_PACKETS_64 = 2048, DI_PACKETS_128 = 4096;
 // Bytes of the rows that are under way at a time, above which more blocks share a row: what is written then pushes out of L2 what is
-// to be read again.  Us: 16384 x 32768 fp32, 1 / 2 / 4 blocks per row (97, 48, 24 MB) 940 / 727 / 933; 8192 x 50257 bf16, 1 / 2 (60,
-// 30 MB) 344 / 406; 4096 x 151936 bf16, 2 / 4 (90, 45 MB) 305 / 284.
+// to be read again.  Us, 1 / 2 / 4 blocks per row: 16384 x 32768 fp32 RENORM (97, 48, 24 MB) 942 / 713 / 833; REST 8192 x 50257 bf16 (60,
+// 30, 15 MB) 337 / 420 / 652; 4096 x 151936 bf16 (180, 90, 45 MB) 576 / 585 / 520.
 constexpr int64_t DI_IN_FLIGHT = 64 << 20;
 constexpr float DI_FAR = -32.0f;  // ln p_rest
 // What 1 - sum q may be of a list that leaves nothing: of log-probabilities t in 32 bits, each within 7 u |t| and together with exp
