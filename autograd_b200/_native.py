@@ -22,6 +22,7 @@ AG_CE_MEAN_ALL_ROWS, AG_CE_MEAN_VALID = 0, 1
 AG_CE_IGNORE_MASKED, AG_CE_IGNORE_COMPAT_UNMASKED = 0, 1
 AG_DISTILL_RENORM, AG_DISTILL_REST = 0, 1
 AG_VOCAB_MAX, AG_TOP_MAX, AG_DISTILL_MAX = 393216, 128, 256
+AG_QK_MAX_D = 1024
 
 
 class FlceDesc(C.Structure):
@@ -103,6 +104,13 @@ SIGNATURES = {
                                    _int, _int]),
     "ag_distill_forward_backward": (_int, [_ctx, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _int,
                                            _int, _f32, _int, _int]),
+    "ag_qk_norm_rope_forward": (_int, [_ctx] + [_ptr] * 9 + [_i64] + [_int] * 6 + [_i64] * 4 + [_f32, _int, _int]),
+    "ag_qk_norm_partials_bytes": (_sz, [_ctx, _int, _int, _int]),
+    "ag_qk_norm_rope_backward": (_int, [_ctx] + [_ptr] * 14 + [_sz, _i64] + [_int] * 6 + [_i64] * 6 + [_f32, _int, _int, _int]),
+    "ag_orthogonalise_scratch_bytes": (_sz, [_int, _int, _int, _int]),
+    "ag_orthogonalise": (_int, [_ctx, _ptr, _ptr, _int, _int, _int, _ptr, _int, _f32, _int, _int, _int, _ptr, _sz]),
+    "ag_muon_step": (_int, [_ctx, _ptr, _ptr, _ptr, _int, _int, _int, _f64, _f64, _int, _f64, _f64, _f64, _ptr, _int, _f32, _int,
+                            _int, _ptr, _sz]),
     "ag_adamw_step": (_int, [_ctx, _ptr, _ptr, _ptr, _ptr, _i64, _f64, _f64, _f64, _f64, _f64, _f64, _f64]),
     "ag_f32_to_bf16": (_int, [_ctx, _ptr, _ptr, _i64, _int]),
     "ag_bf16_to_f32": (_int, [_ctx, _ptr, _ptr, _i64]),
@@ -208,7 +216,8 @@ class _CheckedCalls:
              "ag_bf16_to_f32", "ag_flce_forward", "ag_flce_backward", "ag_flce_forward_keep",
              "ag_flce_backward_kept", "ag_flce_logits_bytes", "ag_linear_add_forward", "ag_linear_add_backward",
              "ag_token_logprobs_forward", "ag_token_logprobs_backward", "ag_distill_forward", "ag_distill_backward",
-             "ag_distill_forward_backward",
+             "ag_distill_forward_backward", "ag_qk_norm_rope_forward", "ag_qk_norm_rope_backward",
+             "ag_qk_norm_partials_bytes", "ag_orthogonalise", "ag_orthogonalise_scratch_bytes", "ag_muon_step",
              "ag_adamw_step", "ag_adamw_step_bf16grad", "ag_event_record", "ag_graph_launch", "ag_copy_h2d",
              "ag_scatter_add_scratch_bytes", "ag_flce_scratch_bytes", "ag_linear_add_scratch_bytes")
 

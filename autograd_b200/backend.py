@@ -17,6 +17,7 @@ callers fall back to `copy_to_host`, runtime.py:118-121) and an attribute named 
 """
 from __future__ import annotations
 
+import ctypes
 from math import copysign, prod
 
 import numpy as np
@@ -627,6 +628,145 @@ class CudaBackend:
         b, t, h, d = q.shape
         hkv = k.shape[2] if k is not None else 0
         _rope_qk(self._context, q, k, cos, sin, b, t, h, hkv, d, sin_sign, _ag_dtype(q.storage.dtype))
+
+    # ------------------------------------------------------------------ heads normalised and rotated
+    # RMSNorm of every head and RoPE in one pass over queries (..., H, D) and keys (..., HKV, D), which may be slices of packed
+    # rows: *_stride elements between tokens, dense where None.  cos, sin (positions, columns / 2) rotate the first `columns` of a
+    # head, all of them stay where the tables are None.  positions (int32, one a token) are rows of the tables; without them the
+    # tensors are (batch, T, heads, D) and token t has position t.  Formulas, limits: include/autograd_b200.h.
+    def _heads(self, q, k, cos, sin, positions, q_gamma, k_gamma, like):
+        t = q if q is not None else k
+        if t is None:
+            raise ValueError("neither queries nor keys")
+        lead, d, dtype = tuple(t.shape[:-2]), t.shape[-1], _ag_dtype(t.storage.dtype)
+        tokens = prod(lead)
+        for name, x, ref in (("q", q, q), ("k", k, k)) + like:
+            if (x is None) != (ref is None):
+                raise ValueError(f"{name} is missing, or has no tensor to belong to")
+            if x is not None and (tuple(x.shape) != lead + (ref.shape[-2], d) or _ag_dtype(x.storage.dtype) != dtype):
+                raise ValueError(f"{name} {tuple(x.shape)} needs the shape {lead + (ref.shape[-2], d)} and the type of the others")
+        check = self._check
+        check("q_gamma", q_gamma, d)
+        check("k_gamma", k_gamma, d)
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin come together")
+        rows, rot, seq = 0, 0, lead[-1] if lead else 1
+        if cos is not None:
+            rows, half = cos.shape
+            rot = 2 * half
+            check("cos", cos, rows * half)
+            check("sin", sin, rows * half)
+            if rot > d:
+                raise ValueError(f"tables of {half} columns for heads of {d}")
+            if positions is not None:
+                check("positions", positions, tokens, np.int32)
+            elif seq > rows:
+                raise ValueError(f"tables of {rows} positions for sequences of {seq}")
+        heads = [0 if x is None else x.shape[-2] for x in (q, k)]
+        return (tokens, seq, rows, *heads, d, rot), dtype
+
+    @staticmethod
+    def _stride(given, t):
+        if t is None:
+            return 0
+        return t.shape[-2] * t.shape[-1] if given is None else given
+
+    def qk_norm_rope_forward(self, q, k, cos, sin, q_out, k_out, eps, q_gamma=None, k_gamma=None, positions=None, sin_sign=1,
+                             q_stride=None, k_stride=None, q_out_stride=None, k_out_stride=None):
+        """q_out, k_out = rotation(x * inv_rms(x) * gamma) of every head of q and k; an output may be its input, then it has the
+        input's stride.  q or k may be None, with its output."""
+        sizes, dtype = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, (("q_out", q_out, q), ("k_out", k_out, k)))
+        stride = self._stride
+        self._context.qk_norm_rope_forward(
+            q, k, q_gamma, k_gamma, cos, sin, positions if cos is not None else None, q_out, k_out, *sizes, stride(q_stride, q),
+            stride(k_stride, k), stride(q_stride if q_out_stride is None and q_out is q else q_out_stride, q_out),
+            stride(k_stride if k_out_stride is None and k_out is k else k_out_stride, k_out), eps, sin_sign, dtype)
+
+    def qk_norm_rope_backward(self, dq_out, dk_out, q, k, cos, sin, dq, dk, eps, q_gamma=None, k_gamma=None, dq_gamma=None,
+                              dk_gamma=None, positions=None, sin_sign=1, accumulate=False, dq_out_stride=None, dk_out_stride=None,
+                              q_stride=None, k_stride=None, dq_stride=None, dk_stride=None, scratch=None):
+        """dq, dk = gradients (added to them with accumulate); dq_gamma, dk_gamma += theirs.  q, k: the forward's inputs; dq may be
+        dq_out or q, with its stride."""
+        like = (("dq_out", dq_out, q), ("dk_out", dk_out, k), ("dq", dq, q), ("dk", dk, k))
+        sizes, dtype = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, like)
+        _, _, _, h, hkv, d, _ = sizes
+        self._check("dq_gamma", dq_gamma, d)
+        self._check("dk_gamma", dk_gamma, d)
+        part, part_bytes = 0, 0
+        if dq_gamma is not None or dk_gamma is not None:
+            part, part_bytes = self._slot(scratch, "partials", self._context.qk_norm_partials_bytes(h, hkv, d))
+        stride = self._stride
+        dqs, dks = stride(dq_out_stride, dq_out), stride(dk_out_stride, dk_out)
+        qs, ks = stride(q_stride, q), stride(k_stride, k)
+
+        def of(given, t, dy, dy_stride, x, x_stride):
+            if given is None and t is not None:
+                return dy_stride if t is dy else x_stride if t is x else stride(None, t)
+            return stride(given, t)
+        self._context.qk_norm_rope_backward(
+            dq_out, dk_out, q, k, q_gamma, k_gamma, cos, sin, positions if cos is not None else None, dq, dk, dq_gamma, dk_gamma,
+            part, part_bytes, *sizes, dqs, dks, qs, ks, of(dq_stride, dq, dq_out, dqs, q, qs), of(dk_stride, dk, dk_out, dks, k, ks),
+            eps, sin_sign, accumulate, dtype)
+
+    # ------------------------------------------------------------------ orthogonal updates
+    # Singular values in (0, 1] end up between 0.7 and 1.2 after five steps; (a, b, c) for all steps, or one triple a step.
+    NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+    @staticmethod
+    def _matrices(name, given, like=None):
+        """(host array of the addresses of all matrices, their number, rows, cols, dtype) of a tensor or storage (..., rows, cols),
+        or a sequence of them."""
+        every = given if isinstance(given, (list, tuple)) else (given,)
+        at, shape, dtype = [], None, None
+        for t in every:
+            st = getattr(t, "storage", t)
+            if len(t.shape) < 2:
+                raise ValueError(f"{name} of shape {tuple(t.shape)}: matrices are wanted")
+            if shape is not None and (tuple(t.shape[-2:]) != shape or _ag_dtype(st.dtype) != dtype):
+                raise ValueError(f"{name}: matrices of one call have one shape and type")
+            shape, dtype = tuple(t.shape[-2:]), _ag_dtype(st.dtype)
+            base, step = address_of(st), prod(shape) * (4 if dtype == N.AG_F32 else 2)
+            at += [base + i * step for i in range(prod(t.shape[:-2]))]
+        if like is not None and (len(at), shape) != like:
+            raise ValueError(f"{name}: {len(at)} matrices of {shape}, expected {like[0]} of {like[1]}")
+        return (ctypes.c_void_p * max(1, len(at)))(*at), len(at), shape, dtype
+
+    @staticmethod
+    def _coefficients(coefficients, steps):
+        each = [tuple(coefficients)] * steps if not steps or np.ndim(coefficients) == 1 else [tuple(c) for c in coefficients]
+        if len(each) != steps or any(len(c) != 3 for c in each):
+            raise ValueError(f"coefficients: three numbers, or three for each of {steps} steps")
+        return (ctypes.c_float * max(1, 3 * steps))(*(x for c in each for x in c))
+
+    def orthogonalise(self, g, out, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=N.AG_CE_3XTF32, scratch=None):
+        """out = the matrices with the singular vectors of g's and singular values near 1, fp32 or bf16 words each; out may be g."""
+        at, n, shape, dtype = self._matrices("g", g)
+        to, _, _, out_dtype = self._matrices("out", out, (n, shape))
+        if not n:
+            return
+        co = self._coefficients(coefficients, steps)
+        sc, sc_bytes = self._slot(scratch, "orthogonalise", self._context.orthogonalise_scratch_bytes(n, *shape, precision))
+        self._context.orthogonalise(ctypes.addressof(at), ctypes.addressof(to), n, *shape, ctypes.addressof(co), steps, eps, precision,
+                                    dtype, out_dtype, sc, sc_bytes)
+
+    def muon_step(self, p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
+                  coefficients=NEWTON_SCHULZ, eps=1e-7, precision=N.AG_CE_3XTF32, scratch=None):
+        """m += (1 - momentum) (g - m); p = p (1 - lr weight_decay) - lr scale factor, the orthogonal factor being that of
+        g + momentum (m - g) (nesterov) or of m.  p, m: fp32, g: fp32 or bf16 words, as tensors or storages (..., rows, cols) or
+        sequences of them.  scale None: 0.2 sqrt(max(rows, cols)), with which elements move about as far as in an AdamW step."""
+        at, n, shape, dtype = self._matrices("p", p)
+        grads, _, _, grad_dtype = self._matrices("g", g, (n, shape))
+        ms, _, _, m_dtype = self._matrices("m", m, (n, shape))
+        if not n:
+            return
+        if dtype != N.AG_F32 or m_dtype != N.AG_F32:
+            raise TypeError("muon_step: parameters and momenta are fp32")
+        co = self._coefficients(coefficients, steps)
+        if scale is None:
+            scale = 0.2 * max(shape) ** 0.5
+        sc, sc_bytes = self._slot(scratch, "orthogonalise", self._context.orthogonalise_scratch_bytes(n, *shape, precision))
+        self._context.muon_step(ctypes.addressof(at), ctypes.addressof(grads), ctypes.addressof(ms), n, *shape, lr, momentum, nesterov,
+                                weight_decay, scale, grad_scale, ctypes.addressof(co), steps, eps, precision, grad_dtype, sc, sc_bytes)
 
     # ------------------------------------------------------------------ rows of logits
     # What a projection onto the vocabulary puts out (ag_linear_add_forward without residual, or the caller's own product):

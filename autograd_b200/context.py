@@ -308,6 +308,37 @@ class CudaContext:
         calls.ag_distill_forward_backward(self._hi, logits, ld, teacher_ids, teacher_logits, row_scale, dloss, loss, row_loss,
                                           stats, dlogits, ld_grad, N_, V_, top, temperature, mode, dtype)
 
+    def qk_norm_rope_forward(self, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out, tokens, seq, table_rows, H, HKV, D,
+                             rot, q_stride, k_stride, q_out_stride, k_out_stride, eps, sin_sign=1, dtype=N.AG_F32):
+        calls.ag_qk_norm_rope_forward(self._hi, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out, tokens, seq, table_rows,
+                                      H, HKV, D, rot, q_stride, k_stride, q_out_stride, k_out_stride, eps, sin_sign, dtype)
+
+    def qk_norm_partials_bytes(self, H, HKV, D):
+        return calls.ag_qk_norm_partials_bytes(self._hi, H, HKV, D)
+
+    def qk_norm_rope_backward(self, dq_out, dk_out, q, k, q_gamma, k_gamma, cos, sin, positions, dq, dk, dq_gamma, dk_gamma,
+                              partials, partials_bytes, tokens, seq, table_rows, H, HKV, D, rot, dq_out_stride, dk_out_stride,
+                              q_stride, k_stride, dq_stride, dk_stride, eps, sin_sign=1, accumulate=False, dtype=N.AG_F32):
+        calls.ag_qk_norm_rope_backward(self._hi, dq_out, dk_out, q, k, q_gamma, k_gamma, cos, sin, positions, dq, dk, dq_gamma,
+                                       dk_gamma, partials, partials_bytes, tokens, seq, table_rows, H, HKV, D, rot,
+                                       dq_out_stride, dk_out_stride, q_stride, k_stride, dq_stride, dk_stride, eps, sin_sign,
+                                       1 if accumulate else 0, dtype)
+
+    @staticmethod
+    def orthogonalise_scratch_bytes(count, rows, cols, precision=N.AG_CE_3XTF32):
+        return calls.ag_orthogonalise_scratch_bytes(count, rows, cols, precision)
+
+    def orthogonalise(self, g, out, count, rows, cols, coefficients, steps, eps, precision, dtype, out_dtype, scratch,
+                      scratch_bytes):
+        """g, out: host addresses of arrays of device addresses; coefficients: that of 3 floats a step."""
+        calls.ag_orthogonalise(self._hi, g, out, count, rows, cols, coefficients, steps, eps, precision, dtype, out_dtype, scratch,
+                               scratch_bytes)
+
+    def muon_step(self, p, g, m, count, rows, cols, lr, momentum, nesterov, weight_decay, scale, grad_scale, coefficients, steps,
+                  eps, precision, grad_dtype, scratch, scratch_bytes):
+        calls.ag_muon_step(self._hi, p, g, m, count, rows, cols, lr, momentum, 1 if nesterov else 0, weight_decay, scale, grad_scale,
+                           coefficients, steps, eps, precision, grad_dtype, scratch, scratch_bytes)
+
     def adamw_step(self, p, g, m, v, n, lr, lr_t, b1, b2, eps, weight_decay, grad_scale=1.0, grad_bf16=False):
         fn = calls.ag_adamw_step_bf16grad if grad_bf16 else calls.ag_adamw_step
         fn(self._hi, p, g, m, v, n, lr, lr_t, b1, b2, eps, weight_decay, grad_scale)

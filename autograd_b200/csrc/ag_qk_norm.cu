@@ -1,0 +1,609 @@
+// Queries and keys normalised per head, scaled by a weight per column and rotated by their position, in one pass, and the
+// gradient of that.
+//
+//   y = R(pos) (gamma * x * inv),  inv = 1 / sqrt(mean(x^2) + eps) over the D columns of a head
+//   w = R(pos)^T dy;  dgamma = sum over tokens and heads of w x inv;  v = gamma w;
+//   dx = inv (v - x inv^2 mean(v x))
+// R turns columns (c, c + rot / 2), c < rot / 2, by the angle of (position, c); columns from rot on stay as they are.
+//
+// A group of 1 to 32 lanes owns a head: a lane has S slots, a slot two packets that the rotation mixes (columns rot and
+// more are split into two halves in the same way, with nothing to mix), so that statistics and rotation need one read, a
+// few shuffles and no shared memory.  A thread keeps U heads of its token in flight and loads the angles once for all of
+// them.  Packets are as wide as addresses, strides and halves allow, 2 to 16 bytes: every shape takes the same code.  All
+// sums are fp32.
+#include "ag_common.cuh"
+
+namespace {
+
+constexpr int QK_THREADS = 256;
+constexpr int QK_BLOCKS_PER_SM = 8;  // of a backward pass, at most: 256 threads each
+
+// NV values of type T as they lie in memory
+template <int BYTES> struct QkWord;
+template <> struct QkWord<2> { using Raw = uint16_t; };
+template <> struct QkWord<4> { using Raw = uint32_t; };
+template <> struct QkWord<8> { using Raw = uint2; };
+template <> struct QkWord<16> { using Raw = uint4; };
+
+template <typename T, int NV>
+struct QkPack {
+  using Raw = typename QkWord<sizeof(T) * NV>::Raw;
+  union Bits {
+    Raw raw;
+    T v[NV];
+    __device__ Bits() {}
+  };
+  __device__ __forceinline__ static Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ static void unpack(const Raw& r, float (&f)[NV]) {
+    Bits b;
+    b.raw = r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f[i] = Pack<T>::load1(&b.v[i]);
+  }
+  __device__ __forceinline__ static void store(T* p, const float (&f)[NV]) {
+    Bits b;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) Pack<T>::store1(&b.v[i], f[i]);
+    *reinterpret_cast<Raw*>(p) = b.raw;
+  }
+};
+
+template <int NV>
+__device__ __forceinline__ void qk_load_f32(const float* p, float (&f)[NV]) {
+  if constexpr (NV >= 4) {
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) {
+      const float4 t = __ldg(reinterpret_cast<const float4*>(p + i));
+      f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f[i] = __ldg(p + i);
+  }
+}
+
+// Queries or keys.  Rows of a token are `*_stride` elements apart, its heads follow one another.
+struct QkSide {
+  const void* x;
+  const void* dy;      // backward
+  void* y;             // forward: output; backward: dx
+  const float* gamma;  // may be null
+  float* dgamma;       // backward, may be null
+  int64_t x_stride, dy_stride, y_stride;
+  int heads;
+  int blocks;          // of U heads each
+};
+
+struct QkArgs {
+  QkSide side[2];
+  const float* cos_tab;
+  const float* sin_tab;
+  const int32_t* positions;  // null: token % seq
+  int64_t tokens;
+  int seq, rows;             // rows of the tables
+  int D, half, slots;        // half = rot / 2, slots = D / 2 / NV
+  int lanes_log2;
+  float eps, sgn;
+  int accumulate;            // backward: dx += ...
+  float* partials;           // backward: [grid.x][grid.y][D], null where a single row of them is enough
+  int* status;
+};
+
+struct QkPlace {  // where a lane stands
+  int64_t tok;
+  int side, head;  // first head of the block
+  bool in;         // the token exists
+};
+
+// Columns of a slot: its first packet's and how far the second one is
+__device__ __forceinline__ void qk_columns(const QkArgs& a, int first, bool& turns, int& col, int& apart) {
+  turns = first < a.half;
+  col = turns ? first : a.half + first;
+  apart = turns ? a.half : (a.D >> 1) - a.half;
+}
+
+template <int S, int NV>
+__device__ __forceinline__ bool qk_angles(const QkArgs& a, int64_t tok, bool in, int lane, float (&c)[S][NV], float (&s)[S][NV]) {
+  int pos = 0;
+  bool ok = true;
+  if (in && a.half) {
+    pos = a.positions ? a.positions[tok] : (int)((uint32_t)tok % (uint32_t)a.seq);
+    ok = (uint32_t)pos < (uint32_t)a.rows;
+    if (!ok && lane == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
+    if (!ok) pos = 0;
+  }
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    const int first = (lane + (k << a.lanes_log2)) * NV;
+    if (in && first < a.half) {
+      qk_load_f32<NV>(a.cos_tab + (int64_t)pos * a.half + first, c[k]);
+      qk_load_f32<NV>(a.sin_tab + (int64_t)pos * a.half + first, s[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) { c[k][i] = 1.0f; s[k][i] = 0.0f; }
+    }
+  }
+  return ok;
+}
+
+__device__ __forceinline__ float qk_group_sum(float v, int lanes_log2) {
+  for (int o = (1 << lanes_log2) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int S, int NV>
+__device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, int lane, float (&lo)[S][NV], float (&hi)[S][NV]) {
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    const int slot = lane + (k << a.lanes_log2);
+    bool turns;
+    int col, apart;
+    qk_columns(a, slot * NV, turns, col, apart);
+    if (gamma && slot < a.slots) {
+      qk_load_f32<NV>(gamma + col, lo[k]);
+      qk_load_f32<NV>(gamma + col + apart, hi[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) lo[k][i] = hi[k][i] = 1.0f;
+    }
+  }
+}
+
+template <typename T, int NV, int S, int U>
+__global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) {
+  using P = QkPack<T, NV>;
+  ag_pdl_wait();
+  ag_pdl_trigger();
+  const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
+  const int64_t tok = (int64_t)blockIdx.x * (QK_THREADS >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const bool in = tok < a.tokens;
+  const int which = (int)blockIdx.y >= a.side[0].blocks;
+  const QkSide& q = a.side[which];
+  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U;
+  typename P::Raw lo[U][S], hi[U][S];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      const int slot = lane + (k << a.lanes_log2);
+      bool turns;
+      int col, apart;
+      qk_columns(a, slot * NV, turns, col, apart);
+      lo[u][k] = hi[u][k] = typename P::Raw{};
+      if (in && slot < a.slots && head + u < q.heads) {
+        const T* x = static_cast<const T*>(q.x) + tok * q.x_stride + (int64_t)(head + u) * a.D + col;
+        lo[u][k] = P::load(x);
+        hi[u][k] = P::load(x + apart);
+      }
+    }
+  float c[S][NV], s[S][NV], glo[S][NV], ghi[S][NV];
+  const bool ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
+  qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
+  float sum[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    sum[u] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      float x[NV], y[NV];
+      P::unpack(lo[u][k], x);
+      P::unpack(hi[u][k], y);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) sum[u] = fmaf(x[i], x[i], fmaf(y[i], y[i], sum[u]));
+    }
+  }
+  for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!in || head + u >= q.heads) continue;
+    const float inv = 1.0f / sqrtf(sum[u] / (float)a.D + a.eps);
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      const int slot = lane + (k << a.lanes_log2);
+      if (slot >= a.slots) continue;
+      bool turns;
+      int col, apart;
+      qk_columns(a, slot * NV, turns, col, apart);
+      float x[NV], y[NV], xo[NV], yo[NV];
+      P::unpack(lo[u][k], x);
+      P::unpack(hi[u][k], y);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float xn = x[i] * inv * glo[k][i], yn = y[i] * inv * ghi[k][i], sn = a.sgn * s[k][i];
+        xo[i] = turns ? xn * c[k][i] - yn * sn : xn;
+        yo[i] = turns ? xn * sn + yn * c[k][i] : yn;
+        if (!ok) xo[i] = yo[i] = 0.0f;
+      }
+      T* out = static_cast<T*>(q.y) + tok * q.y_stride + (int64_t)(head + u) * a.D + col;
+      P::store(out, xo);
+      P::store(out + apart, yo);
+    }
+  }
+}
+
+// W: the gradients of the weights are wanted (of either side)
+template <typename T, int NV, int S, int U, bool W>
+__global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a) {
+  using P = QkPack<T, NV>;
+  extern __shared__ float qk_smem[];  // W: [warps][D]
+  ag_pdl_wait();
+  ag_pdl_trigger();
+  const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
+  const int per_block = QK_THREADS >> a.lanes_log2;
+  const int which = (int)blockIdx.y >= a.side[0].blocks;
+  const QkSide& q = a.side[which];
+  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U;
+  float glo[S][NV], ghi[S][NV];
+  qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
+  float dlo[W ? S : 1][NV], dhi[W ? S : 1][NV];
+#pragma unroll
+  for (int k = 0; k < (W ? S : 1); ++k)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) dlo[k][i] = dhi[k][i] = 0.0f;
+  const float over = 1.0f / (float)a.D;
+  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += (int64_t)gridDim.x * per_block) {
+    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
+    const bool in = tok < a.tokens;
+    typename P::Raw xl[U][S], xh[U][S], gl[U][S], gh[U][S];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        const int slot = lane + (k << a.lanes_log2);
+        bool turns;
+        int col, apart;
+        qk_columns(a, slot * NV, turns, col, apart);
+        xl[u][k] = xh[u][k] = gl[u][k] = gh[u][k] = typename P::Raw{};
+        if (in && slot < a.slots && head + u < q.heads) {
+          const T* x = static_cast<const T*>(q.x) + tok * q.x_stride + (int64_t)(head + u) * a.D + col;
+          const T* g = static_cast<const T*>(q.dy) + tok * q.dy_stride + (int64_t)(head + u) * a.D + col;
+          xl[u][k] = P::load(x);
+          xh[u][k] = P::load(x + apart);
+          gl[u][k] = P::load(g);
+          gh[u][k] = P::load(g + apart);
+        }
+      }
+    float c[S][NV], s[S][NV];
+    const bool ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
+    float sum[U], dot[U];
+    // w of a slot, from its two packets of dy
+    auto turned = [&](int u, int k, float (&wl)[NV], float (&wh)[NV]) {
+      P::unpack(gl[u][k], wl);
+      P::unpack(gh[u][k], wh);
+      const bool turns = (lane + (k << a.lanes_log2)) * NV < a.half;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float x = wl[i], y = wh[i], sn = a.sgn * s[k][i];
+        if (turns) {
+          wl[i] = x * c[k][i] + y * sn;
+          wh[i] = y * c[k][i] - x * sn;
+        }
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      sum[u] = dot[u] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        float x[NV], y[NV], wl[NV], wh[NV];
+        P::unpack(xl[u][k], x);
+        P::unpack(xh[u][k], y);
+        turned(u, k, wl, wh);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          sum[u] = fmaf(x[i], x[i], fmaf(y[i], y[i], sum[u]));
+          dot[u] = fmaf(x[i], wl[i] * glo[k][i], fmaf(y[i], wh[i] * ghi[k][i], dot[u]));
+        }
+      }
+    }
+    for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+        dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!in || head + u >= q.heads) continue;
+      const float inv = 1.0f / sqrtf(sum[u] * over + a.eps);
+      const float back = inv * inv * (dot[u] * over);
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        const int slot = lane + (k << a.lanes_log2);
+        if (slot >= a.slots) continue;
+        bool turns;
+        int col, apart;
+        qk_columns(a, slot * NV, turns, col, apart);
+        float x[NV], y[NV], wl[NV], wh[NV];
+        P::unpack(xl[u][k], x);
+        P::unpack(xh[u][k], y);
+        turned(u, k, wl, wh);
+        T* out = static_cast<T*>(q.y) + tok * q.y_stride + (int64_t)(head + u) * a.D + col;
+        float ol[NV], oh[NV];
+        if (a.accumulate) {
+          P::unpack(P::load(out), ol);
+          P::unpack(P::load(out + apart), oh);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) ol[i] = oh[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (W && ok) {
+            dlo[k][i] = fmaf(wl[i], x[i] * inv, dlo[k][i]);
+            dhi[k][i] = fmaf(wh[i], y[i] * inv, dhi[k][i]);
+          }
+          const float dl = inv * (wl[i] * glo[k][i] - x[i] * back), dh = inv * (wh[i] * ghi[k][i] - y[i] * back);
+          ol[i] += ok ? dl : 0.0f;
+          oh[i] += ok ? dh : 0.0f;
+        }
+        P::store(out, ol);
+        P::store(out + apart, oh);
+      }
+    }
+  }
+  if constexpr (W) {
+    // the groups of a warp, then the warps, in a fixed order
+    const int warp = threadIdx.x >> 5, wl = threadIdx.x & 31;
+    float* mine = qk_smem + warp * a.D;
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      const int slot = lane + (k << a.lanes_log2);
+      bool turns;
+      int col, apart;
+      qk_columns(a, slot * NV, turns, col, apart);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float u = dlo[k][i], v = dhi[k][i];
+        for (int o = 16; o >= (1 << a.lanes_log2); o >>= 1) {
+          u += __shfl_xor_sync(0xffffffffu, u, o);
+          v += __shfl_xor_sync(0xffffffffu, v, o);
+        }
+        if (wl < (1 << a.lanes_log2) && slot < a.slots) {
+          mine[col + i] = u;
+          mine[col + apart + i] = v;
+        }
+      }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += QK_THREADS) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < QK_THREADS / 32; ++w) t += qk_smem[w * a.D + d];
+      a.partials[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * a.D + d] = t;
+    }
+  }
+}
+
+// dgamma += the partial rows of its side.  A block has 32 columns of one side; warps take rows in turn.
+__global__ void __launch_bounds__(QK_THREADS) qk_fold_kernel(const float* __restrict__ partials, int grid_x, int q_blocks,
+                                                             int k_blocks, int D, float* dq_gamma, float* dk_gamma) {
+  __shared__ float part[QK_THREADS / 32][33];
+  ag_pdl_wait();
+  ag_pdl_trigger();
+  float* out = blockIdx.y ? dk_gamma : dq_gamma;
+  if (!out) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
+  const int blocks = blockIdx.y ? k_blocks : q_blocks, first = blockIdx.y ? q_blocks : 0, all = q_blocks + k_blocks;
+  float t = 0.0f;
+  if (d < D)
+    for (int64_t r = warp; r < (int64_t)grid_x * blocks; r += QK_THREADS / 32)
+      t += partials[(r / blocks * all + first + r % blocks) * D + d];
+  part[warp][lane] = t;
+  __syncthreads();
+  if (warp == 0 && d < D) {
+    t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < QK_THREADS / 32; ++w) t += part[w][lane];
+    out[d] += t;
+  }
+}
+
+// ---------------------------------------------------------------------------- host side
+struct QkShape {
+  int nv, lanes_log2, S;
+};
+
+// The widest packets that everything allows, then lanes and slots with as few idle ones as possible
+template <typename T>
+QkShape qk_shape(const QkArgs& a) {
+  int nv = 16 / (int)sizeof(T);
+  auto fits = [&](int n) {
+    if (a.half % n || ((a.D >> 1) - a.half) % n) return false;
+    const uintptr_t bytes = n * sizeof(T), wide = n >= 4 ? 15u : 3u;
+    uintptr_t f = (uintptr_t)a.cos_tab | (uintptr_t)a.sin_tab;
+    for (const QkSide& q : a.side) {
+      if (!q.x) continue;
+      if ((((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.y) & (bytes - 1)) || q.x_stride % n || q.dy_stride % n || q.y_stride % n)
+        return false;
+      f |= (uintptr_t)q.gamma;
+    }
+    return (f & wide) == 0;
+  };
+  while (nv > 1 && !fits(nv)) nv >>= 1;
+  const int slots = a.D / 2 / nv;
+  QkShape best = {nv, 0, 0};
+  int best_cost = 1 << 30;
+  for (int s = 1; s <= 16; s = s < 4 ? s + 1 : s * 2)
+    for (int g = 0; g <= 5; ++g)
+      if ((s << g) >= slots) {
+        const int cost = (s << g) * 8 + s;
+        if (cost < best_cost) best_cost = cost, best = {nv, g, s};
+        break;
+      }
+  return best;
+}
+
+template <typename T, int NV, int S, int U, bool BACK, bool W>
+int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
+  for (QkSide& q : a.side) q.blocks = q.x ? (q.heads + U - 1) / U : 0;
+  const int gy = a.side[0].blocks + a.side[1].blocks, per_block = QK_THREADS >> sh.lanes_log2;
+  AG_REQUIRE(ctx, gy <= 65535, "too many heads");
+  int64_t gx = (a.tokens + per_block - 1) / per_block;
+  if constexpr (!BACK) {
+    AG_LAUNCH_PDL(ctx, "qk_forward_kernel", (qk_forward_kernel<T, NV, S, U>), dim3((unsigned)gx, gy), QK_THREADS, 0, a);
+  } else {
+    const int64_t most = ctx->sm_count * QK_BLOCKS_PER_SM / gy;
+    if (gx > most) gx = most > 0 ? most : 1;
+    AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS,
+                  W ? QK_THREADS / 32 * a.D * sizeof(float) : 0, a);
+    if (W)
+      AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), QK_THREADS, 0, a.partials, (int)gx,
+                    a.side[0].blocks, a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
+  }
+  return AG_OK;
+}
+
+template <typename T, int NV, int S, int U>
+int qk_kind(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
+  if (!back) return qk_launch<T, NV, S, U, false, false>(ctx, a, sh);
+  return w ? qk_launch<T, NV, S, U, true, true>(ctx, a, sh) : qk_launch<T, NV, S, U, true, false>(ctx, a, sh);
+}
+
+template <typename T, int NV>
+int qk_slots(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
+  a.lanes_log2 = sh.lanes_log2;
+  a.slots = a.D / 2 / NV;
+  switch (sh.S) {
+    case 1: return qk_kind<T, NV, 1, 2>(ctx, a, sh, back, w);
+    case 2: return qk_kind<T, NV, 2, 2>(ctx, a, sh, back, w);
+    case 3: return qk_kind<T, NV, 3, 1>(ctx, a, sh, back, w);
+    case 4: return qk_kind<T, NV, 4, 1>(ctx, a, sh, back, w);
+  }
+  if constexpr (NV * sizeof(T) < 16) {  // 16-byte packets: 32 lanes of 4 slots hold 1024 columns
+    if (sh.S == 8) return qk_kind<T, NV, 8, 1>(ctx, a, sh, back, w);
+    if constexpr (NV == 1)
+      if (sh.S == 16) return qk_kind<T, NV, 16, 1>(ctx, a, sh, back, w);
+  }
+  AG_FAIL(ctx, AG_ERR_INVALID, "no kernel for heads of %d columns", a.D);
+}
+
+template <typename T>
+int qk_run(ag_ctx* ctx, QkArgs& a, bool back, bool w) {
+  const QkShape sh = qk_shape<T>(a);
+  switch (sh.nv) {
+    case 1: return qk_slots<T, 1>(ctx, a, sh, back, w);
+    case 2: return qk_slots<T, 2>(ctx, a, sh, back, w);
+    case 4: return qk_slots<T, 4>(ctx, a, sh, back, w);
+  }
+  if constexpr (sizeof(T) == 2) return qk_slots<T, 8>(ctx, a, sh, back, w);
+  AG_FAIL(ctx, AG_ERR_INVALID, "no kernel for packets of %d", sh.nv);
+}
+
+// Rows of `width` elements, `stride` apart
+struct QkRows {
+  const void* p;
+  int64_t stride, width;
+};
+
+// Whether two sets of rows share an element: not if their ranges are apart, nor if rows of the same stride lie beside each
+// other (slices of one packed row)
+bool qk_overlap(const QkRows& x, const QkRows& y, int64_t rows, int64_t size) {
+  if (!x.p || !y.p) return false;
+  const int64_t a = (int64_t)(uintptr_t)x.p, b = (int64_t)(uintptr_t)y.p;
+  const int64_t a_end = a + ((rows - 1) * x.stride + x.width) * size, b_end = b + ((rows - 1) * y.stride + y.width) * size;
+  if (a_end <= b || b_end <= a) return false;
+  if (x.stride != y.stride) return true;
+  const int64_t pitch = x.stride * size, off = (((b - a) % pitch) + pitch) % pitch;  // of y's rows behind x's
+  return off < x.width * size || off + y.width * size > pitch;
+}
+
+int qk_check(ag_ctx* ctx, const char* name, const QkArgs& a, int seq, int rot, float eps, int dtype, bool back) {
+  AG_REQUIRE(ctx, a.tokens > 0 && a.tokens < (1ll << 31), "%s: bad number of tokens %lld", name, (long long)a.tokens);
+  AG_REQUIRE(ctx, a.D > 0 && a.D <= AG_QK_MAX_D && a.D % 2 == 0, "%s: heads of %d columns (even, at most %d)", name, a.D, AG_QK_MAX_D);
+  AG_REQUIRE(ctx, rot >= 0 && rot <= a.D && rot % 2 == 0, "%s: %d of %d columns rotate", name, rot, a.D);
+  AG_REQUIRE(ctx, dtype == AG_F32 || dtype == AG_BF16, "%s: unknown dtype %d", name, dtype);
+  AG_REQUIRE(ctx, eps >= 0.0f && eps <= 1e30f, "%s: eps %g", name, (double)eps);
+  AG_REQUIRE(ctx, rot == 0 || (a.cos_tab && a.sin_tab), "%s: null table", name);
+  AG_REQUIRE(ctx, rot == 0 || (a.rows > 0 && (a.positions || (seq > 0 && seq <= a.rows))),
+             "%s: sequences of %d positions, tables of %d", name, seq, a.rows);
+  AG_REQUIRE(ctx, a.side[0].x || a.side[1].x, "%s: neither queries nor keys", name);
+  const int64_t size = dtype == AG_F32 ? 4 : 2;
+  for (const QkSide& q : a.side) {
+    if (!q.x) continue;
+    AG_REQUIRE(ctx, q.y && (!back || q.dy), "%s: null pointer", name);
+    AG_REQUIRE(ctx, q.heads > 0 && q.heads <= 65535, "%s: %d heads", name, q.heads);
+    const int64_t w = (int64_t)q.heads * a.D;
+    AG_REQUIRE(ctx, q.x_stride >= w && q.y_stride >= w && (!back || q.dy_stride >= w), "%s: token stride smaller than heads * D", name);
+    AG_REQUIRE(ctx, q.x_stride < (1ll << 31) && q.y_stride < (1ll << 31) && q.dy_stride < (1ll << 31), "%s: token stride too large", name);
+    AG_REQUIRE(ctx, (((uintptr_t)q.x | (uintptr_t)q.y | (uintptr_t)q.dy) & (size - 1)) == 0 &&
+                        (((uintptr_t)q.gamma | (uintptr_t)q.dgamma) & 3) == 0, "%s: misaligned pointer", name);
+  }
+  AG_REQUIRE(ctx, (((uintptr_t)a.cos_tab | (uintptr_t)a.sin_tab | (uintptr_t)a.positions) & 3) == 0, "%s: misaligned table", name);
+  // an output may be one of its own side's inputs, row by row; otherwise it shares nothing with any operand
+  for (int i = 0; i < 2; ++i) {
+    const QkSide& q = a.side[i];
+    if (!q.x) continue;
+    const QkRows out = {q.y, q.y_stride, (int64_t)q.heads * a.D};
+    for (int j = 0; j < 2; ++j) {
+      const QkSide& o = a.side[j];
+      if (!o.x) continue;
+      const QkRows rows[3] = {{o.x, o.x_stride, (int64_t)o.heads * a.D},
+                              {back ? o.dy : nullptr, o.dy_stride, (int64_t)o.heads * a.D},
+                              {i != j ? o.y : nullptr, o.y_stride, (int64_t)o.heads * a.D}};
+      for (const QkRows& r : rows) {
+        const bool same = i == j && r.p == q.y && r.stride == q.y_stride;
+        AG_REQUIRE(ctx, same || !qk_overlap(out, r, a.tokens, size), "%s: an output overlaps another operand", name);
+      }
+    }
+  }
+  return AG_OK;
+}
+
+}  // namespace
+
+extern "C" int ag_qk_norm_rope_forward(ag_ctx* ctx, const void* q, const void* k, const float* q_gamma, const float* k_gamma,
+                                       const float* cos_tab, const float* sin_tab, const int32_t* positions, void* q_out,
+                                       void* k_out, int64_t tokens, int seq, int table_rows, int H, int HKV, int D, int rot,
+                                       int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride,
+                                       float eps, int sin_sign, int dtype) {
+  if (!ctx) return AG_ERR_INVALID;
+  if (tokens == 0) return AG_OK;
+  QkArgs a = {};
+  a.side[0] = {q, nullptr, q_out, q_gamma, nullptr, q_stride, 0, q_out_stride, H, 0};
+  a.side[1] = {k, nullptr, k_out, k_gamma, nullptr, k_stride, 0, k_out_stride, HKV, 0};
+  a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.positions = positions;
+  a.tokens = tokens; a.seq = seq; a.rows = table_rows; a.D = D; a.half = rot / 2;
+  a.eps = eps; a.sgn = sin_sign >= 0 ? 1.0f : -1.0f; a.status = ctx->d_status;
+  if (int rc = qk_check(ctx, "ag_qk_norm_rope_forward", a, seq, rot, eps, dtype, false)) return rc;
+  if (rot == 0) a.cos_tab = a.sin_tab = nullptr;
+  return dtype == AG_F32 ? qk_run<float>(ctx, a, false, false) : qk_run<__nv_bfloat16>(ctx, a, false, false);
+}
+
+extern "C" size_t ag_qk_norm_partials_bytes(ag_ctx* ctx, int H, int HKV, int D) {
+  if (!ctx || D <= 0 || H < 0 || HKV < 0) return 0;
+  // a row of D per block: QK_BLOCKS_PER_SM of them per SM, or one per head where there are more heads
+  const int64_t blocks = (int64_t)ctx->sm_count * QK_BLOCKS_PER_SM, heads = (int64_t)H + HKV;
+  return (size_t)((blocks > heads ? blocks : heads) * D) * sizeof(float);
+}
+
+extern "C" int ag_qk_norm_rope_backward(ag_ctx* ctx, const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                        const float* q_gamma, const float* k_gamma, const float* cos_tab,
+                                        const float* sin_tab, const int32_t* positions, void* dq, void* dk,
+                                        float* dq_gamma, float* dk_gamma, void* partials, size_t partials_bytes,
+                                        int64_t tokens, int seq, int table_rows, int H, int HKV, int D, int rot,
+                                        int64_t dq_out_stride, int64_t dk_out_stride, int64_t q_stride, int64_t k_stride,
+                                        int64_t dq_stride, int64_t dk_stride, float eps, int sin_sign, int accumulate,
+                                        int dtype) {
+  if (!ctx) return AG_ERR_INVALID;
+  if (tokens == 0) return AG_OK;
+  QkArgs a = {};
+  a.side[0] = {q, dq_out, dq, q_gamma, q ? dq_gamma : nullptr, q_stride, dq_out_stride, dq_stride, H, 0};
+  a.side[1] = {k, dk_out, dk, k_gamma, k ? dk_gamma : nullptr, k_stride, dk_out_stride, dk_stride, HKV, 0};
+  a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.positions = positions;
+  a.tokens = tokens; a.seq = seq; a.rows = table_rows; a.D = D; a.half = rot / 2;
+  a.eps = eps; a.sgn = sin_sign >= 0 ? 1.0f : -1.0f; a.status = ctx->d_status; a.accumulate = accumulate != 0;
+  if (int rc = qk_check(ctx, "ag_qk_norm_rope_backward", a, seq, rot, eps, dtype, true)) return rc;
+  if (rot == 0) a.cos_tab = a.sin_tab = nullptr;
+  const bool w = a.side[0].dgamma || a.side[1].dgamma;
+  if (w) {
+    const size_t need = ag_qk_norm_partials_bytes(ctx, q ? H : 0, k ? HKV : 0, D);
+    AG_REQUIRE(ctx, partials && ((uintptr_t)partials & 3) == 0, "ag_qk_norm_rope_backward: weight gradients need partials");
+    if (partials_bytes < need)
+      AG_FAIL(ctx, AG_ERR_SCRATCH, "ag_qk_norm_rope_backward: %zu bytes of partials, %zu needed", partials_bytes, need);
+    a.partials = static_cast<float*>(partials);
+  }
+  return dtype == AG_F32 ? qk_run<float>(ctx, a, true, w) : qk_run<__nv_bfloat16>(ctx, a, true, w);
+}

@@ -468,6 +468,12 @@ PyMethodDef methods[] = {
     CALL(ag_distill_forward),
     CALL(ag_distill_backward),
     CALL(ag_distill_forward_backward),
+    CALL(ag_qk_norm_rope_forward),
+    CALL(ag_qk_norm_partials_bytes),
+    CALL(ag_qk_norm_rope_backward),
+    CALL(ag_orthogonalise_scratch_bytes),
+    CALL(ag_orthogonalise),
+    CALL(ag_muon_step),
     CALL(ag_adamw_step),
     CALL(ag_adamw_step_bf16grad),
     CALL(ag_event_record),

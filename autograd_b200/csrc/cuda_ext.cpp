@@ -107,6 +107,12 @@ PYBIND11_MODULE(cuda_ext, m) {
   AG_DEF(ag_distill_forward);
   AG_DEF(ag_distill_backward);
   AG_DEF(ag_distill_forward_backward);
+  AG_DEF(ag_qk_norm_rope_forward);
+  AG_DEF(ag_qk_norm_partials_bytes);
+  AG_DEF(ag_qk_norm_rope_backward);
+  AG_DEF(ag_orthogonalise_scratch_bytes);
+  AG_DEF(ag_orthogonalise);
+  AG_DEF(ag_muon_step);
   AG_DEF(ag_adamw_step);
   AG_DEF(ag_f32_to_bf16);
   AG_DEF(ag_bf16_to_f32);

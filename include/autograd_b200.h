@@ -347,6 +347,59 @@ int ag_distill_forward_backward(ag_ctx* ctx, const void* logits, int64_t ld, con
                                 float* row_loss, float* stats, void* dlogits, int64_t ld_grad, int64_t N, int V,
                                 int top, float temperature, int mode, int dtype);
 
+/* ---- h3 queries and keys normalised per head and rotated ---------------------------------------
+ * No counterpart in the reference, whose heads are only rotated (a7).  For a head x of D columns (even, up to AG_QK_MAX_D) of a
+ * token:  y = R (gamma * x * inv),  inv = 1 / sqrt(mean(x^2) + eps), sums in fp32; gamma (D floats, one for all query heads, one
+ * for all key heads) may be NULL.  R is the rotation of a7 of the first `rot` columns (even, 0 to D; its halves are columns
+ * [0, rot/2) and [rot/2, rot)), the others stay as they are: cos_tab, sin_tab (table_rows, rot/2) fp32, NULL where rot is 0.
+ * positions[token] (int32) is the token's row of the tables; NULL: token % seq, seq <= table_rows.  A position outside the
+ * tables writes zeros, takes no part in the weights' gradients and raises AG_STATUS_BAD_INDEX.
+ * q: `tokens` rows of H heads, q_stride elements apart (slices of packed rows have a larger stride than H * D), likewise k
+ * with HKV heads and the outputs.  q or k may be NULL (with everything of its own).  An output may be its own input, with
+ * the same stride; it overlaps no other operand.
+ * backward: with w = R^T dy and v = gamma * w: dx = inv (v - x inv^2 mean(v x)), added to dq and dk with `accumulate`, else
+ * written; dgamma += sum over tokens and heads of w x inv in a fixed order, either may be NULL; they need
+ * ag_qk_norm_partials_bytes (heads as in the call, 0 for a NULL side) of partials, 4-byte aligned.  q and k are the forward's
+ * inputs.  dq may be dq_out or q, with the same stride. */
+#define AG_QK_MAX_D 1024
+int ag_qk_norm_rope_forward(ag_ctx* ctx, const void* q, const void* k, const float* q_gamma, const float* k_gamma,
+                            const float* cos_tab, const float* sin_tab, const int32_t* positions, void* q_out,
+                            void* k_out, int64_t tokens, int seq, int table_rows, int H, int HKV, int D, int rot,
+                            int64_t q_stride, int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, float eps,
+                            int sin_sign, int dtype);
+size_t ag_qk_norm_partials_bytes(ag_ctx* ctx, int H, int HKV, int D);
+int ag_qk_norm_rope_backward(ag_ctx* ctx, const void* dq_out, const void* dk_out, const void* q, const void* k,
+                             const float* q_gamma, const float* k_gamma, const float* cos_tab, const float* sin_tab,
+                             const int32_t* positions, void* dq, void* dk, float* dq_gamma, float* dk_gamma,
+                             void* partials, size_t partials_bytes, int64_t tokens, int seq, int table_rows, int H,
+                             int HKV, int D, int rot, int64_t dq_out_stride, int64_t dk_out_stride, int64_t q_stride,
+                             int64_t k_stride, int64_t dq_stride, int64_t dk_stride, float eps, int sin_sign,
+                             int accumulate, int dtype);
+
+/* ---- h4 orthogonal factors and the step along them ----------------------------------------------
+ * No counterpart in the reference, whose optimizer is AdamW (f3).  `count` matrices of rows x cols, each contiguous, at the
+ * device addresses that the host arrays g, out, p, m hold (read before the call returns).
+ *   factor(u):  X = u / max(|u|, eps) (Frobenius norm, summed in 64 bits; transposed where rows > cols), `steps` times
+ *               X <- (a I + b A + c A A) X,  A = X X^T,  with (a, b, c) = coefficients[3 i ..] (host) of step i:
+ *               every singular value s of X becomes a s + b s^3 + c s^5, singular vectors stay.
+ *   ag_orthogonalise:  out = factor(g), in out_dtype.  out[i] may be g[i] where its elements are no larger.
+ *   ag_muon_step:  g' = g * grad_scale (g in grad_dtype);  m += (1 - momentum) (g' - m);
+ *               u = g' + momentum (m - g') with nesterov, else m;  p = p (1 - lr weight_decay) - lr scale factor(u).
+ * precision AG_CE_3XTF32: products as exact as fp32 ones (operands carry 22 bits; a factor is off by about 1e-6 of its norm);
+ * AG_CE_BF16: operands rounded once to 16 bits, of which 11 are significant here (1e-3 to 1e-2 of the norm, the more the wider the
+ * singular values range).  Singular values, and a + b s^2 + c s^4 for them, have to stay below 15 throughout.  A matrix of
+ * zeros has the factor 0; NaN or infinities make their matrix NaN and no other.
+ * Matrices and workspace may not overlap (256-byte aligned workspace of ag_orthogonalise_scratch_bytes, 0 for sizes or a
+ * precision that the calls refuse: more than 16384 on the shorter side, 2^20 on the longer or 2^31 elements). */
+size_t ag_orthogonalise_scratch_bytes(int count, int rows, int cols, int precision);
+int ag_orthogonalise(ag_ctx* ctx, const void* const* g, void* const* out, int count, int rows, int cols,
+                     const float* coefficients, int steps, float eps, int precision, int dtype, int out_dtype,
+                     void* scratch, size_t scratch_bytes);
+int ag_muon_step(ag_ctx* ctx, float* const* p, const void* const* g, float* const* m, int count, int rows, int cols,
+                 double lr, double momentum, int nesterov, double weight_decay, double scale, double grad_scale,
+                 const float* coefficients, int steps, float eps, int precision, int grad_dtype, void* scratch,
+                 size_t scratch_bytes);
+
 /* ---- f3 AdamW fp32 step ----------------------------------------------------------------
  * Replaces: backend.py:2013-2038 cpu_adamw_step; metal_ops.metal:10139-10227.
  * g is read as g*grad_scale. */
