@@ -7,9 +7,11 @@
 //   p <- (1 - lr decay) p - lr scale X.
 //
 // Matrices of one size go through every kernel together, as many at a time as the workspace holds.
+#include <math.h>
 #include <stdlib.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ag_tma.cuh"
 
@@ -144,10 +146,6 @@ struct NsPlane {
   __half *hi, *lo;  // lo null: one word
 };
 
-__device__ __forceinline__ float ns_get(const NsPlane& s, int64_t i) {
-  return (__half2float(s.hi[i]) + (s.lo ? __half2float(s.lo[i]) : 0.0f)) * (1.0f / NS_SCALE);
-}
-
 // X = u / max(|u|, eps) in padded rows, transposed where the matrix is tall: tiles of 64 x 64
 __global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices mats, NsPlan t, int bf16, NsUpdate s, float eps,
                                                               const double* norms, int norm_blocks, NsPlane X) {
@@ -204,28 +202,32 @@ __global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices m
 // ---------------------------------------------------------------------------- products
 // One persistent kernel, D = f(L R) for every matrix of the batch: TMA producer, MMA issuer and epilogue warps as in
 // ag_flce_tc.cu, on single CTAs (128 x BN) or on pairs of them (256 x BN).  Operands are planes, three MMAs per 16 elements of
-// the contraction (hi lo, lo hi, hi hi) where there are two.
-//   GRAM:  A = X X^T             both K-major
-//   POLY:  Q = a I + b A + c AA  both symmetric
-//   NEXT:  X' = Q X              symmetric, X MN-major
-//   LAST:  the same, straight into p or out
+// the contraction (hi lo, lo hi, hi hi) where there are two; tiles of high and of low parts come through rings of their own.
+// A step X <- (a I + b G + c G G) X, G = X X^T, is a square once it is completed: with h = b / 2 c
+//   GRAM:  A = G + h I                    both operands K-major
+//   POLY:  Q = (a - h h c) I + c A A      both symmetric
+//   NEXT:  X' = Q X                       symmetric, X MN-major
+// so that no product needs anything beside its operands, and every epilogue is a factor and a number on the diagonal.  Where c is 0,
+// GRAM writes Q = a I + b G itself.
 // A and Q are symmetric (polynomials of one matrix commute): only the tiles on and above the diagonal are computed and
 // stored.  A tile of an operand that lies below is read as the transpose of the one above, as an MN-major tile: which of the
 // two is a matter of the map, the descriptor and a bit of the instruction, chosen for every 64 columns.
-enum { NS_GRAM, NS_POLY, NS_NEXT, NS_LAST };
+enum { NS_GRAM, NS_POLY, NS_NEXT };
 constexpr bool ns_symmetric(int kind) { return kind <= NS_POLY; }
 
 constexpr int NS_EPI_WARPS = 8;
 constexpr int NS_TC_THREADS = 128 + 32 * NS_EPI_WARPS;
-constexpr int NS_MAX_STAGES = 6;
+constexpr int NS_MAX_SLOTS = 12;
 constexpr int NS_SMEM_LIMIT = 227 * 1024;
-constexpr int NS_STAGING = NS_EPI_WARPS * 2048;  // 32 rows of 64 bytes on their way to p or out
-constexpr int NS_SMEM_FIXED = 1024 + NS_STAGING + 256;
-// The tensor core's sums truncate: chains of at most this many steps of 64 elements, added in registers
-#ifndef CH
-#define CH 1
-#endif
-constexpr int NS_CHAIN_PAIRS = CH, NS_CHAIN_SINGLE = 128;
+constexpr int NS_STAGING = NS_EPI_WARPS * 4096;  // per epilogue warp: 32 rows of 64 bytes, twice, on their way to memory
+constexpr int NS_SMEM_FIXED = 1024 + NS_STAGING + 512;
+// The tensor core truncates a sum at every addition, by an amount that grows with it.  So chains are short, two steps of 64 elements
+// (single words: 128 steps, their operands are off by more), the epilogue adds them in registers, and the products with a low part come
+// first, whose sum is 2^-11 of the whole.  What truncation takes of a sum on average, NS_LOSS of it at each of the later additions of
+// 16 elements, is put back by the factor of the epilogue.  Error of the factor of 333 x 1001 with 0, 4e-8, 7e-8 and 1e-7: 3.8e-6, 1.9e-6, 2.9e-6, 4.7e-6
+// (plain fp32 products: 2.6e-6); without it, low parts first in every step, chains of 1, 2 and 4 steps: 2.6e-6, 5.7e-6, 8.7e-6.
+constexpr int NS_CHAIN_PAIRS = 2, NS_CHAIN_SINGLE = 128;
+constexpr double NS_LOSS = 4.6e-8;
 
 // Tensor maps of a plane: tiles with the contraction along its rows (k), and along its columns (mn)
 struct NsMaps {
@@ -234,16 +236,13 @@ struct NsMaps {
 
 struct NsGemm {
   NsMaps l, r;
+  CUtensorMap d_hi, d_lo;  // of the result: boxes of 32 rows x 32 columns
   int batch, tiles_m, tiles_n, tiles;  // tiles of a matrix; symmetric: those on and above the diagonal
-  int k_iters, chain, stages;
-  int M, N;            // rows and columns of a matrix that are stored (padded)
-  int64_t ldd;
-  NsPlane D, A;        // POLY reads A where D is written
-  float diag, add, mul;
-  // LAST
-  NsMatrices mats;
-  int rows, cols, tall, out_kind;
-  float keep, by;
+  int k_iters, chain, k_real;  // steps of 64 elements of the contraction, in chains; elements that are not padding
+  int hi_slots, lo_slots;  // of the two rings of operand tiles: high parts, low parts
+  int M, N;                // rows and columns of a matrix that are stored (padded)
+  int two;                 // the result has a low part
+  float diag, mul;
   int* status;
 };
 
@@ -270,134 +269,47 @@ __device__ __forceinline__ bool ns_tile(const NsGemm& p, int unit, int units, in
   return true;
 }
 
-// 32 columns of a lane's row as words
-template <bool SPLIT>
-__device__ __forceinline__ void ns_store_row(const NsPlane& d, int64_t at, const float (&v)[32]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) split_f16x2(v[16 * j + 2 * k], v[16 * j + 2 * k + 1], hi[k], lo[k]);
-    tc_st_global_v8(d.hi + at + 16 * j, hi);
-    if (SPLIT) tc_st_global_v8(d.lo + at + 16 * j, lo);
-  }
+// 32 x 32 words of 16 bits from a warp's buffer (64 bytes a row, swizzled as tc_stage_at has it) to memory, as a bulk store
+__device__ __forceinline__ void ns_tma_store(const CUtensorMap* tm, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tm), "r"(ag_smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// p <- keep p - by v (kind 0), or v in fp32 (1) or bf16 (2)
-__device__ __forceinline__ void ns_apply(void* p, int64_t i, float v, float old, float keep, float by, int kind) {
-  if (kind == 2) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else static_cast<float*>(p)[i] = kind == 0 ? fmaf(-by, v, keep * old) : v;
-}
+// all but the last `N` stores of this thread have read their buffers
+template <int N>
+__device__ __forceinline__ void ns_stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
-// 32 values of the lane in a column of the matrix, `n` of them inside
-__device__ __forceinline__ void ns_apply_column(const NsGemm& p, int mat, int64_t at, const float (&v)[32], int n) {
-  float* d = p.mats.p[mat];
-#pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    float old[16];
-    if (p.out_kind == 0) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) old[j] = h + j < n ? d[at + (int64_t)(h + j) * p.cols] : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (h + j < n) ns_apply(d, at + (int64_t)(h + j) * p.cols, v[h + j], old[j], p.keep, p.by, p.out_kind);
-  }
-}
-
-// 32 rows x 16 columns from (row0, col), v = the lane's row: four lanes per row, or two rows at a time where rows are not aligned
-__device__ __forceinline__ void ns_apply_block(const NsGemm& p, int mat, unsigned char* stg, int lane, const float* v, int row0, int col) {
-  float* d = p.mats.p[mat];
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) *tc_stage_at(stg, lane, j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  __syncwarp();
-  if (p.out_kind < 2 && (p.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(d) & 15) == 0 && col + 16 <= p.cols) {
-    const int r4 = lane >> 2, piece = lane & 3;
-    float4* q = reinterpret_cast<float4*>(d + (int64_t)(row0 + r4) * p.cols + col) + piece;
-    const int64_t next = (int64_t)p.cols * 2;  // eight rows, in float4
-    float4 old[4];
-    if (p.out_kind == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (row0 + r4 + 8 * i < p.rows) old[i] = q[i * next];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (row0 + r4 + 8 * i >= p.rows) continue;
-      float4 x = *tc_stage_at(stg, r4 + 8 * i, piece);
-      if (p.out_kind == 0)
-        x = make_float4(fmaf(-p.by, x.x, p.keep * old[i].x), fmaf(-p.by, x.y, p.keep * old[i].y), fmaf(-p.by, x.z, p.keep * old[i].z),
-                        fmaf(-p.by, x.w, p.keep * old[i].w));
-      q[i * next] = x;
-    }
-    return;
-  }
-  const int c = lane & 15, first = lane >> 4;
-  if (col + c >= p.cols) return;
-  const int64_t at = (int64_t)(row0 + first) * p.cols + col + c;
-  float old[16];
-  if (p.out_kind == 0) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) old[i] = row0 + first + 2 * i < p.rows ? d[at + (int64_t)(2 * i) * p.cols] : 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (row0 + first + 2 * i < p.rows)
-      ns_apply(d, at + (int64_t)(2 * i) * p.cols, reinterpret_cast<const float*>(tc_stage_at(stg, first + 2 * i, c >> 2))[c & 3], old[i],
-               p.keep, p.by, p.out_kind);
-}
-
-// All MMAs of a stage.  The products with a low part come first: what the tensor core cuts off a sum grows with it, and theirs is
-// 2^-11 of the whole.
-template <bool SPLIT, bool PAIR>
-__device__ __forceinline__ void ns_stage_mmas(uint32_t acc, uint32_t lh, uint32_t ll, uint32_t l_step, uint32_t rh, uint32_t rl,
-                                              uint32_t r_step, uint32_t idesc, uint32_t not_first) {
+// The MMAs of a step of 64 elements: products with a low part, or those of the high parts
+template <bool LOW, bool PAIR>
+__device__ __forceinline__ void ns_step_mmas(uint32_t acc, uint32_t lh, uint32_t ll, uint32_t l_step, uint32_t rh, uint32_t rl,
+                                             uint32_t r_step, uint32_t idesc, uint32_t not_first) {
   constexpr uint32_t hi = TcDesc::hi;
-  if (SPLIT) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k == 0) tc_mma<2, PAIR>(acc, lh, hi, rl, hi, idesc, not_first);
-      else tc_mma<1, PAIR>(acc, lh + k * l_step, hi, rl + k * r_step, hi, idesc, 1u);
-      tc_mma<1, PAIR>(acc, ll + k * l_step, hi, rh + k * r_step, hi, idesc, 1u);
-    }
-  }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if (!SPLIT && k == 0) tc_mma<2, PAIR>(acc, lh, hi, rh, hi, idesc, not_first);
-    else tc_mma<1, PAIR>(acc, lh + k * l_step, hi, rh + k * r_step, hi, idesc, 1u);
+    const uint32_t lo = k * l_step, ro = k * r_step, r0 = LOW ? rl : rh;
+    if (k == 0) tc_mma<2, PAIR>(acc, lh, hi, r0, hi, idesc, not_first);
+    else tc_mma<1, PAIR>(acc, lh + lo, hi, r0 + ro, hi, idesc, 1u);
+    if (LOW) tc_mma<1, PAIR>(acc, ll + lo, hi, rh + ro, hi, idesc, 1u);
   }
 }
-
-// four 16-byte loads at once of 32 words of 16 bits
-struct NsWords {
-  uint4 v[4];
-  __device__ __forceinline__ void load(const __half* p) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(p + 8 * j);
-  }
-  __device__ __forceinline__ float2 pair(int k) const {  // words 2 k and 2 k + 1
-    const uint4& q = v[k >> 2];
-    const uint32_t w = (k & 3) == 0 ? q.x : (k & 3) == 1 ? q.y : (k & 3) == 2 ? q.z : q.w;
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  }
-};
 
 template <int KIND, bool SPLIT, bool PAIR, int BN>
 __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_constant__ NsGemm p) {
   extern __shared__ unsigned char ns_smem_raw[];
   constexpr bool R_MN = !ns_symmetric(KIND);          // the right operand is stored with its columns contiguous
   constexpr uint32_t A_BYTES = TC_BM * 128, BN_CTA = PAIR ? BN / 2 : BN, B_BYTES = BN_CTA * 128;
-  constexpr uint32_t STAGE = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);
+  constexpr uint32_t SLOT = A_BYTES + B_BYTES;        // both operands' tiles of 64 elements of the contraction
   constexpr int BM = PAIR ? 2 * TC_BM : TC_BM;
   constexpr uint32_t COLUMNS = 2 * BN;                // of tensor memory: two accumulators
   constexpr int CHUNKS = BN / 64;                     // 32-column chunks of an epilogue warp
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
   static_assert(!ns_symmetric(KIND) || BM == BN, "tiles on the diagonal are square");
   unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ns_smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* staging = tiles + (size_t)p.stages * STAGE;
+  unsigned char* staging = tiles + (size_t)(p.hi_slots + p.lo_slots) * SLOT;
+  // barriers of the slots: those of the ring of high parts, then of low parts
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + NS_STAGING);
-  uint64_t* empty = full + NS_MAX_STAGES;
-  uint64_t* acc_full = empty + NS_MAX_STAGES;
+  uint64_t* empty = full + NS_MAX_SLOTS;
+  uint64_t* acc_full = empty + NS_MAX_SLOTS;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -409,7 +321,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   const int row_off = PAIR ? (int)rank * TC_BM : 0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
+    for (int s = 0; s < p.hi_slots + p.lo_slots; ++s) {
       ag_mbar_init(&full[s], 1);
       ag_mbar_init(&empty[s], 1);
     }
@@ -443,107 +355,109 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA producer
-      uint32_t stage = 0, phase = 0;
+      uint32_t slot[2] = {0, 0}, phase[2] = {0, 0};
       NsTile t;
       for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
         const int l_at = t.tm * BM + row_off;
         const int r_at = t.tn * BN + (int)rank * (PAIR ? (int)BN_CTA : 0);
-        for (int k = 0; k < p.k_iters; ++k) {
-          if (!tc_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-            expired = true;
-            break;
-          }
-          unsigned char* s = tiles + (size_t)stage * STAGE;
-          uint32_t full_addr = ag_smem_u32(&full[stage]);
-          if (PAIR) {
-            if (rank == 0) ag_mbar_expect_tx(&full[stage], 2u * STAGE);
-            full_addr = tc_map_to_cta(full_addr, 0u);
-          } else {
-            ag_mbar_expect_tx(&full[stage], STAGE);
-          }
-          const int kx = k * TC_BK;
-          const int blk = kx / BM;  // tile of the contraction
-          auto load = [&](const CUtensorMap& k_map, const CUtensorMap& mn_map, unsigned char* dst, int at, bool mn) {
-            if (!mn) {
-              if (PAIR) tc_tma_load_2d_pair(&k_map, dst, full_addr, kx, t.mat * p.M + at);
-              else tc_tma_load_2d(&k_map, dst, &full[stage], kx, t.mat * p.M + at);
-            } else {
-              if (PAIR) tc_tma_load_3d_pair(&mn_map, dst, full_addr, 0, t.mat * p.M + kx, at / TC_MN_GROUP);
-              else tc_tma_load_3d(&mn_map, dst, &full[stage], 0, t.mat * p.M + kx, at / TC_MN_GROUP);
-            }
-          };
+        for (int k = 0; k < p.k_iters && !expired; ++k) {
+          const int kx = k * TC_BK, blk = kx / BM;  // blk: tile of the contraction
           const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
-          load(p.l.k_hi, p.l.mn_hi, s, l_at, l_mn);
-          if (SPLIT) {
-            load(p.l.k_lo, p.l.mn_lo, s + A_BYTES, l_at, l_mn);
-            load(p.r.k_hi, p.r.mn_hi, s + 2 * A_BYTES, r_at, r_mn);
-            load(p.r.k_lo, p.r.mn_lo, s + 2 * A_BYTES + B_BYTES, r_at, r_mn);
-          } else {
-            load(p.r.k_hi, p.r.mn_hi, s + A_BYTES, r_at, r_mn);
-          }
-          if (++stage == (uint32_t)p.stages) {
-            stage = 0;
-            phase ^= 1u;
+#pragma unroll
+          for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
+            const uint32_t at = (part ? p.hi_slots : 0) + slot[part];
+            if (!tc_wait(&empty[at], phase[part] ^ 1u, abort_flag)) {
+              expired = true;
+              break;
+            }
+            unsigned char* s = tiles + (size_t)at * SLOT;
+            uint32_t full_addr = ag_smem_u32(&full[at]);
+            if (PAIR) {
+              if (rank == 0) ag_mbar_expect_tx(&full[at], 2u * SLOT);
+              full_addr = tc_map_to_cta(full_addr, 0u);
+            } else {
+              ag_mbar_expect_tx(&full[at], SLOT);
+            }
+            auto load = [&](const CUtensorMap& k_map, const CUtensorMap& mn_map, unsigned char* dst, int row, bool mn) {
+              if (!mn) {
+                if (PAIR) tc_tma_load_2d_pair(&k_map, dst, full_addr, kx, t.mat * p.M + row);
+                else tc_tma_load_2d(&k_map, dst, &full[at], kx, t.mat * p.M + row);
+              } else {
+                if (PAIR) tc_tma_load_3d_pair(&mn_map, dst, full_addr, 0, t.mat * p.M + kx, row / TC_MN_GROUP);
+                else tc_tma_load_3d(&mn_map, dst, &full[at], 0, t.mat * p.M + kx, row / TC_MN_GROUP);
+              }
+            };
+            load(part ? p.l.k_lo : p.l.k_hi, part ? p.l.mn_lo : p.l.mn_hi, s, l_at, l_mn);
+            load(part ? p.r.k_lo : p.r.k_hi, part ? p.r.mn_lo : p.r.mn_hi, s + A_BYTES, r_at, r_mn);
+            if (++slot[part] == (uint32_t)(part ? p.lo_slots : p.hi_slots)) {
+              slot[part] = 0;
+              phase[part] ^= 1u;
+            }
           }
         }
       }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------------------------------------------------------- MMA issuer (pair: the leader only)
-      uint32_t stage = 0, phase = 0, acc_par = 0;
+      uint32_t hi_slot = 0, hi_phase = 0, lo_slot = 0, lo_phase = 0, acc_par = 0;
       int buf = 0;
       const uint32_t tiles_u = ag_smem_u32(tiles) >> 4;
       TcDesc dk, dmn;
       dk.init(0);
       dmn.init(1);
+      auto arrive = [&](uint64_t* bar) {  // when the MMAs so far are done (pair: in both CTAs)
+        if (PAIR) {
+          const uint32_t e = ag_smem_u32(bar);
+          tc_commit_pair(tc_map_to_cta(e, 0u));
+          tc_commit_pair(tc_map_to_cta(e, 1u));
+        } else {
+          tc_commit(bar);
+        }
+      };
       NsTile t;
       for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
-        uint32_t tacc = 0;
-        int left = 0;
-        for (int k = 0; k < p.k_iters; ++k) {
-          uint32_t not_first = 1u;
-          if (left == 0) {
-            if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
-              expired = true;
-              break;
-            }
-            acc_par ^= 1u << buf;
-            tacc = tmem_base + (uint32_t)buf * BN;
-            left = p.k_iters - k < p.chain ? p.k_iters - k : p.chain;
-            not_first = 0u;
-          }
-          if (!tc_wait(&full[stage], phase, abort_flag)) {
+        for (int k = 0; k < p.k_iters && !expired; k += p.chain) {
+          const int n = p.k_iters - k < p.chain ? p.k_iters - k : p.chain;
+          if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
             expired = true;
             break;
           }
-          tc_fence_after();
-          const uint32_t su = tiles_u + stage * (STAGE >> 4);
-          const int blk = k * TC_BK / BM;
-          const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
-          const uint32_t ah = su + (l_mn ? dmn.lo_const : dk.lo_const), al = ah + (A_BYTES >> 4);
-          const uint32_t bh = su + ((SPLIT ? 2u * A_BYTES : A_BYTES) >> 4) + (r_mn ? dmn.lo_const : dk.lo_const), bl = bh + (B_BYTES >> 4);
-          ns_stage_mmas<SPLIT, PAIR>(tacc, ah, al, l_mn ? dmn.step : dk.step, bh, bl, r_mn ? dmn.step : dk.step,
-                                     IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u), not_first);
-          if (PAIR) {
-            const uint32_t e = ag_smem_u32(&empty[stage]);
-            tc_commit_pair(tc_map_to_cta(e, 0u));
-            tc_commit_pair(tc_map_to_cta(e, 1u));
-          } else {
-            tc_commit(&empty[stage]);
-          }
-          if (++stage == (uint32_t)p.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          if (--left == 0) {
-            if (PAIR) {
-              const uint32_t f = ag_smem_u32(&acc_full[buf]);
-              tc_commit_pair(tc_map_to_cta(f, 0u));
-              tc_commit_pair(tc_map_to_cta(f, 1u));
-            } else {
-              tc_commit(&acc_full[buf]);
+          acc_par ^= 1u << buf;
+          const uint32_t tacc = tmem_base + (uint32_t)buf * BN;
+          uint32_t not_first = 0u;
+          // SPLIT: the low products of the chain's steps, then the high ones; both wait for nothing but their tiles
+          uint32_t slot = hi_slot, phase = hi_phase;
+#pragma unroll
+          for (int part = SPLIT ? 1 : 0; part >= 0 && !expired; --part) {
+            if (part == 0) slot = hi_slot, phase = hi_phase;
+            for (int j = 0; j < n; ++j) {
+              if (!tc_wait(&full[slot], phase, abort_flag) || (part && !tc_wait(&full[p.hi_slots + lo_slot], lo_phase, abort_flag))) {
+                expired = true;
+                break;
+              }
+              tc_fence_after();
+              const int blk = (k + j) * TC_BK / BM;
+              const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
+              const uint32_t l_const = l_mn ? dmn.lo_const : dk.lo_const, r_const = (r_mn ? dmn.lo_const : dk.lo_const) + (A_BYTES >> 4);
+              const uint32_t hs = tiles_u + slot * (SLOT >> 4), ls = tiles_u + (p.hi_slots + lo_slot) * (SLOT >> 4);
+              const uint32_t idesc = IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u);
+              const uint32_t l_step = l_mn ? dmn.step : dk.step, r_step = r_mn ? dmn.step : dk.step;
+              if (part) {
+                ns_step_mmas<true, PAIR>(tacc, hs + l_const, ls + l_const, l_step, hs + r_const, ls + r_const, r_step, idesc, not_first);
+                arrive(&empty[p.hi_slots + lo_slot]);
+                if (++lo_slot == (uint32_t)p.lo_slots) lo_slot = 0, lo_phase ^= 1u;
+              } else {
+                ns_step_mmas<false, PAIR>(tacc, hs + l_const, 0, l_step, hs + r_const, 0, r_step, idesc, not_first);
+                arrive(&empty[slot]);
+              }
+              not_first = 1u;
+              if (++slot == (uint32_t)p.hi_slots) slot = 0, phase ^= 1u;
             }
-            buf ^= 1;
           }
+          hi_slot = slot;
+          hi_phase = phase;
+          if (expired) break;
+          arrive(&acc_full[buf]);
+          buf ^= 1;
         }
       }
     }
@@ -551,57 +465,43 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     // ------------------------------------------------------------------ epilogue (warps 4..11)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int quarter = warp & 3, slice = (warp - 4) >> 2;
-    unsigned char* stg = staging + (warp - 4) * 2048;
+    unsigned char* stg = staging + (warp - 4) * 4096;
     uint32_t full_par = 0;
-    int buf = 0;
+    int buf = 0, half = 0;
     NsTile t;
     for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
       const int row0 = t.tm * BM + row_off + quarter * 32, row = row0 + lane, col0 = t.tn * BN + slice * (BN / 2);
       const uint32_t toff = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slice * (BN / 2));
       const bool rows_in = row0 < p.M;  // padded sizes are multiples of 32
-      const int64_t at = (int64_t)t.mat * p.M * p.ldd + (int64_t)row * p.ldd + col0;
-      NsWords ah[2], al[2];             // POLY: A where the tile goes, a chunk ahead
-      auto fetch = [&](const int c) {
-        if (KIND == NS_POLY && rows_in && col0 + c * 32 < p.N) {
-          ah[c & 1].load(p.A.hi + at + c * 32);
-          if (SPLIT) al[c & 1].load(p.A.lo + at + c * 32);
-        }
+      // one word of each of the lane's 32 columns: through the half of the buffer that was stored from before the last
+      auto put = [&](const CUtensorMap& map, const uint32_t (&w)[16], int col) {
+        if (lane == 0) ns_stores_read<1>();
+        __syncwarp();
+        unsigned char* s = stg + half * 2048;
+        half ^= 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(tc_stage_at(s, lane, j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        ag_fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) ns_tma_store(&map, s, col, t.mat * p.M + row0);
       };
       auto chunk = [&](const int c, float (&v)[32]) {
         const int col = col0 + c * 32;
-        if (c + 1 < CHUNKS) fetch(c + 1);
         if (!rows_in || col >= p.N) return;
-        if constexpr (KIND != NS_LAST) {
-          if constexpr (KIND == NS_POLY) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float2 x = ah[c & 1].pair(k);
-              if (SPLIT) {
-                const float2 y = al[c & 1].pair(k);
-                x.x += y.x; x.y += y.y;
-              }
-              v[2 * k] = fmaf(p.mul, v[2 * k], p.add * x.x);
-              v[2 * k + 1] = fmaf(p.mul, v[2 * k + 1], p.add * x.y);
-            }
-            const int hit = row - col;
+        for (int j = 0; j < 32; ++j) v[j] *= p.mul;
+        if (ns_symmetric(KIND)) {
+          const int hit = row - col;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j == hit) v[j] += p.diag;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= p.mul;
-          }
-          ns_store_row<SPLIT>(p.D, at + c * 32, v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= p.mul;
-          if (p.tall) {  // row of X = column of the matrix: lanes are neighbours in memory
-            if (row < p.cols) ns_apply_column(p, t.mat, (int64_t)col * p.cols + row, v, p.rows - col);
-          } else {       // through shared memory, 32 rows x 16 columns at a time
-#pragma unroll
-            for (int h = 0; h < 2; ++h) ns_apply_block(p, t.mat, stg, lane, v + 16 * h, row0, col + 16 * h);
-          }
+          for (int j = 0; j < 32; ++j)
+            if (j == hit) v[j] += p.diag;
         }
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) split_f16x2(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+        put(p.d_hi, hi, col);
+        if (SPLIT || p.two) put(p.d_lo, lo, col);
       };
       auto wait_full = [&]() {
         if (!tc_wait(&acc_full[buf], (full_par >> buf) & 1u, abort_flag)) {
@@ -624,7 +524,6 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
       float acc[CHUNKS][32];
       bool gone = false;
       for (int k = 0; k < p.k_iters; k += p.chain) {
-        if (k + p.chain >= p.k_iters) fetch(0);
         if (!wait_full()) {
           gone = true;
           break;
@@ -656,6 +555,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) chunk(c, acc[c]);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
   tc_fence_before();
@@ -669,54 +569,96 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   }
 }
 
-// No steps: X itself
+// p <- keep p - by X (kind 0), or X in fp32 (1) or bf16 (2): tiles of 64 x 64 of X, as in ns_start_kernel
 __global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices mats, NsPlan t, NsPlane X, float keep, float by,
                                                                int out_kind) {
+  __shared__ float tile[64][65];
   ag_pdl_wait();
   ag_pdl_trigger();
-  const int64_t x = (int64_t)blockIdx.y * t.mp * t.np, elements = (int64_t)t.rows * t.cols;
-  for (int64_t i = (int64_t)blockIdx.x * NS_THREADS + threadIdx.x; i < elements; i += (int64_t)gridDim.x * NS_THREADS) {
-    const int64_t row = i / t.cols, col = i - row * t.cols;
-    float* p = mats.p[blockIdx.y];
-    ns_apply(p, i, ns_get(X, x + (t.rows > t.cols ? col * t.np + row : row * t.np + col)), out_kind == 0 ? p[i] : 0.0f, keep, by, out_kind);
+  const bool tall = t.rows > t.cols;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int row = tall ? c0 + ty : r0 + ty, col = tall ? r0 + tx : c0 + tx;  // of the matrix: rows 4 apart
+  const int64_t at = (int64_t)row * t.cols + col, x = (int64_t)blockIdx.z * t.mp * t.np;
+  float* p = mats.p[blockIdx.z];
+  float old[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) old[k] = out_kind == 0 && row + 4 * k < t.rows && col < t.cols ? p[at + (int64_t)(4 * k) * t.cols] : 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = threadIdx.x + h * NS_THREADS, r = i >> 3, c = (i & 7) * 8;
+    const int64_t from = x + (int64_t)(r0 + r) * t.np + c0 + c;
+    const uint4 hi = *reinterpret_cast<const uint4*>(X.hi + from);
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u);
+    if (X.lo) lo = *reinterpret_cast<const uint4*>(X.lo + from);
+    const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w}, lw[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hw[k])), v = __half22float2(*reinterpret_cast<const __half2*>(&lw[k]));
+      const float a = (u.x + v.x) * (1.0f / NS_SCALE), b = (u.y + v.y) * (1.0f / NS_SCALE);
+      tile[tall ? c + 2 * k : r][tall ? r : c + 2 * k] = a;
+      tile[tall ? c + 2 * k + 1 : r][tall ? r : c + 2 * k + 1] = b;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    if (row + 4 * k >= t.rows || col >= t.cols) continue;
+    const float v = tile[ty + 4 * k][tx];
+    const int64_t i = at + (int64_t)(4 * k) * t.cols;
+    if (out_kind == 2) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else p[i] = out_kind == 0 ? fmaf(-by, v, keep * old[k]) : v;
   }
 }
 
 // ---------------------------------------------------------------------------- host side
-// Tensor map of a plane of `rows` rows (of all matrices) of `cols` columns: tiles of TC_BK columns and box_rows rows, or seen as
-// {64, rows, cols / 64}, for the columns of a product, boxes of TC_BK rows and `box_rows` columns.
-int ns_map(ag_ctx* ctx, CUtensorMap* tm, const void* plane, int64_t rows, int64_t cols, int box, bool mn_major) {
+// Tensor maps of a plane of `rows` rows (of all matrices) of `cols` columns.  NS_K: tiles of TC_BK columns and `box` rows; NS_MN: seen
+// as {64, rows, cols / 64}, boxes of TC_BK rows and `box` columns; NS_OUT: 32 x 32.
+enum { NS_K, NS_MN, NS_OUT };
+int ns_map(ag_ctx* ctx, CUtensorMap* tm, const void* plane, int64_t rows, int64_t cols, int box, int form) {
   EncodeTiledFn encode = tc_encode_fn(ctx);
   if (!encode) return AG_ERR_CUDA;
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1}, strides[2] = {(cuuint64_t)cols * 2, TC_MN_GROUP * 2};
   cuuint32_t boxes[3] = {TC_BK, (cuuint32_t)box, 1}, estr[3] = {1, 1, 1};
-  if (mn_major) {
+  if (form == NS_MN) {
     dims[0] = TC_MN_GROUP; dims[2] = (cuuint64_t)(cols / TC_MN_GROUP);
     boxes[0] = TC_MN_GROUP; boxes[1] = TC_BK; boxes[2] = (cuuint32_t)(box / TC_MN_GROUP);
+  } else if (form == NS_OUT) {
+    boxes[0] = boxes[1] = 32;
   }
-  const CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, mn_major ? 3 : 2, const_cast<void*>(plane), dims, strides, boxes, estr,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, form == NS_MN ? 3 : 2, const_cast<void*>(plane), dims, strides, boxes, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, form == NS_OUT ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     AG_FAIL(ctx, AG_ERR_CUDA, "cuTensorMapEncodeTiled failed: CUresult %d (ptr %p, %lld x %lld, box %d)", (int)r, plane, (long long)rows,
             (long long)cols, box);
   return AG_OK;
 }
 
-int ns_maps(ag_ctx* ctx, NsMaps& m, const NsPlane& plane, int64_t rows, int64_t cols, int box) {
-  int rc;
-  if ((rc = ns_map(ctx, &m.k_hi, plane.hi, rows, cols, box, false)) || (rc = ns_map(ctx, &m.mn_hi, plane.hi, rows, cols, box, true))) return rc;
-  m.k_lo = m.k_hi;
-  m.mn_lo = m.mn_hi;
-  if (plane.lo && ((rc = ns_map(ctx, &m.k_lo, plane.lo, rows, cols, box, false)) || (rc = ns_map(ctx, &m.mn_lo, plane.lo, rows, cols, box, true))))
-    return rc;
-  return AG_OK;
+// Planes and their maps: as operands, and as a result
+struct NsBuffer {
+  NsPlane plane;
+  NsMaps maps;
+  CUtensorMap out_hi, out_lo;
+};
+
+int ns_maps(ag_ctx* ctx, NsBuffer& b, int64_t rows, int64_t cols) {
+  int rc = AG_OK;
+  auto make = [&](CUtensorMap& hi, CUtensorMap& lo, int form) {
+    if (!rc) rc = ns_map(ctx, &hi, b.plane.hi, rows, cols, TC_BM, form);
+    lo = hi;
+    if (!rc && b.plane.lo) rc = ns_map(ctx, &lo, b.plane.lo, rows, cols, TC_BM, form);
+  };
+  make(b.maps.k_hi, b.maps.k_lo, NS_K);
+  make(b.maps.mn_hi, b.maps.mn_lo, NS_MN);
+  make(b.out_hi, b.out_lo, NS_OUT);
+  return rc;
 }
 
 template <int KIND, bool SPLIT, bool PAIR, int BN>
 int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int BM = PAIR ? 256 : 128, BN_CTA = PAIR ? BN / 2 : BN;
-  constexpr size_t STAGE = (size_t)(TC_BM + BN_CTA) * 128 * (SPLIT ? 2 : 1);
+  constexpr size_t SLOT = (size_t)(TC_BM + BN_CTA) * 128;
   static std::atomic<int> known[AG_MAX_DEVICES];  // 1 + units that are resident at once
   auto kern = ns_gemm_kernel<KIND, SPLIT, PAIR, BN>;
   std::atomic<int>& slot = known[ag_dev_slot(ctx)];
@@ -748,10 +690,15 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   p.tiles = ns_symmetric(KIND) ? p.tiles_n * (p.tiles_n + 1) / 2 : p.tiles_m * p.tiles_n;
   const int chain = SPLIT ? NS_CHAIN_PAIRS : NS_CHAIN_SINGLE, parts = (p.k_iters + chain - 1) / chain;
   p.chain = (p.k_iters + parts - 1) / parts;
-  p.stages = std::min<int>(NS_MAX_STAGES, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / STAGE));
+  if (SPLIT) p.mul *= (float)(1.0 + NS_LOSS * std::max(0.0, ((p.k_real + 15) / 16 - parts) / (double)parts));
+  // A chain's high tiles stay until its low products are through: twice as many slots of them
+  constexpr int SLOTS = std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
+  p.lo_slots = SPLIT ? SLOTS / 3 : 0;
+  p.hi_slots = SLOTS - p.lo_slots;
+  static_assert(SLOTS >= 6, "two chains of high tiles and one of low ones");
   units = std::min<int64_t>(units, (int64_t)p.batch * p.tiles);
   cfg.gridDim = dim3(PAIR ? 2 * units : units);
-  cfg.dynamicSmemBytes = NS_SMEM_FIXED + p.stages * STAGE;
+  cfg.dynamicSmemBytes = NS_SMEM_FIXED + SLOTS * SLOT;
   cfg.stream = ctx->stream;
   if (ctx->pdl) {
     at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -769,43 +716,24 @@ int ns_product(ag_ctx* ctx, NsGemm& p) {
   return p.M > 256 ? ns_launch<KIND, SPLIT, true, 256>(ctx, p) : ns_launch<KIND, SPLIT, false, 128>(ctx, p);
 }
 
-struct NsBuffer {
-  NsPlane plane;
-  NsMaps maps;
-};
-
+// X[0] -> the factor in X[steps & 1]
 template <bool SPLIT>
-int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsPlane Xp, NsPlane Yp, NsPlane Ap, NsPlane Qp, const float* coefficients,
-               int steps) {
-  NsBuffer X[2], A, Q;
-  X[0].plane = Xp; X[1].plane = Yp; A.plane = Ap; Q.plane = Qp;
-  const int64_t rows = (int64_t)p.batch * t.mp;
-  int rc;
-  for (NsBuffer* b : {&X[0], &X[1], &A, &Q})
-    if ((rc = ns_maps(ctx, b->maps, b->plane, rows, b == &A || b == &Q ? t.mp : t.np, TC_BM))) return rc;
+int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsBuffer* X, NsBuffer& A, NsBuffer& Q, const float* coefficients, int steps) {
+  const float unit = 1.0f / NS_SCALE;  // operands carry NS_SCALE each, a result one of them
   for (int i = 0; i < steps; ++i) {
-    const float *co = coefficients + 3 * i, unit = 1.0f / NS_SCALE;
+    const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2], h = c != 0.0 ? b / (2.0 * c) : 0.0;
     NsBuffer &x = X[i & 1], &y = X[~i & 1];
-    p.M = p.N = t.mp; p.ldd = t.mp;
-    p.k_iters = t.np / TC_BK;
-    p.l = p.r = x.maps;
-    p.D = A.plane; p.mul = unit;
-    if ((rc = ns_product<NS_GRAM, SPLIT>(ctx, p))) return rc;
-    p.k_iters = t.mp / TC_BK;
-    p.l = p.r = A.maps;
-    p.D = Q.plane; p.A = A.plane;
-    p.diag = co[0] * NS_SCALE; p.add = co[1]; p.mul = co[2] * unit;
-    if ((rc = ns_product<NS_POLY, SPLIT>(ctx, p))) return rc;
-    p.N = t.np; p.ldd = t.np;
-    p.l = Q.maps; p.r = x.maps;
-    p.D = y.plane;
-    if (i + 1 < steps) {
-      p.mul = unit;
-      rc = ns_product<NS_NEXT, SPLIT>(ctx, p);
-    } else {
-      p.mul = unit * unit;
-      rc = ns_product<NS_LAST, SPLIT>(ctx, p);
-    }
+    auto product = [&](auto kind, const NsMaps& l, const NsMaps& r, NsBuffer& d, int n, int k, double mul, double diag) {
+      p.l = l; p.r = r;
+      p.d_hi = d.out_hi; p.d_lo = d.out_lo;
+      p.two = d.plane.lo && (SPLIT || (&d == &y && i + 1 == steps));
+      p.N = n; p.k_iters = (k + TC_BK - 1) / TC_BK; p.k_real = k;
+      p.mul = (float)mul * unit; p.diag = (float)(diag * NS_SCALE);
+      return ns_product<decltype(kind)::value, SPLIT>(ctx, p);
+    };
+    int rc = product(std::integral_constant<int, NS_GRAM>(), x.maps, x.maps, c != 0.0 ? A : Q, t.mp, t.n, c != 0.0 ? 1.0 : b, c != 0.0 ? h : a);
+    if (!rc && c != 0.0) rc = product(std::integral_constant<int, NS_POLY>(), A.maps, A.maps, Q, t.mp, t.m, c, a - h * h * c);
+    if (!rc) rc = product(std::integral_constant<int, NS_NEXT>(), Q.maps, x.maps, y, t.np, t.m, 1.0, 0.0);
     if (rc) return rc;
   }
   return AG_OK;
@@ -813,13 +741,14 @@ int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsPlane Xp, NsPlane Yp, 
 
 int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int bf16, const NsUpdate& s, float eps,
            const float* coefficients, int steps, float keep, float by, int out_kind, char* scratch, bool split) {
-  auto plane = [&](size_t at, size_t bytes) {
-    NsPlane r = {reinterpret_cast<__half*>(scratch + at), nullptr};
-    if (split || steps == 0) r.lo = reinterpret_cast<__half*>(scratch + at + bytes / 2);
-    return r;
+  // 16-bit operands have one word, but for the last result, which nothing multiplies
+  auto plane = [&](size_t at, size_t bytes, bool two) {
+    return NsPlane{reinterpret_cast<__half*>(scratch + at), two ? reinterpret_cast<__half*>(scratch + at + bytes / 2) : nullptr};
   };
-  const NsPlane X = plane(0, t.x_bytes), Y = plane(t.x_bytes, t.x_bytes), A = plane(2 * t.x_bytes, t.a_bytes),
-                Q = plane(2 * t.x_bytes + t.a_bytes, t.a_bytes);
+  NsBuffer X[2], A, Q;
+  for (int i = 0; i < 2; ++i) X[i].plane = plane(i * t.x_bytes, t.x_bytes, split || i == (steps & 1));
+  A.plane = plane(2 * t.x_bytes, t.a_bytes, split);
+  Q.plane = plane(2 * t.x_bytes + t.a_bytes, t.a_bytes, split);
   double* norms = reinterpret_cast<double*>(scratch + 2 * t.x_bytes + 2 * t.a_bytes);
   const int64_t elements = (int64_t)t.rows * t.cols;
   bool vec = true;
@@ -833,20 +762,23 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
   else
     AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", ns_momentum_kernel<false>, dim3(blocks, count), NS_THREADS, 0, mats, elements, bf16, s, norms);
   AG_LAUNCH_PDL(ctx, "ns_start_kernel", ns_start_kernel, dim3(t.np / 64, t.mp / 64, count), NS_THREADS, 0, mats, t, bf16, s, eps,
-                (const double*)norms, blocks, X);
-  if (steps == 0) {
-    int many = ag_ceil_div(elements, NS_THREADS * 4);
-    if (many > 1024) many = 1024;
-    AG_LAUNCH_PDL(ctx, "ns_finish_kernel", ns_finish_kernel, dim3(many, count), NS_THREADS, 0, mats, t, X, keep, by, out_kind);
-    return AG_OK;
+                (const double*)norms, blocks, X[0].plane);
+  if (steps > 0) {
+    const int64_t rows = (int64_t)count * t.mp;
+    int rc;
+    if ((rc = ns_maps(ctx, X[0], rows, t.np)) || (rc = ns_maps(ctx, X[1], rows, t.np)) || (rc = ns_maps(ctx, A, rows, t.mp)) ||
+        (rc = ns_maps(ctx, Q, rows, t.mp)))
+      return rc;
+    NsGemm p = {};
+    p.batch = count;
+    p.M = t.mp;
+    p.status = ctx->d_status;
+    if ((rc = split ? ns_iterate<true>(ctx, t, p, X, A, Q, coefficients, steps) : ns_iterate<false>(ctx, t, p, X, A, Q, coefficients, steps)))
+      return rc;
   }
-  NsGemm p = {};
-  p.batch = count;
-  p.mats = mats;
-  p.rows = t.rows; p.cols = t.cols; p.tall = t.rows > t.cols; p.out_kind = out_kind;
-  p.keep = keep; p.by = by;
-  p.status = ctx->d_status;
-  return split ? ns_iterate<true>(ctx, t, p, X, Y, A, Q, coefficients, steps) : ns_iterate<false>(ctx, t, p, X, Y, A, Q, coefficients, steps);
+  AG_LAUNCH_PDL(ctx, "ns_finish_kernel", ns_finish_kernel, dim3(t.np / 64, t.mp / 64, count), NS_THREADS, 0, mats, t, X[steps & 1].plane,
+                keep, by, out_kind);
+  return AG_OK;
 }
 
 bool ns_fits(int rows, int cols) {
@@ -862,6 +794,11 @@ int ns_check(ag_ctx* ctx, const char* name, int count, int rows, int cols, const
   AG_REQUIRE(ctx, ns_fits(rows, cols), "%s: %d x %d is too large", name, rows, cols);
   AG_REQUIRE(ctx, steps >= 0 && steps <= NS_MAX_STEPS && (steps == 0 || coefficients), "%s: %d steps", name, steps);
   for (int i = 0; i < 3 * steps; ++i) AG_REQUIRE(ctx, ns_finite(coefficients[i]), "%s: coefficient %g", name, (double)coefficients[i]);
+  for (int i = 0; i < steps; ++i) {
+    const double b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    AG_REQUIRE(ctx, c == 0.0 || (fabs(b) <= 16.0 * fabs(c) && b * b <= 256.0 * fabs(c)), "%s: coefficients b %g and c %g are too far apart",
+               name, b, c);
+  }
   AG_REQUIRE(ctx, eps > 0.0f && ns_finite(eps), "%s: eps %g", name, (double)eps);
   AG_REQUIRE(ctx, precision == AG_CE_3XTF32 || precision == AG_CE_BF16, "%s: precision %d", name, precision);
   AG_REQUIRE(ctx, count == 0 || (scratch && ((uintptr_t)scratch & 255) == 0), "%s: the workspace has to be 256-byte aligned", name);

@@ -77,19 +77,52 @@ def kept(x, bits):
     return (hi.astype(np.float64) + (y - hi.astype(np.float32)).astype(np.float16).astype(np.float64)) / 4096.0
 
 
-def factor_error(u, coefficients, steps, eps, bits):
-    """(factor, how far one is off whose operands are rounded to `bits` significant bits, as a Frobenius norm).
+def truncated(x):
+    """x with 23 significant bits, cut off: what a sum in a tensor core keeps (the number with which 512 additions of one sign lose
+    3e-5 of their sum, as they do)."""
+    m, e = np.frexp(x)
+    return np.ldexp(np.trunc(m * 2.0 ** 23), e - 23)
 
-    The rounded form rounds where a kernel does and has exact products.  A kernel's sums are of 32 bits: its roundings fall otherwise
-    where a sum is next to the middle of two numbers, which makes other errors of the same size, and each sum is off by up to 48
-    truncations (2^-23 each at most, half of that on average and less while the sum grows): 2^-18."""
+
+def product(x, y, bits):
+    """x @ y of operands as they are kept: sums of 16 products are exact and truncated as they are added up, 128 elements at a time with
+    22 bits, the products with a low part first; 32-bit sums of those."""
+    high = [kept(v, 11) for v in (x, y)]
+    low = [kept(v, 22) - h for v, h in zip((x, y), high)]
+    out = np.zeros((x.shape[0], y.shape[1]), np.float32)
+    chain = 128 if bits == 22 else 8192
+    for k in range(0, x.shape[1], chain):
+        acc = np.zeros(out.shape)
+        blocks = [slice(j, min(j + 16, k + chain, x.shape[1])) for j in range(k, min(k + chain, x.shape[1]), 16)]
+        if bits == 22:
+            for s in blocks:
+                acc = truncated(acc + high[0][:, s] @ low[1][s])
+                acc = truncated(acc + low[0][:, s] @ high[1][s])
+        for s in blocks:
+            acc = truncated(acc + high[0][:, s] @ high[1][s])
+        out += acc.astype(np.float32)
+    return out.astype(np.float64)
+
+
+def factor_error(u, coefficients, steps, eps, bits):
+    """(factor, how far one is off whose operands are rounded to `bits` significant bits and whose sums are truncated, as a Frobenius
+    norm).
+
+    The form rounds and truncates where a kernel does: operands of every product, the completed square of a step, 23 bits of a sum.
+    That way what each of the products adds is taken along through the steps that follow, which multiply it by up to their largest
+    coefficient (8.2, 4 and 1.9 make 62); as one term of the result alone it is underrated by that.  A kernel's errors fall otherwise, and are of
+    the same size."""
     ref = factor(u, coefficients, steps, eps)
     x = np.asarray(u, np.float64)
     x = x / max(np.sqrt(np.sum(x * x)), eps)
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
+    one = np.eye(len(x))
     for a, b, c in triples(coefficients, steps):
-        x = kept(x, bits)
-        g = kept(x @ x.T, bits)
-        x = kept(a * np.eye(len(g)) + b * g + c * (g @ g), bits) @ x
+        if c == 0:
+            q = a * one + b * product(x, x.T, bits)
+        else:
+            g = product(x, x.T, bits) + b / (2 * c) * one
+            q = (a - b * b / (4 * c)) * one + c * product(g, g, bits)
+        x = product(q, x, bits)
     return ref, np.linalg.norm((x.T if tall else x) - ref)

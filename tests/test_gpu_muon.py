@@ -1,8 +1,8 @@
 """Orthogonal factors and the step along them against the 64-bit forms.
 
-A factor may be off by four times what the form with rounded operands is (oracle.heads_and_updates.factor_error: 22 significant bits,
-or 11 of products of 16-bit operands) and by 2^-18 of its norm, what truncated sums leave out.  An update adds the roundings of its own
-arithmetic: p by 2^-24 of each of |p| (twice) and of its change (four times); m by 4 u (|m| + |g|)."""
+A factor may be off by four times what the form with rounded operands and truncated sums is (oracle.heads_and_updates.factor_error:
+operands of 22 significant bits, or 11 of products of 16-bit operands), by 2^-18 of its norm (the error of a form with one
+number or a few may be small by chance), and by half a step of its type.  An update adds the roundings of its own arithmetic: p by 2^-24 of each of |p| (twice) and of its change (four times); m by 4 u (|m| + |g|)."""
 import numpy as np
 import pytest
 

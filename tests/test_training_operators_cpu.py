@@ -108,7 +108,9 @@ REFUSED = (
         dict(ctx=0), dict(count=-1), dict(rows=0), dict(cols=-3), dict(rows=16385, cols=16385), dict(rows=2, cols=(1 << 20) + 1),
         dict(rows=16384, cols=1 << 17), dict(steps=-1), dict(steps=33), dict(coefficients=None), dict(eps=0.0), dict(eps=-1.0), dict(eps=NAN),
         dict(eps=INF), dict(precision=N.AG_CE_FP32), dict(precision=N.AG_CE_BF16X3), dict(precision=9), dict(dtype=2), dict(g=None),
-        dict(coefficients=_array(ctypes.c_float, [3.4, -4.7, 2.0] * 4 + [NAN, 1, 1])), dict(scratch=0), dict(scratch=BASE + 3 * FAR + 128),
+        dict(coefficients=_array(ctypes.c_float, [3.4, -4.7, 2.0] * 4 + [NAN, 1, 1])),
+        dict(coefficients=_array(ctypes.c_float, [3.4, -4.7, 2.0] * 4 + [3.4, -4.7, 0.2])),
+        dict(coefficients=_array(ctypes.c_float, [3.4, 1e3, 100.0] * 5)), dict(scratch=0), dict(scratch=BASE + 3 * FAR + 128),
         dict(g=_array(ctypes.c_void_p, [BASE + FAR, 0, BASE + 2 * FAR])), dict(g=_addresses(BASE + FAR + 2)), dict(g=_addresses(BASE + 4)),
         dict(scratch=BASE + FAR), dict(scratch=BASE - 256))] +
     [("ag_orthogonalise", c) for c in (
