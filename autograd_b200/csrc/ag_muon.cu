@@ -202,7 +202,9 @@ __global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices m
 // ---------------------------------------------------------------------------- products
 // One persistent kernel, D = f(L R) for every matrix of the batch: TMA producer, MMA issuer and epilogue warps as in
 // ag_flce_tc.cu, on single CTAs (128 x BN) or on pairs of them (256 x BN).  Operands are planes, three MMAs per 16 elements of
-// the contraction (hi lo, lo hi, hi hi) where there are two; tiles of high and of low parts come through rings of their own.
+// the contraction (hi lo, lo hi, hi hi) where there are two.  What one thread issues between MMAs takes their time where they do not
+// queue up, a tcgen05.commit above all (ten of them to 24 MMAs: 171 cycles for each of 128): slots hold 128 elements, a commit
+// arrives in both CTAs of a pair, and where a chain is a slot, the commit that hands its sum over frees it too.
 // A step X <- (a I + b G + c G G) X, G = X X^T, is a square once it is completed: with h = b / 2 c
 //   GRAM:  A = G + h I                    both operands K-major
 //   POLY:  Q = (a - h h c) I + c A A      both symmetric
@@ -217,16 +219,16 @@ constexpr bool ns_symmetric(int kind) { return kind <= NS_POLY; }
 
 constexpr int NS_EPI_WARPS = 8;
 constexpr int NS_TC_THREADS = 128 + 32 * NS_EPI_WARPS;
-constexpr int NS_MAX_SLOTS = 12;
+constexpr int NS_MAX_SLOTS = 4;
 constexpr int NS_SMEM_LIMIT = 227 * 1024;
 constexpr int NS_STAGING = NS_EPI_WARPS * 4096;  // per epilogue warp: 32 rows of 64 bytes, twice, on their way to memory
 constexpr int NS_SMEM_FIXED = 1024 + NS_STAGING + 512;
-// The tensor core truncates a sum at every addition, by an amount that grows with it.  So chains are short, two steps of 64 elements
-// (single words: 128 steps, their operands are off by more), the epilogue adds them in registers, and the products with a low part come
+// The tensor core truncates a sum at every addition, by an amount that grows with it.  So chains are short, 128 elements
+// (single words: 8192, their operands are off by more), the epilogue adds them in registers, and the products with a low part come
 // first, whose sum is 2^-11 of the whole.  What truncation takes of a sum on average, NS_LOSS of it at each of the later additions of
 // 16 elements, is put back by the factor of the epilogue.  Error of the factor of 333 x 1001 with 0, 4e-8, 7e-8 and 1e-7: 3.8e-6, 1.9e-6, 2.9e-6, 4.7e-6
 // (plain fp32 products: 2.6e-6); without it, low parts first in every step, chains of 1, 2 and 4 steps: 2.6e-6, 5.7e-6, 8.7e-6.
-constexpr int NS_CHAIN_PAIRS = 2, NS_CHAIN_SINGLE = 128;
+constexpr int NS_CHAIN_PAIRS = 1, NS_CHAIN_SINGLE = 64;  // in double steps of 128 elements
 constexpr double NS_LOSS = 4.6e-8;
 
 // Tensor maps of a plane: tiles with the contraction along its rows (k), and along its columns (mn)
@@ -238,8 +240,8 @@ struct NsGemm {
   NsMaps l, r;
   CUtensorMap d_hi, d_lo;  // of the result: boxes of 32 rows x 32 columns
   int batch, tiles_m, tiles_n, tiles;  // tiles of a matrix; symmetric: those on and above the diagonal
-  int k_iters, chain, k_real;  // steps of 64 elements of the contraction, in chains; elements that are not padding
-  int hi_slots, lo_slots;  // of the two rings of operand tiles: high parts, low parts
+  int k_iters, chain, k_real;  // steps of 64 elements of the contraction; double steps to a chain; elements that are not padding
+  int slots;                   // of operand tiles of a double step
   int M, N;                // rows and columns of a matrix that are stored (padded)
   int two;                 // the result has a low part
   float diag, mul;
@@ -279,6 +281,13 @@ __device__ __forceinline__ void ns_tma_store(const CUtensorMap* tm, const void* 
 template <int N>
 __device__ __forceinline__ void ns_stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
+// an arrival at the barrier of both CTAs of a pair once the MMAs so far are done
+__device__ __forceinline__ void ns_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(ag_smem_u32(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+
 // The MMAs of a step of 64 elements: products with a low part, or those of the high parts
 template <bool LOW, bool PAIR>
 __device__ __forceinline__ void ns_step_mmas(uint32_t acc, uint32_t lh, uint32_t ll, uint32_t l_step, uint32_t rh, uint32_t rl,
@@ -298,18 +307,21 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   extern __shared__ unsigned char ns_smem_raw[];
   constexpr bool R_MN = !ns_symmetric(KIND);          // the right operand is stored with its columns contiguous
   constexpr uint32_t A_BYTES = TC_BM * 128, BN_CTA = PAIR ? BN / 2 : BN, B_BYTES = BN_CTA * 128;
-  constexpr uint32_t SLOT = A_BYTES + B_BYTES;        // both operands' tiles of 64 elements of the contraction
+  constexpr uint32_t STEP = A_BYTES + B_BYTES;        // both operands' tiles of 64 elements of the contraction
+  constexpr uint32_t SLOT = 2 * STEP;
   constexpr int BM = PAIR ? 2 * TC_BM : TC_BM;
   constexpr uint32_t COLUMNS = 2 * BN;                // of tensor memory: two accumulators
   constexpr int CHUNKS = BN / 64;                     // 32-column chunks of an epilogue warp
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
   static_assert(!ns_symmetric(KIND) || BM == BN, "tiles on the diagonal are square");
   unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ns_smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* staging = tiles + (size_t)(p.hi_slots + p.lo_slots) * SLOT;
-  // barriers of the slots: those of the ring of high parts, then of low parts
+  unsigned char* lows = tiles + (size_t)p.slots * SLOT;  // SPLIT: two slots of a step's low parts
+  unsigned char* staging = lows + (SPLIT ? SLOT : 0);
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + NS_STAGING);
-  uint64_t* empty = full + NS_MAX_SLOTS;
-  uint64_t* acc_full = empty + NS_MAX_SLOTS;
+  uint64_t* empty = full + NS_MAX_SLOTS;              // not SPLIT: a chain's slot is free when its sum is complete
+  uint64_t* low_full = empty + NS_MAX_SLOTS;
+  uint64_t* low_empty = low_full + 2;
+  uint64_t* acc_full = low_empty + 2;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -321,11 +333,13 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   const int row_off = PAIR ? (int)rank * TC_BM : 0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.hi_slots + p.lo_slots; ++s) {
+    for (int s = 0; s < p.slots; ++s) {
       ag_mbar_init(&full[s], 1);
       ag_mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
+      ag_mbar_init(&low_full[b], 1);
+      ag_mbar_init(&low_empty[b], 1);
       ag_mbar_init(&acc_full[b], 1);
       ag_mbar_init(&acc_empty[b], PAIR ? 2 * NS_EPI_WARPS : NS_EPI_WARPS);
     }
@@ -355,109 +369,115 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- TMA producer
-      uint32_t slot[2] = {0, 0}, phase[2] = {0, 0};
+      uint32_t slot = 0, phase = 0, low = 0, low_phase = 0;
       NsTile t;
       for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
-        const int l_at = t.tm * BM + row_off;
-        const int r_at = t.tn * BN + (int)rank * (PAIR ? (int)BN_CTA : 0);
-        for (int k = 0; k < p.k_iters && !expired; ++k) {
-          const int kx = k * TC_BK, blk = kx / BM;  // blk: tile of the contraction
+        const int l_at = t.tm * BM + row_off, r_at = t.tn * BN + (int)rank * (PAIR ? (int)BN_CTA : 0);
+        for (int k = 0; k < p.k_iters && !expired; k += 2) {
+          const int n = p.k_iters - k < 2 ? 1 : 2, blk = k * TC_BK / BM;  // blk: tile of the contraction
           const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
-#pragma unroll
-          for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
-            const uint32_t at = (part ? p.hi_slots : 0) + slot[part];
-            if (!tc_wait(&empty[at], phase[part] ^ 1u, abort_flag)) {
-              expired = true;
-              break;
-            }
-            unsigned char* s = tiles + (size_t)at * SLOT;
-            uint32_t full_addr = ag_smem_u32(&full[at]);
-            if (PAIR) {
-              if (rank == 0) ag_mbar_expect_tx(&full[at], 2u * SLOT);
-              full_addr = tc_map_to_cta(full_addr, 0u);
+          auto load = [&](const CUtensorMap& k_map, const CUtensorMap& mn_map, uint64_t* bar, unsigned char* dst, int kx, int row, bool mn) {
+            const uint32_t at = PAIR ? tc_map_to_cta(ag_smem_u32(bar), 0u) : 0u;  // the leader counts the bytes of both
+            if (!mn) {
+              if (PAIR) tc_tma_load_2d_pair(&k_map, dst, at, kx, t.mat * p.M + row);
+              else tc_tma_load_2d(&k_map, dst, bar, kx, t.mat * p.M + row);
             } else {
-              ag_mbar_expect_tx(&full[at], SLOT);
+              if (PAIR) tc_tma_load_3d_pair(&mn_map, dst, at, 0, t.mat * p.M + kx, row / TC_MN_GROUP);
+              else tc_tma_load_3d(&mn_map, dst, bar, 0, t.mat * p.M + kx, row / TC_MN_GROUP);
             }
-            auto load = [&](const CUtensorMap& k_map, const CUtensorMap& mn_map, unsigned char* dst, int row, bool mn) {
-              if (!mn) {
-                if (PAIR) tc_tma_load_2d_pair(&k_map, dst, full_addr, kx, t.mat * p.M + row);
-                else tc_tma_load_2d(&k_map, dst, &full[at], kx, t.mat * p.M + row);
-              } else {
-                if (PAIR) tc_tma_load_3d_pair(&mn_map, dst, full_addr, 0, t.mat * p.M + kx, row / TC_MN_GROUP);
-                else tc_tma_load_3d(&mn_map, dst, &full[at], 0, t.mat * p.M + kx, row / TC_MN_GROUP);
+          };
+          if (!tc_wait(SPLIT ? &acc_full[slot] : &empty[slot], phase ^ 1u, abort_flag)) {
+            expired = true;
+            break;
+          }
+          unsigned char* s = tiles + (size_t)slot * SLOT;
+          if (rank == 0) ag_mbar_expect_tx(&full[slot], (PAIR ? 2u : 1u) * n * STEP);
+          for (int j = 0; j < n; ++j, s += STEP) {
+            const int kx = (k + j) * TC_BK;
+            load(p.l.k_hi, p.l.mn_hi, &full[slot], s, kx, l_at, l_mn);
+            load(p.r.k_hi, p.r.mn_hi, &full[slot], s + A_BYTES, kx, r_at, r_mn);
+            if (SPLIT) {
+              if (!tc_wait(&low_empty[low], low_phase ^ 1u, abort_flag)) {
+                expired = true;
+                break;
               }
-            };
-            load(part ? p.l.k_lo : p.l.k_hi, part ? p.l.mn_lo : p.l.mn_hi, s, l_at, l_mn);
-            load(part ? p.r.k_lo : p.r.k_hi, part ? p.r.mn_lo : p.r.mn_hi, s + A_BYTES, r_at, r_mn);
-            if (++slot[part] == (uint32_t)(part ? p.lo_slots : p.hi_slots)) {
-              slot[part] = 0;
-              phase[part] ^= 1u;
+              unsigned char* d = lows + (size_t)low * STEP;
+              if (rank == 0) ag_mbar_expect_tx(&low_full[low], (PAIR ? 2u : 1u) * STEP);
+              load(p.l.k_lo, p.l.mn_lo, &low_full[low], d, kx, l_at, l_mn);
+              load(p.r.k_lo, p.r.mn_lo, &low_full[low], d + A_BYTES, kx, r_at, r_mn);
+              low ^= 1u;
+              low_phase ^= low ^ 1u;
             }
           }
+          if (++slot == (uint32_t)p.slots) slot = 0, phase ^= 1u;
         }
       }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------------------------------------------------------- MMA issuer (pair: the leader only)
-      uint32_t hi_slot = 0, hi_phase = 0, lo_slot = 0, lo_phase = 0, acc_par = 0;
+      uint32_t slot = 0, phase = 0, low = 0, low_phase = 0, acc_par = 0;
       int buf = 0;
-      const uint32_t tiles_u = ag_smem_u32(tiles) >> 4;
+      const uint32_t tiles_u = ag_smem_u32(tiles) >> 4, lows_u = ag_smem_u32(lows) >> 4;
       TcDesc dk, dmn;
       dk.init(0);
       dmn.init(1);
       auto arrive = [&](uint64_t* bar) {  // when the MMAs so far are done (pair: in both CTAs)
-        if (PAIR) {
-          const uint32_t e = ag_smem_u32(bar);
-          tc_commit_pair(tc_map_to_cta(e, 0u));
-          tc_commit_pair(tc_map_to_cta(e, 1u));
-        } else {
-          tc_commit(bar);
-        }
+        if (PAIR) ns_commit_both(bar);
+        else tc_commit(bar);
       };
       NsTile t;
       for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
-        for (int k = 0; k < p.k_iters && !expired; k += p.chain) {
-          const int n = p.k_iters - k < p.chain ? p.k_iters - k : p.chain;
-          if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
+        uint32_t tacc = 0, more = 0;
+        int left = 0;  // double steps of the chain
+        for (int k = 0; k < p.k_iters; k += 2) {
+          const int n = p.k_iters - k < 2 ? 1 : 2, blk = k * TC_BK / BM;
+          const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
+          const uint32_t idesc = IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u);
+          const uint32_t l_step = l_mn ? dmn.step : dk.step, r_step = r_mn ? dmn.step : dk.step;
+          const uint32_t l_const = l_mn ? dmn.lo_const : dk.lo_const, r_const = (A_BYTES >> 4) + (r_mn ? dmn.lo_const : dk.lo_const);
+          if (left == 0) {
+            if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
+              expired = true;
+              break;
+            }
+            acc_par ^= 1u << buf;
+            tacc = tmem_base + (uint32_t)buf * BN;
+            left = p.chain;
+            more = 0u;
+          }
+          if (!tc_wait(&full[slot], phase, abort_flag)) {
             expired = true;
             break;
           }
-          acc_par ^= 1u << buf;
-          const uint32_t tacc = tmem_base + (uint32_t)buf * BN;
-          uint32_t not_first = 0u;
-          // SPLIT: the low products of the chain's steps, then the high ones; both wait for nothing but their tiles
-          uint32_t slot = hi_slot, phase = hi_phase;
-#pragma unroll
-          for (int part = SPLIT ? 1 : 0; part >= 0 && !expired; --part) {
-            if (part == 0) slot = hi_slot, phase = hi_phase;
+          tc_fence_after();
+          const uint32_t hs = tiles_u + slot * (SLOT >> 4);
+          if (SPLIT) {
             for (int j = 0; j < n; ++j) {
-              if (!tc_wait(&full[slot], phase, abort_flag) || (part && !tc_wait(&full[p.hi_slots + lo_slot], lo_phase, abort_flag))) {
+              if (!tc_wait(&low_full[low], low_phase, abort_flag)) {
                 expired = true;
                 break;
               }
               tc_fence_after();
-              const int blk = (k + j) * TC_BK / BM;
-              const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
-              const uint32_t l_const = l_mn ? dmn.lo_const : dk.lo_const, r_const = (r_mn ? dmn.lo_const : dk.lo_const) + (A_BYTES >> 4);
-              const uint32_t hs = tiles_u + slot * (SLOT >> 4), ls = tiles_u + (p.hi_slots + lo_slot) * (SLOT >> 4);
-              const uint32_t idesc = IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u);
-              const uint32_t l_step = l_mn ? dmn.step : dk.step, r_step = r_mn ? dmn.step : dk.step;
-              if (part) {
-                ns_step_mmas<true, PAIR>(tacc, hs + l_const, ls + l_const, l_step, hs + r_const, ls + r_const, r_step, idesc, not_first);
-                arrive(&empty[p.hi_slots + lo_slot]);
-                if (++lo_slot == (uint32_t)p.lo_slots) lo_slot = 0, lo_phase ^= 1u;
-              } else {
-                ns_step_mmas<false, PAIR>(tacc, hs + l_const, 0, l_step, hs + r_const, 0, r_step, idesc, not_first);
-                arrive(&empty[slot]);
-              }
-              not_first = 1u;
-              if (++slot == (uint32_t)p.hi_slots) slot = 0, phase ^= 1u;
+              const uint32_t h = hs + j * (STEP >> 4), l = lows_u + low * (STEP >> 4);
+              ns_step_mmas<true, PAIR>(tacc, h + l_const, l + l_const, l_step, h + r_const, l + r_const, r_step, idesc, more);
+              more = 1u;
+              arrive(&low_empty[low]);
+              low ^= 1u;
+              low_phase ^= low ^ 1u;
             }
+            if (expired) break;
           }
-          hi_slot = slot;
-          hi_phase = phase;
-          if (expired) break;
-          arrive(&acc_full[buf]);
-          buf ^= 1;
+          for (int j = 0; j < n; ++j) {
+            const uint32_t h = hs + j * (STEP >> 4);
+            ns_step_mmas<false, PAIR>(tacc, h + l_const, 0, l_step, h + r_const, 0, r_step, idesc, more);
+            more = 1u;
+          }
+          if (!SPLIT) arrive(&empty[slot]);
+          if (++slot == (uint32_t)p.slots) slot = 0, phase ^= 1u;
+          if (--left == 0 || k + 2 >= p.k_iters) {
+            arrive(&acc_full[buf]);
+            buf ^= 1;
+            left = 0;
+          }
         }
       }
     }
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
       };
       float acc[CHUNKS][32];
       bool gone = false;
-      for (int k = 0; k < p.k_iters; k += p.chain) {
+      for (int k = 0; k < p.k_iters; k += 2 * p.chain) {
         if (!wait_full()) {
           gone = true;
           break;
@@ -552,8 +572,16 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         }
       }
       if (gone) break;
+      // one copy of the code for all chunks, which move up to acc[0] one after the other: what every tile runs through once is
+      // fetched anew each time
+#pragma unroll 1
+      for (int c = 0; c < CHUNKS; ++c) {
+        chunk(c, acc[0]);
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) chunk(c, acc[c]);
+        for (int k = 1; k < CHUNKS; ++k)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[k - 1][j] = acc[k][j];
+      }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -658,7 +686,7 @@ int ns_maps(ag_ctx* ctx, NsBuffer& b, int64_t rows, int64_t cols) {
 template <int KIND, bool SPLIT, bool PAIR, int BN>
 int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int BM = PAIR ? 256 : 128, BN_CTA = PAIR ? BN / 2 : BN;
-  constexpr size_t SLOT = (size_t)(TC_BM + BN_CTA) * 128;
+  constexpr size_t SLOT = (size_t)(TC_BM + BN_CTA) * 256;
   static std::atomic<int> known[AG_MAX_DEVICES];  // 1 + units that are resident at once
   auto kern = ns_gemm_kernel<KIND, SPLIT, PAIR, BN>;
   std::atomic<int>& slot = known[ag_dev_slot(ctx)];
@@ -688,17 +716,16 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
   p.tiles = ns_symmetric(KIND) ? p.tiles_n * (p.tiles_n + 1) / 2 : p.tiles_m * p.tiles_n;
-  const int chain = SPLIT ? NS_CHAIN_PAIRS : NS_CHAIN_SINGLE, parts = (p.k_iters + chain - 1) / chain;
-  p.chain = (p.k_iters + parts - 1) / parts;
-  if (SPLIT) p.mul *= (float)(1.0 + NS_LOSS * std::max(0.0, ((p.k_real + 15) / 16 - parts) / (double)parts));
-  // A chain's high tiles stay until its low products are through: twice as many slots of them
-  constexpr int SLOTS = std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
-  p.lo_slots = SPLIT ? SLOTS / 3 : 0;
-  p.hi_slots = SLOTS - p.lo_slots;
-  static_assert(SLOTS >= 6, "two chains of high tiles and one of low ones");
+  p.chain = SPLIT ? NS_CHAIN_PAIRS : NS_CHAIN_SINGLE;
+  const int chains = (p.k_iters + 2 * p.chain - 1) / (2 * p.chain);
+  if (SPLIT) p.mul *= (float)(1.0 + NS_LOSS * std::max(0.0, ((p.k_real + 15) / 16 - chains) / (double)chains));
+  // a slot per accumulator, and two steps' low parts: more slots would be free no earlier
+  constexpr int SLOTS = SPLIT ? 2 : std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
+  static_assert(NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT <= NS_SMEM_LIMIT && SLOTS >= 2, "operand tiles");
+  p.slots = SLOTS;
   units = std::min<int64_t>(units, (int64_t)p.batch * p.tiles);
   cfg.gridDim = dim3(PAIR ? 2 * units : units);
-  cfg.dynamicSmemBytes = NS_SMEM_FIXED + SLOTS * SLOT;
+  cfg.dynamicSmemBytes = NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT;
   cfg.stream = ctx->stream;
   if (ctx->pdl) {
     at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
