@@ -18,7 +18,7 @@
 namespace {
 
 constexpr int NS_BATCH = 32;          // matrices of one launch
-constexpr int NS_NORM_BLOCKS = 128;   // blocks per matrix of the momentum kernel, at most
+constexpr int NS_NORM_BLOCKS = 256;   // blocks per matrix of the momentum kernel, at most
 constexpr int NS_THREADS = 256;
 constexpr int NS_PAD_M = 128, NS_PAD_N = 64;
 constexpr int NS_MAX_SHORT = 16384, NS_MAX_LONG = 1 << 20, NS_MAX_STEPS = 32;
@@ -62,72 +62,95 @@ NsPlan ns_plan(int count, int rows, int cols) {
   return s;
 }
 
-__device__ __forceinline__ float ns_load(const void* g, int bf16, int64_t i) {
-  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]) : static_cast<const float*>(g)[i];
-}
 __device__ __forceinline__ float ns_direction(float g, float m, const NsUpdate& s) {
   return s.nesterov ? fmaf(s.beta, m - g, g) : m;
 }
 
-// m <- m + (1 - beta) (g - m); the squares of the update's elements, in 64 bits, summed by every block.  VEC: four elements to a
-// thread, all addresses being aligned to that.
-template <bool VEC>
-__global__ void __launch_bounds__(NS_THREADS) ns_momentum_kernel(const NsMatrices mats, int64_t elements, int bf16, NsUpdate s,
-                                                                 double* norms) {
+// EACH consecutive elements of a gradient; EACH 1: any address
+template <typename T, int EACH>
+__device__ __forceinline__ void ns_load(const void* g, int64_t at, float (&v)[EACH]) {
+  const T* p = static_cast<const T*>(g) + at;
+  if constexpr (EACH == 1) {
+    v[0] = Pack<T>::load1(p);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+  } else {
+    Pack<float>::load(p, v);
+  }
+}
+template <int EACH>
+__device__ __forceinline__ void ns_load_f32(const float* p, float (&v)[EACH]) {
+  if constexpr (EACH == 1) v[0] = *p;
+  else Pack<float>::load(p, v);
+}
+
+// Sum of squares of numbers of any size: those whose square is well inside 32 bits are added in 32 bits, a few dozen at a time, the
+// others, and NaN, in 64 (which alone would take twice the time of reading bf16 gradients: 124 us for 55 million).
+struct NsSquares {
+  double sum = 0.0;
+  float some = 0.0f;
+  __device__ __forceinline__ void add(float u) {
+    const float t = u * u;
+    if (t > 0x1p-100f && t < 0x1p100f) some += t;
+    else if (u != 0.0f) sum = fma((double)u, (double)u, sum);
+  }
+  __device__ __forceinline__ void flush() {
+    sum += (double)some;
+    some = 0.0f;
+  }
+};
+
+// m <- m + (1 - beta) (g - m); the squares of the update's elements, summed by every block.  EACH elements to an access:
+// 4 where all addresses are aligned to that, else 1; eight accesses under way in a thread.
+template <typename T, int EACH>
+__global__ void __launch_bounds__(NS_THREADS) ns_momentum_kernel(const NsMatrices mats, int64_t elements, NsUpdate s, double* norms) {
   __shared__ double part[NS_THREADS / 32];
   ag_pdl_wait();
   ag_pdl_trigger();
   const void* g = mats.g[blockIdx.y];
   float* m = mats.m[blockIdx.y];
-  double sum = 0.0;
+  NsSquares squares;
   auto element = [&](float gi, float& mi) {
     float u = gi * s.grad_scale;
     if (m) {
       mi = fmaf(1.0f - s.beta, u - mi, mi);
       u = ns_direction(u, mi, s);
     }
-    sum = fma((double)u, (double)u, sum);
+    squares.add(u);
   };
-  constexpr int EACH = VEC ? 4 : 1, AHEAD = 4;
+  constexpr int AHEAD = EACH == 1 || sizeof(T) == 2 ? 8 : 4;
   const int64_t stride = (int64_t)gridDim.x * NS_THREADS, packets = elements / EACH;
   for (int64_t i = (int64_t)blockIdx.x * NS_THREADS + threadIdx.x; i < packets; i += stride * AHEAD) {
     float gv[AHEAD][EACH], mv[AHEAD][EACH];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int64_t at = (i + k * stride) * EACH;
       if (i + k * stride >= packets) continue;
-      if constexpr (VEC) {
-        if (bf16) {
-          const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(g) + at);
-          gv[k][0] = __uint_as_float(w.x << 16); gv[k][1] = __uint_as_float(w.x & 0xffff0000u);
-          gv[k][2] = __uint_as_float(w.y << 16); gv[k][3] = __uint_as_float(w.y & 0xffff0000u);
-        } else {
-          Pack<float>::load(static_cast<const float*>(g) + at, gv[k]);
-        }
-        if (m) Pack<float>::load(m + at, mv[k]);
-      } else {
-        gv[k][0] = ns_load(g, bf16, at);
-        if (m) mv[k][0] = m[at];
-      }
+      ns_load<T, EACH>(g, (i + k * stride) * EACH, gv[k]);
+      if (m) ns_load_f32<EACH>(m + (i + k * stride) * EACH, mv[k]);
     }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int64_t at = (i + k * stride) * EACH;
       if (i + k * stride >= packets) continue;
 #pragma unroll
       for (int e = 0; e < EACH; ++e) element(gv[k][e], mv[k][e]);
       if (m) {
-        if constexpr (VEC) Pack<float>::store(m + at, mv[k]);
-        else m[at] = mv[k][0];
+        if constexpr (EACH == 4) Pack<float>::store(m + (i + k * stride) * EACH, mv[k]);
+        else m[i + k * stride] = mv[k][0];
       }
     }
+    squares.flush();
   }
-  if (VEC && blockIdx.x == 0 && threadIdx.x < elements % EACH) {
+  if (EACH > 1 && blockIdx.x == 0 && threadIdx.x < elements % EACH) {
     const int64_t at = elements - 1 - threadIdx.x;
-    float mi = m ? m[at] : 0.0f;
-    element(ns_load(g, bf16, at), mi);
+    float gi[1], mi = m ? m[at] : 0.0f;
+    ns_load<T, 1>(g, at, gi);
+    element(gi[0], mi);
     if (m) m[at] = mi;
+    squares.flush();
   }
+  double sum = squares.sum;
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
   __syncthreads();
@@ -146,9 +169,16 @@ struct NsPlane {
   __half *hi, *lo;  // lo null: one word
 };
 
-// X = u / max(|u|, eps) in padded rows, transposed where the matrix is tall: tiles of 64 x 64
-__global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices mats, NsPlan t, int bf16, NsUpdate s, float eps,
-                                                              const double* norms, int norm_blocks, NsPlane X) {
+// What an element of the update is multiplied by: NS_SCALE over its norm, whose square is `sum`
+__device__ __forceinline__ double ns_factor(double sum, float eps) {
+  const double norm = sqrt(sum);
+  return (double)NS_SCALE / (norm > eps || norm != norm ? norm : (double)eps);
+}
+
+// X = u / max(|u|, eps) in padded rows, transposed where the matrix is tall: tiles of 64 x 64, EACH elements to an access of the matrix
+template <typename T, int EACH>
+__global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices mats, NsPlan t, NsUpdate s, float eps, const double* norms,
+                                                              int norm_blocks, NsPlane X) {
   __shared__ float tile[64][65];
   __shared__ double factor;
   ag_pdl_wait();
@@ -157,31 +187,36 @@ __global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices m
   const float* m = mats.m[blockIdx.z];
   const bool tall = t.rows > t.cols;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  float u[16], mv[16];
-  const int row = tall ? c0 + ty : r0 + ty, col = tall ? r0 + tx : c0 + tx;  // of the matrix: rows 4 apart
+  constexpr int ACROSS = 64 / EACH, DOWN = NS_THREADS / ACROSS, TIMES = 64 / DOWN;
+  const int tx = threadIdx.x % ACROSS * EACH, ty = threadIdx.x / ACROSS;
+  float u[TIMES][EACH], mv[TIMES][EACH];
+  const int row = (tall ? c0 : r0) + ty, col = (tall ? r0 : c0) + tx;  // of the matrix: rows DOWN apart
   const int64_t at = (int64_t)row * t.cols + col;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const bool in = row + 4 * k < t.rows && col < t.cols;
-    u[k] = in ? ns_load(g, bf16, at + (int64_t)(4 * k) * t.cols) : 0.0f;
-    mv[k] = in && m ? m[at + (int64_t)(4 * k) * t.cols] : 0.0f;
+  for (int k = 0; k < TIMES; ++k) {
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) u[k][e] = mv[k][e] = 0.0f;
+    if (row + DOWN * k < t.rows && col < t.cols) {
+      ns_load<T, EACH>(g, at + (int64_t)(DOWN * k) * t.cols, u[k]);
+      if (m) ns_load_f32<EACH>(m + at + (int64_t)(DOWN * k) * t.cols, mv[k]);
+    }
   }
   if (threadIdx.x < 32) {
     double sum = 0.0;
     for (int i = threadIdx.x; i < norm_blocks; i += 32) sum += norms[blockIdx.z * NS_NORM_BLOCKS + i];
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double norm = sqrt(sum);
-    if (threadIdx.x == 0) factor = (double)NS_SCALE / (norm > eps || norm != norm ? norm : (double)eps);
+    if (threadIdx.x == 0) factor = ns_factor(sum, eps);
   }
   __syncthreads();
   const double by = factor;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    float v = u[k] * s.grad_scale;
-    if (m) v = ns_direction(v, mv[k], s);
-    tile[ty + 4 * k][tx] = (float)(v * by);
-  }
+  for (int k = 0; k < TIMES; ++k)
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      float v = u[k][e] * s.grad_scale;
+      if (m) v = ns_direction(v, mv[k][e], s);
+      tile[ty + DOWN * k][tx + e] = (float)(v * by);
+    }
   __syncthreads();
   const int64_t x = (int64_t)blockIdx.z * t.mp * t.np;
 #pragma unroll
@@ -434,29 +469,29 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
           const uint32_t idesc = IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u);
           const uint32_t l_step = l_mn ? dmn.step : dk.step, r_step = r_mn ? dmn.step : dk.step;
           const uint32_t l_const = l_mn ? dmn.lo_const : dk.lo_const, r_const = (A_BYTES >> 4) + (r_mn ? dmn.lo_const : dk.lo_const);
+          // the accumulator last: it is what is late
+          if (!tc_wait(&full[slot], phase, abort_flag) || (SPLIT && !tc_wait(&low_full[low], low_phase, abort_flag)) ||
+              (left == 0 && !tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag))) {
+            expired = true;
+            break;
+          }
+          tc_fence_after();
           if (left == 0) {
-            if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
-              expired = true;
-              break;
-            }
             acc_par ^= 1u << buf;
             tacc = tmem_base + (uint32_t)buf * BN;
             left = p.chain;
             more = 0u;
           }
-          if (!tc_wait(&full[slot], phase, abort_flag)) {
-            expired = true;
-            break;
-          }
-          tc_fence_after();
           const uint32_t hs = tiles_u + slot * (SLOT >> 4);
           if (SPLIT) {
             for (int j = 0; j < n; ++j) {
-              if (!tc_wait(&low_full[low], low_phase, abort_flag)) {
-                expired = true;
-                break;
+              if (j > 0) {
+                if (!tc_wait(&low_full[low], low_phase, abort_flag)) {
+                  expired = true;
+                  break;
+                }
+                tc_fence_after();
               }
-              tc_fence_after();
               const uint32_t h = hs + j * (STEP >> 4), l = lows_u + low * (STEP >> 4);
               ns_step_mmas<true, PAIR>(tacc, h + l_const, l + l_const, l_step, h + r_const, l + r_const, r_step, idesc, more);
               more = 1u;
@@ -490,7 +525,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     int buf = 0, half = 0;
     NsTile t;
     for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
-      const int row0 = t.tm * BM + row_off + quarter * 32, row = row0 + lane, col0 = t.tn * BN + slice * (BN / 2);
+      const int row0 = t.tm * BM + row_off + quarter * 32, col0 = t.tn * BN + slice * (BN / 2);
       const uint32_t toff = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slice * (BN / 2));
       const bool rows_in = row0 < p.M;  // padded sizes are multiples of 32
       // one word of each of the lane's 32 columns: through the half of the buffer that was stored from before the last
@@ -511,11 +546,10 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         if (!rows_in || col >= p.N) return;
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= p.mul;
-        if (ns_symmetric(KIND)) {
-          const int hit = row - col;
+        if (ns_symmetric(KIND) && row0 == col) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (j == hit) v[j] += p.diag;
+            if (j == lane) v[j] += p.diag;
         }
         uint32_t hi[16], lo[16];
 #pragma unroll
@@ -597,21 +631,46 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   }
 }
 
-// p <- keep p - by X (kind 0), or X in fp32 (1) or bf16 (2): tiles of 64 x 64 of X, as in ns_start_kernel
-__global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices mats, NsPlan t, NsPlane X, float keep, float by,
-                                                               int out_kind) {
+// p <- keep p - by X (NS_STEP), or X in fp32 (NS_F32) or bf16 (NS_BF16)
+enum { NS_STEP, NS_F32, NS_BF16 };
+template <int EACH>
+__device__ __forceinline__ void ns_put(float* p, int64_t at, float (&v)[EACH], const float (&old)[EACH], float keep, float by, int kind) {
+  if (kind == NS_BF16) {
+    __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(p) + at;
+    if constexpr (EACH == 4) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(q) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      *q = __float2bfloat16_rn(v[0]);
+    }
+    return;
+  }
+  if (kind == NS_STEP) {
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) v[e] = fmaf(-by, v[e], keep * old[e]);
+  }
+  if constexpr (EACH == 4) Pack<float>::store(p + at, v);
+  else p[at] = v[0];
+}
+
+// The factor goes where it belongs: tiles of 64 x 64 of X, as in ns_start_kernel
+template <int EACH>
+__global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices mats, NsPlan t, NsPlane X, float keep, float by, int kind) {
   __shared__ float tile[64][65];
   ag_pdl_wait();
   ag_pdl_trigger();
   const bool tall = t.rows > t.cols;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int row = tall ? c0 + ty : r0 + ty, col = tall ? r0 + tx : c0 + tx;  // of the matrix: rows 4 apart
+  constexpr int ACROSS = 64 / EACH, DOWN = NS_THREADS / ACROSS, TIMES = 64 / DOWN;
+  const int tx = threadIdx.x % ACROSS * EACH, ty = threadIdx.x / ACROSS;
+  const int row = (tall ? c0 : r0) + ty, col = (tall ? r0 : c0) + tx;  // of the matrix: rows DOWN apart
   const int64_t at = (int64_t)row * t.cols + col, x = (int64_t)blockIdx.z * t.mp * t.np;
   float* p = mats.p[blockIdx.z];
-  float old[16];
+  float old[TIMES][EACH];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) old[k] = out_kind == 0 && row + 4 * k < t.rows && col < t.cols ? p[at + (int64_t)(4 * k) * t.cols] : 0.0f;
+  for (int k = 0; k < TIMES; ++k) {
+    if (kind == NS_STEP && row + DOWN * k < t.rows && col < t.cols) ns_load_f32<EACH>(p + at + (int64_t)(DOWN * k) * t.cols, old[k]);
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = threadIdx.x + h * NS_THREADS, r = i >> 3, c = (i & 7) * 8;
@@ -630,12 +689,12 @@ __global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices 
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    if (row + 4 * k >= t.rows || col >= t.cols) continue;
-    const float v = tile[ty + 4 * k][tx];
-    const int64_t i = at + (int64_t)(4 * k) * t.cols;
-    if (out_kind == 2) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else p[i] = out_kind == 0 ? fmaf(-by, v, keep * old[k]) : v;
+  for (int k = 0; k < TIMES; ++k) {
+    if (row + DOWN * k >= t.rows || col >= t.cols) continue;
+    float v[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) v[e] = tile[ty + DOWN * k][tx + e];
+    ns_put<EACH>(p, at + (int64_t)(DOWN * k) * t.cols, v, old[k], keep, by, kind);
   }
 }
 
@@ -778,18 +837,33 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
   Q.plane = plane(2 * t.x_bytes + t.a_bytes, t.a_bytes, split);
   double* norms = reinterpret_cast<double*>(scratch + 2 * t.x_bytes + 2 * t.a_bytes);
   const int64_t elements = (int64_t)t.rows * t.cols;
-  bool vec = true;
-  for (int i = 0; i < count; ++i)
+  // accesses of four elements where all addresses are multiples of their size, in every row for the tiles
+  bool vec = true, vec_out = true;
+  for (int i = 0; i < count; ++i) {
     vec = vec && ag_aligned16(mats.m[i]) && ((uintptr_t)mats.g[i] & (bf16 ? 7 : 15)) == 0;
-  const int each = vec ? 4 : 1;
-  int blocks = ag_ceil_div(elements, (int64_t)NS_THREADS * 4 * each);
+    vec_out = vec_out && ((uintptr_t)mats.p[i] & (out_kind == NS_BF16 ? 7 : 15)) == 0;
+  }
+  const bool vec_rows = vec && (t.cols & 3) == 0;
+  vec_out = vec_out && (t.cols & 3) == 0;
+  int blocks = ag_ceil_div(elements, (int64_t)NS_THREADS * 4 * (vec ? 4 : 1));
   if (blocks > NS_NORM_BLOCKS) blocks = NS_NORM_BLOCKS;
-  if (vec)
-    AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", ns_momentum_kernel<true>, dim3(blocks, count), NS_THREADS, 0, mats, elements, bf16, s, norms);
-  else
-    AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", ns_momentum_kernel<false>, dim3(blocks, count), NS_THREADS, 0, mats, elements, bf16, s, norms);
-  AG_LAUNCH_PDL(ctx, "ns_start_kernel", ns_start_kernel, dim3(t.np / 64, t.mp / 64, count), NS_THREADS, 0, mats, t, bf16, s, eps,
-                (const double*)norms, blocks, X[0].plane);
+  const dim3 tiles(t.np / 64, t.mp / 64, count);
+#define NS_FORMS(T, EACH_M, EACH_S)                                                                                              \
+  do {                                                                                                                           \
+    AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", (ns_momentum_kernel<T, EACH_M>), dim3(blocks, count), NS_THREADS, 0, mats, elements, s, norms); \
+    AG_LAUNCH_PDL(ctx, "ns_start_kernel", (ns_start_kernel<T, EACH_S>), tiles, NS_THREADS, 0, mats, t, s, eps, (const double*)norms, blocks, \
+                  X[0].plane);                                                                                                    \
+  } while (0)
+  if (bf16) {
+    if (vec_rows) NS_FORMS(__nv_bfloat16, 4, 4);
+    else if (vec) NS_FORMS(__nv_bfloat16, 4, 1);
+    else NS_FORMS(__nv_bfloat16, 1, 1);
+  } else {
+    if (vec_rows) NS_FORMS(float, 4, 4);
+    else if (vec) NS_FORMS(float, 4, 1);
+    else NS_FORMS(float, 1, 1);
+  }
+#undef NS_FORMS
   if (steps > 0) {
     const int64_t rows = (int64_t)count * t.mp;
     int rc;
@@ -803,8 +877,10 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
     if ((rc = split ? ns_iterate<true>(ctx, t, p, X, A, Q, coefficients, steps) : ns_iterate<false>(ctx, t, p, X, A, Q, coefficients, steps)))
       return rc;
   }
-  AG_LAUNCH_PDL(ctx, "ns_finish_kernel", ns_finish_kernel, dim3(t.np / 64, t.mp / 64, count), NS_THREADS, 0, mats, t, X[steps & 1].plane,
-                keep, by, out_kind);
+  if (vec_out)
+    AG_LAUNCH_PDL(ctx, "ns_finish_kernel", ns_finish_kernel<4>, tiles, NS_THREADS, 0, mats, t, X[steps & 1].plane, keep, by, out_kind);
+  else
+    AG_LAUNCH_PDL(ctx, "ns_finish_kernel", ns_finish_kernel<1>, tiles, NS_THREADS, 0, mats, t, X[steps & 1].plane, keep, by, out_kind);
   return AG_OK;
 }
 
@@ -905,7 +981,7 @@ extern "C" int ag_orthogonalise(ag_ctx* ctx, const void* const* g, void* const* 
       mats.g[i] = g[first + i];
       mats.p[i] = static_cast<float*>(out[first + i]);
     }
-    if (int rc = ns_run(ctx, t, mats, here, dtype == AG_BF16, s, eps, coefficients, steps, 0.0f, 0.0f, out_dtype == AG_F32 ? 1 : 2,
+    if (int rc = ns_run(ctx, t, mats, here, dtype == AG_BF16, s, eps, coefficients, steps, 0.0f, 0.0f, out_dtype == AG_F32 ? NS_F32 : NS_BF16,
                         static_cast<char*>(scratch), precision == AG_CE_3XTF32))
       return rc;
   }
@@ -942,7 +1018,7 @@ extern "C" int ag_muon_step(ag_ctx* ctx, float* const* p, const void* const* g, 
       mats.m[i] = m[first + i];
     }
     if (int rc = ns_run(ctx, t, mats, here, grad_dtype == AG_BF16, s, eps, coefficients, steps, (float)(1.0 - lr * weight_decay),
-                        (float)(lr * scale), 0, static_cast<char*>(scratch), precision == AG_CE_3XTF32))
+                        (float)(lr * scale), NS_STEP, static_cast<char*>(scratch), precision == AG_CE_3XTF32))
       return rc;
   }
   return AG_OK;
