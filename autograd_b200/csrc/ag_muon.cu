@@ -103,45 +103,49 @@ struct NsSquares {
 };
 
 // m <- m + (1 - beta) (g - m); the squares of the update's elements, summed by every block.  EACH elements to an access:
-// 4 where all addresses are aligned to that, else 1; eight accesses under way in a thread.
-template <typename T, int EACH>
-__global__ void __launch_bounds__(NS_THREADS) ns_momentum_kernel(const NsMatrices mats, int64_t elements, NsUpdate s, double* norms) {
+// 4 where all addresses are aligned to that, else 1; four or eight accesses of each array under way in a thread.
+// HAS: there is a momentum.
+template <typename T, int EACH, bool HAS>
+__global__ void __launch_bounds__(NS_THREADS, 4) ns_momentum_kernel(const NsMatrices mats, int64_t elements, NsUpdate s, double* norms) {
   __shared__ double part[NS_THREADS / 32];
   ag_pdl_wait();
   ag_pdl_trigger();
   const void* g = mats.g[blockIdx.y];
-  float* m = mats.m[blockIdx.y];
+  float* m = HAS ? mats.m[blockIdx.y] : nullptr;
   NsSquares squares;
   auto element = [&](float gi, float& mi) {
     float u = gi * s.grad_scale;
-    if (m) {
+    if (HAS) {
       mi = fmaf(1.0f - s.beta, u - mi, mi);
       u = ns_direction(u, mi, s);
     }
     squares.add(u);
   };
-  constexpr int AHEAD = EACH == 1 || sizeof(T) == 2 ? 8 : 4;
+  constexpr int AHEAD = EACH == 1 || !HAS ? 8 : 4;
   const int64_t stride = (int64_t)gridDim.x * NS_THREADS, packets = elements / EACH;
-  for (int64_t i = (int64_t)blockIdx.x * NS_THREADS + threadIdx.x; i < packets; i += stride * AHEAD) {
-    float gv[AHEAD][EACH], mv[AHEAD][EACH];
+  int64_t i = (int64_t)blockIdx.x * NS_THREADS + threadIdx.x;
+  auto run = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+    float gv[N][EACH], mv[N][EACH];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (i + k * stride >= packets) continue;
-      ns_load<T, EACH>(g, (i + k * stride) * EACH, gv[k]);
-      if (m) ns_load_f32<EACH>(m + (i + k * stride) * EACH, mv[k]);
+    for (int k = 0; k < N; ++k) ns_load<T, EACH>(g, (i + k * stride) * EACH, gv[k]);
+    if (HAS) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) ns_load_f32<EACH>(m + (i + k * stride) * EACH, mv[k]);
     }
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (i + k * stride >= packets) continue;
+    for (int k = 0; k < N; ++k) {
 #pragma unroll
       for (int e = 0; e < EACH; ++e) element(gv[k][e], mv[k][e]);
-      if (m) {
+      if (HAS) {
         if constexpr (EACH == 4) Pack<float>::store(m + (i + k * stride) * EACH, mv[k]);
         else m[i + k * stride] = mv[k][0];
       }
     }
     squares.flush();
-  }
+  };
+  for (; i + (AHEAD - 1) * stride < packets; i += AHEAD * stride) run(std::integral_constant<int, AHEAD>());
+  for (; i < packets; i += stride) run(std::integral_constant<int, 1>());
   if (EACH > 1 && blockIdx.x == 0 && threadIdx.x < elements % EACH) {
     const int64_t at = elements - 1 - threadIdx.x;
     float gi[1], mi = m ? m[at] : 0.0f;
@@ -850,7 +854,10 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
   const dim3 tiles(t.np / 64, t.mp / 64, count);
 #define NS_FORMS(T, EACH_M, EACH_S)                                                                                              \
   do {                                                                                                                           \
-    AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", (ns_momentum_kernel<T, EACH_M>), dim3(blocks, count), NS_THREADS, 0, mats, elements, s, norms); \
+    if (mats.m[0])                                                                                                                \
+      AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", (ns_momentum_kernel<T, EACH_M, true>), dim3(blocks, count), NS_THREADS, 0, mats, elements, s, norms); \
+    else                                                                                                                         \
+      AG_LAUNCH_PDL(ctx, "ns_momentum_kernel", (ns_momentum_kernel<T, EACH_M, false>), dim3(blocks, count), NS_THREADS, 0, mats, elements, s, norms); \
     AG_LAUNCH_PDL(ctx, "ns_start_kernel", (ns_start_kernel<T, EACH_S>), tiles, NS_THREADS, 0, mats, t, s, eps, (const double*)norms, blocks, \
                   X[0].plane);                                                                                                    \
   } while (0)
