@@ -702,6 +702,395 @@ __global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices 
   }
 }
 
+// ---------------------------------------------------------------------------- small matrices
+// Matrices of up to 128 rows (their shorter side) in one launch, from gradient to parameter: a cluster of CTAs per matrix, each with a
+// slice of 64 to 320 columns of X in shared memory, as pairs in the layout that serves as a K-major operand (X X^T) and as an MN-major
+// one (Q X) alike.  A step is three products of 128 rows:
+//   G = X X^T of the slice into tensor memory; each CTA of the cluster owns 128 / S rows of the sum: it gets the others' parts of them
+//   through distributed shared memory, adds them in the order of the ranks, and sends A = G + h I to all;
+//   Q = (a - h h c) I + c A A and X <- Q X by every CTA for itself.
+// What bounds it is latency: 15 dependent products of a few thousand cycles, where the launches of the general path cost 7 us each.
+constexpr int NS_SMALL_THREADS = 256, NS_SMALL_M = 128, NS_SMALL_GROUPS = 5, NS_SMALL_CLUSTER = 16;
+constexpr uint32_t NS_GROUP_BYTES = NS_SMALL_M * 128;       // 64 columns of one plane
+constexpr uint32_t NS_SQUARE_BYTES = 4 * NS_GROUP_BYTES;    // 128 x 128: two planes, or 32-bit sums
+
+struct NsSmall {
+  NsMatrices mats;
+  NsUpdate s;
+  int rows, cols, m, n, groups, cluster, steps, out_kind;
+  float eps, keep, by, loss_gram, loss_square;
+  float co[3 * NS_MAX_STEPS];
+  int* status;
+};
+
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+// generic writes before it, of this CTA's memory or another's, and products after it
+__device__ __forceinline__ void ns_fence_proxy() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+// Byte of (row, byte of the row) in a group of rows of 128 bytes, swizzled as the products read it
+__device__ __forceinline__ uint32_t ns_swizzled(int row, uint32_t byte) { return (uint32_t)row * 128u + (byte ^ (((uint32_t)row & 7u) << 4)); }
+
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __grid_constant__ NsSmall p) {
+  extern __shared__ unsigned char ns_smem_raw[];
+  unsigned char* X = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ns_smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int G = p.groups, S = p.cluster, W = G * 64;
+  const uint32_t plane = (uint32_t)G * NS_GROUP_BYTES;                 // X: high words, low words; at the end its 32-bit values
+  unsigned char* AQ = X + 2 * plane;                                   // A or Q: high words, low words; partial sums in between
+  double* norms = reinterpret_cast<double*>(AQ + NS_SQUARE_BYTES);     // of every rank
+  uint64_t* bar = reinterpret_cast<uint64_t*>(norms + NS_SMALL_CLUSTER);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  double* part = reinterpret_cast<double*>(tmem_slot + 2);             // of every warp
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int mat = blockIdx.x / S, rank = blockIdx.x - mat * S;
+  auto cluster_sync = [&]() {
+    if (S > 1) tc_cluster_sync(); else __syncthreads();
+  };
+  if (tid == 0) {
+    ag_mbar_init(bar, 1);
+    *abort_flag = 0;
+    ag_fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync();  // all CTAs are there, too, before anything goes to their memory
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ag_pdl_wait();
+  ag_pdl_trigger();
+
+  // ---- the momentum and the norm; then X.  Elements in the order of memory: a slice is whole rows of a tall matrix, pieces of the
+  // rows of another
+  const bool tall = p.rows > p.cols;
+  const int first = rank * W, width = max(0, min(W, p.n - first)), inner = tall ? p.m : width, count = p.m * width;
+  auto place = [&](int i, int& r, int& c) {  // row and column of the slice of X
+    const int q = i / inner, k = i - q * inner;
+    r = tall ? k : q;
+    c = tall ? q : k;
+    return tall ? (int64_t)(first + q) * p.cols + k : (int64_t)q * p.cols + first + k;
+  };
+  const void* g = p.mats.g[mat];
+  float* mom = p.mats.m[mat];
+  constexpr int AHEAD = 8;
+  NsSquares squares;
+  for (int i = tid; i < count; i += NS_SMALL_THREADS * AHEAD) {
+    float gv[AHEAD][1], mv[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      gv[k][0] = mv[k] = 0.0f;
+      if (j < count) {
+        int r, c;
+        const int64_t at = place(j, r, c);
+        ns_load<T, 1>(g, at, gv[k]);
+        if (mom) mv[k] = mom[at];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      if (j >= count) continue;
+      float u = gv[k][0] * p.s.grad_scale;
+      if (mom) {
+        int r, c;
+        const float v = fmaf(1.0f - p.s.beta, u - mv[k], mv[k]);
+        mom[place(j, r, c)] = v;
+        u = ns_direction(u, v, p.s);
+      }
+      squares.add(u);
+    }
+    squares.flush();
+  }
+  double sum = squares.sum;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) part[warp] = sum;
+  // padding of X is zero
+  for (uint32_t i = tid; i < 2 * plane / 16; i += NS_SMALL_THREADS) reinterpret_cast<uint4*>(X)[i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  if (tid < S) {
+    sum = 0.0;
+    for (int w = 0; w < NS_SMALL_THREADS / 32; ++w) sum += part[w];
+    if (S > 1) ns_st_cluster(tc_map_to_cta(ag_smem_u32(norms + rank), tid), sum);
+    else norms[0] = sum;
+  }
+  cluster_sync();
+  sum = 0.0;
+  for (int r = 0; r < S; ++r) sum += norms[r];
+  const double by = ns_factor(sum, p.eps);
+  for (int i = tid; i < count; i += NS_SMALL_THREADS * AHEAD) {
+    float gv[AHEAD][1], mv[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      gv[k][0] = mv[k] = 0.0f;
+      if (j < count) {
+        int r, c;
+        const int64_t at = place(j, r, c);
+        ns_load<T, 1>(g, at, gv[k]);
+        if (mom) mv[k] = mom[at];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      if (j >= count) continue;
+      int r, c;
+      place(j, r, c);
+      float u = gv[k][0] * p.s.grad_scale;
+      if (mom) u = ns_direction(u, mv[k], p.s);
+      u = (float)(u * by);
+      const __half h = __float2half_rn(u);
+      const uint32_t at = (uint32_t)(c >> 6) * NS_GROUP_BYTES + ns_swizzled(r, (uint32_t)(c & 63) * 2u);
+      *reinterpret_cast<__half*>(X + at) = h;
+      if (SPLIT || p.steps == 0) *reinterpret_cast<__half*>(X + plane + at) = __float2half_rn(u - __half2float(h));
+    }
+  }
+  ns_fence_proxy();
+  __syncthreads();
+
+  // ---- the steps
+  uint32_t phase = 0;
+  bool expired = false;
+  auto products_done = [&]() {
+    if (!tc_wait(bar, phase, abort_flag)) expired = true;  // the steps go on, all CTAs meet at the same barriers
+    phase ^= 1u;
+    tc_fence_after();
+  };
+  constexpr uint32_t HI = TcDesc::hi, K_CONST = 1u << 16, MN_CONST = (NS_GROUP_BYTES >> 4) << 16;
+  auto idesc = [](uint32_t n, bool mn) { return (1u << 4) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((NS_SMALL_M >> 4) << 24); };
+  // D (128 x 128 at column `d`) = B B^T over `groups` groups of a K-major buffer: the products with a low part first
+  auto gram = [&](uint32_t d, uint32_t hi, uint32_t lo, int groups) {
+    uint32_t more = 0;
+    if (SPLIT)
+      for (int k = 0; k < groups * 4; ++k) {
+        const uint32_t at = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST;
+        tc_mma<2, false>(d, hi + at, HI, lo + at, HI, idesc(128, false), more);
+        tc_mma<1, false>(d, lo + at, HI, hi + at, HI, idesc(128, false), 1u);
+        more = 1u;
+      }
+    for (int k = 0; k < groups * 4; ++k) {
+      const uint32_t at = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST;
+      tc_mma<2, false>(d, hi + at, HI, hi + at, HI, idesc(128, false), more);
+      more = 1u;
+    }
+  };
+  const uint32_t xu = ag_smem_u32(X) >> 4, xl = xu + (plane >> 4), au = ag_smem_u32(AQ) >> 4, al = au + ((2 * NS_GROUP_BYTES) >> 4);
+  const int quarter = warp & 3, slice = warp >> 2, row = quarter * 32 + lane;
+  const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+  const int chains = SPLIT ? (G + 1) / 2 : 1, chain_groups = SPLIT ? 2 : G;
+  // 32 columns of the lane's row into the words of a buffer
+  auto put = [&](unsigned char* dst, uint32_t low, int col, const float (&v)[32]) {
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) split_f16x2(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+    unsigned char* d = dst + (uint32_t)(col >> 6) * NS_GROUP_BYTES;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = ns_swizzled(row, (uint32_t)(col & 63) * 2u + 16u * j);
+      *reinterpret_cast<uint4*>(d + at) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+      if (SPLIT) *reinterpret_cast<uint4*>(d + low + at) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+    }
+  };
+  auto finish_value = [&](int col, const float (&v)[32]) {  // 32-bit values in X's place, in the order in which they leave
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (tall) {
+        reinterpret_cast<float*>(X)[(col + j) * NS_SMALL_M + row] = v[j];
+      } else if ((j & 3) == 0) {
+        *reinterpret_cast<float4*>(X + (uint32_t)row * W * 4u + ((((uint32_t)(col + j) >> 2) ^ ((uint32_t)row & 7u)) << 4)) =
+            make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    }
+  };
+  const float unit = 1.0f / NS_SCALE;
+  for (int step = 0; step < p.steps; ++step) {
+    const float a = p.co[3 * step], b = p.co[3 * step + 1], c = p.co[3 * step + 2];
+    const bool square = c != 0.0f;
+    const float h = square ? b / (2.0f * c) : 0.0f;
+    const float gram_mul = (square ? 1.0f : b) * unit * p.loss_gram, gram_diag = (square ? h : a) * NS_SCALE;
+    if (tid == 0) {
+      for (int i = 0; i < chains; ++i)
+        gram(tmem + i * 128, xu + i * chain_groups * (NS_GROUP_BYTES >> 4), xl + i * chain_groups * (NS_GROUP_BYTES >> 4),
+             min(chain_groups, G - i * chain_groups));
+      tc_commit(bar);
+    }
+    products_done();
+    const int own = NS_SMALL_M / S;  // rows of the sum that a CTA owns
+    if (S > 1) tc_cluster_sync();    // nobody multiplies with its Q any more
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+      const int col = slice * 64 + ch * 32;
+      float v[32];
+      tc_tmem_ld32(trow + col, reinterpret_cast<uint32_t(&)[32]>(v));
+      tc_tmem_ld_wait();
+      for (int i = 1; i < chains; ++i) {
+        uint32_t r[32];
+        tc_tmem_ld32(trow + i * 128 + col, r);
+        tc_tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+      }
+      if (S == 1) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j] * gram_mul + (row == col + j ? gram_diag : 0.0f);
+        put(AQ, 2 * NS_GROUP_BYTES, col, v);
+      } else {
+        const uint32_t to = tc_map_to_cta(ag_smem_u32(AQ), row / own) + (uint32_t)(rank * own + row % own) * 512u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          ns_st_cluster(to + ((((uint32_t)col >> 2) + j ^ ((uint32_t)row & 7u)) << 4), make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+      }
+    }
+    if (S > 1) {
+      tc_cluster_sync();
+      // own rows: four columns to a thread and turn, 32 x own of them
+      float4 sums[8];
+      const int turns = own / 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= turns) continue;
+        const int i = tid + k * NS_SMALL_THREADS, r = i >> 5, q = i & 31, global = rank * own + r;
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < S; ++s) {
+          const float4 x = *reinterpret_cast<const float4*>(AQ + (uint32_t)(s * own + r) * 512u + ((uint32_t)(q ^ (global & 7)) << 4));
+          t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+        }
+        const int d = global - q * 4;  // the diagonal's place among the four
+        t.x = t.x * gram_mul + (d == 0 ? gram_diag : 0.f);
+        t.y = t.y * gram_mul + (d == 1 ? gram_diag : 0.f);
+        t.z = t.z * gram_mul + (d == 2 ? gram_diag : 0.f);
+        t.w = t.w * gram_mul + (d == 3 ? gram_diag : 0.f);
+        sums[k] = t;
+      }
+      tc_cluster_sync();  // all have read the parts: A takes their place
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= turns) continue;
+        const int i = tid + k * NS_SMALL_THREADS, r = i >> 5, q = i & 31, global = rank * own + r;
+        uint32_t hi[2], lo[2];
+        split_f16x2(sums[k].x, sums[k].y, hi[0], lo[0]);
+        split_f16x2(sums[k].z, sums[k].w, hi[1], lo[1]);
+        const uint32_t at = ag_smem_u32(AQ) + (uint32_t)(q >> 4) * NS_GROUP_BYTES + ns_swizzled(global, (uint32_t)(q & 15) * 8u);
+        for (int s = 0; s < S; ++s) {
+          const uint32_t to = tc_map_to_cta(at, s);
+          ns_st_cluster(to, hi[0], hi[1]);
+          if (SPLIT) ns_st_cluster(to + 2 * NS_GROUP_BYTES, lo[0], lo[1]);
+        }
+      }
+    }
+    ns_fence_proxy();
+    tc_fence_before();
+    cluster_sync();
+    if (square) {
+      if (tid == 0) {
+        tc_fence_after();
+        ns_fence_proxy();
+        gram(tmem, au, al, 2);
+        tc_commit(bar);
+      }
+      products_done();
+      const float mul = c * unit * p.loss_square, diag = (a - h * h * c) * NS_SCALE;
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch) {
+        const int col = slice * 64 + ch * 32;
+        float v[32];
+        tc_tmem_ld32(trow + col, reinterpret_cast<uint32_t(&)[32]>(v));
+        tc_tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j] * mul + (row == col + j ? diag : 0.0f);
+        put(AQ, 2 * NS_GROUP_BYTES, col, v);
+      }
+      ns_fence_proxy();
+      tc_fence_before();
+      __syncthreads();
+    }
+    if (tid == 0) {
+      tc_fence_after();
+      ns_fence_proxy();
+      for (int c0 = 0; c0 < G; c0 += 4) {  // up to 256 columns at a time
+        const uint32_t n = (uint32_t)min(4, G - c0) * 64u, d = tmem + c0 * 64, x0 = c0 * (NS_GROUP_BYTES >> 4) + MN_CONST;
+        uint32_t more = 0;
+        if (SPLIT)
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t l = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST, r = x0 + k * 128;
+            tc_mma<2, false>(d, au + l, HI, xl + r, HI, idesc(n, true), more);
+            tc_mma<1, false>(d, al + l, HI, xu + r, HI, idesc(n, true), 1u);
+            more = 1u;
+          }
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t l = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST, r = x0 + k * 128;
+          tc_mma<2, false>(d, au + l, HI, xu + r, HI, idesc(n, true), more);
+          more = 1u;
+        }
+      }
+      tc_commit(bar);
+    }
+    products_done();
+    const bool last = step + 1 == p.steps;
+    const float mul = (last ? unit * unit : unit) * p.loss_square;
+    for (int ch = slice; ch < 2 * G; ch += 2) {
+      float v[32];
+      tc_tmem_ld32(trow + ch * 32, reinterpret_cast<uint32_t(&)[32]>(v));
+      tc_tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= mul;
+      if (last) finish_value(ch * 32, v);
+      else put(X, plane, ch * 32, v);
+    }
+    ns_fence_proxy();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  // ---- out
+  float* out = p.mats.p[mat];
+  for (int i = tid; i < count; i += NS_SMALL_THREADS * AHEAD) {
+    float old[AHEAD][1];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      int r, c;
+      if (j < count && p.out_kind == NS_STEP) old[k][0] = out[place(j, r, c)];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * NS_SMALL_THREADS;
+      if (j >= count) continue;
+      int r, c;
+      const int64_t at = place(j, r, c);
+      float v[1];
+      if (p.steps == 0) {
+        const uint32_t x = (uint32_t)(c >> 6) * NS_GROUP_BYTES + ns_swizzled(r, (uint32_t)(c & 63) * 2u);
+        v[0] = (__half2float(*reinterpret_cast<const __half*>(X + x)) + __half2float(*reinterpret_cast<const __half*>(X + plane + x))) * unit;
+      } else if (tall) {
+        v[0] = reinterpret_cast<const float*>(X)[c * NS_SMALL_M + r];
+      } else {
+        v[0] = *reinterpret_cast<const float*>(X + (uint32_t)r * W * 4u + ((((uint32_t)c >> 2) ^ ((uint32_t)r & 7u)) << 4) + ((uint32_t)c & 3u) * 4u);
+      }
+      ns_put<1>(out, at, v, old[k], p.keep, p.by, p.out_kind);
+    }
+  }
+  if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // ---------------------------------------------------------------------------- host side
 // Tensor maps of a plane of `rows` rows (of all matrices) of `cols` columns.  NS_K: tiles of TC_BK columns and `box` rows; NS_MN: seen
 // as {64, rows, cols / 64}, boxes of TC_BK rows and `box` columns; NS_OUT: 32 x 32.
@@ -829,8 +1218,64 @@ int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsBuffer* X, NsBuffer& A
   return AG_OK;
 }
 
+// Columns of X in groups of 64 over the CTAs of a cluster: as many CTAs as there are SMs for all matrices, as a CTA's time is that of its
+// slice; false where a slice would not fit, or another path serves the matrices better.
+bool ns_small_shape(const ag_ctx* ctx, const NsPlan& t, int count, int* cluster, int* groups) {
+  if (t.m > NS_SMALL_M) return false;
+  const int all = (t.n + 63) / 64;
+  int s = NS_SMALL_CLUSTER;
+  while (s > 1 && (s / 2 >= all || (int64_t)count * s > ctx->sm_count)) s /= 2;
+  while (s < NS_SMALL_CLUSTER && (all + s - 1) / s > NS_SMALL_GROUPS) s *= 2;
+  *cluster = s;
+  *groups = (all + s - 1) / s;
+  return *groups <= NS_SMALL_GROUPS;
+}
+
+template <typename T, bool SPLIT>
+int ns_small_launch(ag_ctx* ctx, NsSmall& p, int count) {
+  static std::atomic<bool> attr_done[AG_MAX_DEVICES];
+  auto kern = ns_small_kernel<T, SPLIT>;
+  if (!attr_done[ag_dev_slot(ctx)].load(std::memory_order_relaxed)) {
+    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM_LIMIT));
+    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    attr_done[ag_dev_slot(ctx)].store(true, std::memory_order_relaxed);
+  }
+  static_assert(1024 + 2 * NS_SMALL_GROUPS * NS_GROUP_BYTES + NS_SQUARE_BYTES + 512 <= NS_SMEM_LIMIT, "slice and square");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3(count * p.cluster);
+  cfg.blockDim = dim3(NS_SMALL_THREADS);
+  cfg.dynamicSmemBytes = NS_SMEM_LIMIT;  // whatever the slice needs: a CTA has its SM, and all of tensor memory, for itself
+  cfg.stream = ctx->stream;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = ctx->pdl ? 2 : 1;
+  AG_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, p));
+  ctx->launches++;
+  ag_enqueued(ctx);
+  return AG_OK;
+}
+
 int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int bf16, const NsUpdate& s, float eps,
            const float* coefficients, int steps, float keep, float by, int out_kind, char* scratch, bool split) {
+  int cluster, groups;
+  if (ns_small_shape(ctx, t, count, &cluster, &groups)) {
+    NsSmall p = {};
+    p.mats = mats; p.s = s;
+    p.rows = t.rows; p.cols = t.cols; p.m = t.m; p.n = t.n; p.groups = groups; p.cluster = cluster; p.steps = steps; p.out_kind = out_kind;
+    p.eps = eps; p.keep = keep; p.by = by; p.status = ctx->d_status;
+    const double chains = cluster * ((groups + 1) / 2);
+    p.loss_gram = split ? (float)(1.0 + NS_LOSS * std::max(0.0, ((t.n + 15) / 16 - chains) / chains)) : 1.0f;
+    p.loss_square = split ? (float)(1.0 + NS_LOSS * ((t.m + 15) / 16 - 1)) : 1.0f;
+    for (int i = 0; i < 3 * steps; ++i) p.co[i] = coefficients[i];
+    if (bf16) return split ? ns_small_launch<__nv_bfloat16, true>(ctx, p, count) : ns_small_launch<__nv_bfloat16, false>(ctx, p, count);
+    return split ? ns_small_launch<float, true>(ctx, p, count) : ns_small_launch<float, false>(ctx, p, count);
+  }
   // 16-bit operands have one word, but for the last result, which nothing multiplies
   auto plane = [&](size_t at, size_t bytes, bool two) {
     return NsPlane{reinterpret_cast<__half*>(scratch + at), two ? reinterpret_cast<__half*>(scratch + at + bytes / 2) : nullptr};
