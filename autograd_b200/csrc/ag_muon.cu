@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int NS_BATCH = 32;          // matrices of one launch
+constexpr int NS_BATCH = 96;          // matrices of one launch
 constexpr int NS_NORM_BLOCKS = 256;   // blocks per matrix of the momentum kernel, at most
 constexpr int NS_THREADS = 256;
 constexpr int NS_PAD_M = 128, NS_PAD_N = 64;
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(NS_THREADS) ns_finish_kernel(const NsMatrices 
 //   through distributed shared memory, adds them in the order of the ranks, and sends A = G + h I to all;
 //   Q = (a - h h c) I + c A A and X <- Q X by every CTA for itself.
 // What bounds it is latency: 15 dependent products of a few thousand cycles, where the launches of the general path cost 7 us each.
-constexpr int NS_SMALL_THREADS = 256, NS_SMALL_M = 128, NS_SMALL_GROUPS = 5, NS_SMALL_CLUSTER = 16;
+constexpr int NS_SMALL_THREADS = 512, NS_SMALL_M = 128, NS_SMALL_GROUPS = 5, NS_SMALL_APART = 3, NS_SMALL_CLUSTER = 16;
 constexpr uint32_t NS_GROUP_BYTES = NS_SMALL_M * 128;       // 64 columns of one plane
 constexpr uint32_t NS_SQUARE_BYTES = 4 * NS_GROUP_BYTES;    // 128 x 128: two planes, or 32-bit sums
 
@@ -744,8 +744,10 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
   unsigned char* X = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ns_smem_raw) + 1023) & ~(uintptr_t)1023);
   const int G = p.groups, S = p.cluster, W = G * 64;
   const uint32_t plane = (uint32_t)G * NS_GROUP_BYTES;                 // X: high words, low words; at the end its 32-bit values
-  unsigned char* AQ = X + 2 * plane;                                   // A or Q: high words, low words; partial sums in between
-  double* norms = reinterpret_cast<double*>(AQ + NS_SQUARE_BYTES);     // of every rank
+  unsigned char* AQ = X + 2 * plane;                                   // A or Q: high words, low words
+  const bool apart = S > 1 && G <= NS_SMALL_APART;                     // there is room for partial sums beside it
+  unsigned char* parts = apart ? AQ + NS_SQUARE_BYTES : AQ;
+  double* norms = reinterpret_cast<double*>(parts + NS_SQUARE_BYTES);  // of every rank
   uint64_t* bar = reinterpret_cast<uint64_t*>(norms + NS_SMALL_CLUSTER);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -816,8 +818,8 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
   double sum = squares.sum;
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) part[warp] = sum;
-  // padding of X is zero
-  for (uint32_t i = tid; i < 2 * plane / 16; i += NS_SMALL_THREADS) reinterpret_cast<uint4*>(X)[i] = make_uint4(0u, 0u, 0u, 0u);
+  // padding of X is zero, and rows and columns of the square that are not written
+  for (uint32_t i = tid; i < (2 * plane + NS_SQUARE_BYTES) / 16; i += NS_SMALL_THREADS) reinterpret_cast<uint4*>(X)[i] = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
   if (tid < S) {
     sum = 0.0;
@@ -870,31 +872,40 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
   };
   constexpr uint32_t HI = TcDesc::hi, K_CONST = 1u << 16, MN_CONST = (NS_GROUP_BYTES >> 4) << 16;
   auto idesc = [](uint32_t n, bool mn) { return (1u << 4) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((NS_SMALL_M >> 4) << 24); };
-  // D (128 x 128 at column `d`) = B B^T over `groups` groups of a K-major buffer: the products with a low part first
-  auto gram = [&](uint32_t d, uint32_t hi, uint32_t lo, int groups) {
+  // D (at column `d` of tensor memory) = B B^T over `steps16` steps of a K-major buffer: the products with a low part first
+  auto gram = [&](uint32_t d, uint32_t hi, uint32_t lo, int steps16, uint32_t n) {
+    const uint32_t form = idesc(n, false);
     uint32_t more = 0;
     if (SPLIT)
-      for (int k = 0; k < groups * 4; ++k) {
+      for (int k = 0; k < steps16; ++k) {
         const uint32_t at = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST;
-        tc_mma<2, false>(d, hi + at, HI, lo + at, HI, idesc(128, false), more);
-        tc_mma<1, false>(d, lo + at, HI, hi + at, HI, idesc(128, false), 1u);
+        tc_mma<2, false>(d, hi + at, HI, lo + at, HI, form, more);
+        tc_mma<1, false>(d, lo + at, HI, hi + at, HI, form, 1u);
         more = 1u;
       }
-    for (int k = 0; k < groups * 4; ++k) {
+    for (int k = 0; k < steps16; ++k) {
       const uint32_t at = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST;
-      tc_mma<2, false>(d, hi + at, HI, hi + at, HI, idesc(128, false), more);
+      tc_mma<2, false>(d, hi + at, HI, hi + at, HI, form, more);
       more = 1u;
     }
   };
-  const uint32_t xu = ag_smem_u32(X) >> 4, xl = xu + (plane >> 4), au = ag_smem_u32(AQ) >> 4, al = au + ((2 * NS_GROUP_BYTES) >> 4);
+  // descriptors take the address within the CTA: the higher bits of a shared address may name the CTA of the cluster, and would
+  // run into the next field
+  const uint32_t xu = (ag_smem_u32(X) & 0x3FFFFu) >> 4, xl = xu + (plane >> 4), au = (ag_smem_u32(AQ) & 0x3FFFFu) >> 4, al = au + ((2 * NS_GROUP_BYTES) >> 4);
+  constexpr int SLICES = NS_SMALL_THREADS / 128;
   const int quarter = warp & 3, slice = warp >> 2, row = quarter * 32 + lane;
+  // what is not padding: steps of 16 elements, chunks of 32 columns of a square
+  const int m16 = (p.m + 15) / 16, m32 = (p.m + 31) / 32;
   const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
-  const int chains = SPLIT ? (G + 1) / 2 : 1, chain_groups = SPLIT ? 2 : G;
-  // 32 columns of the lane's row into the words of a buffer
+  const int w16 = max(1, (width + 15) / 16), chain16 = SPLIT ? 8 : 4 * NS_SMALL_GROUPS, chains = (w16 + chain16 - 1) / chain16;
+  // 32 columns of the lane's row into the words of a buffer; rows of padding are zero
   auto put = [&](unsigned char* dst, uint32_t low, int col, const float (&v)[32]) {
     uint32_t hi[16], lo[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) split_f16x2(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+    for (int k = 0; k < 16; ++k) {
+      split_f16x2(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+      if (row >= p.m) hi[k] = lo[k] = 0u;
+    }
     unsigned char* d = dst + (uint32_t)(col >> 6) * NS_GROUP_BYTES;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -922,16 +933,14 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
     const float gram_mul = (square ? 1.0f : b) * unit * p.loss_gram, gram_diag = (square ? h : a) * NS_SCALE;
     if (tid == 0) {
       for (int i = 0; i < chains; ++i)
-        gram(tmem + i * 128, xu + i * chain_groups * (NS_GROUP_BYTES >> 4), xl + i * chain_groups * (NS_GROUP_BYTES >> 4),
-             min(chain_groups, G - i * chain_groups));
+        gram(tmem + i * 128, xu + 2 * i * (NS_GROUP_BYTES >> 4), xl + 2 * i * (NS_GROUP_BYTES >> 4), min(chain16, w16 - i * chain16), m16 * 16);
       tc_commit(bar);
     }
     products_done();
-    const int own = NS_SMALL_M / S;  // rows of the sum that a CTA owns
-    if (S > 1) tc_cluster_sync();    // nobody multiplies with its Q any more
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch) {
-      const int col = slice * 64 + ch * 32;
+    const int own = NS_SMALL_M / S;          // rows of the sum that a CTA owns
+    if (S > 1 && !apart) tc_cluster_sync();  // nobody multiplies with its Q any more
+    for (int ch = slice; ch < m32; ch += SLICES) {
+      const int col = ch * 32;
       float v[32];
       tc_tmem_ld32(trow + col, reinterpret_cast<uint32_t(&)[32]>(v));
       tc_tmem_ld_wait();
@@ -947,38 +956,41 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
         for (int j = 0; j < 32; ++j) v[j] = v[j] * gram_mul + (row == col + j ? gram_diag : 0.0f);
         put(AQ, 2 * NS_GROUP_BYTES, col, v);
       } else {
-        const uint32_t to = tc_map_to_cta(ag_smem_u32(AQ), row / own) + (uint32_t)(rank * own + row % own) * 512u;
+        const uint32_t to = tc_map_to_cta(ag_smem_u32(parts), row / own) + (uint32_t)(rank * own + row % own) * 512u;
+        if (row < p.m) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          ns_st_cluster(to + ((((uint32_t)col >> 2) + j ^ ((uint32_t)row & 7u)) << 4), make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+          for (int j = 0; j < 8; ++j)
+            ns_st_cluster(to + (((((uint32_t)col >> 2) + j) ^ ((uint32_t)row & 7u)) << 4), make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+        }
+        __syncwarp();
       }
     }
     if (S > 1) {
       tc_cluster_sync();
       // own rows: four columns to a thread and turn, 32 x own of them
-      float4 sums[8];
-      const int turns = own / 8;
+      constexpr int TURNS = NS_SMALL_M / 2 * 32 / NS_SMALL_THREADS;
+      float4 sums[TURNS];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k >= turns) continue;
+      for (int k = 0; k < TURNS; ++k) {
         const int i = tid + k * NS_SMALL_THREADS, r = i >> 5, q = i & 31, global = rank * own + r;
+        if (r >= own || global >= m16 * 16 || q >= m32 * 8) continue;
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < S; ++s) {
-          const float4 x = *reinterpret_cast<const float4*>(AQ + (uint32_t)(s * own + r) * 512u + ((uint32_t)(q ^ (global & 7)) << 4));
+        for (int s = 0; s < (global < p.m ? S : 0); ++s) {
+          const float4 x = *reinterpret_cast<const float4*>(parts + (uint32_t)(s * own + r) * 512u + ((uint32_t)(q ^ (global & 7)) << 4));
           t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
         }
-        const int d = global - q * 4;  // the diagonal's place among the four
+        const int d = global < p.m ? global - q * 4 : -1;  // the diagonal's place among the four; rows of padding are zero
         t.x = t.x * gram_mul + (d == 0 ? gram_diag : 0.f);
         t.y = t.y * gram_mul + (d == 1 ? gram_diag : 0.f);
         t.z = t.z * gram_mul + (d == 2 ? gram_diag : 0.f);
         t.w = t.w * gram_mul + (d == 3 ? gram_diag : 0.f);
         sums[k] = t;
       }
-      tc_cluster_sync();  // all have read the parts: A takes their place
+      if (!apart) tc_cluster_sync();  // all have read the parts: A takes their place
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k >= turns) continue;
+      for (int k = 0; k < TURNS; ++k) {
         const int i = tid + k * NS_SMALL_THREADS, r = i >> 5, q = i & 31, global = rank * own + r;
+        if (r >= own || global >= m16 * 16 || q >= m32 * 8) continue;
         uint32_t hi[2], lo[2];
         split_f16x2(sums[k].x, sums[k].y, hi[0], lo[0]);
         split_f16x2(sums[k].z, sums[k].w, hi[1], lo[1]);
@@ -997,14 +1009,13 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
       if (tid == 0) {
         tc_fence_after();
         ns_fence_proxy();
-        gram(tmem, au, al, 2);
+        gram(tmem, au, al, m16, m16 * 16);
         tc_commit(bar);
       }
       products_done();
       const float mul = c * unit * p.loss_square, diag = (a - h * h * c) * NS_SCALE;
-#pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        const int col = slice * 64 + ch * 32;
+      for (int ch = slice; ch < m32; ch += SLICES) {
+        const int col = ch * 32;
         float v[32];
         tc_tmem_ld32(trow + col, reinterpret_cast<uint32_t(&)[32]>(v));
         tc_tmem_ld_wait();
@@ -1023,13 +1034,13 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
         const uint32_t n = (uint32_t)min(4, G - c0) * 64u, d = tmem + c0 * 64, x0 = c0 * (NS_GROUP_BYTES >> 4) + MN_CONST;
         uint32_t more = 0;
         if (SPLIT)
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < m16; ++k) {
             const uint32_t l = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST, r = x0 + k * 128;
             tc_mma<2, false>(d, au + l, HI, xl + r, HI, idesc(n, true), more);
             tc_mma<1, false>(d, al + l, HI, xu + r, HI, idesc(n, true), 1u);
             more = 1u;
           }
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < m16; ++k) {
           const uint32_t l = (uint32_t)(k >> 2) * (NS_GROUP_BYTES >> 4) + (uint32_t)(k & 3) * 2u + K_CONST, r = x0 + k * 128;
           tc_mma<2, false>(d, au + l, HI, xu + r, HI, idesc(n, true), more);
           more = 1u;
@@ -1040,7 +1051,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
     products_done();
     const bool last = step + 1 == p.steps;
     const float mul = (last ? unit * unit : unit) * p.loss_square;
-    for (int ch = slice; ch < 2 * G; ch += 2) {
+    for (int ch = slice; ch < 2 * G; ch += SLICES) {
       float v[32];
       tc_tmem_ld32(trow + ch * 32, reinterpret_cast<uint32_t(&)[32]>(v));
       tc_tmem_ld_wait();
@@ -1218,44 +1229,92 @@ int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsBuffer* X, NsBuffer& A
   return AG_OK;
 }
 
-// Columns of X in groups of 64 over the CTAs of a cluster: as many CTAs as there are SMs for all matrices, as a CTA's time is that of its
-// slice; false where a slice would not fit, or another path serves the matrices better.
-bool ns_small_shape(const ag_ctx* ctx, const NsPlan& t, int count, int* cluster, int* groups) {
+void ns_cluster_launch(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int cluster, int blocks) {
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(NS_SMALL_THREADS);
+  cfg.dynamicSmemBytes = NS_SMEM_LIMIT;  // whatever the slice needs: a CTA has its SM, and all of tensor memory, for itself
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+}
+
+template <typename T, bool SPLIT>
+int ns_small_setup(ag_ctx* ctx) {
+  static std::atomic<bool> done[AG_MAX_DEVICES];
+  auto kern = ns_small_kernel<T, SPLIT>;
+  if (!done[ag_dev_slot(ctx)].load(std::memory_order_relaxed)) {
+    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM_LIMIT));
+    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    done[ag_dev_slot(ctx)].store(true, std::memory_order_relaxed);
+  }
+  return AG_OK;
+}
+
+// Clusters of 2^log2 CTAs of the small kernel that are resident at once; 0: none, or not known
+int ns_small_resident(ag_ctx* ctx, int log2) {
+  static std::atomic<int> known[AG_MAX_DEVICES][5];  // 1 + the answer
+  std::atomic<int>& slot = known[ag_dev_slot(ctx)][log2];
+  if (const int k = slot.load(std::memory_order_relaxed)) return k - 1;
+  int n = 0;
+  if (ns_small_setup<float, true>(ctx) == AG_OK) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    ns_cluster_launch(cfg, at, 1 << log2, ctx->sm_count << log2);
+    if (cudaOccupancyMaxActiveClusters(&n, ns_small_kernel<float, true>, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+  }
+  slot.store(1 + n, std::memory_order_relaxed);
+  return n;
+}
+
+// How the columns of X, in groups of 64, go to the CTAs of a cluster; false where the general path serves the matrices better.  Times in
+// us, fitted to measurements of 16 to 128 rows and 16 to 5000 columns: a round of clusters takes 13 + 0.17 m, 3 + 0.15 m a group and, with
+// S > 1 CTAs, 12 + m m S / 10^4 (64 x 256: 51 on four CTAs, 64 on two, 73 on one; 128 x 256: 78, 93, 116; 64 x 64: 36 on one, 49 on four;
+// 128 x 1024, 2048, 4096 on sixteen: 93, 114, 160), and there are as many rounds as it takes to hold all matrices; the general path
+// 85 + 0.065 n + 0.0013 n for each matrix (64 x 64: 90, 2 of 64 x 1024: 154, 2 of 128 x 4096: 355, 16 of them: 433 against 501, 32 of 100 x
+// 5000: 656 against 836).
+bool ns_small_shape(ag_ctx* ctx, const NsPlan& t, int count, int* cluster, int* groups) {
   if (t.m > NS_SMALL_M) return false;
   const int all = (t.n + 63) / 64;
-  int s = NS_SMALL_CLUSTER;
-  while (s > 1 && (s / 2 >= all || (int64_t)count * s > ctx->sm_count)) s /= 2;
-  while (s < NS_SMALL_CLUSTER && (all + s - 1) / s > NS_SMALL_GROUPS) s *= 2;
-  *cluster = s;
-  *groups = (all + s - 1) / s;
-  return *groups <= NS_SMALL_GROUPS;
+  double best = 85.0 + 0.065 * t.n + 0.0013 * t.n * count;
+  bool found = false;
+  for (int log2 = 0; (1 << log2) <= NS_SMALL_CLUSTER && (log2 == 0 || (1 << log2) < 2 * all); ++log2) {
+    const int g = (all + (1 << log2) - 1) >> log2;
+    if (g > NS_SMALL_GROUPS) continue;
+    const int resident = ns_small_resident(ctx, log2);
+    if (resident < 1) continue;
+    const double cost = ((count + resident - 1) / resident) *
+                        (13.0 + 0.17 * t.m + (3.0 + 0.15 * t.m) * g + (log2 ? 12.0 + 1e-4 * t.m * t.m * (1 << log2) : 0.0));
+    if (cost < best) {
+      best = cost;
+      found = true;
+      *cluster = 1 << log2;
+      *groups = g;
+    }
+  }
+  return found;
 }
 
 template <typename T, bool SPLIT>
 int ns_small_launch(ag_ctx* ctx, NsSmall& p, int count) {
-  static std::atomic<bool> attr_done[AG_MAX_DEVICES];
-  auto kern = ns_small_kernel<T, SPLIT>;
-  if (!attr_done[ag_dev_slot(ctx)].load(std::memory_order_relaxed)) {
-    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM_LIMIT));
-    AG_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    attr_done[ag_dev_slot(ctx)].store(true, std::memory_order_relaxed);
-  }
-  static_assert(1024 + 2 * NS_SMALL_GROUPS * NS_GROUP_BYTES + NS_SQUARE_BYTES + 512 <= NS_SMEM_LIMIT, "slice and square");
+  static_assert(1024 + 2 * NS_SMALL_GROUPS * NS_GROUP_BYTES + NS_SQUARE_BYTES + 512 <= NS_SMEM_LIMIT &&
+                1024 + 2 * NS_SMALL_APART * NS_GROUP_BYTES + 2 * NS_SQUARE_BYTES + 512 <= NS_SMEM_LIMIT, "slice and square");
+  if (int rc = ns_small_setup<T, SPLIT>(ctx)) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
-  cfg.gridDim = dim3(count * p.cluster);
-  cfg.blockDim = dim3(NS_SMALL_THREADS);
-  cfg.dynamicSmemBytes = NS_SMEM_LIMIT;  // whatever the slice needs: a CTA has its SM, and all of tensor memory, for itself
+  ns_cluster_launch(cfg, at, p.cluster, count * p.cluster);
   cfg.stream = ctx->stream;
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.cluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = ctx->pdl ? 2 : 1;
-  AG_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, p));
+  if (ctx->pdl) {
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  AG_CUDA(ctx, cudaLaunchKernelEx(&cfg, ns_small_kernel<T, SPLIT>, p));
   ctx->launches++;
   ag_enqueued(ctx);
   return AG_OK;

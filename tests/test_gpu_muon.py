@@ -74,7 +74,9 @@ def close(got, u, precision, steps=5, coefficients=R.NEWTON_SCHULZ, eps=1e-7, ou
 
 
 SHAPES = [(1, 1, 1), (1, 1, 9), (2, 7, 1), (2, 2, 2), (3, 16, 16), (2, 64, 256), (1, 100, 33), (2, 129, 65), (1, 127, 257), (3, 333, 201),
-          (1, 384, 384), (2, 200, 64), (1, 64, 1000), (1, 1000, 3), (2, 128, 128), (1, 256, 640), (1, 257, 255), (1, 513, 520), (35, 20, 30)]
+          (1, 384, 384), (2, 200, 64), (1, 64, 1000), (1, 1000, 3), (2, 128, 128), (1, 256, 640), (1, 257, 255), (1, 513, 520), (35, 20, 30),
+          # clusters of several CTAs, slices of one to five groups, the last of them in part or not at all; more rounds than one
+          (1, 20, 500), (1, 128, 1030), (1, 33, 2100), (1, 2900, 77), (1, 70, 4000), (2, 5100, 128), (160, 40, 65), (20, 17, 700), (1, 100, 5200)]
 
 
 @PRECISIONS
