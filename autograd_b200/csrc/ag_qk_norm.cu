@@ -9,7 +9,7 @@
 // A group of 1 to 32 lanes owns a head: a lane has S slots, a slot two packets that the rotation mixes (columns rot and
 // more are split into two halves in the same way, with nothing to mix), so that statistics and rotation need one read, a
 // few shuffles and no shared memory.  A thread keeps U heads of its token in flight and loads the angles once for all of
-// them.  Packets are as wide as addresses, strides and halves allow, 2 to 16 bytes: every shape takes the same code.  All
+// them.  Packets are as wide as addresses, strides and halves allow, one to four elements: every shape takes the same code.  All
 // sums are fp32.
 #include "ag_common.cuh"
 
@@ -85,7 +85,7 @@ struct QkArgs {
   int lanes_log2;
   float eps, sgn;
   int accumulate;            // backward: dx += ...
-  float* partials;           // backward: [grid.x][grid.y][D], null where a single row of them is enough
+  float* partials;           // backward: [grid.y][grid.x][D]
   int* status;
 };
 
@@ -372,31 +372,38 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
       float t = 0.0f;
 #pragma unroll
       for (int w = 0; w < QK_THREADS / 32; ++w) t += qk_smem[w * a.D + d];
-      a.partials[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * a.D + d] = t;
+      a.partials[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.D + d] = t;
     }
   }
 }
 
-// dgamma += the partial rows of its side.  A block has 32 columns of one side; warps take rows in turn.
-__global__ void __launch_bounds__(QK_THREADS) qk_fold_kernel(const float* __restrict__ partials, int grid_x, int q_blocks,
-                                                             int k_blocks, int D, float* dq_gamma, float* dk_gamma) {
-  __shared__ float part[QK_THREADS / 32][33];
+// dgamma += the partial rows of its side: those of queries are the first.  A block has 32 columns of one side, its warps take rows in
+// turn, eight under way each (one at a time, of eight warps, took 72 us for 1183 rows of 128).
+constexpr int QK_FOLD_WARPS = 32;
+__global__ void __launch_bounds__(32 * QK_FOLD_WARPS) qk_fold_kernel(const float* __restrict__ partials, int q_rows, int k_rows, int D,
+                                                                     float* dq_gamma, float* dk_gamma) {
+  __shared__ float part[QK_FOLD_WARPS][33];
   ag_pdl_wait();
   ag_pdl_trigger();
   float* out = blockIdx.y ? dk_gamma : dq_gamma;
   if (!out) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
-  const int blocks = blockIdx.y ? k_blocks : q_blocks, first = blockIdx.y ? q_blocks : 0, all = q_blocks + k_blocks;
+  const int rows = blockIdx.y ? k_rows : q_rows;
+  const float* p = partials + (blockIdx.y ? (int64_t)q_rows * D : 0) + d;
   float t = 0.0f;
-  if (d < D)
-    for (int64_t r = warp; r < (int64_t)grid_x * blocks; r += QK_THREADS / 32)
-      t += partials[(r / blocks * all + first + r % blocks) * D + d];
+  for (int r = warp; r < rows; r += 8 * QK_FOLD_WARPS) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = d < D && r + k * QK_FOLD_WARPS < rows ? p[(int64_t)(r + k * QK_FOLD_WARPS) * D] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += v[k];
+  }
   part[warp][lane] = t;
   __syncthreads();
   if (warp == 0 && d < D) {
     t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < QK_THREADS / 32; ++w) t += part[w][lane];
+    for (int w = 0; w < QK_FOLD_WARPS; ++w) t += part[w][lane];
     out[d] += t;
   }
 }
@@ -409,7 +416,7 @@ struct QkShape {
 // The widest packets that everything allows, then lanes and slots with as few idle ones as possible
 template <typename T>
 QkShape qk_shape(const QkArgs& a) {
-  int nv = 16 / (int)sizeof(T);
+  int nv = 4;
   auto fits = [&](int n) {
     if (a.half % n || ((a.D >> 1) - a.half) % n) return false;
     const uintptr_t bytes = n * sizeof(T), wide = n >= 4 ? 15u : 3u;
@@ -450,8 +457,8 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
     AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS,
                   W ? QK_THREADS / 32 * a.D * sizeof(float) : 0, a);
     if (W)
-      AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), QK_THREADS, 0, a.partials, (int)gx,
-                    a.side[0].blocks, a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
+      AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), 32 * QK_FOLD_WARPS, 0, a.partials,
+                    (int)gx * a.side[0].blocks, (int)gx * a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
   }
   return AG_OK;
 }
@@ -472,7 +479,7 @@ int qk_slots(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
     case 3: return qk_kind<T, NV, 3, 1>(ctx, a, sh, back, w);
     case 4: return qk_kind<T, NV, 4, 1>(ctx, a, sh, back, w);
   }
-  if constexpr (NV * sizeof(T) < 16) {  // 16-byte packets: 32 lanes of 4 slots hold 1024 columns
+  if constexpr (NV < 4) {  // packets of four: 32 lanes of 4 slots hold 1024 columns
     if (sh.S == 8) return qk_kind<T, NV, 8, 1>(ctx, a, sh, back, w);
     if constexpr (NV == 1)
       if (sh.S == 16) return qk_kind<T, NV, 16, 1>(ctx, a, sh, back, w);
@@ -486,10 +493,8 @@ int qk_run(ag_ctx* ctx, QkArgs& a, bool back, bool w) {
   switch (sh.nv) {
     case 1: return qk_slots<T, 1>(ctx, a, sh, back, w);
     case 2: return qk_slots<T, 2>(ctx, a, sh, back, w);
-    case 4: return qk_slots<T, 4>(ctx, a, sh, back, w);
+    default: return qk_slots<T, 4>(ctx, a, sh, back, w);
   }
-  if constexpr (sizeof(T) == 2) return qk_slots<T, 8>(ctx, a, sh, back, w);
-  AG_FAIL(ctx, AG_ERR_INVALID, "no kernel for packets of %d", sh.nv);
 }
 
 // Rows of `width` elements, `stride` apart
