@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (!in || head + u >= q.heads) continue;
-    const float inv = 1.0f / sqrtf(sum[u] / (float)a.D + a.eps);
+    const float inv = rsqrtf(sum[u] * (1.0f / (float)a.D) + a.eps);
 #pragma unroll
     for (int k = 0; k < S; ++k) {
       const int slot = lane + (k << a.lanes_log2);
@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
   }
 }
 
-// W: the gradients of the weights are wanted (of either side)
+// W: the gradients of the weights are wanted (of either side).  A group goes from token to token, with the sums of its columns in
+// registers.  What keeps memory busy is blocks, not packets a token ahead: with those, registers leave half of the blocks (187 us instead of 165 for 16 x
+// 2048 tokens of 2 x 10 heads fp32, 40 instead of 36 for 8192 of 12 + 2 bf16).
 template <typename T, int NV, int S, int U, bool W>
 __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a) {
   using P = QkPack<T, NV>;
@@ -234,67 +236,68 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
   const int per_block = QK_THREADS >> a.lanes_log2;
   const int which = (int)blockIdx.y >= a.side[0].blocks;
   const QkSide& q = a.side[which];
-  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U;
+  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U, heads = min(U, q.heads - head);
   float glo[S][NV], ghi[S][NV];
   qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
+  int col[S], apart[S];
+  bool turns[S];
+#pragma unroll
+  for (int k = 0; k < S; ++k) qk_columns(a, (lane + (k << a.lanes_log2)) * NV, turns[k], col[k], apart[k]);
   float dlo[W ? S : 1][NV], dhi[W ? S : 1][NV];
 #pragma unroll
   for (int k = 0; k < (W ? S : 1); ++k)
 #pragma unroll
     for (int i = 0; i < NV; ++i) dlo[k][i] = dhi[k][i] = 0.0f;
   const float over = 1.0f / (float)a.D;
-  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += (int64_t)gridDim.x * per_block) {
-    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
+  const int64_t first = (int64_t)blockIdx.x * per_block + (threadIdx.x >> a.lanes_log2), stride = (int64_t)gridDim.x * per_block;
+  const T* x = static_cast<const T*>(q.x) + first * q.x_stride + (int64_t)head * a.D;
+  const T* dy = static_cast<const T*>(q.dy) + first * q.dy_stride + (int64_t)head * a.D;
+  T* out = static_cast<T*>(q.y) + first * q.y_stride + (int64_t)head * a.D;
+  typename P::Raw xl[U][S], xh[U][S], gl[U][S], gh[U][S];
+  float c[S][NV], s[S][NV];
+  bool ok = true;
+  auto fetch = [&](int64_t tok) {
     const bool in = tok < a.tokens;
-    typename P::Raw xl[U][S], xh[U][S], gl[U][S], gh[U][S];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int k = 0; k < S; ++k) {
-        const int slot = lane + (k << a.lanes_log2);
-        bool turns;
-        int col, apart;
-        qk_columns(a, slot * NV, turns, col, apart);
         xl[u][k] = xh[u][k] = gl[u][k] = gh[u][k] = typename P::Raw{};
-        if (in && slot < a.slots && head + u < q.heads) {
-          const T* x = static_cast<const T*>(q.x) + tok * q.x_stride + (int64_t)(head + u) * a.D + col;
-          const T* g = static_cast<const T*>(q.dy) + tok * q.dy_stride + (int64_t)(head + u) * a.D + col;
-          xl[u][k] = P::load(x);
-          xh[u][k] = P::load(x + apart);
-          gl[u][k] = P::load(g);
-          gh[u][k] = P::load(g + apart);
+        if (in && u < heads && lane + (k << a.lanes_log2) < a.slots) {
+          const int at = u * a.D + col[k];
+          xl[u][k] = P::load(x + at);
+          xh[u][k] = P::load(x + at + apart[k]);
+          gl[u][k] = P::load(dy + at);
+          gh[u][k] = P::load(dy + at + apart[k]);
         }
       }
-    float c[S][NV], s[S][NV];
-    const bool ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
-    float sum[U], dot[U];
-    // w of a slot, from its two packets of dy
-    auto turned = [&](int u, int k, float (&wl)[NV], float (&wh)[NV]) {
-      P::unpack(gl[u][k], wl);
-      P::unpack(gh[u][k], wh);
-      const bool turns = (lane + (k << a.lanes_log2)) * NV < a.half;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const float x = wl[i], y = wh[i], sn = a.sgn * s[k][i];
-        if (turns) {
-          wl[i] = x * c[k][i] + y * sn;
-          wh[i] = y * c[k][i] - x * sn;
-        }
-      }
-    };
+    ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
+    x += stride * q.x_stride;
+    dy += stride * q.dy_stride;
+  };
+  // all threads of a block make as many turns: the sums are over groups of lanes
+  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += stride) {
+    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
+    fetch(tok);
+    const bool in = tok < a.tokens, good = ok;
+    float vx[U][S][NV], vy[U][S][NV], wl[U][S][NV], wh[U][S][NV], sum[U], dot[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       sum[u] = dot[u] = 0.0f;
 #pragma unroll
       for (int k = 0; k < S; ++k) {
-        float x[NV], y[NV], wl[NV], wh[NV];
-        P::unpack(xl[u][k], x);
-        P::unpack(xh[u][k], y);
-        turned(u, k, wl, wh);
+        P::unpack(xl[u][k], vx[u][k]);
+        P::unpack(xh[u][k], vy[u][k]);
+        P::unpack(gl[u][k], wl[u][k]);
+        P::unpack(gh[u][k], wh[u][k]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          sum[u] = fmaf(x[i], x[i], fmaf(y[i], y[i], sum[u]));
-          dot[u] = fmaf(x[i], wl[i] * glo[k][i], fmaf(y[i], wh[i] * ghi[k][i], dot[u]));
+          // the angles of columns that do not turn are (1, 0)
+          const float p = wl[u][k][i], r = wh[u][k][i], sn = a.sgn * s[k][i];
+          wl[u][k][i] = turns[k] ? p * c[k][i] + r * sn : p;
+          wh[u][k][i] = turns[k] ? r * c[k][i] - p * sn : r;
+          sum[u] = fmaf(vx[u][k][i], vx[u][k][i], fmaf(vy[u][k][i], vy[u][k][i], sum[u]));
+          dot[u] = fmaf(vx[u][k][i], wl[u][k][i] * glo[k][i], fmaf(vy[u][k][i], wh[u][k][i] * ghi[k][i], dot[u]));
         }
       }
     }
@@ -306,43 +309,36 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
       }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!in || head + u >= q.heads) continue;
-      const float inv = 1.0f / sqrtf(sum[u] * over + a.eps);
+      if (!in || u >= heads) continue;
+      const float inv = rsqrtf(sum[u] * over + a.eps);
       const float back = inv * inv * (dot[u] * over);
 #pragma unroll
       for (int k = 0; k < S; ++k) {
-        const int slot = lane + (k << a.lanes_log2);
-        if (slot >= a.slots) continue;
-        bool turns;
-        int col, apart;
-        qk_columns(a, slot * NV, turns, col, apart);
-        float x[NV], y[NV], wl[NV], wh[NV];
-        P::unpack(xl[u][k], x);
-        P::unpack(xh[u][k], y);
-        turned(u, k, wl, wh);
-        T* out = static_cast<T*>(q.y) + tok * q.y_stride + (int64_t)(head + u) * a.D + col;
+        if (lane + (k << a.lanes_log2) >= a.slots) continue;
+        T* d = out + u * a.D + col[k];
         float ol[NV], oh[NV];
-        if (a.accumulate) {
-          P::unpack(P::load(out), ol);
-          P::unpack(P::load(out + apart), oh);
-        } else {
-#pragma unroll
-          for (int i = 0; i < NV; ++i) ol[i] = oh[i] = 0.0f;
-        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          if (W && ok) {
-            dlo[k][i] = fmaf(wl[i], x[i] * inv, dlo[k][i]);
-            dhi[k][i] = fmaf(wh[i], y[i] * inv, dhi[k][i]);
+          const float xi = vx[u][k][i], yi = vy[u][k][i], wi = wl[u][k][i], ui = wh[u][k][i];
+          if (W && good) {
+            dlo[k][i] = fmaf(wi, xi * inv, dlo[k][i]);
+            dhi[k][i] = fmaf(ui, yi * inv, dhi[k][i]);
           }
-          const float dl = inv * (wl[i] * glo[k][i] - x[i] * back), dh = inv * (wh[i] * ghi[k][i] - y[i] * back);
-          ol[i] += ok ? dl : 0.0f;
-          oh[i] += ok ? dh : 0.0f;
+          ol[i] = good ? inv * (wi * glo[k][i] - xi * back) : 0.0f;
+          oh[i] = good ? inv * (ui * ghi[k][i] - yi * back) : 0.0f;
         }
-        P::store(out, ol);
-        P::store(out + apart, oh);
+        if (a.accumulate) {
+          float pl[NV], ph[NV];
+          P::unpack(P::load(d), pl);
+          P::unpack(P::load(d + apart[k]), ph);
+#pragma unroll
+          for (int i = 0; i < NV; ++i) ol[i] += pl[i], oh[i] += ph[i];
+        }
+        P::store(d, ol);
+        P::store(d + apart[k], oh);
       }
     }
+    out += stride * q.y_stride;
   }
   if constexpr (W) {
     // the groups of a warp, then the warps, in a fixed order
@@ -452,10 +448,22 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
   if constexpr (!BACK) {
     AG_LAUNCH_PDL(ctx, "qk_forward_kernel", (qk_forward_kernel<T, NV, S, U>), dim3((unsigned)gx, gy), QK_THREADS, 0, a);
   } else {
-    const int64_t most = ctx->sm_count * QK_BLOCKS_PER_SM / gy;
-    if (gx > most) gx = most > 0 ? most : 1;
+    // blocks that are resident at once, with as many turns each
+    static AgOccupancy known[AG_MAX_DEVICES];
+    const size_t smem = W ? QK_THREADS / 32 * a.D * sizeof(float) : 0;
+    int occ = known[ag_dev_slot(ctx)].get(QK_THREADS, smem, [&] {
+      int n = 0;
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, qk_backward_kernel<T, NV, S, U, W>, QK_THREADS, smem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        n = 0;
+      }
+      return n;
+    });
+    occ = occ < 1 ? 1 : occ > QK_BLOCKS_PER_SM ? QK_BLOCKS_PER_SM : occ;
+    const int64_t most = ctx->sm_count * occ / gy > 0 ? ctx->sm_count * occ / gy : 1, turns = (gx + most - 1) / most;
+    gx = (gx + turns - 1) / turns;
     AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS,
-                  W ? QK_THREADS / 32 * a.D * sizeof(float) : 0, a);
+                  smem, a);
     if (W)
       AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), 32 * QK_FOLD_WARPS, 0, a.partials,
                     (int)gx * a.side[0].blocks, (int)gx * a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
@@ -466,7 +474,10 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
 template <typename T, int NV, int S, int U>
 int qk_kind(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
   if (!back) return qk_launch<T, NV, S, U, false, false>(ctx, a, sh);
-  return w ? qk_launch<T, NV, S, U, true, true>(ctx, a, sh) : qk_launch<T, NV, S, U, true, false>(ctx, a, sh);
+  // backward, heads a thread has: two of fp32, one of bf16 (16 x 2048 tokens of 2 x 10 heads fp32 165 us against 186, 8192 of 12 + 2 bf16 36
+  // against 45: with two, registers leave two blocks to an SM)
+  constexpr int B = sizeof(T) == 4 ? U : 1;
+  return w ? qk_launch<T, NV, S, B, true, true>(ctx, a, sh) : qk_launch<T, NV, S, B, true, false>(ctx, a, sh);
 }
 
 template <typename T, int NV>
