@@ -634,79 +634,97 @@ class CudaBackend:
     # rows: *_stride elements between tokens, dense where None.  cos, sin (positions, columns / 2) rotate the first `columns` of a
     # head, all of them stay where the tables are None.  positions (int32, one a token) are rows of the tables; without them the
     # tensors are (batch, T, heads, D) and token t has position t.  Formulas, limits: include/autograd_b200.h.
-    def _heads(self, q, k, cos, sin, positions, q_gamma, k_gamma, like):
-        t = q if q is not None else k
+    @staticmethod
+    def _alike(name, x, shape, dtype):
+        if tuple(x.shape) != tuple(shape) or _ag_dtype(x.storage.dtype) != _ag_dtype(dtype):
+            raise ValueError(f"{name} {tuple(x.shape)} needs the shape {tuple(shape)} and the type of the others")
+
+    # The usual tensors pass by comparisons in place (a call for one token takes the host longer than the device); the rest, and all
+    # refusals, go through _alike and _check.
+    def _heads(self, q, k, cos, sin, positions, q_gamma, k_gamma, with_q, with_k):
+        t = k if q is None else q
         if t is None:
             raise ValueError("neither queries nor keys")
-        lead, d, dtype = tuple(t.shape[:-2]), t.shape[-1], _ag_dtype(t.storage.dtype)
+        shape, dtype = t.shape, t.storage.dtype
+        lead, d, h, hkv = shape[:-2], shape[-1], 0, 0
+        if q is not None:
+            h = shape[-2]
+        if k is not None:
+            hkv = k.shape[-2]
+            if q is not None and (k.shape[:-2] != lead or k.shape[-1] != d or k.storage.dtype is not dtype):
+                self._alike("k", k, (*lead, hkv, d), dtype)
+        for ref, every in ((q, with_q), (k, with_k)):
+            for x in every:
+                if ref is None or x is None:
+                    if x is not ref:
+                        raise ValueError("queries or keys without their output or gradient, or the other way round")
+                elif x is not ref and (x.shape != ref.shape or x.storage.dtype is not dtype):
+                    self._alike("a tensor of the " + ("queries" if ref is q else "keys"), x, ref.shape, dtype)
+        for name, g in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+            if g is not None and (g.shape != (d,) or g.dtype is not np.float32):
+                self._check(name, g, d)
         tokens = prod(lead)
-        for name, x, ref in (("q", q, q), ("k", k, k)) + like:
-            if (x is None) != (ref is None):
-                raise ValueError(f"{name} is missing, or has no tensor to belong to")
-            if x is not None and (tuple(x.shape) != lead + (ref.shape[-2], d) or _ag_dtype(x.storage.dtype) != dtype):
-                raise ValueError(f"{name} {tuple(x.shape)} needs the shape {lead + (ref.shape[-2], d)} and the type of the others")
-        check = self._check
-        check("q_gamma", q_gamma, d)
-        check("k_gamma", k_gamma, d)
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin come together")
         rows, rot, seq = 0, 0, lead[-1] if lead else 1
         if cos is not None:
             rows, half = cos.shape
             rot = 2 * half
-            check("cos", cos, rows * half)
-            check("sin", sin, rows * half)
+            if sin is None:
+                raise ValueError("cos and sin come together")
+            if sin.shape != (rows, half) or sin.dtype is not np.float32 or cos.dtype is not np.float32:
+                self._check("cos", cos, rows * half)
+                self._check("sin", sin, rows * half)
             if rot > d:
                 raise ValueError(f"tables of {half} columns for heads of {d}")
             if positions is not None:
-                check("positions", positions, tokens, np.int32)
+                if positions.dtype is not np.int32 or _size(positions) != tokens:
+                    self._check("positions", positions, tokens, np.int32)
             elif seq > rows:
                 raise ValueError(f"tables of {rows} positions for sequences of {seq}")
-        heads = [0 if x is None else x.shape[-2] for x in (q, k)]
-        return (tokens, seq, rows, *heads, d, rot), dtype
-
-    @staticmethod
-    def _stride(given, t):
-        if t is None:
-            return 0
-        return t.shape[-2] * t.shape[-1] if given is None else given
+        elif sin is not None:
+            raise ValueError("cos and sin come together")
+        else:
+            positions = None
+        return tokens, seq, rows, h, hkv, d, rot, _ag_dtype(dtype), positions
 
     def qk_norm_rope_forward(self, q, k, cos, sin, q_out, k_out, eps, q_gamma=None, k_gamma=None, positions=None, sin_sign=1,
                              q_stride=None, k_stride=None, q_out_stride=None, k_out_stride=None):
         """q_out, k_out = rotation(x * inv_rms(x) * gamma) of every head of q and k; an output may be its input, then it has the
         input's stride.  q or k may be None, with its output."""
-        sizes, dtype = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, (("q_out", q_out, q), ("k_out", k_out, k)))
-        stride = self._stride
-        self._context.qk_norm_rope_forward(
-            q, k, q_gamma, k_gamma, cos, sin, positions if cos is not None else None, q_out, k_out, *sizes, stride(q_stride, q),
-            stride(k_stride, k), stride(q_stride if q_out_stride is None and q_out is q else q_out_stride, q_out),
-            stride(k_stride if k_out_stride is None and k_out is k else k_out_stride, k_out), eps, sin_sign, dtype)
+        tokens, seq, rows, h, hkv, d, rot, dtype, positions = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, (q_out,), (k_out,))
+        if q_stride is None:
+            q_stride = h * d
+        if k_stride is None:
+            k_stride = hkv * d
+        if q_out_stride is None:
+            q_out_stride = q_stride if q_out is q else h * d
+        if k_out_stride is None:
+            k_out_stride = k_stride if k_out is k else hkv * d
+        self._context.qk_norm_rope_forward(q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out, tokens, seq, rows, h, hkv, d, rot,
+                                           q_stride, k_stride, q_out_stride, k_out_stride, eps, sin_sign, dtype)
 
     def qk_norm_rope_backward(self, dq_out, dk_out, q, k, cos, sin, dq, dk, eps, q_gamma=None, k_gamma=None, dq_gamma=None,
                               dk_gamma=None, positions=None, sin_sign=1, accumulate=False, dq_out_stride=None, dk_out_stride=None,
                               q_stride=None, k_stride=None, dq_stride=None, dk_stride=None, scratch=None):
         """dq, dk = gradients (added to them with accumulate); dq_gamma, dk_gamma += theirs.  q, k: the forward's inputs; dq may be
         dq_out or q, with its stride."""
-        like = (("dq_out", dq_out, q), ("dk_out", dk_out, k), ("dq", dq, q), ("dk", dk, k))
-        sizes, dtype = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, like)
-        _, _, _, h, hkv, d, _ = sizes
-        self._check("dq_gamma", dq_gamma, d)
-        self._check("dk_gamma", dk_gamma, d)
+        tokens, seq, rows, h, hkv, d, rot, dtype, positions = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, (dq_out, dq),
+                                                                          (dk_out, dk))
         part, part_bytes = 0, 0
         if dq_gamma is not None or dk_gamma is not None:
+            self._check("dq_gamma", dq_gamma, d)
+            self._check("dk_gamma", dk_gamma, d)
             part, part_bytes = self._slot(scratch, "partials", self._context.qk_norm_partials_bytes(h, hkv, d))
-        stride = self._stride
-        dqs, dks = stride(dq_out_stride, dq_out), stride(dk_out_stride, dk_out)
-        qs, ks = stride(q_stride, q), stride(k_stride, k)
 
-        def of(given, t, dy, dy_stride, x, x_stride):
-            if given is None and t is not None:
-                return dy_stride if t is dy else x_stride if t is x else stride(None, t)
-            return stride(given, t)
+        def strides(dense, x, x_stride, dy, dy_stride, dx, dx_stride):
+            x_stride, dy_stride = dense if x_stride is None else x_stride, dense if dy_stride is None else dy_stride
+            if dx_stride is None:
+                dx_stride = dy_stride if dx is dy else x_stride if dx is x else dense
+            return x_stride, dy_stride, dx_stride
+        qs, dqos, dqs = strides(h * d, q, q_stride, dq_out, dq_out_stride, dq, dq_stride)
+        ks, dkos, dks = strides(hkv * d, k, k_stride, dk_out, dk_out_stride, dk, dk_stride)
         self._context.qk_norm_rope_backward(
-            dq_out, dk_out, q, k, q_gamma, k_gamma, cos, sin, positions if cos is not None else None, dq, dk, dq_gamma, dk_gamma,
-            part, part_bytes, *sizes, dqs, dks, qs, ks, of(dq_stride, dq, dq_out, dqs, q, qs), of(dk_stride, dk, dk_out, dks, k, ks),
-            eps, sin_sign, accumulate, dtype)
+            dq_out, dk_out, q, k, q_gamma, k_gamma, cos, sin, positions, dq, dk, dq_gamma, dk_gamma, part, part_bytes, tokens, seq, rows, h,
+            hkv, d, rot, dqos, dkos, qs, ks, dqs, dks, eps, sin_sign, accumulate, dtype)
 
     # ------------------------------------------------------------------ orthogonal updates
     # Singular values in (0, 1] end up between 0.7 and 1.2 after five steps; (a, b, c) for all steps, or one triple a step.
