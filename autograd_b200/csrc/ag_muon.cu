@@ -250,9 +250,11 @@ __global__ void __launch_bounds__(NS_THREADS) ns_start_kernel(const NsMatrices m
 //   NEXT:  X' = Q X                       symmetric, X MN-major
 // so that no product needs anything beside its operands, and every epilogue is a factor and a number on the diagonal.  Where c is 0,
 // GRAM writes Q = a I + b G itself.
-// A and Q are symmetric (polynomials of one matrix commute): only the tiles on and above the diagonal are computed and
-// stored.  A tile of an operand that lies below is read as the transpose of the one above, as an MN-major tile: which of the
-// two is a matter of the map, the descriptor and a bit of the instruction, chosen for every 64 columns.
+// A and Q are symmetric (polynomials of one matrix commute): only the 256 x 256 blocks on and above the diagonal are computed and
+// stored, by tiles of either size.  A tile of an operand that lies below is read as the transpose of the one above, as an MN-major
+// tile: which of the two is a matter of the map, the descriptor and a bit of the instruction.
+// Few tiles with a long contraction (X X^T of a wide matrix) are shared by a cluster of up to 8 CTAs, each with a part of the contraction (ZSPLIT):
+// they send their sums to the CTA that owns the rows, which adds them in the order of the ranks.
 enum { NS_GRAM, NS_POLY, NS_NEXT };
 constexpr bool ns_symmetric(int kind) { return kind <= NS_POLY; }
 
@@ -283,6 +285,8 @@ struct NsGemm {
   int slots;                   // of operand tiles of a double step
   int M, N;                // rows and columns of a matrix that are stored (padded)
   int two;                 // the result has a low part
+  int cluster, k_each;     // ZSPLIT: CTAs to a tile, steps of each (even)
+  NsPlane D;               // and where the result goes
   float diag, mul;
   int* status;
 };
@@ -291,18 +295,26 @@ struct NsTile {
   int mat, tm, tn;
 };
 
-template <int KIND>
+template <int KIND, bool PAIR>
 __device__ __forceinline__ bool ns_tile(const NsGemm& p, int unit, int units, int step, NsTile& t) {
   int i = unit + step * units;
   if (i >= p.batch * p.tiles) return false;
   t.mat = i / p.tiles;
   i -= t.mat * p.tiles;
-  if (ns_symmetric(KIND)) {  // columns of tiles, the diagonal last in each
+  if (ns_symmetric(KIND) && PAIR) {  // columns of tiles, the diagonal last in each
     int n = (int)((sqrtf(8.0f * (float)i + 1.0f) - 1.0f) * 0.5f);
     while (n * (n + 1) / 2 > i) --n;
     while ((n + 1) * (n + 2) / 2 <= i) ++n;
     t.tn = n;
     t.tm = i - n * (n + 1) / 2;
+  } else if (ns_symmetric(KIND)) {   // two columns of 128-row tiles to a block: 2 j + 2 tiles in each
+    int j = (int)((sqrtf(2.0f * (float)i + 1.0f) - 1.0f) * 0.5f);
+    while (2 * j * (j + 1) > i) --j;
+    while (2 * (j + 1) * (j + 2) <= i) ++j;
+    i -= 2 * j * (j + 1);
+    const int rows = min(2 * j + 2, p.tiles_m);
+    t.tn = 2 * j + i / rows;
+    t.tm = i - i / rows * rows;
   } else {
     t.tn = i / p.tiles_m;
     t.tm = i - t.tn * p.tiles_m;
@@ -341,8 +353,20 @@ __device__ __forceinline__ void ns_step_mmas(uint32_t acc, uint32_t lh, uint32_t
   }
 }
 
-template <int KIND, bool SPLIT, bool PAIR, int BN>
+// into the shared memory of a CTA of the cluster
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
+template <int KIND, bool SPLIT, bool PAIR, int BN, bool ZSPLIT = false>
 __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_constant__ NsGemm p) {
+  static_assert(!ZSPLIT || (KIND == NS_GRAM && !PAIR), "sums of a cluster: X X^T on single CTAs");
   extern __shared__ unsigned char ns_smem_raw[];
   constexpr bool R_MN = !ns_symmetric(KIND);          // the right operand is stored with its columns contiguous
   constexpr uint32_t A_BYTES = TC_BM * 128, BN_CTA = PAIR ? BN / 2 : BN, B_BYTES = BN_CTA * 128;
@@ -367,8 +391,10 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? tc_cluster_rank() : 0u;
-  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
-  const int units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const int unit = PAIR ? (int)(blockIdx.x >> 1) : ZSPLIT ? (int)blockIdx.x / p.cluster : (int)blockIdx.x;
+  const int units = PAIR ? (int)(gridDim.x >> 1) : ZSPLIT ? (int)gridDim.x / p.cluster : (int)gridDim.x;  // ZSPLIT: one tile each
+  const int zrank = ZSPLIT ? (int)blockIdx.x - unit * p.cluster : 0;
+  const int k_first = ZSPLIT ? zrank * p.k_each : 0, k_last = ZSPLIT ? min(p.k_iters, k_first + p.k_each) : p.k_iters;
   const int row_off = PAIR ? (int)rank * TC_BM : 0;
 
   if (threadIdx.x == 0) {
@@ -385,7 +411,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     *abort_flag = 0;
     ag_fence_mbar_init();
   }
-  if (PAIR) tc_cluster_sync(); else __syncthreads();
+  if (PAIR || ZSPLIT) tc_cluster_sync(); else __syncthreads();
   if (warp == 1) {
     if (PAIR) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem_u32(tmem_slot)), "r"(COLUMNS)
@@ -410,11 +436,11 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
       // ---------------------------------------------------------------- TMA producer
       uint32_t slot = 0, phase = 0, low = 0, low_phase = 0;
       NsTile t;
-      for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
+      for (int step = 0; !expired && ns_tile<KIND, PAIR>(p, unit, units, step, t); ++step) {
         const int l_at = t.tm * BM + row_off, r_at = t.tn * BN + (int)rank * (PAIR ? (int)BN_CTA : 0);
-        for (int k = 0; k < p.k_iters && !expired; k += 2) {
-          const int n = p.k_iters - k < 2 ? 1 : 2, blk = k * TC_BK / BM;  // blk: tile of the contraction
-          const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
+        for (int k = k_first; k < k_last && !expired; k += 2) {
+          const int n = k_last - k < 2 ? 1 : 2, blk = k * TC_BK / 256;  // blk: block of the contraction
+          const bool l_mn = KIND != NS_GRAM && t.tm * BM / 256 > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn * BN / 256 > blk);
           auto load = [&](const CUtensorMap& k_map, const CUtensorMap& mn_map, uint64_t* bar, unsigned char* dst, int kx, int row, bool mn) {
             const uint32_t at = PAIR ? tc_map_to_cta(ag_smem_u32(bar), 0u) : 0u;  // the leader counts the bytes of both
             if (!mn) {
@@ -455,7 +481,8 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
       // ---------------------------------------------------------------- MMA issuer (pair: the leader only)
       uint32_t slot = 0, phase = 0, low = 0, low_phase = 0, acc_par = 0;
       int buf = 0;
-      const uint32_t tiles_u = ag_smem_u32(tiles) >> 4, lows_u = ag_smem_u32(lows) >> 4;
+      // descriptors take the address within the CTA: higher bits may name the CTA of the cluster
+      const uint32_t tiles_u = (ag_smem_u32(tiles) & 0x3FFFFu) >> 4, lows_u = (ag_smem_u32(lows) & 0x3FFFFu) >> 4;
       TcDesc dk, dmn;
       dk.init(0);
       dmn.init(1);
@@ -464,12 +491,12 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         else tc_commit(bar);
       };
       NsTile t;
-      for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
+      for (int step = 0; !expired && ns_tile<KIND, PAIR>(p, unit, units, step, t); ++step) {
         uint32_t tacc = 0, more = 0;
         int left = 0;  // double steps of the chain
-        for (int k = 0; k < p.k_iters; k += 2) {
-          const int n = p.k_iters - k < 2 ? 1 : 2, blk = k * TC_BK / BM;
-          const bool l_mn = KIND != NS_GRAM && t.tm > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn > blk);
+        for (int k = k_first; k < k_last; k += 2) {
+          const int n = k_last - k < 2 ? 1 : 2, blk = k * TC_BK / 256;
+          const bool l_mn = KIND != NS_GRAM && t.tm * BM / 256 > blk, r_mn = R_MN || (KIND == NS_POLY && t.tn * BN / 256 > blk);
           const uint32_t idesc = IDESC | (l_mn ? 1u << 15 : 0u) | (r_mn ? 1u << 16 : 0u);
           const uint32_t l_step = l_mn ? dmn.step : dk.step, r_step = r_mn ? dmn.step : dk.step;
           const uint32_t l_const = l_mn ? dmn.lo_const : dk.lo_const, r_const = (A_BYTES >> 4) + (r_mn ? dmn.lo_const : dk.lo_const);
@@ -512,13 +539,18 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
           }
           if (!SPLIT) arrive(&empty[slot]);
           if (++slot == (uint32_t)p.slots) slot = 0, phase ^= 1u;
-          if (--left == 0 || k + 2 >= p.k_iters) {
+          if (--left == 0 || k + 2 >= k_last) {
             arrive(&acc_full[buf]);
             buf ^= 1;
             left = 0;
           }
         }
       }
+    }
+    if constexpr (ZSPLIT) {
+      __syncwarp();
+      tc_cluster_sync();
+      tc_cluster_sync();
     }
   } else {
     // ------------------------------------------------------------------ epilogue (warps 4..11)
@@ -528,7 +560,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     uint32_t full_par = 0;
     int buf = 0, half = 0;
     NsTile t;
-    for (int step = 0; !expired && ns_tile<KIND>(p, unit, units, step, t); ++step) {
+    for (int step = 0; !expired && ns_tile<KIND, PAIR>(p, unit, units, step, t); ++step) {
       const int row0 = t.tm * BM + row_off + quarter * 32, col0 = t.tn * BN + slice * (BN / 2);
       const uint32_t toff = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slice * (BN / 2));
       const bool rows_in = row0 < p.M;  // padded sizes are multiples of 32
@@ -580,14 +612,20 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         buf ^= 1;
       };
       float acc[CHUNKS][32];
+      if (ZSPLIT) {  // a part may be empty
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
+      }
       bool gone = false;
-      for (int k = 0; k < p.k_iters; k += 2 * p.chain) {
+      for (int k = k_first; k < k_last; k += 2 * p.chain) {
         if (!wait_full()) {
           gone = true;
           break;
         }
         const uint32_t from = toff + (uint32_t)buf * BN;
-        if (k == 0) {
+        if (k == k_first) {
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) tc_tmem_ld32(from + c * 32, reinterpret_cast<uint32_t(&)[32]>(acc[c]));
           tc_tmem_ld_wait();
@@ -609,6 +647,36 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
           }
         }
       }
+      if constexpr (ZSPLIT) {
+        // The sums go to the CTAs that own the rows, where the operands were (all CTAs meet twice, whatever became of them)
+        const int own = TC_BM / p.cluster, r = quarter * 32 + lane;
+        tc_cluster_sync();
+        const uint32_t to = tc_map_to_cta(ag_smem_u32(tiles), r / own) + (uint32_t)(zrank * own + r % own) * 512u;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            ns_st_cluster(to + ((((uint32_t)(slice * (BN / 8) + c * 8 + j)) ^ ((uint32_t)r & 7u)) << 4),
+                          make_float4(acc[c][4 * j], acc[c][4 * j + 1], acc[c][4 * j + 2], acc[c][4 * j + 3]));
+        tc_cluster_sync();
+        for (int i = threadIdx.x - 128; i < own * 32; i += 32 * NS_EPI_WARPS) {
+          const int q = i & 31, at = zrank * own + (i >> 5), row = t.tm * BM + at, col = t.tn * BN + q * 4;
+          if (row >= p.M || col >= p.N) continue;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int s = 0; s < p.cluster; ++s) {
+            const float4 x = *reinterpret_cast<const float4*>(tiles + (uint32_t)(s * own + (i >> 5)) * 512u + ((uint32_t)(q ^ (at & 7)) << 4));
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+          }
+          const int d = row - col;  // the diagonal's place among the four
+          uint32_t hi[2], lo[2];
+          split_f16x2(v.x * p.mul + (d == 0 ? p.diag : 0.f), v.y * p.mul + (d == 1 ? p.diag : 0.f), hi[0], lo[0]);
+          split_f16x2(v.z * p.mul + (d == 2 ? p.diag : 0.f), v.w * p.mul + (d == 3 ? p.diag : 0.f), hi[1], lo[1]);
+          const int64_t out = ((int64_t)t.mat * p.M + row) * p.M + col;
+          *reinterpret_cast<uint2*>(p.D.hi + out) = make_uint2(hi[0], hi[1]);
+          if (SPLIT || p.two) *reinterpret_cast<uint2*>(p.D.lo + out) = make_uint2(lo[0], lo[1]);
+        }
+        break;
+      }
       if (gone) break;
       // one copy of the code for all chunks, which move up to acc[0] one after the other: what every tile runs through once is
       // fetched anew each time
@@ -625,7 +693,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   }
   if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
   tc_fence_before();
-  if (PAIR) tc_cluster_sync(); else __syncthreads();
+  if (PAIR || ZSPLIT) tc_cluster_sync(); else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     if (PAIR)
@@ -723,15 +791,6 @@ struct NsSmall {
   int* status;
 };
 
-__device__ __forceinline__ void ns_st_cluster(uint32_t addr, const float4& v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-}
-__device__ __forceinline__ void ns_st_cluster(uint32_t addr, uint32_t x, uint32_t y) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void ns_st_cluster(uint32_t addr, double v) {
-  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
-}
 // generic writes before it, of this CTA's memory or another's, and products after it
 __device__ __forceinline__ void ns_fence_proxy() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
@@ -889,8 +948,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
       more = 1u;
     }
   };
-  // descriptors take the address within the CTA: the higher bits of a shared address may name the CTA of the cluster, and would
-  // run into the next field
+  // descriptors take the address within the CTA: higher bits, which may name the CTA of the cluster, would run into the next field
   const uint32_t xu = (ag_smem_u32(X) & 0x3FFFFu) >> 4, xl = xu + (plane >> 4), au = (ag_smem_u32(AQ) & 0x3FFFFu) >> 4, al = au + ((2 * NS_GROUP_BYTES) >> 4);
   constexpr int SLICES = NS_SMALL_THREADS / 128;
   const int quarter = warp & 3, slice = warp >> 2, row = quarter * 32 + lane;
@@ -1146,12 +1204,19 @@ int ns_maps(ag_ctx* ctx, NsBuffer& b, int64_t rows, int64_t cols) {
   return rc;
 }
 
-template <int KIND, bool SPLIT, bool PAIR, int BN>
+int ns_tiles(int kind, int M, int N, int BM, int BN) {
+  const int m = (M + BM - 1) / BM, n = (N + BN - 1) / BN;
+  if (!ns_symmetric(kind)) return m * n;
+  if (BM == 256) return n * (n + 1) / 2;
+  return 2 * (n / 2) * (n / 2 + 1) + (n & 1 ? n : 0);  // two columns of 2 j + 2 each, and what an odd number leaves
+}
+
+template <int KIND, bool SPLIT, bool PAIR, int BN, bool ZSPLIT>
 int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int BM = PAIR ? 256 : 128, BN_CTA = PAIR ? BN / 2 : BN;
   constexpr size_t SLOT = (size_t)(TC_BM + BN_CTA) * 256;
   static std::atomic<int> known[AG_MAX_DEVICES];  // 1 + units that are resident at once
-  auto kern = ns_gemm_kernel<KIND, SPLIT, PAIR, BN>;
+  auto kern = ns_gemm_kernel<KIND, SPLIT, PAIR, BN, ZSPLIT>;
   std::atomic<int>& slot = known[ag_dev_slot(ctx)];
   int units = slot.load(std::memory_order_relaxed) - 1;
   cudaLaunchConfig_t cfg = {};
@@ -1159,9 +1224,9 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   cfg.blockDim = dim3(NS_TC_THREADS);
   cfg.dynamicSmemBytes = NS_SMEM_LIMIT;
   cfg.attrs = at;
-  if (PAIR) {
+  if (PAIR || ZSPLIT) {
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.x = PAIR ? 2 : p.cluster;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
@@ -1178,16 +1243,16 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   }
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  p.tiles = ns_symmetric(KIND) ? p.tiles_n * (p.tiles_n + 1) / 2 : p.tiles_m * p.tiles_n;
+  p.tiles = ns_tiles(KIND, p.M, p.N, BM, BN);
   p.chain = SPLIT ? NS_CHAIN_PAIRS : NS_CHAIN_SINGLE;
-  const int chains = (p.k_iters + 2 * p.chain - 1) / (2 * p.chain);
+  const int chains = (p.k_iters + 2 * p.chain - 1) / (2 * p.chain);  // parts of a cluster are whole chains
   if (SPLIT) p.mul *= (float)(1.0 + NS_LOSS * std::max(0.0, ((p.k_real + 15) / 16 - chains) / (double)chains));
   // a slot per accumulator, and two steps' low parts: more slots would be free no earlier
   constexpr int SLOTS = SPLIT ? 2 : std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
   static_assert(NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT <= NS_SMEM_LIMIT && SLOTS >= 2, "operand tiles");
   p.slots = SLOTS;
-  units = std::min<int64_t>(units, (int64_t)p.batch * p.tiles);
-  cfg.gridDim = dim3(PAIR ? 2 * units : units);
+  const int64_t work = (int64_t)p.batch * p.tiles;
+  cfg.gridDim = dim3(ZSPLIT ? work * p.cluster : (PAIR ? 2 : 1) * std::min<int64_t>(units, work));
   cfg.dynamicSmemBytes = NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT;
   cfg.stream = ctx->stream;
   if (ctx->pdl) {
@@ -1201,9 +1266,25 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   return AG_OK;
 }
 
+// Tiles of 256 x 256 on pairs of CTAs or of 128 x 128 on single ones: a round of them takes 7 + 1.15 k or 6 + 0.78 k us for k steps of 64
+// elements with pairs of words (1280 x 1280 alone: 402 us on pairs, 327 on single CTAs; four of them 630 and 737).  Where X X^T
+// leaves most SMs without a tile, clusters share the contraction, four steps or more to each CTA.
 template <int KIND, bool SPLIT>
 int ns_product(ag_ctx* ctx, NsGemm& p) {
-  return p.M > 256 ? ns_launch<KIND, SPLIT, true, 256>(ctx, p) : ns_launch<KIND, SPLIT, false, 128>(ctx, p);
+  const int64_t pairs = (int64_t)p.batch * ns_tiles(KIND, p.M, p.N, 256, 256), singles = (int64_t)p.batch * ns_tiles(KIND, p.M, p.N, 128, 128);
+  const double on_pairs = ag_ceil_div(pairs, ctx->sm_count / 2) * (7.0 + 1.15 * p.k_iters);
+  const double on_singles = ag_ceil_div(singles, ctx->sm_count) * (6.0 + 0.78 * p.k_iters);
+  if (p.M > 256 && on_pairs <= on_singles) return ns_launch<KIND, SPLIT, true, 256, false>(ctx, p);
+  if constexpr (KIND == NS_GRAM) {
+    int z = 8;
+    while (z > 1 && (singles * z > ctx->sm_count || p.k_iters < 4 * z)) z /= 2;
+    if (z > 1) {
+      p.k_each = ((p.k_iters + z - 1) / z + 1) & ~1;
+      p.cluster = z;
+      return ns_launch<KIND, SPLIT, false, 128, true>(ctx, p);
+    }
+  }
+  return ns_launch<KIND, SPLIT, false, 128, false>(ctx, p);
 }
 
 // X[0] -> the factor in X[steps & 1]
@@ -1215,7 +1296,7 @@ int ns_iterate(ag_ctx* ctx, const NsPlan& t, NsGemm& p, NsBuffer* X, NsBuffer& A
     NsBuffer &x = X[i & 1], &y = X[~i & 1];
     auto product = [&](auto kind, const NsMaps& l, const NsMaps& r, NsBuffer& d, int n, int k, double mul, double diag) {
       p.l = l; p.r = r;
-      p.d_hi = d.out_hi; p.d_lo = d.out_lo;
+      p.d_hi = d.out_hi; p.d_lo = d.out_lo; p.D = d.plane;
       p.two = d.plane.lo && (SPLIT || (&d == &y && i + 1 == steps));
       p.N = n; p.k_iters = (k + TC_BK - 1) / TC_BK; p.k_real = k;
       p.mul = (float)mul * unit; p.diag = (float)(diag * NS_SCALE);
