@@ -8,15 +8,17 @@
 //
 // A group of 1 to 32 lanes owns a head: a lane has S slots, a slot two packets that the rotation mixes (columns rot and
 // more are split into two halves in the same way, with nothing to mix), so that statistics and rotation need one read, a
-// few shuffles and no shared memory.  A thread keeps U heads of its token in flight and loads the angles once for all of
-// them.  Packets are as wide as addresses, strides and halves allow, one to four elements: every shape takes the same code.  All
-// sums are fp32.
+// few shuffles and no shared memory.  A thread has one or two heads of a token under way, loads the angles once for them, and goes on to the next
+// token of its turn with the weights in registers.  Packets are as wide as addresses, strides and halves allow, one to four
+// elements: every shape takes the same code.  All sums are fp32.
+// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 114 us, 0.90 of the copy rate; the gradient 165 us, 0.93), instructions
+// with bf16 ones (78 us, 0.66) and with packets of one element (heads of 74 columns: 98 us fp32, 0.61).
 #include "ag_common.cuh"
 
 namespace {
 
 constexpr int QK_THREADS = 256;
-constexpr int QK_BLOCKS_PER_SM = 8;  // of a backward pass, at most: 256 threads each
+constexpr int QK_BLOCKS_PER_SM = 8;  // at most: 256 threads each
 
 // NV values of type T as they lie in memory
 template <int BYTES> struct QkWord;
@@ -126,11 +128,6 @@ __device__ __forceinline__ bool qk_angles(const QkArgs& a, int64_t tok, bool in,
   return ok;
 }
 
-__device__ __forceinline__ float qk_group_sum(float v, int lanes_log2) {
-  for (int o = (1 << lanes_log2) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 template <int S, int NV>
 __device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, int lane, float (&lo)[S][NV], float (&hi)[S][NV]) {
 #pragma unroll
@@ -149,77 +146,84 @@ __device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, in
   }
 }
 
+// A group goes from token to token with its weights in registers
 template <typename T, int NV, int S, int U>
 __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) {
   using P = QkPack<T, NV>;
   ag_pdl_wait();
   ag_pdl_trigger();
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
-  const int64_t tok = (int64_t)blockIdx.x * (QK_THREADS >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
-  const bool in = tok < a.tokens;
+  const int per_block = QK_THREADS >> a.lanes_log2;
   const int which = (int)blockIdx.y >= a.side[0].blocks;
   const QkSide& q = a.side[which];
-  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U;
-  typename P::Raw lo[U][S], hi[U][S];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int k = 0; k < S; ++k) {
-      const int slot = lane + (k << a.lanes_log2);
-      bool turns;
-      int col, apart;
-      qk_columns(a, slot * NV, turns, col, apart);
-      lo[u][k] = hi[u][k] = typename P::Raw{};
-      if (in && slot < a.slots && head + u < q.heads) {
-        const T* x = static_cast<const T*>(q.x) + tok * q.x_stride + (int64_t)(head + u) * a.D + col;
-        lo[u][k] = P::load(x);
-        hi[u][k] = P::load(x + apart);
-      }
-    }
-  float c[S][NV], s[S][NV], glo[S][NV], ghi[S][NV];
-  const bool ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
+  const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U, heads = min(U, q.heads - head);
+  float glo[S][NV], ghi[S][NV];
   qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
-  float sum[U];
+  int col[S], apart[S];
+  bool turns[S];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    sum[u] = 0.0f;
+  for (int k = 0; k < S; ++k) qk_columns(a, (lane + (k << a.lanes_log2)) * NV, turns[k], col[k], apart[k]);
+  const float over = 1.0f / (float)a.D;
+  const int64_t first = (int64_t)blockIdx.x * per_block + (threadIdx.x >> a.lanes_log2), stride = (int64_t)gridDim.x * per_block;
+  const T* x = static_cast<const T*>(q.x) + first * q.x_stride + (int64_t)head * a.D;
+  T* out = static_cast<T*>(q.y) + first * q.y_stride + (int64_t)head * a.D;
+  // all threads of a block make as many turns: the sums are over groups of lanes
+  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += stride) {
+    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
+    const bool in = tok < a.tokens;
+    typename P::Raw xl[U][S], xh[U][S];
 #pragma unroll
-    for (int k = 0; k < S; ++k) {
-      float x[NV], y[NV];
-      P::unpack(lo[u][k], x);
-      P::unpack(hi[u][k], y);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) sum[u] = fmaf(x[i], x[i], fmaf(y[i], y[i], sum[u]));
-    }
-  }
-  for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
-#pragma unroll
-    for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (!in || head + u >= q.heads) continue;
-    const float inv = rsqrtf(sum[u] * (1.0f / (float)a.D) + a.eps);
-#pragma unroll
-    for (int k = 0; k < S; ++k) {
-      const int slot = lane + (k << a.lanes_log2);
-      if (slot >= a.slots) continue;
-      bool turns;
-      int col, apart;
-      qk_columns(a, slot * NV, turns, col, apart);
-      float x[NV], y[NV], xo[NV], yo[NV];
-      P::unpack(lo[u][k], x);
-      P::unpack(hi[u][k], y);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const float xn = x[i] * inv * glo[k][i], yn = y[i] * inv * ghi[k][i], sn = a.sgn * s[k][i];
-        xo[i] = turns ? xn * c[k][i] - yn * sn : xn;
-        yo[i] = turns ? xn * sn + yn * c[k][i] : yn;
-        if (!ok) xo[i] = yo[i] = 0.0f;
+      for (int k = 0; k < S; ++k) {
+        xl[u][k] = xh[u][k] = typename P::Raw{};
+        if (in && u < heads && lane + (k << a.lanes_log2) < a.slots) {
+          xl[u][k] = P::load(x + u * a.D + col[k]);
+          xh[u][k] = P::load(x + u * a.D + col[k] + apart[k]);
+        }
       }
-      T* out = static_cast<T*>(q.y) + tok * q.y_stride + (int64_t)(head + u) * a.D + col;
-      P::store(out, xo);
-      P::store(out + apart, yo);
+    float c[S][NV], s[S][NV];
+    const bool good = qk_angles<S, NV>(a, tok, in, lane, c, s);
+    float sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      sum[u] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        float vx[NV], vy[NV];
+        P::unpack(xl[u][k], vx);
+        P::unpack(xh[u][k], vy);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sum[u] = fmaf(vx[i], vx[i], fmaf(vy[i], vy[i], sum[u]));
+      }
     }
+    for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!in || u >= heads) continue;
+      const float inv = rsqrtf(sum[u] * over + a.eps);
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        if (lane + (k << a.lanes_log2) >= a.slots) continue;
+        float vx[NV], vy[NV];
+        P::unpack(xl[u][k], vx);
+        P::unpack(xh[u][k], vy);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const float xn = vx[i] * inv * glo[k][i], yn = vy[i] * inv * ghi[k][i], sn = a.sgn * s[k][i];
+          vx[i] = turns[k] ? xn * c[k][i] - yn * sn : xn;
+          vy[i] = turns[k] ? xn * sn + yn * c[k][i] : yn;
+          if (!good) vx[i] = vy[i] = 0.0f;
+        }
+        T* d = out + u * a.D + col[k];
+        P::store(d, vx);
+        P::store(d + apart[k], vy);
+      }
+    }
+    x += stride * q.x_stride;
+    out += stride * q.y_stride;
   }
 }
 
@@ -445,25 +449,28 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
   const int gy = a.side[0].blocks + a.side[1].blocks, per_block = QK_THREADS >> sh.lanes_log2;
   AG_REQUIRE(ctx, gy <= 65535, "too many heads");
   int64_t gx = (a.tokens + per_block - 1) / per_block;
+  const size_t smem = BACK && W ? QK_THREADS / 32 * a.D * sizeof(float) : 0;
+  // blocks that are resident at once, with as many turns each
+  static AgOccupancy known[AG_MAX_DEVICES];
+  const auto resident = [&] {
+    int n = 0;
+    cudaError_t e;
+    if constexpr (BACK) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, qk_backward_kernel<T, NV, S, U, W>, QK_THREADS, smem);
+    else e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, qk_forward_kernel<T, NV, S, U>, QK_THREADS, smem);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    return n;
+  };
+  int occ = known[ag_dev_slot(ctx)].get(QK_THREADS, smem, resident);
+  occ = occ < 1 ? 1 : occ > QK_BLOCKS_PER_SM ? QK_BLOCKS_PER_SM : occ;
+  const int64_t most = ctx->sm_count * occ / gy > 0 ? ctx->sm_count * occ / gy : 1, turns = (gx + most - 1) / most;
+  gx = (gx + turns - 1) / turns;
   if constexpr (!BACK) {
     AG_LAUNCH_PDL(ctx, "qk_forward_kernel", (qk_forward_kernel<T, NV, S, U>), dim3((unsigned)gx, gy), QK_THREADS, 0, a);
   } else {
-    // blocks that are resident at once, with as many turns each
-    static AgOccupancy known[AG_MAX_DEVICES];
-    const size_t smem = W ? QK_THREADS / 32 * a.D * sizeof(float) : 0;
-    int occ = known[ag_dev_slot(ctx)].get(QK_THREADS, smem, [&] {
-      int n = 0;
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, qk_backward_kernel<T, NV, S, U, W>, QK_THREADS, smem) != cudaSuccess) {
-        (void)cudaGetLastError();
-        n = 0;
-      }
-      return n;
-    });
-    occ = occ < 1 ? 1 : occ > QK_BLOCKS_PER_SM ? QK_BLOCKS_PER_SM : occ;
-    const int64_t most = ctx->sm_count * occ / gy > 0 ? ctx->sm_count * occ / gy : 1, turns = (gx + most - 1) / most;
-    gx = (gx + turns - 1) / turns;
-    AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS,
-                  smem, a);
+    AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS, smem, a);
     if (W)
       AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), 32 * QK_FOLD_WARPS, 0, a.partials,
                     (int)gx * a.side[0].blocks, (int)gx * a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
@@ -471,12 +478,14 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
   return AG_OK;
 }
 
-template <typename T, int NV, int S, int U>
+// Heads that a thread has under way.  Forward, two where a lane has 16 bytes of a half or fewer, else one (16 x 2048 tokens of 2 x 10 heads of 128:
+// fp32 114 us, 115 with one; bf16 78, 99 with one, 83 with four; fp32 heads of 256 columns 225 with one, 231 with two).  Backward, two where a lane
+// has four fp32 pairs or fewer, else one (the same tokens fp32 165 us against 186 with one; 8192 of 12 + 2 heads bf16 34 against 45
+// with two: their registers leave two blocks to an SM).
+template <typename T, int NV, int S>
 int qk_kind(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
+  constexpr int BYTES = S * NV * (int)sizeof(T), U = BYTES < 32 ? 2 : 1, B = sizeof(T) == 4 && S * NV <= 4 ? 2 : 1;
   if (!back) return qk_launch<T, NV, S, U, false, false>(ctx, a, sh);
-  // backward, heads a thread has: two of fp32, one of bf16 (16 x 2048 tokens of 2 x 10 heads fp32 165 us against 186, 8192 of 12 + 2 bf16 36
-  // against 45: with two, registers leave two blocks to an SM)
-  constexpr int B = sizeof(T) == 4 ? U : 1;
   return w ? qk_launch<T, NV, S, B, true, true>(ctx, a, sh) : qk_launch<T, NV, S, B, true, false>(ctx, a, sh);
 }
 
@@ -485,15 +494,15 @@ int qk_slots(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
   a.lanes_log2 = sh.lanes_log2;
   a.slots = a.D / 2 / NV;
   switch (sh.S) {
-    case 1: return qk_kind<T, NV, 1, 2>(ctx, a, sh, back, w);
-    case 2: return qk_kind<T, NV, 2, 2>(ctx, a, sh, back, w);
-    case 3: return qk_kind<T, NV, 3, 1>(ctx, a, sh, back, w);
-    case 4: return qk_kind<T, NV, 4, 1>(ctx, a, sh, back, w);
+    case 1: return qk_kind<T, NV, 1>(ctx, a, sh, back, w);
+    case 2: return qk_kind<T, NV, 2>(ctx, a, sh, back, w);
+    case 3: return qk_kind<T, NV, 3>(ctx, a, sh, back, w);
+    case 4: return qk_kind<T, NV, 4>(ctx, a, sh, back, w);
   }
   if constexpr (NV < 4) {  // packets of four: 32 lanes of 4 slots hold 1024 columns
-    if (sh.S == 8) return qk_kind<T, NV, 8, 1>(ctx, a, sh, back, w);
+    if (sh.S == 8) return qk_kind<T, NV, 8>(ctx, a, sh, back, w);
     if constexpr (NV == 1)
-      if (sh.S == 16) return qk_kind<T, NV, 16, 1>(ctx, a, sh, back, w);
+      if (sh.S == 16) return qk_kind<T, NV, 16>(ctx, a, sh, back, w);
   }
   AG_FAIL(ctx, AG_ERR_INVALID, "no kernel for heads of %d columns", a.D);
 }
