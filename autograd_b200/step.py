@@ -10,6 +10,9 @@ forward is kept per layer exactly as a real model would keep it (h1, h2 for the 
 backward; u for the GELU backward); everything else rotates through a few transient buffers.
 All transient buffers are larger than the L2 cache, so every pass streams from HBM.
 
+With `qk_norm` the heads of q and k are normalised, weighted and rotated in one pass instead of rotated in place, and the gradients of
+the two weight vectors of every layer join those of the norms.
+
 The step covers: 1 gather, 2L+1 fused (add+)LayerNorm forward and backward, L RoPE(q,k)
 forward and backward, L GELU forward and backward, 1 fused linear+CE forward and backward, 1
 deterministic scatter-add into the tied table, plus the zero-fills of the gradient buffers.
@@ -36,6 +39,7 @@ class StepConfig:
     mlp_ratio: int = 4
     eps: float = 1e-5
     rope_theta: float = 1e5    # module.py:146 (GPT2 uses 100000.0)
+    qk_norm: bool = False      # RMSNorm of every head of q and k before the rotation (no counterpart in the reference)
     ce_precision: int = N.AG_CE_3XTF32
     ce_vocab_chunk: int = 4096
     # Memory that only saves time, in bytes, 0: none.  Logits kept from the head's forward to its backward, where that pays
@@ -110,7 +114,8 @@ class FusedLayerStep:
         self.beta = self._dev((self.n_norms, C), f32, host=bet)
         # gradient buckets (contiguous, so that one allreduce covers each)
         # [dgamma | dbeta] per norm, then the loss scalar: one small allreduce carries all of them
-        self.n_small = self.n_norms * 2 * C
+        # (qk_norm: then [dq_gamma | dk_gamma] per layer)
+        self.n_small = self.n_norms * 2 * C + (2 * L * c.head_dim if c.qk_norm else 0)
         self.small_bucket = self._dev((self.n_small + 4,), f32)
         self.loss = self.small_bucket + self.n_small * 4
         self.dtable = self._dev((V, C), f32)                           # dW_vocab == embedding grad (tied)
@@ -138,6 +143,14 @@ class FusedLayerStep:
         self.du = self._dev((Nn, I), f32)                              # GELU input grad
         self.dh = self._dev((Nn, C), f32)                              # residual-stream gradient
         self.lse = self._dev((Nn,), f32)
+        if c.qk_norm:
+            qk = Nn * c.n_head * c.head_dim
+            self.head_gamma = self._dev((L, 2, c.head_dim), f32, host=np.ones((L, 2, c.head_dim), f32))
+            self.qk_out = [self._dev((qk,), f32) for _ in range(2)]              # what attention reads
+            self.dqk_out = [self._dev((qk,), f32, normal=1.0) for _ in range(2)]  # and its gradients, stand-ins
+            self.dqk = [self._dev((qk,), f32) for _ in range(2)]
+            self.head_partials_bytes = ctx.qk_norm_partials_bytes(c.n_head, c.n_head, c.head_dim)
+            self.head_partials = self._raw(self.head_partials_bytes)
         self.partials_bytes = ctx.norm_partials_bytes(C)
         self.scatter_bytes = ctx.scatter_add_scratch_bytes(Nn, C, V)
         self.scatter = self._raw(self.scatter_bytes)
@@ -229,6 +242,24 @@ class FusedLayerStep:
         return (self.gamma + i * C * 4, self.beta + i * C * 4,
                 self.small_bucket + (2 * i) * C * 4, self.small_bucket + (2 * i + 1) * C * 4)
 
+    def _rotate(self, layer, backward):
+        """q and k on their way to attention, or their gradients on the way back."""
+        ctx, c = self.ctx, self.cfg
+        if not c.qk_norm:
+            ctx.rope_qk(self.q, self.k, self.cos, self.sin, c.batch, c.seq_len, c.n_head, c.n_head, c.head_dim,
+                        sin_sign=+1 if backward else -1)
+            return
+        d, w = c.head_dim, c.n_head * c.head_dim
+        gq = self.head_gamma + layer * 2 * d * 4
+        sizes = (self.N, c.seq_len, c.seq_len, c.n_head, c.n_head, d, d)
+        if backward:
+            dg = self.small_bucket + (self.n_norms * 2 * self.C + layer * 2 * d) * 4
+            ctx.qk_norm_rope_backward(*self.dqk_out, self.q, self.k, gq, gq + d * 4, self.cos, self.sin, 0, *self.dqk, dg, dg + d * 4,
+                                      self.head_partials, self.head_partials_bytes, *sizes, w, w, w, w, w, w, c.eps, sin_sign=-1)
+        else:
+            ctx.qk_norm_rope_forward(self.q, self.k, gq, gq + d * 4, self.cos, self.sin, 0, *self.qk_out, *sizes, w, w, w, w, c.eps,
+                                     sin_sign=-1)
+
     def forward(self):
         ctx, t, c = self.ctx, self.timer, self.cfg
         Nn, C, V, L, I = self.N, self.C, self.V, self.L, self.I
@@ -240,8 +271,7 @@ class FusedLayerStep:
             ctx.add_layernorm_forward(x, self.branch[(2 * l) % 4], g1, b1, self.h1[l], self.y[0], 0, 0, Nn, C, c.eps)
             t.end(k)
             k = t.begin("rope")
-            ctx.rope_qk(self.q, self.k, self.cos, self.sin, c.batch, c.seq_len, c.n_head, c.n_head, c.head_dim,
-                        sin_sign=-1)
+            self._rotate(l, False)
             t.end(k)
             g2, b2, _, _ = self._norm_params(2 * l + 1)
             k = t.begin("ln_fwd")
@@ -300,8 +330,7 @@ class FusedLayerStep:
             self._norm_backward(2 * l + 1, self.dy[1], self.h2[l], self.dh)
             t.end(k)
             k = t.begin("rope")     # backward of RoPE = the transposed rotation on dq, dk
-            ctx.rope_qk(self.q, self.k, self.cos, self.sin, c.batch, c.seq_len, c.n_head, c.n_head, c.head_dim,
-                        sin_sign=+1)
+            self._rotate(l, True)
             t.end(k)
             k = t.begin("ln_bwd")
             self._norm_backward(2 * l, self.dy[l % 2], self.h1[l], self.dh)
@@ -379,7 +408,7 @@ class FusedLayerStep:
             "gather_fwd": 8 * Nn * C,                              # read rows + write out
             "ln_fwd": self.n_norms * 16 * Nn * C,                  # read x, r; write h, y
             "ln_bwd": (self.n_norms * 16 - 4) * Nn * C,            # read dy, h, dres; write dx (first has no dres)
-            "rope": 2 * L * 8 * qk,                                # fwd + bwd: read + write q, k
+            "rope": (20 if self.cfg.qk_norm else 16) * L * qk,     # fwd + bwd: read + write q, k (normalised: their inputs too)
             "gelu_fwd": L * 8 * Nn * I,
             "gelu_bwd": L * 12 * Nn * I,
             "scatter_add": 4 * Nn * C + 8 * min(Nn, V) * C,        # read dOut; read-modify-write touched rows

@@ -75,3 +75,49 @@ def test_projection_heads_loss_gradient_and_step():
     slope = (loss(w + 1e-5 * step) - loss(w - 1e-5 * step)) / 2e-5
     assert abs((got * step).sum() - slope) <= 1e-4 * np.linalg.norm(got) * np.linalg.norm(step)
     check_clean_status()
+
+
+def test_step_with_normalised_heads():
+    """The step's heads against the 64-bit form: outputs, input gradients, the weights' gradients in the bucket that is reduced, the loss
+    behind them; the same result from a recorded step."""
+    from autograd_b200.step import FusedLayerStep, StepConfig
+    ctx, alloc, be = env()
+    cfg = StepConfig(n_layer=2, n_embd=64, n_head=2, head_dim=32, seq_len=24, vocab=128, batch=2, qk_norm=True)
+    plain = FusedLayerStep(ctx, alloc, be, StepConfig(**{**cfg.__dict__, "qk_norm": False}))
+    step = FusedLayerStep(ctx, alloc, be, cfg)
+    n, h, d, c = cfg.tokens, cfg.n_head, cfg.head_dim, cfg.n_embd
+    rng = np.random.default_rng(0)
+    ids = rng.integers(0, cfg.vocab, (2, n)).astype(np.int32)
+    gamma = (1 + 0.3 * rng.standard_normal((2, 2, d))).astype(np.float32)
+    ctx.copy_from_host(step.head_gamma, gamma)
+    for s in (plain, step):
+        ctx.copy_from_host(s.ids, ids[0])
+        ctx.copy_from_host(s.targets, ids[1])
+
+    def read(address, *shape):
+        return ctx.copy_to_host(address, shape, np.float32)
+    cos, sin = read(step.cos, cfg.seq_len, d // 2), read(step.sin, cfg.seq_len, d // 2)
+    at = np.arange(n) % cfg.seq_len
+    results = []
+    for _ in range(3):
+        step.step()
+        results.append([read(a, n, h, d) for a in (*step.qk_out, *step.dqk)] + [read(step.small_bucket, step.n_small + 1)])
+    assert all(np.array_equal(a, b) for r in results[1:] for a, b in zip(results[0], r))
+    plain.step()
+    *heads, small = results[0]
+    assert step.n_small == plain.n_small + 2 * 2 * d and small[-1] == plain.read_loss()
+    assert np.array_equal(small[:plain.n_small], read(plain.small_bucket, plain.n_small))
+    for layer in range(2):
+        for side, x in enumerate((step.q, step.k)):
+            x, dy = read(x, n, h, d), read(step.dqk_out[side], n, h, d)
+            dx, dgamma = R.heads_backward(dy, x, gamma[layer, side], cos[at], -sin[at], cfg.eps)
+            got = small[plain.n_small + (2 * layer + side) * d:][:d]
+            assert np.abs(got - dgamma).max() <= 1e-5 * np.abs(dgamma).max() + 1e-5
+            if layer == 1:   # the last forward pass
+                ref = R.heads(x, gamma[layer, side], cos[at], -sin[at], cfg.eps)
+                assert np.abs(heads[side] - ref).max() <= 1e-5 * np.abs(ref).max()
+            else:            # the last backward pass
+                assert np.abs(heads[2 + side] - dx).max() <= 1e-5 * np.abs(dx).max()
+    check_clean_status()
+    plain.close()
+    step.close()
