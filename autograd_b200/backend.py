@@ -705,7 +705,8 @@ class CudaBackend:
     def qk_norm_rope_backward(self, dq_out, dk_out, q, k, cos, sin, dq, dk, eps, q_gamma=None, k_gamma=None, dq_gamma=None,
                               dk_gamma=None, positions=None, sin_sign=1, accumulate=False, dq_out_stride=None, dk_out_stride=None,
                               q_stride=None, k_stride=None, dq_stride=None, dk_stride=None, scratch=None):
-        """dq, dk = gradients (added to them with accumulate); dq_gamma, dk_gamma += theirs.  q, k: the forward's inputs; dq may be
+        """dq, dk = gradients (added to them with accumulate); dq_gamma, dk_gamma += theirs (the same
+        tensor: both).  q, k: the forward's inputs; dq may be
         dq_out or q, with its stride."""
         tokens, seq, rows, h, hkv, d, rot, dtype, positions = self._heads(q, k, cos, sin, positions, q_gamma, k_gamma, (dq_out, dq),
                                                                           (dk_out, dk))

@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
   }
 }
 
-// dgamma += the partial rows of its side: those of queries are the first.  A block has 32 columns of one side, its warps take rows in
+// dgamma += the partial rows of its side: those of queries are the first (one weight for both sides: all rows are its).  A block has 32 columns of one side, its warps take rows in
 // turn, eight under way each (one at a time, of eight warps, took 72 us for 1183 rows of 128).
 constexpr int QK_FOLD_WARPS = 32;
 __global__ void __launch_bounds__(32 * QK_FOLD_WARPS) qk_fold_kernel(const float* __restrict__ partials, int q_rows, int k_rows, int D,
@@ -471,9 +471,12 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
     AG_LAUNCH_PDL(ctx, "qk_forward_kernel", (qk_forward_kernel<T, NV, S, U>), dim3((unsigned)gx, gy), QK_THREADS, 0, a);
   } else {
     AG_LAUNCH_PDL(ctx, "qk_backward_kernel", (qk_backward_kernel<T, NV, S, U, W>), dim3((unsigned)gx, gy), QK_THREADS, smem, a);
-    if (W)
-      AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, 2), 32 * QK_FOLD_WARPS, 0, a.partials,
-                    (int)gx * a.side[0].blocks, (int)gx * a.side[1].blocks, a.D, a.side[0].dgamma, a.side[1].dgamma);
+    if (W) {
+      const int q_rows = (int)gx * a.side[0].blocks, k_rows = (int)gx * a.side[1].blocks;
+      const bool one = a.side[0].dgamma == a.side[1].dgamma;
+      AG_LAUNCH_PDL(ctx, "qk_fold_kernel", qk_fold_kernel, dim3((a.D + 31) / 32, one ? 1 : 2), 32 * QK_FOLD_WARPS, 0, a.partials,
+                    one ? q_rows + k_rows : q_rows, k_rows, a.D, a.side[0].dgamma, a.side[1].dgamma);
+    }
   }
   return AG_OK;
 }
@@ -557,6 +560,9 @@ int qk_check(ag_ctx* ctx, const char* name, const QkArgs& a, int seq, int rot, f
                         (((uintptr_t)q.gamma | (uintptr_t)q.dgamma) & 3) == 0, "%s: misaligned pointer", name);
   }
   AG_REQUIRE(ctx, (((uintptr_t)a.cos_tab | (uintptr_t)a.sin_tab | (uintptr_t)a.positions) & 3) == 0, "%s: misaligned table", name);
+  const uintptr_t dg[2] = {(uintptr_t)a.side[0].dgamma, (uintptr_t)a.side[1].dgamma}, wide = (uintptr_t)a.D * 4;
+  AG_REQUIRE(ctx, !dg[0] || !dg[1] || dg[0] == dg[1] || dg[0] + wide <= dg[1] || dg[1] + wide <= dg[0],
+             "%s: the weights' gradients overlap", name);
   // an output may be one of its own side's inputs, row by row; otherwise it shares nothing with any operand
   for (int i = 0; i < 2; ++i) {
     const QkSide& q = a.side[i];

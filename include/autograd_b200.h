@@ -358,7 +358,8 @@ int ag_distill_forward_backward(ag_ctx* ctx, const void* logits, int64_t ld, con
  * with HKV heads and the outputs.  q or k may be NULL (with everything of its own).  An output may be its own input, with
  * the same stride; it overlaps no other operand.
  * backward: with w = R^T dy and v = gamma * w: dx = inv (v - x inv^2 mean(v x)), added to dq and dk with `accumulate`, else
- * written; dgamma += sum over tokens and heads of w x inv in a fixed order, either may be NULL; they need
+ * written; dgamma += sum over tokens and heads of w x inv in a fixed order, either may be NULL, and
+ * both may be the same, which then gets both sums (one weight for queries and keys); they need
  * ag_qk_norm_partials_bytes (heads as in the call, 0 for a NULL side) of partials, 4-byte aligned.  q and k are the forward's
  * inputs.  dq may be dq_out or q, with the same stride. */
 #define AG_QK_MAX_D 1024

@@ -236,6 +236,36 @@ def test_in_place_and_by_the_backend(dtype):
     free(packed, saved, dgamma, c, s, gq, gk)
 
 
+@pytest.mark.parametrize("n,h,kv,d", [(1, 1, 1, 8), (600, 6, 2, 128), (37, 3, 3, 74)])
+def test_one_weight_for_queries_and_keys(n, h, kv, d):
+    """Its gradient is the sum of both sides', many times over the same."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(n)
+    x = [inputs(rng, n, heads, d, "f32").reshape(1, n, heads, d) for heads in (h, kv)]
+    dy = [rng.standard_normal(t.shape).astype(np.float32) for t in x]
+    cos, sin = tables(n, d)
+    gamma = (1 + 0.3 * rng.standard_normal(d)).astype(np.float32)
+    c, s, g, q, k, dq, dk, ox, ok = (up(t) for t in (cos, sin, gamma, *x, *dy, *(np.zeros_like(t) for t in x)))
+    ref, bound = np.ones(d), U * np.ones(d)
+    for t, dyt in zip(x, dy):
+        dgamma = R.heads_backward(dyt[0], t[0], gamma, cos, sin, EPS)[1]
+        y = t[0].astype(np.float64)
+        inv = 1 / np.sqrt(np.mean(y * y, -1, keepdims=True) + EPS)
+        ref = ref + dgamma
+        bound = bound + (n * (h + kv) + 32) * U * (partner(dyt[0].astype(np.float64), d) * np.abs(y) * inv).reshape(-1, d).sum(0)
+    first = None
+    for _ in range(20):
+        dg = up(np.ones(d, np.float32))
+        be.qk_norm_rope_backward(dq, dk, q, k, c, s, ox, ok, EPS, q_gamma=g, k_gamma=g, dq_gamma=dg, dk_gamma=dg)
+        got = be.copy_to_host(dg)
+        near(got.astype(np.float64), ref, bound + U * np.abs(ref), "f32", "dgamma")
+        first = got if first is None else first
+        assert np.array_equal(got, first)
+        free(dg)
+    check_clean_status()
+    free(c, s, g, q, k, dq, dk, ox, ok)
+
+
 @pytest.mark.parametrize("only", ["q", "k"])
 def test_one_side_alone(only):
     ctx, alloc, be = env()

@@ -103,7 +103,9 @@ REFUSED = (
     [("ag_qk_norm_rope_backward", c) for c in (
         dict(dq=0), dict(dk=0), dict(dq_out=0), dict(dk_out=0), dict(dq_stride=63), dict(dq_out_stride=63), dict(dq=BASE + 4),
         dict(dq=BASE + 6 * FAR), dict(dk=BASE + 3 * FAR), dict(dq=BASE + 5 * FAR, dq_stride=70), dict(dq_gamma=BASE + 8 * FAR),
-        dict(dq_gamma=BASE + 8 * FAR + 2, partials=BASE + 9 * FAR, bytes=1 << 20), dict(dk_gamma=BASE + 8 * FAR, partials=BASE + 9 * FAR + 2, bytes=1 << 20))] +
+        dict(dq_gamma=BASE + 8 * FAR + 2, partials=BASE + 9 * FAR, bytes=1 << 20), dict(dk_gamma=BASE + 8 * FAR, partials=BASE + 9 * FAR + 2, bytes=1 << 20),
+        dict(dq_gamma=BASE + 8 * FAR, dk_gamma=BASE + 8 * FAR + 60, partials=BASE + 9 * FAR, bytes=1 << 24),
+        dict(dq_gamma=BASE + 8 * FAR + 60, dk_gamma=BASE + 8 * FAR, partials=BASE + 9 * FAR, bytes=1 << 24))] +
     [(n, c) for n in NS for c in (
         dict(ctx=0), dict(count=-1), dict(rows=0), dict(cols=-3), dict(rows=16385, cols=16385), dict(rows=2, cols=(1 << 20) + 1),
         dict(rows=16384, cols=1 << 17), dict(steps=-1), dict(steps=33), dict(coefficients=None), dict(eps=0.0), dict(eps=-1.0), dict(eps=NAN),
