@@ -919,6 +919,8 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
     }
   }
   ns_fence_proxy();
+  // without steps nothing else stands between what a CTA reads and what another may write in its place (narrower words)
+  if (p.steps == 0) cluster_sync();
   __syncthreads();
 
   // ---- the steps
@@ -1529,9 +1531,10 @@ int ns_check_ranges(ag_ctx* ctx, const char* name, const void* const* p, size_t 
     r[n++] = {(uintptr_t)at, (uintptr_t)at + bytes, written};
   };
   for (int i = 0; i < count; ++i) {
-    add(p[i], elements * p_size, true);
+    const bool in_place = !m && g[i] == p[i] && g_size >= p_size;  // the factor may take its matrix's place
+    add(p[i], elements * (in_place ? g_size : p_size), true);
     if (m) add(m[i], elements * 4, true);
-    if (m || g[i] != p[i] || g_size < p_size) add(g[i], elements * g_size, false);  // the factor may take its matrix's place
+    if (!in_place) add(g[i], elements * g_size, false);
   }
   add(scratch, scratch_bytes, true);
   const bool apart = ns_apart(r, n);

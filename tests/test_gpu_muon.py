@@ -104,6 +104,31 @@ def test_factor(shape, dtype, out, precision):
 
 
 @PRECISIONS
+@pytest.mark.parametrize("steps", [0, 1, 5])
+@pytest.mark.parametrize("shape", [(2, 64, 256), (1, 300, 20), (2, 5, 9), (2, 130, 140)], ids=lambda s: "x".join(map(str, s)))
+def test_narrower_words_in_the_matrix_place(shape, steps, precision):
+    """bf16 factors begin where their fp32 matrices do: what a CTA writes is what others read."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(sum(shape) + steps)
+    g = gradient(rng, *shape)
+    n = shape[1] * shape[2]
+    for _ in range(10):
+        a = Matrices(g, apart=True)
+        outs = []
+        for t in a.tensors:
+            o = hg.HostTensor(shape[1:], np.uint16, requires_grad=False)
+            o.storage = alloc.view(t.storage, 0, shape[1:], np.uint16)
+            outs.append(o)
+        be.orthogonalise(a.argument, outs, steps=steps, precision=precision)
+        for i, whole in enumerate(a.buffers):
+            words = np.asarray(be.copy_to_host(whole)).view(np.uint16)
+            close(bf16_bits_to_f32(words[:n].copy()).reshape(shape[1:]).astype(np.float64), g[i], precision, steps, out="bf16")
+            assert np.array_equal(words[n:2 * n], np.ascontiguousarray(g[i]).reshape(-1).view(np.uint16)[n:]), "more than the factor was written"
+        a.free()
+    check_clean_status()
+
+
+@PRECISIONS
 @pytest.mark.parametrize("steps,coefficients", [(0, R.NEWTON_SCHULZ), (1, R.NEWTON_SCHULZ), (2, (1.5, -0.5, 0.0)), (3, (2.0, -1.5, 0.5)),
                                                 (3, [(8.2, -23.0, 16.5), (4.0, -2.9, 0.55), (1.9, -1.25, 0.4)])])
 def test_steps_and_coefficients(steps, coefficients, precision):

@@ -118,7 +118,9 @@ REFUSED = (
     [("ag_orthogonalise", c) for c in (
         dict(out=None), dict(out_dtype=5), dict(out=_addresses(BASE + 1)), dict(out=_array(ctypes.c_void_p, [BASE, BASE + 2396, BASE + FAR // 2])),
         dict(out=_array(ctypes.c_void_p, [BASE, BASE, BASE + FAR // 2])), dict(out=_addresses(BASE + FAR), dtype=1),
-        dict(g=_addresses(BASE + 4)), dict(g=_array(ctypes.c_void_p, [BASE + (1 << 20), BASE, BASE + FAR])))] +
+        dict(g=_addresses(BASE + 4)), dict(g=_array(ctypes.c_void_p, [BASE + (1 << 20), BASE, BASE + FAR])),
+        # a factor of 16-bit words in its matrix's place, and another one in what is left of it
+        dict(g=_array(ctypes.c_void_p, [BASE, BASE + 2400, BASE + FAR]), out=_array(ctypes.c_void_p, [BASE, BASE + 1200, BASE + FAR]), out_dtype=1))] +
     [("ag_muon_step", c) for c in (
         dict(p=None), dict(m=None), dict(lr=NAN), dict(lr=INF), dict(momentum=-0.1), dict(momentum=1.1), dict(momentum=NAN), dict(decay=INF),
         dict(scale=NAN), dict(grad_scale=INF), dict(m=_addresses(BASE)), dict(m=_addresses(BASE + FAR)), dict(g=_addresses(BASE)),
