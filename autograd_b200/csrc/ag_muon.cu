@@ -692,6 +692,9 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
+  // after a wait that ran out: copies under way land before this CTA's memory is someone else's (0.2 ms are a hundred times what one takes)
+  if (warp == 0 && lane == 0 && *abort_flag)
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
   tc_fence_before();
   if (PAIR || ZSPLIT) tc_cluster_sync(); else __syncthreads();
   if (warp == 1) {
