@@ -11,14 +11,41 @@
 // few shuffles and no shared memory.  A thread has one or two heads of a token under way, loads the angles once for them, and goes on to the next
 // token of its turn with the weights in registers.  Packets are as wide as addresses, strides and halves allow, one to four
 // elements: every shape takes the same code.  All sums are fp32.
-// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 114 us, 0.90 of the copy rate; the gradient 165 us, 0.93), instructions
-// with bf16 ones (78 us, 0.66) and with packets of one element (heads of 74 columns: 98 us fp32, 0.61).
+// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 108 us, 0.95 of the copy rate; the gradient 169 us, 0.91), instructions
+// with bf16 ones (73 us, 0.70; the gradient 117 us, 0.66) and with packets of one element (heads of 74 columns: 93 us fp32, 0.64).
+#include <type_traits>
+
 #include "ag_common.cuh"
 
 namespace {
 
 constexpr int QK_THREADS = 256;
 constexpr int QK_BLOCKS_PER_SM = 8;  // at most: 256 threads each
+
+// One fp32 number, or two that arithmetic takes at once: bf16 rows, whose time is that of the instructions (gradient of 8192 tokens of 12 + 2
+// heads 34 -> 27 us; fp32 rows are bound by memory and lost 3 % with pairs, 114 -> 119 us for 16 x 2048 tokens of 2 x 10 heads).
+struct QkOne {
+  float v;
+  __device__ __forceinline__ static QkOne make(float a, float = 0.0f) { return {a}; }
+  __device__ __forceinline__ void get(float& a, float&) const { a = v; }
+  __device__ __forceinline__ float sum() const { return v; }
+};
+struct QkTwo {
+  uint64_t v;
+  __device__ __forceinline__ static QkTwo make(float a, float b) { return {ag_pair(a, b)}; }
+  __device__ __forceinline__ void get(float& a, float& b) const { ag_unpair(v, a, b); }
+  __device__ __forceinline__ float sum() const {
+    float a, b;
+    get(a, b);
+    return a + b;
+  }
+};
+__device__ __forceinline__ QkOne qk_mul(QkOne a, QkOne b) { return {a.v * b.v}; }
+__device__ __forceinline__ QkOne qk_add(QkOne a, QkOne b) { return {a.v + b.v}; }
+__device__ __forceinline__ QkOne qk_fma(QkOne a, QkOne b, QkOne c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ QkTwo qk_mul(QkTwo a, QkTwo b) { return {ag_mul2(a.v, b.v)}; }
+__device__ __forceinline__ QkTwo qk_add(QkTwo a, QkTwo b) { return {ag_add2(a.v, b.v)}; }
+__device__ __forceinline__ QkTwo qk_fma(QkTwo a, QkTwo b, QkTwo c) { return {ag_fma2(a.v, b.v, c.v)}; }
 
 // NV values of type T as they lie in memory
 template <int BYTES> struct QkWord;
@@ -27,41 +54,83 @@ template <> struct QkWord<4> { using Raw = uint32_t; };
 template <> struct QkWord<8> { using Raw = uint2; };
 template <> struct QkWord<16> { using Raw = uint4; };
 
+// and as numbers: N of E, TWO in each or one
 template <typename T, int NV>
-struct QkPack {
-  using Raw = typename QkWord<sizeof(T) * NV>::Raw;
-  union Bits {
-    Raw raw;
-    T v[NV];
-    __device__ Bits() {}
-  };
-  __device__ __forceinline__ static Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
-  __device__ __forceinline__ static void unpack(const Raw& r, float (&f)[NV]) {
-    Bits b;
-    b.raw = r;
+struct QkVec {
+  static constexpr bool TWO = NV > 1 && sizeof(T) == 2;
+  using E = std::conditional_t<TWO, QkTwo, QkOne>;
+  static constexpr int N = TWO ? NV / 2 : NV;
+  E e[N];
+  __device__ __forceinline__ void fill(float x) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = Pack<T>::load1(&b.v[i]);
-  }
-  __device__ __forceinline__ static void store(T* p, const float (&f)[NV]) {
-    Bits b;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) Pack<T>::store1(&b.v[i], f[i]);
-    *reinterpret_cast<Raw*>(p) = b.raw;
+    for (int i = 0; i < N; ++i) e[i] = E::make(x, x);
   }
 };
 
-template <int NV>
-__device__ __forceinline__ void qk_load_f32(const float* p, float (&f)[NV]) {
+template <typename T, int NV>
+struct QkPack {
+  using Raw = typename QkWord<sizeof(T) * NV>::Raw;
+  using V = QkVec<T, NV>;
+  union Bits {
+    Raw raw;
+    uint16_t half[sizeof(T) * NV / 2];
+    uint32_t word[sizeof(T) * NV >= 4 ? sizeof(T) * NV / 4 : 1];
+    __device__ Bits() {}
+  };
+  __device__ __forceinline__ static Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  // What is read or written once leaves the cache first (114 -> 108 us forward for the tokens above, fp32), but for narrow packets, whose
+  // neighbours read the same sectors again (93 us against 99 with heads of 74 columns)
+  __device__ __forceinline__ static Raw load_once(const T* p) {
+    if constexpr (NV >= 4) return __ldcs(reinterpret_cast<const Raw*>(p));
+    else return load(p);
+  }
+  __device__ __forceinline__ static void unpack(const Raw& r, V& f) {
+    Bits b;
+    b.raw = r;
+#pragma unroll
+    for (int i = 0; i < V::N; ++i) {
+      if constexpr (sizeof(T) == 4) f.e[i] = V::E::make(__uint_as_float(b.word[i]));
+      else if constexpr (NV == 1) f.e[i] = V::E::make(__uint_as_float((uint32_t)b.half[0] << 16));
+      else f.e[i] = V::E::make(__uint_as_float(b.word[i] << 16), __uint_as_float(b.word[i] & 0xffff0000u));
+    }
+  }
+  template <bool ONCE>
+  __device__ __forceinline__ static void store(T* p, const V& f) {
+    Bits b;
+#pragma unroll
+    for (int i = 0; i < V::N; ++i) {
+      float x, y = 0.0f;
+      f.e[i].get(x, y);
+      if constexpr (sizeof(T) == 4) {
+        b.word[i] = __float_as_uint(x);
+      } else if constexpr (NV == 1) {
+        b.half[0] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        b.word[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    if constexpr (NV >= 4 && ONCE) __stcs(reinterpret_cast<Raw*>(p), b.raw);
+    else *reinterpret_cast<Raw*>(p) = b.raw;
+  }
+};
+
+template <typename T, int NV>
+__device__ __forceinline__ void qk_load_f32(const float* p, QkVec<T, NV>& f) {
+  using V = QkVec<T, NV>;
+  float v[NV];
   if constexpr (NV >= 4) {
 #pragma unroll
     for (int i = 0; i < NV; i += 4) {
       const float4 t = __ldg(reinterpret_cast<const float4*>(p + i));
-      f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
+      v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = __ldg(p + i);
+    for (int i = 0; i < NV; ++i) v[i] = __ldg(p + i);
   }
+#pragma unroll
+  for (int i = 0; i < V::N; ++i) f.e[i] = V::TWO ? V::E::make(v[2 * i % NV], v[(2 * i + 1) % NV]) : V::E::make(v[i], 0.0f);
 }
 
 // Queries or keys.  Rows of a token are `*_stride` elements apart, its heads follow one another.
@@ -104,13 +173,29 @@ __device__ __forceinline__ void qk_columns(const QkArgs& a, int first, bool& tur
   apart = turns ? a.half : (a.D >> 1) - a.half;
 }
 
-template <int S, int NV>
-__device__ __forceinline__ bool qk_angles(const QkArgs& a, int64_t tok, bool in, int lane, float (&c)[S][NV], float (&s)[S][NV]) {
-  int pos = 0;
+// The row of the tables of the token that a group has, which goes `stride` tokens on: no division on the way
+struct QkTurn {
+  uint32_t pos, step;
+  __device__ __forceinline__ QkTurn(const QkArgs& a, int64_t first, int64_t stride) {
+    pos = step = 0;
+    if (a.half && !a.positions) {
+      pos = (uint32_t)first % (uint32_t)a.seq;  // both are below 2^32: there are fewer than 2^31 tokens
+      step = (uint32_t)stride % (uint32_t)a.seq;
+    }
+  }
+  __device__ __forceinline__ void next(const QkArgs& a) {
+    pos += step;  // both below seq, which is below 2^31
+    if (pos >= (uint32_t)a.seq) pos -= (uint32_t)a.seq;
+  }
+};
+
+// Cosines, and sines with the direction's sign, of a token; 1 and 0 for columns that do not turn.  False: a bad position
+template <typename T, int S, int NV>
+__device__ __forceinline__ bool qk_angles(const QkArgs& a, int64_t tok, uint32_t pos, bool in, int lane, QkVec<T, NV> (&c)[S], QkVec<T, NV> (&s)[S]) {
   bool ok = true;
-  if (in && a.half) {
-    pos = a.positions ? a.positions[tok] : (int)((uint32_t)tok % (uint32_t)a.seq);
-    ok = (uint32_t)pos < (uint32_t)a.rows;
+  if (in && a.half && a.positions) {
+    pos = (uint32_t)a.positions[tok];
+    ok = pos < (uint32_t)a.rows;
     if (!ok && lane == 0) atomicOr(a.status, AG_STATUS_BAD_INDEX);
     if (!ok) pos = 0;
   }
@@ -118,18 +203,18 @@ __device__ __forceinline__ bool qk_angles(const QkArgs& a, int64_t tok, bool in,
   for (int k = 0; k < S; ++k) {
     const int first = (lane + (k << a.lanes_log2)) * NV;
     if (in && first < a.half) {
-      qk_load_f32<NV>(a.cos_tab + (int64_t)pos * a.half + first, c[k]);
-      qk_load_f32<NV>(a.sin_tab + (int64_t)pos * a.half + first, s[k]);
+      qk_load_f32<T, NV>(a.cos_tab + (int64_t)pos * a.half + first, c[k]);
+      qk_load_f32<T, NV>(a.sin_tab + (int64_t)pos * a.half + first, s[k]);
     } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) { c[k][i] = 1.0f; s[k][i] = 0.0f; }
+      c[k].fill(1.0f);
+      s[k].fill(0.0f);
     }
   }
   return ok;
 }
 
-template <int S, int NV>
-__device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, int lane, float (&lo)[S][NV], float (&hi)[S][NV]) {
+template <typename T, int S, int NV>
+__device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, int lane, QkVec<T, NV> (&lo)[S], QkVec<T, NV> (&hi)[S]) {
 #pragma unroll
   for (int k = 0; k < S; ++k) {
     const int slot = lane + (k << a.lanes_log2);
@@ -137,11 +222,11 @@ __device__ __forceinline__ void qk_gamma(const QkArgs& a, const float* gamma, in
     int col, apart;
     qk_columns(a, slot * NV, turns, col, apart);
     if (gamma && slot < a.slots) {
-      qk_load_f32<NV>(gamma + col, lo[k]);
-      qk_load_f32<NV>(gamma + col + apart, hi[k]);
+      qk_load_f32<T, NV>(gamma + col, lo[k]);
+      qk_load_f32<T, NV>(gamma + col + apart, hi[k]);
     } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) lo[k][i] = hi[k][i] = 1.0f;
+      lo[k].fill(1.0f);
+      hi[k].fill(1.0f);
     }
   }
 }
@@ -157,8 +242,10 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
   const int which = (int)blockIdx.y >= a.side[0].blocks;
   const QkSide& q = a.side[which];
   const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U, heads = min(U, q.heads - head);
-  float glo[S][NV], ghi[S][NV];
-  qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
+  using V = QkVec<T, NV>;
+  using E = typename V::E;
+  V glo[S], ghi[S];
+  qk_gamma<T, S, NV>(a, q.gamma, lane, glo, ghi);
   int col[S], apart[S];
   bool turns[S];
 #pragma unroll
@@ -167,6 +254,8 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
   const int64_t first = (int64_t)blockIdx.x * per_block + (threadIdx.x >> a.lanes_log2), stride = (int64_t)gridDim.x * per_block;
   const T* x = static_cast<const T*>(q.x) + first * q.x_stride + (int64_t)head * a.D;
   T* out = static_cast<T*>(q.y) + first * q.y_stride + (int64_t)head * a.D;
+  QkTurn turn(a, first, stride);
+  const E sign = E::make(a.sgn, a.sgn), minus = E::make(-a.sgn, -a.sgn);
   // all threads of a block make as many turns: the sums are over groups of lanes
   for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += stride) {
     const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
@@ -178,24 +267,26 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
       for (int k = 0; k < S; ++k) {
         xl[u][k] = xh[u][k] = typename P::Raw{};
         if (in && u < heads && lane + (k << a.lanes_log2) < a.slots) {
-          xl[u][k] = P::load(x + u * a.D + col[k]);
-          xh[u][k] = P::load(x + u * a.D + col[k] + apart[k]);
+          xl[u][k] = P::load_once(x + u * a.D + col[k]);
+          xh[u][k] = P::load_once(x + u * a.D + col[k] + apart[k]);
         }
       }
-    float c[S][NV], s[S][NV];
-    const bool good = qk_angles<S, NV>(a, tok, in, lane, c, s);
+    V c[S], s[S];
+    const bool good = qk_angles<T, S, NV>(a, tok, turn.pos, in, lane, c, s);
+    turn.next(a);
     float sum[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      sum[u] = 0.0f;
+      E all = E::make(0.0f, 0.0f);
 #pragma unroll
       for (int k = 0; k < S; ++k) {
-        float vx[NV], vy[NV];
+        V vx, vy;
         P::unpack(xl[u][k], vx);
         P::unpack(xh[u][k], vy);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) sum[u] = fmaf(vx[i], vx[i], fmaf(vy[i], vy[i], sum[u]));
+        for (int i = 0; i < V::N; ++i) all = qk_fma(vx.e[i], vx.e[i], qk_fma(vy.e[i], vy.e[i], all));
       }
+      sum[u] = all.sum();
     }
     for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
 #pragma unroll
@@ -204,22 +295,33 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
     for (int u = 0; u < U; ++u) {
       if (!in || u >= heads) continue;
       const float inv = rsqrtf(sum[u] * over + a.eps);
+      const E by = E::make(inv, inv);
 #pragma unroll
       for (int k = 0; k < S; ++k) {
         if (lane + (k << a.lanes_log2) >= a.slots) continue;
-        float vx[NV], vy[NV];
+        V vx, vy;
         P::unpack(xl[u][k], vx);
         P::unpack(xh[u][k], vy);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const float xn = vx[i] * inv * glo[k][i], yn = vy[i] * inv * ghi[k][i], sn = a.sgn * s[k][i];
-          vx[i] = turns[k] ? xn * c[k][i] - yn * sn : xn;
-          vy[i] = turns[k] ? xn * sn + yn * c[k][i] : yn;
-          if (!good) vx[i] = vy[i] = 0.0f;
+        for (int i = 0; i < V::N; ++i) {
+          vx.e[i] = qk_mul(qk_mul(vx.e[i], by), glo[k].e[i]);
+          vy.e[i] = qk_mul(qk_mul(vy.e[i], by), ghi[k].e[i]);
+        }
+        if (turns[k]) {
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) {
+            const E xn = vx.e[i], yn = vy.e[i];
+            vx.e[i] = qk_fma(xn, c[k].e[i], qk_mul(yn, qk_mul(s[k].e[i], minus)));
+            vy.e[i] = qk_fma(yn, c[k].e[i], qk_mul(xn, qk_mul(s[k].e[i], sign)));
+          }
+        }
+        if (!good) {
+          vx.fill(0.0f);
+          vy.fill(0.0f);
         }
         T* d = out + u * a.D + col[k];
-        P::store(d, vx);
-        P::store(d + apart[k], vy);
+        P::template store<true>(d, vx);
+        P::template store<true>(d + apart[k], vy);
       }
     }
     x += stride * q.x_stride;
@@ -228,10 +330,11 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(const QkArgs a) 
 }
 
 // W: the gradients of the weights are wanted (of either side).  A group goes from token to token, with the sums of its columns in
-// registers.  What keeps memory busy is blocks, not packets a token ahead: with those, registers leave half of the blocks (187 us instead of 165 for 16 x
-// 2048 tokens of 2 x 10 heads fp32, 40 instead of 36 for 8192 of 12 + 2 bf16).
+// registers.  What keeps memory busy is blocks, not packets a token ahead: with those, registers leave half of the blocks (187 us
+// instead of 165 for 16 x 2048 tokens of 2 x 10 heads fp32).  bf16 rows get three or two blocks to an SM by the bound on registers (heads of 80 columns, 40 of
+// which rotate, S = 3: 188 -> 92 us); fp32 ones that many by themselves, and three are too many (177 us), as is a hint that they leave the cache.
 template <typename T, int NV, int S, int U, bool W>
-__global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a) {
+__global__ void __launch_bounds__(QK_THREADS, sizeof(T) == 4 || S * NV > 12 ? 1 : S == 1 ? 3 : 2) qk_backward_kernel(const QkArgs a) {
   using P = QkPack<T, NV>;
   extern __shared__ float qk_smem[];  // W: [warps][D]
   ag_pdl_wait();
@@ -241,27 +344,37 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
   const int which = (int)blockIdx.y >= a.side[0].blocks;
   const QkSide& q = a.side[which];
   const int head = ((int)blockIdx.y - (which ? a.side[0].blocks : 0)) * U, heads = min(U, q.heads - head);
-  float glo[S][NV], ghi[S][NV];
-  qk_gamma<S, NV>(a, q.gamma, lane, glo, ghi);
+  using V = QkVec<T, NV>;
+  using E = typename V::E;
+  V glo[S], ghi[S];
+  qk_gamma<T, S, NV>(a, q.gamma, lane, glo, ghi);
   int col[S], apart[S];
   bool turns[S];
 #pragma unroll
   for (int k = 0; k < S; ++k) qk_columns(a, (lane + (k << a.lanes_log2)) * NV, turns[k], col[k], apart[k]);
-  float dlo[W ? S : 1][NV], dhi[W ? S : 1][NV];
+  V dlo[W ? S : 1], dhi[W ? S : 1];
 #pragma unroll
-  for (int k = 0; k < (W ? S : 1); ++k)
-#pragma unroll
-    for (int i = 0; i < NV; ++i) dlo[k][i] = dhi[k][i] = 0.0f;
+  for (int k = 0; k < (W ? S : 1); ++k) {
+    dlo[k].fill(0.0f);
+    dhi[k].fill(0.0f);
+  }
   const float over = 1.0f / (float)a.D;
   const int64_t first = (int64_t)blockIdx.x * per_block + (threadIdx.x >> a.lanes_log2), stride = (int64_t)gridDim.x * per_block;
   const T* x = static_cast<const T*>(q.x) + first * q.x_stride + (int64_t)head * a.D;
   const T* dy = static_cast<const T*>(q.dy) + first * q.dy_stride + (int64_t)head * a.D;
   T* out = static_cast<T*>(q.y) + first * q.y_stride + (int64_t)head * a.D;
-  typename P::Raw xl[U][S], xh[U][S], gl[U][S], gh[U][S];
-  float c[S][NV], s[S][NV];
-  bool ok = true;
-  auto fetch = [&](int64_t tok) {
+  QkTurn turn(a, first, stride);
+  const E sign = E::make(a.sgn, a.sgn), minus = E::make(-a.sgn, -a.sgn);
+  constexpr bool ONCE = sizeof(T) == 2;  // see above
+  auto fetch = [](const T* p) {
+    if constexpr (ONCE) return P::load_once(p);
+    else return P::load(p);
+  };
+  // all threads of a block make as many turns: the sums are over groups of lanes
+  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += stride) {
+    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
     const bool in = tok < a.tokens;
+    typename P::Raw xl[U][S], xh[U][S], gl[U][S], gh[U][S];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -269,41 +382,45 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
         xl[u][k] = xh[u][k] = gl[u][k] = gh[u][k] = typename P::Raw{};
         if (in && u < heads && lane + (k << a.lanes_log2) < a.slots) {
           const int at = u * a.D + col[k];
-          xl[u][k] = P::load(x + at);
-          xh[u][k] = P::load(x + at + apart[k]);
-          gl[u][k] = P::load(dy + at);
-          gh[u][k] = P::load(dy + at + apart[k]);
+          xl[u][k] = fetch(x + at);
+          xh[u][k] = fetch(x + at + apart[k]);
+          gl[u][k] = fetch(dy + at);
+          gh[u][k] = fetch(dy + at + apart[k]);
         }
       }
-    ok = qk_angles<S, NV>(a, tok, in, lane, c, s);
+    V c[S], s[S];
+    const bool good = qk_angles<T, S, NV>(a, tok, turn.pos, in, lane, c, s);
+    turn.next(a);
     x += stride * q.x_stride;
     dy += stride * q.dy_stride;
-  };
-  // all threads of a block make as many turns: the sums are over groups of lanes
-  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.tokens; base += stride) {
-    const int64_t tok = base + (threadIdx.x >> a.lanes_log2);
-    fetch(tok);
-    const bool in = tok < a.tokens, good = ok;
-    float vx[U][S][NV], vy[U][S][NV], wl[U][S][NV], wh[U][S][NV], sum[U], dot[U];
+    V vx[U][S], vy[U][S], wl[U][S], wh[U][S];
+    float sum[U], dot[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      sum[u] = dot[u] = 0.0f;
+      E squares = E::make(0.0f, 0.0f), products = squares;
 #pragma unroll
       for (int k = 0; k < S; ++k) {
         P::unpack(xl[u][k], vx[u][k]);
         P::unpack(xh[u][k], vy[u][k]);
         P::unpack(gl[u][k], wl[u][k]);
         P::unpack(gh[u][k], wh[u][k]);
+        if (turns[k]) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          // the angles of columns that do not turn are (1, 0)
-          const float p = wl[u][k][i], r = wh[u][k][i], sn = a.sgn * s[k][i];
-          wl[u][k][i] = turns[k] ? p * c[k][i] + r * sn : p;
-          wh[u][k][i] = turns[k] ? r * c[k][i] - p * sn : r;
-          sum[u] = fmaf(vx[u][k][i], vx[u][k][i], fmaf(vy[u][k][i], vy[u][k][i], sum[u]));
-          dot[u] = fmaf(vx[u][k][i], wl[u][k][i] * glo[k][i], fmaf(vy[u][k][i], wh[u][k][i] * ghi[k][i], dot[u]));
+          for (int i = 0; i < V::N; ++i) {
+            const E p = wl[u][k].e[i], r = wh[u][k].e[i];
+            wl[u][k].e[i] = qk_fma(p, c[k].e[i], qk_mul(r, qk_mul(s[k].e[i], sign)));
+            wh[u][k].e[i] = qk_fma(r, c[k].e[i], qk_mul(p, qk_mul(s[k].e[i], minus)));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) {
+          squares = qk_fma(vx[u][k].e[i], vx[u][k].e[i], qk_fma(vy[u][k].e[i], vy[u][k].e[i], squares));
+          products = qk_fma(vx[u][k].e[i], qk_mul(wl[u][k].e[i], glo[k].e[i]), products);
+          products = qk_fma(vy[u][k].e[i], qk_mul(wh[u][k].e[i], ghi[k].e[i]), products);
         }
       }
+      sum[u] = squares.sum();
+      dot[u] = products.sum();
     }
     for (int o = (1 << a.lanes_log2) >> 1; o > 0; o >>= 1)
 #pragma unroll
@@ -315,31 +432,37 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
     for (int u = 0; u < U; ++u) {
       if (!in || u >= heads) continue;
       const float inv = rsqrtf(sum[u] * over + a.eps);
-      const float back = inv * inv * (dot[u] * over);
+      const float back = -(inv * inv * (dot[u] * over));
+      const E by = E::make(inv, inv), less = E::make(back, back);
 #pragma unroll
       for (int k = 0; k < S; ++k) {
         if (lane + (k << a.lanes_log2) >= a.slots) continue;
         T* d = out + u * a.D + col[k];
-        float ol[NV], oh[NV];
+        V ol, oh;
+        if (good) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const float xi = vx[u][k][i], yi = vy[u][k][i], wi = wl[u][k][i], ui = wh[u][k][i];
-          if (W && good) {
-            dlo[k][i] = fmaf(wi, xi * inv, dlo[k][i]);
-            dhi[k][i] = fmaf(ui, yi * inv, dhi[k][i]);
+          for (int i = 0; i < V::N; ++i) {
+            const E xi = vx[u][k].e[i], yi = vy[u][k].e[i], wi = wl[u][k].e[i], ui = wh[u][k].e[i];
+            if (W) {
+              dlo[k].e[i] = qk_fma(wi, qk_mul(xi, by), dlo[k].e[i]);
+              dhi[k].e[i] = qk_fma(ui, qk_mul(yi, by), dhi[k].e[i]);
+            }
+            ol.e[i] = qk_mul(by, qk_fma(wi, glo[k].e[i], qk_mul(xi, less)));
+            oh.e[i] = qk_mul(by, qk_fma(ui, ghi[k].e[i], qk_mul(yi, less)));
           }
-          ol[i] = good ? inv * (wi * glo[k][i] - xi * back) : 0.0f;
-          oh[i] = good ? inv * (ui * ghi[k][i] - yi * back) : 0.0f;
+        } else {
+          ol.fill(0.0f);
+          oh.fill(0.0f);
         }
         if (a.accumulate) {
-          float pl[NV], ph[NV];
+          V pl, ph;
           P::unpack(P::load(d), pl);
           P::unpack(P::load(d + apart[k]), ph);
 #pragma unroll
-          for (int i = 0; i < NV; ++i) ol[i] += pl[i], oh[i] += ph[i];
+          for (int i = 0; i < V::N; ++i) ol.e[i] = qk_add(ol.e[i], pl.e[i]), oh.e[i] = qk_add(oh.e[i], ph.e[i]);
         }
-        P::store(d, ol);
-        P::store(d + apart[k], oh);
+        P::template store<ONCE>(d, ol);
+        P::template store<ONCE>(d + apart[k], oh);
       }
     }
     out += stride * q.y_stride;
@@ -356,7 +479,11 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(const QkArgs a)
       qk_columns(a, slot * NV, turns, col, apart);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        float u = dlo[k][i], v = dhi[k][i];
+        constexpr int EACH = V::TWO ? 2 : 1;
+        float of_lo[2] = {}, of_hi[2] = {};
+        dlo[k].e[i / EACH].get(of_lo[0], of_lo[1]);
+        dhi[k].e[i / EACH].get(of_hi[0], of_hi[1]);
+        float u = of_lo[i % EACH], v = of_hi[i % EACH];
         for (int o = 16; o >= (1 << a.lanes_log2); o >>= 1) {
           u += __shfl_xor_sync(0xffffffffu, u, o);
           v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -483,11 +610,10 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
 
 // Heads that a thread has under way.  Forward, two where a lane has 16 bytes of a half or fewer, else one (16 x 2048 tokens of 2 x 10 heads of 128:
 // fp32 114 us, 115 with one; bf16 78, 99 with one, 83 with four; fp32 heads of 256 columns 225 with one, 231 with two).  Backward, two where a lane
-// has four fp32 pairs or fewer, else one (the same tokens fp32 165 us against 186 with one; 8192 of 12 + 2 heads bf16 34 against 45
-// with two: their registers leave two blocks to an SM).
+// has four pairs of columns or fewer, else one (the same tokens fp32 165 us against 186 with one; 8192 of 12 + 2 heads bf16 27 against 29).
 template <typename T, int NV, int S>
 int qk_kind(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
-  constexpr int BYTES = S * NV * (int)sizeof(T), U = BYTES < 32 ? 2 : 1, B = sizeof(T) == 4 && S * NV <= 4 ? 2 : 1;
+  constexpr int BYTES = S * NV * (int)sizeof(T), U = BYTES < 32 ? 2 : 1, B = S * NV <= 4 ? 2 : 1;
   if (!back) return qk_launch<T, NV, S, U, false, false>(ctx, a, sh);
   return w ? qk_launch<T, NV, S, B, true, true>(ctx, a, sh) : qk_launch<T, NV, S, B, true, false>(ctx, a, sh);
 }

@@ -82,29 +82,6 @@ __device__ __forceinline__ float ag_max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// pairs of fp32 in one instruction
-__device__ __forceinline__ uint64_t ag_pair(float a, float b) {
-  uint64_t y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
-  return y;
-}
-__device__ __forceinline__ void ag_unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
-__device__ __forceinline__ uint64_t ag_add2(uint64_t a, uint64_t b) {
-  uint64_t y;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-  return y;
-}
-__device__ __forceinline__ uint64_t ag_mul2(uint64_t a, uint64_t b) {
-  uint64_t y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-  return y;
-}
-__device__ __forceinline__ uint64_t ag_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t y;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-  return y;
-}
-
 // Statistics of a part of a row: m its largest logit, s = sum 2^(c y), t = sum 2^(c y) y with y = x - m, c = log2(e) / temperature.
 // The difference is formed before the product: x c - m c in one fma would be off by the rounding of m c, which differs between the
 // parts of a row, and overflows for rows of the lowest numbers.  Terms whose power is 0 add nothing to t, however far y is.
