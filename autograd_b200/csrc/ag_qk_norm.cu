@@ -608,9 +608,10 @@ int qk_launch(ag_ctx* ctx, QkArgs& a, const QkShape& sh) {
   return AG_OK;
 }
 
-// Heads that a thread has under way.  Forward, two where a lane has 16 bytes of a half or fewer, else one (16 x 2048 tokens of 2 x 10 heads of 128:
-// fp32 114 us, 115 with one; bf16 78, 99 with one, 83 with four; fp32 heads of 256 columns 225 with one, 231 with two).  Backward, two where a lane
-// has four pairs of columns or fewer, else one (the same tokens fp32 165 us against 186 with one; 8192 of 12 + 2 heads bf16 27 against 29).
+// Heads that a thread has under way.  Forward, two where a lane has 16 bytes of a half or fewer, else one (16 x 2048 tokens of 2 x 10 heads of 128
+// with two, one and four: fp32 108, 114 and 116 us, bf16 71, 84 and 77; heads of 256 columns fp32 214, 214 and 230).  Backward, two where a
+// lane has four pairs of columns or fewer, else one (with two and one: the same tokens fp32 164 and 174 us, bf16 112 and 136; 8192 of 12 + 2
+// heads bf16 26 and 30).
 template <typename T, int NV, int S>
 int qk_kind(ag_ctx* ctx, QkArgs& a, const QkShape& sh, bool back, bool w) {
   constexpr int BYTES = S * NV * (int)sizeof(T), U = BYTES < 32 ? 2 : 1, B = S * NV <= 4 ? 2 : 1;
