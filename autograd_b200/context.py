@@ -198,6 +198,10 @@ class CudaContext:
         """Test hook: the next norm kernel gives up its staging wait at once (see the header)."""
         self._check(lib.ag_debug_expire_staging(self._h))
 
+    def debug_expire_products(self, after=0):
+        """Test hook: a product of an orthogonal factor gives its waits up at once (see the header)."""
+        self._check(lib.ag_debug_expire_products(self._h, int(after)))
+
     def rmsnorm_forward(self, x, gamma, y, inv_rms, N_, C_, eps, dtype=N.AG_F32):
         calls.ag_rmsnorm_forward(self._hi, x, gamma, y, inv_rms, N_, C_, eps, dtype)
 

@@ -33,6 +33,7 @@ struct ag_ctx {
   int norm_pair;        // norm backward with two warps per row: 0 never, 1 always, 2 per shape
   int scatter_group;    // sorted entries per group of the scatter-add: 32, 64, 128, or 0 = by the size of the call
   int debug_stage_expire;  // ag_debug_expire_staging: the next staging wait gives up at once (tests)
+  int debug_wait_expire;   // ag_debug_expire_products: 1 + the products until one gives its waits up at once, 0: none does (tests)
   int linear_k_chunk;   // contraction elements per accumulation chain, forward of the linear+bias+residual op
   int tc_timing;        // ag_tc_timing: bracket tensor-core GEMM launches with pool events
   int tc_timing_base;

@@ -298,7 +298,7 @@ extern "C" int ag_graph_begin(ag_ctx* ctx, ag_ctx** recorder) {
   ag_ctx* r = new ag_ctx(*ctx);
   r->stream = stream;
   r->launches = 0;
-  r->tc_timing = r->debug_stage_expire = 0;
+  r->tc_timing = r->debug_stage_expire = r->debug_wait_expire = 0;
   pthread_mutex_init(&r->run_lock, nullptr);
   r->run_at = 0;
   *recorder = r;

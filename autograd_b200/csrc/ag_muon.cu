@@ -288,6 +288,7 @@ struct NsGemm {
   int cluster, k_each;     // ZSPLIT: CTAs to a tile, steps of each (even)
   NsPlane D;               // and where the result goes
   float diag, mul;
+  int expire;              // the issuer gives up at once
   int* status;
 };
 
@@ -360,6 +361,9 @@ __device__ __forceinline__ void ns_st_cluster(uint32_t addr, const float4& v) {
 __device__ __forceinline__ void ns_st_cluster(uint32_t addr, uint32_t x, uint32_t y) {
   asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void ns_st_cluster(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ void ns_st_cluster(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
@@ -428,6 +432,12 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   bool expired = false;
+  // a wait ran out: all roles give up, those of the pair's other CTA too
+  auto give_up = [&]() {
+    expired = true;
+    *abort_flag = 1;
+    if (PAIR) ns_st_cluster(tc_map_to_cta(ag_smem_u32(tmem_slot + 1), rank ^ 1u), 1);
+  };
   ag_pdl_wait();
 
   if (warp < 4) {
@@ -452,7 +462,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
             }
           };
           if (!tc_wait(SPLIT ? &acc_full[slot] : &empty[slot], phase ^ 1u, abort_flag)) {
-            expired = true;
+            give_up();
             break;
           }
           unsigned char* s = tiles + (size_t)slot * SLOT;
@@ -463,7 +473,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
             load(p.r.k_hi, p.r.mn_hi, &full[slot], s + A_BYTES, kx, r_at, r_mn);
             if (SPLIT) {
               if (!tc_wait(&low_empty[low], low_phase ^ 1u, abort_flag)) {
-                expired = true;
+                give_up();
                 break;
               }
               unsigned char* d = lows + (size_t)low * STEP;
@@ -490,6 +500,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         if (PAIR) ns_commit_both(bar);
         else tc_commit(bar);
       };
+      if (p.expire) give_up();
       NsTile t;
       for (int step = 0; !expired && ns_tile<KIND, PAIR>(p, unit, units, step, t); ++step) {
         uint32_t tacc = 0, more = 0;
@@ -503,7 +514,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
           // the accumulator last: it is what is late
           if (!tc_wait(&full[slot], phase, abort_flag) || (SPLIT && !tc_wait(&low_full[low], low_phase, abort_flag)) ||
               (left == 0 && !tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag))) {
-            expired = true;
+            give_up();
             break;
           }
           tc_fence_after();
@@ -518,7 +529,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
             for (int j = 0; j < n; ++j) {
               if (j > 0) {
                 if (!tc_wait(&low_full[low], low_phase, abort_flag)) {
-                  expired = true;
+                  give_up();
                   break;
                 }
                 tc_fence_after();
@@ -594,8 +605,9 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
         if (SPLIT || p.two) put(p.d_lo, lo, col);
       };
       auto wait_full = [&]() {
-        if (!tc_wait(&acc_full[buf], (full_par >> buf) & 1u, abort_flag)) {
-          expired = true;
+        // one answer for the warp: what follows is for all lanes together
+        if (!__all_sync(0xffffffffu, tc_wait(&acc_full[buf], (full_par >> buf) & 1u, abort_flag))) {
+          give_up();
           return false;
         }
         full_par ^= 1u << buf;
@@ -692,12 +704,10 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
-  // after a wait that ran out: copies under way land before this CTA's memory is someone else's (0.2 ms are a hundred times what one takes)
-  if (warp == 0 && lane == 0 && *abort_flag)
-    for (int i = 0; i < 200; ++i) __nanosleep(1000);
   tc_fence_before();
-  if (PAIR || ZSPLIT) tc_cluster_sync(); else __syncthreads();
+  tc_meet<PAIR || ZSPLIT>();
   if (warp == 1) {
+    tc_drain(abort_flag);
     tc_fence_after();
     if (PAIR)
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLUMNS) : "memory");
@@ -791,6 +801,7 @@ struct NsSmall {
   int rows, cols, m, n, groups, cluster, steps, out_kind;
   float eps, keep, by, loss_gram, loss_square;
   float co[3 * NS_MAX_STEPS];
+  uint32_t wait_limit;  // polls of a wait for products
   int* status;
 };
 
@@ -930,7 +941,8 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
   uint32_t phase = 0;
   bool expired = false;
   auto products_done = [&]() {
-    if (!tc_wait(bar, phase, abort_flag)) expired = true;  // the steps go on, all CTAs meet at the same barriers
+    if (!tc_wait(bar, phase, abort_flag, p.wait_limit)) expired = true;  // the steps go on without products, all CTAs meet at the same barriers
+    __syncwarp();
     phase ^= 1u;
     tc_fence_after();
   };
@@ -994,7 +1006,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
     const bool square = c != 0.0f;
     const float h = square ? b / (2.0f * c) : 0.0f;
     const float gram_mul = (square ? 1.0f : b) * unit * p.loss_gram, gram_diag = (square ? h : a) * NS_SCALE;
-    if (tid == 0) {
+    if (tid == 0 && !expired) {
       for (int i = 0; i < chains; ++i)
         gram(tmem + i * 128, xu + 2 * i * (NS_GROUP_BYTES >> 4), xl + 2 * i * (NS_GROUP_BYTES >> 4), min(chain16, w16 - i * chain16), m16 * 16);
       tc_commit(bar);
@@ -1069,7 +1081,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
     tc_fence_before();
     cluster_sync();
     if (square) {
-      if (tid == 0) {
+      if (tid == 0 && !expired) {
         tc_fence_after();
         ns_fence_proxy();
         gram(tmem, au, al, m16, m16 * 16);
@@ -1090,7 +1102,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
       tc_fence_before();
       __syncthreads();
     }
-    if (tid == 0) {
+    if (tid == 0 && !expired) {
       tc_fence_after();
       ns_fence_proxy();
       for (int c0 = 0; c0 < G; c0 += 4) {  // up to 256 columns at a time
@@ -1156,10 +1168,11 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS, 1) ns_small_kernel(const __g
       ns_put<1>(out, at, v, old[k], p.keep, p.by, p.out_kind);
     }
   }
-  if (expired && lane == 0) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
+  if (expired) atomicOr(p.status, AG_STATUS_WAIT_EXPIRED);
   tc_fence_before();
-  cluster_sync();
+  if (S > 1) tc_meet<true>(); else tc_meet<false>();
   if (warp == 0) {
+    tc_drain(abort_flag);
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -1216,6 +1229,9 @@ int ns_tiles(int kind, int M, int N, int BM, int BN) {
   return 2 * (n / 2) * (n / 2 + 1) + (n & 1 ? n : 0);  // two columns of 2 j + 2 each, and what an odd number leaves
 }
 
+// Whether ag_debug_expire_products means this launch
+bool ns_expires(ag_ctx* ctx) { return ctx->debug_wait_expire && --ctx->debug_wait_expire == 0; }
+
 template <int KIND, bool SPLIT, bool PAIR, int BN, bool ZSPLIT>
 int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int BM = PAIR ? 256 : 128, BN_CTA = PAIR ? BN / 2 : BN;
@@ -1256,6 +1272,7 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int SLOTS = SPLIT ? 2 : std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
   static_assert(NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT <= NS_SMEM_LIMIT && SLOTS >= 2, "operand tiles");
   p.slots = SLOTS;
+  p.expire = ns_expires(ctx);
   const int64_t work = (int64_t)p.batch * p.tiles;
   cfg.gridDim = dim3(ZSPLIT ? work * p.cluster : (PAIR ? 2 : 1) * std::min<int64_t>(units, work));
   cfg.dynamicSmemBytes = NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT;
@@ -1413,7 +1430,7 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
     NsSmall p = {};
     p.mats = mats; p.s = s;
     p.rows = t.rows; p.cols = t.cols; p.m = t.m; p.n = t.n; p.groups = groups; p.cluster = cluster; p.steps = steps; p.out_kind = out_kind;
-    p.eps = eps; p.keep = keep; p.by = by; p.status = ctx->d_status;
+    p.eps = eps; p.keep = keep; p.by = by; p.wait_limit = ns_expires(ctx) ? 0u : TC_WAIT_LIMIT; p.status = ctx->d_status;
     const double chains = cluster * ((groups + 1) / 2);
     p.loss_gram = split ? (float)(1.0 + NS_LOSS * std::max(0.0, ((t.n + 15) / 16 - chains) / chains)) : 1.0f;
     p.loss_square = split ? (float)(1.0 + NS_LOSS * ((t.m + 15) / 16 - 1)) : 1.0f;
@@ -1547,6 +1564,13 @@ int ns_check_ranges(ag_ctx* ctx, const char* name, const void* const* p, size_t 
 }
 
 }  // namespace
+
+extern "C" int ag_debug_expire_products(ag_ctx* ctx, int after) {
+  if (!ctx) return AG_ERR_INVALID;
+  AG_REQUIRE(ctx, after >= 0 && after < 1 << 30, "ag_debug_expire_products: after %d products", after);
+  ctx->debug_wait_expire = 1 + after;
+  return AG_OK;
+}
 
 extern "C" size_t ag_orthogonalise_scratch_bytes(int count, int rows, int cols, int precision) {
   if (count <= 0 || !ns_fits(rows, cols) || (precision != AG_CE_3XTF32 && precision != AG_CE_BF16)) return 0;

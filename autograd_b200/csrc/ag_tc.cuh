@@ -80,8 +80,8 @@ __device__ __forceinline__ void tc_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) 
 __device__ __forceinline__ void tc_tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Bounded wait that also gives up when another role of the CTA has already given up.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t i = 0; i < TC_WAIT_LIMIT; ++i) {
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit = TC_WAIT_LIMIT) {
+  for (uint32_t i = 0; i < limit; ++i) {
     if (ag_mbar_try_wait(bar, parity)) return true;
     if ((i & 127u) == 127u) {
       if (*abort_flag) return false;
@@ -90,6 +90,21 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
   }
   *abort_flag = 1;
   return false;
+}
+
+// Where the roles of a CTA, or of all CTAs of a cluster, meet at the end; the lanes of a warp may come one by one.
+template <bool CLUSTER>
+__device__ __forceinline__ void tc_meet() {
+  if (CLUSTER) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  else asm volatile("barrier.sync 0;" ::: "memory");
+}
+
+// Called after that by the warp that frees tensor memory, when nothing is issued any more: where a wait ran out, copies and products under way
+// get 0.2 ms to end, a hundred times what one takes, before the memory is someone else's.
+__device__ __forceinline__ void tc_drain(volatile int* abort_flag) {
+  if (__builtin_expect(*abort_flag, 0))
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  __syncwarp();
 }
 
 __device__ __forceinline__ float tc_exp2(float x) {  // 2^x by the PTX instruction, ~2 ulp

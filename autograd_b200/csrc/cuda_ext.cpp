@@ -80,6 +80,7 @@ PYBIND11_MODULE(cuda_ext, m) {
   AG_DEF(ag_layernorm_backward);
   AG_DEF(ag_layernorm_backward_noalloc);
   AG_DEF(ag_debug_expire_staging);
+  AG_DEF(ag_debug_expire_products);
   AG_DEF(ag_rmsnorm_forward);
   AG_DEF(ag_rmsnorm_backward);
   AG_DEF(ag_gelu_forward);

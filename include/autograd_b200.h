@@ -402,6 +402,12 @@ int ag_muon_step(ag_ctx* ctx, float* const* p, const void* const* g, float* cons
                  const float* coefficients, int steps, float eps, int precision, int grad_dtype, void* scratch,
                  size_t scratch_bytes);
 
+/* Test hook: of the launches that ag_orthogonalise and ag_muon_step make for products through ctx from now on, the one behind the next
+ * `after` gives its waits for operands (all of a small matrix's products are one launch: for products) up at once, so that the unwind path
+ * runs with copies or products under way: AG_STATUS_WAIT_EXPIRED is set, what is under way is given time to end, the kernel returns by itself,
+ * and the call's results are invalid.  One-shot. */
+int ag_debug_expire_products(ag_ctx* ctx, int after);
+
 /* ---- f3 AdamW fp32 step ----------------------------------------------------------------
  * Replaces: backend.py:2013-2038 cpu_adamw_step; metal_ops.metal:10139-10227.
  * g is read as g*grad_scale. */
