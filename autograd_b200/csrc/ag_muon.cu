@@ -173,10 +173,11 @@ struct NsPlane {
   __half *hi, *lo;  // lo null: one word
 };
 
-// What an element of the update is multiplied by: NS_SCALE over its norm, whose square is `sum`
+// What an element of the update is multiplied by: NS_SCALE over its norm, whose square is `sum`; NaN, and so a matrix of NaN after any
+// number of steps, where the norm is infinite or none (32-bit numbers have squares that 64 bits can add up)
 __device__ __forceinline__ double ns_factor(double sum, float eps) {
-  const double norm = sqrt(sum);
-  return (double)NS_SCALE / (norm > eps || norm != norm ? norm : (double)eps);
+  const double norm = sqrt(sum), none = norm - norm;
+  return none != 0.0 ? none : (double)NS_SCALE / (norm > eps ? norm : (double)eps);
 }
 
 // X = u / max(|u|, eps) in padded rows, transposed where the matrix is tall: tiles of 64 x 64, EACH elements to an access of the matrix
