@@ -165,7 +165,8 @@ __global__ void __launch_bounds__(NS_THREADS, 4) ns_momentum_kernel(const NsMatr
 }
 
 // What is kept between products: x * 2^12 as one or two 16-bit floats (`hi`, and what hi leaves), in planes of padded rows.
-// Singular values stay near 1 or below, so that no element of X, A or Q is beyond a few units, and the smallest that
+// Singular values stay near 1 or below, so that no element of X, A or Q is beyond a few units (15.99 is the largest: a limit on what
+// coefficients of the caller's may do, A = X X^T + h I being the first to reach it), and the smallest that
 // keep all bits are 2^-26 (one word) or next to nothing (two): elements err by at most 2^-37 or 2^-38 beside that.
 constexpr float NS_SCALE = 4096.0f;
 

@@ -386,10 +386,12 @@ int ag_qk_norm_rope_backward(ag_ctx* ctx, const void* dq_out, const void* dk_out
  *   ag_orthogonalise:  out = factor(g), in out_dtype.  out[i] may be g[i] where its elements are no larger.
  *   ag_muon_step:  g' = g * grad_scale (g in grad_dtype);  m += (1 - momentum) (g' - m);
  *               u = g' + momentum (m - g') with nesterov, else m;  p = p (1 - lr weight_decay) - lr scale factor(u).
- * precision AG_CE_3XTF32: products as exact as fp32 ones (operands carry 22 bits; a factor is off by about 1e-6 of its norm);
+ * precision AG_CE_3XTF32: products as exact as fp32 ones (operands carry 22 bits; a factor is off by about 1e-6 of its norm,
+ * more with coefficients whose b^2 / 4c, which is added and taken off again, is far above the usual 3);
  * AG_CE_BF16: operands rounded once to 16 bits, of which 11 are significant here (1e-3 to 1e-2 of the norm, the more the wider the
- * singular values range).  Singular values, and a + b s^2 + c s^4 for them, have to stay below 15 throughout; c is 0, or |b| at most
- * 16 |c| and b^2 at most 256 |c|.  A matrix of
+ * singular values range).  What is kept between products has to stay below 15 throughout, or its matrix may become NaN: singular values s
+ * before and after every step, |a + b s^2 + c s^4| and, where c is not 0, |s^2 + b / 2c| (s below about 4 for the usual coefficients, whose
+ * steps stay near 1).  c is 0, or |b| at most 16 |c| and b^2 at most 256 |c|.  A matrix of
  * zeros has the factor 0; NaN or infinities make their matrix NaN and no other.
  * Matrices and workspace may not overlap (256-byte aligned workspace of ag_orthogonalise_scratch_bytes, 0 for sizes or a
  * precision that the calls refuse: more than 16384 on the shorter side, 2^20 on the longer or 2^31 elements). */

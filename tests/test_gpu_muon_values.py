@@ -1,12 +1,11 @@
 """Orthogonal factors of matrices with numbers that are none: a matrix with a NaN or an infinity becomes NaN altogether, whatever the steps,
-and those beside it come out as without it."""
+and those beside it come out as without it; and coefficients at the limits of what is kept between products."""
 import numpy as np
 import pytest
 
-from autograd_b200 import _native as N
 from gpu_util import check_clean_status, env
-from oracle import heads_and_updates as R
-from test_gpu_muon import PRECISIONS, Matrices, gradient
+from test_gpu_muon import BITS, PRECISIONS, Matrices, close, gradient
+from test_muon_limits_cpu import EDGES
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +60,48 @@ def test_a_step_with_an_infinite_gradient(shape):
     m1[1, 2, 3] = m0[1, 2, 3]
     assert np.array_equal(m0, m1) and np.array_equal(p0[[0, 2]], p1[[0, 2]])
     check_clean_status()
+
+
+def one_direction_error(steps, bits):
+    """How far the singular value 1 may be off after the steps.
+
+    A product errs by e of itself: two operands by half a step each (2^-23 or 2^-12), and the kernel's factor for what truncation loses on
+    average, 3.2e-7 for 128 elements, stays whole where a sum has one term and loses nothing: 2^-20 or 2^-10 in all.  What is stored is rounded by
+    half a step.  A = s^2 + h is off by d = e s^2 + r |A|, Q = (a - h^2 c) + c A^2 by 2 |c A| d + e |c| A^2 + r |Q| (of the whole square: where
+    h^2 c is large, most of it cancels), s Q by |s| times that, by e |s Q| and by what s was off, times the step's derivative."""
+    e, r = (2.0 ** -20, 2.0 ** -23) if bits == 22 else (2.0 ** -10, 2.0 ** -12)
+    s, off = 1.0, r
+    for a, b, c in steps:
+        h = b / (2 * c) if c else 0.0
+        if c:
+            d = e * s * s + r * abs(s * s + h)
+            dq = 2 * abs(c * (s * s + h)) * d + e * abs(c) * (s * s + h) ** 2
+        else:
+            dq = e * abs(b) * s * s
+        q = a + b * s * s + c * s ** 4
+        off = abs(a + 3 * b * s * s + 5 * c * s ** 4) * off + abs(s) * (dq + r * abs(q)) + (e + r) * abs(s * q)
+        s *= q
+    return off
+
+
+@PRECISIONS
+@pytest.mark.parametrize("steps", EDGES, ids=lambda s: str(len(s)))
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 70, 90), (1, 40, 700), (2, 150, 140), (1, 140, 1500), (24, 270, 300)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_singular_values_up_to_the_limits(shape, steps, precision):
+    """Matrices of one direction, the singular value of which is 1: one element that has it all (in a corner, beside the padding), and rows
+    and columns that share it."""
+    ctx, alloc, be = env()
+    rng = np.random.default_rng(sum(shape))
+    g = np.zeros(shape, np.float32)
+    g[:, -1, -1] = 3.0
+    if shape[0] > 1:
+        g[1] = np.outer(rng.standard_normal(shape[1]), rng.standard_normal(shape[2]))
+    a = Matrices(g)
+    b = Matrices(np.ones_like(g))
+    be.orthogonalise(a.argument, b.argument, steps=len(steps), coefficients=steps, precision=precision)
+    got = b.read()
+    for i in sorted({0, min(1, shape[0] - 1), shape[0] - 1}):
+        close(got[i], g[i], precision, len(steps), steps, more=one_direction_error(steps, BITS[precision]))
+    check_clean_status()
+    a.free(), b.free()
