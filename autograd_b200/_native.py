@@ -23,6 +23,7 @@ AG_CE_IGNORE_MASKED, AG_CE_IGNORE_COMPAT_UNMASKED = 0, 1
 AG_DISTILL_RENORM, AG_DISTILL_REST = 0, 1
 AG_VOCAB_MAX, AG_TOP_MAX, AG_DISTILL_MAX = 393216, 128, 256
 AG_QK_MAX_D = 1024
+AG_NS_ONE_LAUNCH, AG_NS_SINGLE, AG_NS_PAIRS, AG_NS_CLUSTERS = 0, 1, 2, 3
 
 
 class FlceDesc(C.Structure):
@@ -109,6 +110,7 @@ SIGNATURES = {
     "ag_qk_norm_partials_bytes": (_sz, [_ctx, _int, _int, _int]),
     "ag_qk_norm_rope_backward": (_int, [_ctx] + [_ptr] * 14 + [_sz, _i64] + [_int] * 6 + [_i64] * 6 + [_f32, _int, _int, _int]),
     "ag_orthogonalise_scratch_bytes": (_sz, [_int, _int, _int, _int]),
+    "ag_orthogonalise_form": (_int, [_ctx, _int, _int, _int, _int, _ptr, _ptr]),
     "ag_orthogonalise": (_int, [_ctx, _ptr, _ptr, _int, _int, _int, _ptr, _int, _f32, _int, _int, _int, _ptr, _sz]),
     "ag_muon_step": (_int, [_ctx, _ptr, _ptr, _ptr, _int, _int, _int, _f64, _f64, _int, _f64, _f64, _f64, _ptr, _int, _f32, _int,
                             _int, _ptr, _sz]),

@@ -332,6 +332,12 @@ class CudaContext:
     def orthogonalise_scratch_bytes(count, rows, cols, precision=N.AG_CE_3XTF32):
         return calls.ag_orthogonalise_scratch_bytes(count, rows, cols, precision)
 
+    def orthogonalise_form(self, count, rows, cols, product):
+        """(N.AG_NS_*: what computes product 0, 1 or 2 of a step, matrices that share a launch)"""
+        form, batch = C.c_int(), C.c_int()
+        self._check(lib.ag_orthogonalise_form(self._h, int(count), int(rows), int(cols), int(product), C.byref(form), C.byref(batch)))
+        return form.value, batch.value
+
     def orthogonalise(self, g, out, count, rows, cols, coefficients, steps, eps, precision, dtype, out_dtype, scratch,
                       scratch_bytes):
         """g, out: host addresses of arrays of device addresses; coefficients: that of 3 floats a step."""

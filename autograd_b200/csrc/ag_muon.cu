@@ -1293,18 +1293,25 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
 // Tiles of 256 x 256 on pairs of CTAs or of 128 x 128 on single ones: a round of them takes 7 + 1.15 k or 6 + 0.78 k us for k steps of 64
 // elements with pairs of words (1280 x 1280 alone: 402 us on pairs, 327 on single CTAs; four of them 630 and 737).  Where X X^T
 // leaves most SMs without a tile, clusters share the contraction, four steps or more to each CTA.
+int ns_form(ag_ctx* ctx, int kind, int batch, int M, int N, int k_iters, int* cluster) {
+  const int64_t pairs = (int64_t)batch * ns_tiles(kind, M, N, 256, 256), singles = (int64_t)batch * ns_tiles(kind, M, N, 128, 128);
+  const double on_pairs = ag_ceil_div(pairs, ctx->sm_count / 2) * (7.0 + 1.15 * k_iters);
+  const double on_singles = ag_ceil_div(singles, ctx->sm_count) * (6.0 + 0.78 * k_iters);
+  if (M > 256 && on_pairs <= on_singles) return AG_NS_PAIRS;
+  if (kind != NS_GRAM) return AG_NS_SINGLE;
+  int z = 8;
+  while (z > 1 && (singles * z > ctx->sm_count || k_iters < 4 * z)) z /= 2;
+  *cluster = z;
+  return z > 1 ? AG_NS_CLUSTERS : AG_NS_SINGLE;
+}
+
 template <int KIND, bool SPLIT>
 int ns_product(ag_ctx* ctx, NsGemm& p) {
-  const int64_t pairs = (int64_t)p.batch * ns_tiles(KIND, p.M, p.N, 256, 256), singles = (int64_t)p.batch * ns_tiles(KIND, p.M, p.N, 128, 128);
-  const double on_pairs = ag_ceil_div(pairs, ctx->sm_count / 2) * (7.0 + 1.15 * p.k_iters);
-  const double on_singles = ag_ceil_div(singles, ctx->sm_count) * (6.0 + 0.78 * p.k_iters);
-  if (p.M > 256 && on_pairs <= on_singles) return ns_launch<KIND, SPLIT, true, 256, false>(ctx, p);
+  const int form = ns_form(ctx, KIND, p.batch, p.M, p.N, p.k_iters, &p.cluster);
+  if (form == AG_NS_PAIRS) return ns_launch<KIND, SPLIT, true, 256, false>(ctx, p);
   if constexpr (KIND == NS_GRAM) {
-    int z = 8;
-    while (z > 1 && (singles * z > ctx->sm_count || p.k_iters < 4 * z)) z /= 2;
-    if (z > 1) {
-      p.k_each = ((p.k_iters + z - 1) / z + 1) & ~1;
-      p.cluster = z;
+    if (form == AG_NS_CLUSTERS) {
+      p.k_each = ((p.k_iters + p.cluster - 1) / p.cluster + 1) & ~1;
       return ns_launch<KIND, SPLIT, false, 128, true>(ctx, p);
     }
   }
@@ -1571,6 +1578,20 @@ extern "C" int ag_debug_expire_products(ag_ctx* ctx, int after) {
   if (!ctx) return AG_ERR_INVALID;
   AG_REQUIRE(ctx, after >= 0 && after < 1 << 30, "ag_debug_expire_products: after %d products", after);
   ctx->debug_wait_expire = 1 + after;
+  return AG_OK;
+}
+
+extern "C" int ag_orthogonalise_form(ag_ctx* ctx, int count, int rows, int cols, int product, int* form, int* batch) {
+  if (!ctx) return AG_ERR_INVALID;
+  AG_REQUIRE(ctx, count > 0 && rows > 0 && cols > 0 && ns_fits(rows, cols), "ag_orthogonalise_form: bad shape count=%d rows=%d cols=%d", count, rows,
+             cols);
+  AG_REQUIRE(ctx, product >= NS_GRAM && product <= NS_NEXT && form && batch, "ag_orthogonalise_form: product %d", product);
+  const NsPlan t = ns_plan(count, rows, cols);
+  int cluster = 1, groups;
+  *batch = t.batch;
+  *form = ns_small_shape(ctx, t, t.batch, &cluster, &groups)
+              ? AG_NS_ONE_LAUNCH
+              : ns_form(ctx, product, t.batch, t.mp, product == NS_NEXT ? t.np : t.mp, ((product == NS_GRAM ? t.n : t.m) + TC_BK - 1) / TC_BK, &cluster);
   return AG_OK;
 }
 

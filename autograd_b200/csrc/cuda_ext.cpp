@@ -112,6 +112,7 @@ PYBIND11_MODULE(cuda_ext, m) {
   AG_DEF(ag_qk_norm_partials_bytes);
   AG_DEF(ag_qk_norm_rope_backward);
   AG_DEF(ag_orthogonalise_scratch_bytes);
+  AG_DEF(ag_orthogonalise_form);
   AG_DEF(ag_orthogonalise);
   AG_DEF(ag_muon_step);
   AG_DEF(ag_adamw_step);

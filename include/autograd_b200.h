@@ -386,7 +386,7 @@ int ag_qk_norm_rope_backward(ag_ctx* ctx, const void* dq_out, const void* dk_out
  *   ag_orthogonalise:  out = factor(g), in out_dtype.  out[i] may be g[i] where its elements are no larger.
  *   ag_muon_step:  g' = g * grad_scale (g in grad_dtype);  m += (1 - momentum) (g' - m);
  *               u = g' + momentum (m - g') with nesterov, else m;  p = p (1 - lr weight_decay) - lr scale factor(u).
- * precision AG_CE_3XTF32: products as exact as fp32 ones (operands carry 22 bits; a factor is off by about 1e-6 of its norm,
+ * precision AG_CE_3XTF32: products as exact as fp32 ones (operands carry 22 bits; a factor is off by 1e-6 to 3e-6 of its norm,
  * more with coefficients whose b^2 / 4c, which is added and taken off again, is far above the usual 3);
  * AG_CE_BF16: operands rounded once to 16 bits, of which 11 are significant here (1e-3 to 1e-2 of the norm, the more the wider the
  * singular values range).  What is kept between products has to stay below 15 throughout, or its matrix may become NaN: singular values s
@@ -399,6 +399,11 @@ size_t ag_orthogonalise_scratch_bytes(int count, int rows, int cols, int precisi
 int ag_orthogonalise(ag_ctx* ctx, const void* const* g, void* const* out, int count, int rows, int cols,
                      const float* coefficients, int steps, float eps, int precision, int dtype, int out_dtype,
                      void* scratch, size_t scratch_bytes);
+/* How the calls above go about the first matrices of a list: *batch, how many of them share a launch; *form, what computes product 0 (X X^T),
+ * 1 (its square) or 2 (the next X) of their steps, with either precision: one launch for everything, single CTAs, pairs of CTAs, or
+ * clusters of CTAs that share a contraction.  A part of the list behind a whole number of batches may take another form. */
+enum { AG_NS_ONE_LAUNCH = 0, AG_NS_SINGLE = 1, AG_NS_PAIRS = 2, AG_NS_CLUSTERS = 3 };
+int ag_orthogonalise_form(ag_ctx* ctx, int count, int rows, int cols, int product, int* form, int* batch);
 int ag_muon_step(ag_ctx* ctx, float* const* p, const void* const* g, float* const* m, int count, int rows, int cols,
                  double lr, double momentum, int nesterov, double weight_decay, double scale, double grad_scale,
                  const float* coefficients, int steps, float eps, int precision, int grad_dtype, void* scratch,
