@@ -199,7 +199,7 @@ class CudaContext:
         self._check(lib.ag_debug_expire_staging(self._h))
 
     def debug_expire_products(self, after=0):
-        """Test hook: a product of an orthogonal factor gives its waits up at once (see the header)."""
+        """Test hook: a launch of products on tensor cores gives its waits up at once (see the header)."""
         self._check(lib.ag_debug_expire_products(self._h, int(after)))
 
     def rmsnorm_forward(self, x, gamma, y, inv_rms, N_, C_, eps, dtype=N.AG_F32):

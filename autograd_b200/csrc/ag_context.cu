@@ -280,6 +280,13 @@ static int not_capturing(ag_ctx* ctx, const char* what) {
   return AG_OK;
 }
 
+extern "C" int ag_debug_expire_products(ag_ctx* ctx, int after) {
+  if (!ctx) return AG_ERR_INVALID;
+  AG_REQUIRE(ctx, after >= 0 && after < 1 << 30, "ag_debug_expire_products: after %d products", after);
+  ctx->debug_wait_expire = 1 + after;
+  return AG_OK;
+}
+
 // The recorder is a copy of the context with a stream of its own: what other threads enqueue on the context meanwhile
 // stays out of the recording, and the context's stream may be one that cannot be captured.
 extern "C" int ag_graph_begin(ag_ctx* ctx, ag_ctx** recorder) {

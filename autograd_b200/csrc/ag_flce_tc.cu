@@ -45,8 +45,8 @@
 // group when the MN extent is ragged) and described to the MMA with the transposing descriptor forms
 // (see TcDesc).
 // Every output tile has exactly one writer, so accumulation order is fixed.
-// Every mbarrier wait is bounded; on expiry the CTA raises AG_STATUS_WAIT_EXPIRED, all roles
-// leave their loops, TMEM is released and the kernel returns.  Larger problems run on clusters
+// Every mbarrier wait is bounded; on expiry the CTA raises AG_STATUS_WAIT_EXPIRED, all roles (a pair's: of both CTAs)
+// leave their loops, copies and products under way get time to end, TMEM is released and the kernel returns.  Larger problems run on clusters
 // of two CTAs (see tc_gemm_kernel); every CTA loads its own tiles with plain (single-destination) TMA
 // loads.
 #include "ag_flce.cuh"
@@ -152,6 +152,7 @@ struct TcLaunch {
   TcSchedule sched;
   int stages;
   uint32_t stage_bytes;
+  int expire;  // the issuer gives up at once
   int* status;
 };
 
@@ -300,6 +301,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   bool expired = false;
+  // a wait ran out: all roles give up, those of the pair's other CTA too
+  auto give_up = [&]() {
+    expired = true;
+    *abort_flag = 1;
+    if (PAIR) tc_st_cluster(tc_map_to_cta(ag_smem_u32(tmem_slot + 1), rank ^ 1u), 1);
+  };
   // Everything above touched no global memory and may overlap the tail of the previous kernel of the
   // stream; from here on its results are read.  No trigger for the next kernel: beside 227 KB of shared memory none of its CTAs
   // finds room anyway, and where they move in one by one as these leave, an SM is never empty and its L1 stays what is left beside
@@ -330,7 +337,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
         const int m0 = it.tm * bm_tile + row_off, n0 = it.tn * p.BN + (PAIR ? (int)rank * bn_cta : 0);
         for (int k = it.k_begin; k < it.k_end; ++k) {
           if (!tc_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-            expired = true;
+            give_up();
             break;
           }
           unsigned char* s = tiles + (size_t)stage * stage_bytes;
@@ -388,6 +395,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
       uint32_t acc_par = 0;  // phase bits of the two accumulators' "free" barriers
       int buf = 0;
       const uint32_t stage_units = stage_bytes >> 4;
+      if (L.expire) give_up();
       const uint32_t tiles_u = ag_smem_u32(tiles) >> 4;
       TcItem it;
       for (int step = 0; !expired && tc_item(L, unit, units, step, it); ++step) {
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
           uint32_t not_first = 1u;
           if (left == 0) {
             if (!tc_wait(&acc_empty[buf], ((acc_par >> buf) & 1u) ^ 1u, abort_flag)) {
-              expired = true;
+              give_up();
               break;
             }
             acc_par ^= 1u << buf;
@@ -415,7 +423,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
             not_first = 0u;
           }
           if (!tc_wait(&full[stage], phase, abort_flag)) {
-            expired = true;
+            give_up();
             break;
           }
           tc_fence_after();
@@ -494,8 +502,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
         if (EPI == EPI_COLMAX) cols1 = tc_load_cols(h.w_norm, col0 + 4 * lane, p.N);
       }
       auto wait_full = [&]() {
-        if (!tc_wait(&acc_full[buf], (full_par >> buf) & 1u, abort_flag)) {
-          expired = true;
+        // one answer for the warp: what follows is for all lanes together
+        if (!__all_sync(0xffffffffu, tc_wait(&acc_full[buf], (full_par >> buf) & 1u, abort_flag))) {
+          give_up();
           return false;
         }
         full_par ^= 1u << buf;
@@ -744,8 +753,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_gemm_kernel(const __grid_con
   tc_fence_before();
   // pair: neither CTA may leave, or free its tensor memory, while the other can still read its shared
   // memory or arrive on its barriers
-  if (PAIR) tc_cluster_sync(); else __syncthreads();
+  tc_meet<PAIR>();
   if (warp == 1) {
+    tc_drain(abort_flag);
     tc_fence_after();
     if (PAIR)
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
@@ -1157,6 +1167,7 @@ int tc_gemm(ag_ctx* ctx, const TcGemm* g, int n, int epi = EPI_STORE, const TcHe
   if (head) L.head = *head;
   L.sched = pl.sched;
   L.status = ctx->d_status;
+  L.expire = tc_expires(ctx);
   const int order[2] = {n == 2 && pl.shape[1].tile_cost > pl.shape[0].tile_cost ? 1 : 0, 0};
   int64_t total = 0;
   for (int i = 0; i < n; ++i) {

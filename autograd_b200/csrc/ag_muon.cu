@@ -363,9 +363,6 @@ __device__ __forceinline__ void ns_st_cluster(uint32_t addr, const float4& v) {
 __device__ __forceinline__ void ns_st_cluster(uint32_t addr, uint32_t x, uint32_t y) {
   asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void ns_st_cluster(uint32_t addr, int v) {
-  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 __device__ __forceinline__ void ns_st_cluster(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
@@ -438,7 +435,7 @@ __global__ void __launch_bounds__(NS_TC_THREADS, 1) ns_gemm_kernel(const __grid_
   auto give_up = [&]() {
     expired = true;
     *abort_flag = 1;
-    if (PAIR) ns_st_cluster(tc_map_to_cta(ag_smem_u32(tmem_slot + 1), rank ^ 1u), 1);
+    if (PAIR) tc_st_cluster(tc_map_to_cta(ag_smem_u32(tmem_slot + 1), rank ^ 1u), 1);
   };
   ag_pdl_wait();
 
@@ -1231,9 +1228,6 @@ int ns_tiles(int kind, int M, int N, int BM, int BN) {
   return 2 * (n / 2) * (n / 2 + 1) + (n & 1 ? n : 0);  // two columns of 2 j + 2 each, and what an odd number leaves
 }
 
-// Whether ag_debug_expire_products means this launch
-bool ns_expires(ag_ctx* ctx) { return ctx->debug_wait_expire && --ctx->debug_wait_expire == 0; }
-
 template <int KIND, bool SPLIT, bool PAIR, int BN, bool ZSPLIT>
 int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int BM = PAIR ? 256 : 128, BN_CTA = PAIR ? BN / 2 : BN;
@@ -1274,7 +1268,7 @@ int ns_launch(ag_ctx* ctx, NsGemm& p) {
   constexpr int SLOTS = SPLIT ? 2 : std::min<int>(NS_MAX_SLOTS, (int)((NS_SMEM_LIMIT - NS_SMEM_FIXED) / SLOT));
   static_assert(NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT <= NS_SMEM_LIMIT && SLOTS >= 2, "operand tiles");
   p.slots = SLOTS;
-  p.expire = ns_expires(ctx);
+  p.expire = tc_expires(ctx);
   const int64_t work = (int64_t)p.batch * p.tiles;
   cfg.gridDim = dim3(ZSPLIT ? work * p.cluster : (PAIR ? 2 : 1) * std::min<int64_t>(units, work));
   cfg.dynamicSmemBytes = NS_SMEM_FIXED + (SLOTS + (SPLIT ? 1 : 0)) * SLOT;
@@ -1439,7 +1433,7 @@ int ns_run(ag_ctx* ctx, const NsPlan& t, const NsMatrices& mats, int count, int 
     NsSmall p = {};
     p.mats = mats; p.s = s;
     p.rows = t.rows; p.cols = t.cols; p.m = t.m; p.n = t.n; p.groups = groups; p.cluster = cluster; p.steps = steps; p.out_kind = out_kind;
-    p.eps = eps; p.keep = keep; p.by = by; p.wait_limit = ns_expires(ctx) ? 0u : TC_WAIT_LIMIT; p.status = ctx->d_status;
+    p.eps = eps; p.keep = keep; p.by = by; p.wait_limit = tc_expires(ctx) ? 0u : TC_WAIT_LIMIT; p.status = ctx->d_status;
     const double chains = cluster * ((groups + 1) / 2);
     p.loss_gram = split ? (float)(1.0 + NS_LOSS * std::max(0.0, ((t.n + 15) / 16 - chains) / chains)) : 1.0f;
     p.loss_square = split ? (float)(1.0 + NS_LOSS * ((t.m + 15) / 16 - 1)) : 1.0f;
@@ -1573,13 +1567,6 @@ int ns_check_ranges(ag_ctx* ctx, const char* name, const void* const* p, size_t 
 }
 
 }  // namespace
-
-extern "C" int ag_debug_expire_products(ag_ctx* ctx, int after) {
-  if (!ctx) return AG_ERR_INVALID;
-  AG_REQUIRE(ctx, after >= 0 && after < 1 << 30, "ag_debug_expire_products: after %d products", after);
-  ctx->debug_wait_expire = 1 + after;
-  return AG_OK;
-}
 
 extern "C" int ag_orthogonalise_form(ag_ctx* ctx, int count, int rows, int cols, int product, int* form, int* batch) {
   if (!ctx) return AG_ERR_INVALID;

@@ -107,6 +107,9 @@ __device__ __forceinline__ void tc_drain(volatile int* abort_flag) {
   __syncwarp();
 }
 
+// Whether ag_debug_expire_products means this launch
+inline bool tc_expires(ag_ctx* ctx) { return ctx->debug_wait_expire && --ctx->debug_wait_expire == 0; }
+
 __device__ __forceinline__ float tc_exp2(float x) {  // 2^x by the PTX instruction, ~2 ulp
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

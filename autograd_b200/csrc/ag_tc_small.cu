@@ -64,6 +64,7 @@ struct TcsLaunch {
   int tiles0, tiles;  // of problem 0, of both
   AgTcsHead head;
   int* status;
+  int expire;   // the issuer gives up at once
   int trigger;  // let the next kernel be scheduled early
 };
 
@@ -288,6 +289,10 @@ __global__ void __launch_bounds__(TCS_THREADS, 1) tcs_gemm_kernel(const __grid_c
       const uint32_t tiles_u = ag_smem_u32(tiles) >> 4;
       int buf = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 1;
+      if (L.expire) {
+        expired = true;
+        *abort_flag = 1;
+      }
       for (int at = blockIdx.x; !expired && at < L.tiles; at += gridDim.x) {
         const TcsTile t = tcs_tile(L, at);
         const TcsProblem& p = L.pr[t.which];
@@ -374,7 +379,8 @@ __global__ void __launch_bounds__(TCS_THREADS, 1) tcs_gemm_kernel(const __grid_c
         la.now = lb.now = 0u;
         la.whole = lb.whole = false;
       }
-      if (!tc_wait(&empty[buf], phase, abort_flag)) {
+      if (!__all_sync(0xffffffffu, tc_wait(&empty[buf], phase, abort_flag))) {
+        *abort_flag = 1;
         expired = true;
         break;
       }
@@ -467,7 +473,9 @@ __global__ void __launch_bounds__(TCS_THREADS, 1) tcs_gemm_kernel(const __grid_c
       // argument, an error of 2^-18 of p at a loss gradient of 2^-60 instead of 2^-22.
       const float first = shift < 0.0f ? sc : one, second = shift < 0.0f ? one : sc;
       float mx = -INFINITY, sum = 0.0f;
-      if (!tc_wait(&acc_full[acc], acc_phase, abort_flag)) {
+      // one answer for the warp: what follows is for all lanes together
+      if (!__all_sync(0xffffffffu, tc_wait(&acc_full[acc], acc_phase, abort_flag))) {
+        *abort_flag = 1;
         expired = true;
         break;
       }
@@ -538,8 +546,9 @@ __global__ void __launch_bounds__(TCS_THREADS, 1) tcs_gemm_kernel(const __grid_c
   }
   if (expired && lane == 0) atomicOr(L.status, AG_STATUS_WAIT_EXPIRED);
   tc_fence_before();
-  __syncthreads();
+  tc_meet<false>();
   if (warp == TCS_MMA_WARP) {
+    tc_drain(abort_flag);
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * ACC) : "memory");
   }
@@ -767,6 +776,7 @@ int ag_tcs_gemm(ag_ctx* ctx, int epi, int parts, const AgTcsGemm* g, int n, int 
   TcsLaunch L = {};
   if (head) L.head = *head;
   L.status = ctx->d_status;
+  L.expire = tc_expires(ctx);
   TcsReduces R = {};
   int64_t ctas = 0, n_red = 0, red_blocks = 0;
   bool vec = true;

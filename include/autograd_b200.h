@@ -166,6 +166,12 @@ int ag_layernorm_backward_noalloc(ag_ctx* ctx, const float* dy, const float* x, 
  * are filled with plain loads and the results are still correct.  One-shot. */
 int ag_debug_expire_staging(ag_ctx* ctx);
 
+/* Test hook: of the launches that make products on tensor cores through ctx from now on (heads, projections, orthogonal factors), the one
+ * behind the next `after` gives up its waits for operands at once (all products of a small matrix's factor are one launch: its waits for
+ * products), so that the unwind path runs with copies or products under way: AG_STATUS_WAIT_EXPIRED is set, what is under way is given time
+ * to end, the kernel returns by itself, and the call's results are invalid.  One-shot. */
+int ag_debug_expire_products(ag_ctx* ctx, int after);
+
 /* ---- a4 RMSNorm -----------------------------------------------------------------------
  * Replaces: the RMSNorm stage of backend.py:1097-1108 / :1228-1251 (also :741-749,
  * :862-886, :1737-1745, :1990-2011); metal_ops.metal:3412-3537, :8107-8240, :14542.
@@ -408,12 +414,6 @@ int ag_muon_step(ag_ctx* ctx, float* const* p, const void* const* g, float* cons
                  double lr, double momentum, int nesterov, double weight_decay, double scale, double grad_scale,
                  const float* coefficients, int steps, float eps, int precision, int grad_dtype, void* scratch,
                  size_t scratch_bytes);
-
-/* Test hook: of the launches that ag_orthogonalise and ag_muon_step make for products through ctx from now on, the one behind the next
- * `after` gives its waits for operands (all of a small matrix's products are one launch: for products) up at once, so that the unwind path
- * runs with copies or products under way: AG_STATUS_WAIT_EXPIRED is set, what is under way is given time to end, the kernel returns by itself,
- * and the call's results are invalid.  One-shot. */
-int ag_debug_expire_products(ag_ctx* ctx, int after);
 
 /* ---- f3 AdamW fp32 step ----------------------------------------------------------------
  * Replaces: backend.py:2013-2038 cpu_adamw_step; metal_ops.metal:10139-10227.
