@@ -11,8 +11,8 @@
 // few shuffles and no shared memory.  A thread has one or two heads of a token under way, loads the angles once for them, and goes on to the next
 // token of its turn with the weights in registers.  Packets are as wide as addresses, strides and halves allow, one to four
 // elements: every shape takes the same code.  All sums are fp32.
-// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 108 us, 0.95 of the copy rate; the gradient 169 us, 0.91), instructions
-// with bf16 ones (73 us, 0.70; the gradient 117 us, 0.66) and with packets of one element (heads of 74 columns: 93 us fp32, 0.64).
+// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 108 us, 0.95 of the copy rate; the gradient 167 us, 0.92), instructions
+// with bf16 ones (73 us, 0.70; the gradient 117 us, 0.66) and with packets of one element (heads of 74 columns: 93 us fp32, 0.64; the gradient 143).
 #include <type_traits>
 
 #include "ag_common.cuh"
@@ -366,6 +366,10 @@ __global__ void __launch_bounds__(QK_THREADS, sizeof(T) == 4 || S * NV > 12 ? 1 
   QkTurn turn(a, first, stride);
   const E sign = E::make(a.sgn, a.sgn), minus = E::make(-a.sgn, -a.sgn);
   constexpr bool ONCE = sizeof(T) == 2;  // see above
+  // What turns, and what has a place, is selected in fp32 rows where a lane has four pairs of columns or fewer, and branched on elsewhere
+  // (16 x 2048 tokens of 2 x 10 heads fp32: 166.6 us with selects, 168.9 with branches; heads of 74 columns 143 and 149, heads of 80, 40 of which
+  // rotate, twelve pairs of columns to a lane, 150.6 and 149.0)
+  constexpr bool SELECT = sizeof(T) == 4 && S * NV <= 4;
   auto fetch = [](const T* p) {
     if constexpr (ONCE) return P::load_once(p);
     else return P::load(p);
@@ -404,12 +408,14 @@ __global__ void __launch_bounds__(QK_THREADS, sizeof(T) == 4 || S * NV > 12 ? 1 
         P::unpack(xh[u][k], vy[u][k]);
         P::unpack(gl[u][k], wl[u][k]);
         P::unpack(gh[u][k], wh[u][k]);
-        if (turns[k]) {
+        if (SELECT || turns[k]) {
 #pragma unroll
           for (int i = 0; i < V::N; ++i) {
             const E p = wl[u][k].e[i], r = wh[u][k].e[i];
-            wl[u][k].e[i] = qk_fma(p, c[k].e[i], qk_mul(r, qk_mul(s[k].e[i], sign)));
-            wh[u][k].e[i] = qk_fma(r, c[k].e[i], qk_mul(p, qk_mul(s[k].e[i], minus)));
+            const E tl = qk_fma(p, c[k].e[i], qk_mul(r, qk_mul(s[k].e[i], sign)));
+            const E th = qk_fma(r, c[k].e[i], qk_mul(p, qk_mul(s[k].e[i], minus)));
+            wl[u][k].e[i] = !SELECT || turns[k] ? tl : p;
+            wh[u][k].e[i] = !SELECT || turns[k] ? th : r;
           }
         }
 #pragma unroll
@@ -439,18 +445,19 @@ __global__ void __launch_bounds__(QK_THREADS, sizeof(T) == 4 || S * NV > 12 ? 1 
         if (lane + (k << a.lanes_log2) >= a.slots) continue;
         T* d = out + u * a.D + col[k];
         V ol, oh;
-        if (good) {
+        if (SELECT || good) {
 #pragma unroll
           for (int i = 0; i < V::N; ++i) {
             const E xi = vx[u][k].e[i], yi = vy[u][k].e[i], wi = wl[u][k].e[i], ui = wh[u][k].e[i];
-            if (W) {
+            if (W && (!SELECT || good)) {
               dlo[k].e[i] = qk_fma(wi, qk_mul(xi, by), dlo[k].e[i]);
               dhi[k].e[i] = qk_fma(ui, qk_mul(yi, by), dhi[k].e[i]);
             }
             ol.e[i] = qk_mul(by, qk_fma(wi, glo[k].e[i], qk_mul(xi, less)));
             oh.e[i] = qk_mul(by, qk_fma(ui, ghi[k].e[i], qk_mul(yi, less)));
           }
-        } else {
+        }
+        if (!good) {
           ol.fill(0.0f);
           oh.fill(0.0f);
         }
