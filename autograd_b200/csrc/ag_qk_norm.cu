@@ -11,8 +11,9 @@
 // few shuffles and no shared memory.  A thread has one or two heads of a token under way, loads the angles once for them, and goes on to the next
 // token of its turn with the weights in registers.  Packets are as wide as addresses, strides and halves allow, one to four
 // elements: every shape takes the same code.  All sums are fp32.
-// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 108 us, 0.95 of the copy rate; the gradient 167 us, 0.92), instructions
-// with bf16 ones (73 us, 0.70; the gradient 117 us, 0.66) and with packets of one element (heads of 74 columns: 93 us fp32, 0.64; the gradient 143).
+// Bound: HBM with fp32 rows (16 x 2048 tokens of 2 x 10 heads of 128: 108 us, 0.95 of the copy rate; the gradient 167 us, 0.92); with bf16 ones (73 us, 0.70;
+// the gradient 117 us, 0.66) waits for loads at 31 to 41 % of the warps beside two thirds of the issue slots; instructions with packets of one
+// element (heads of 74 columns: 93 us fp32, 0.64; the gradient 143).
 #include <type_traits>
 
 #include "ag_common.cuh"
@@ -22,7 +23,7 @@ namespace {
 constexpr int QK_THREADS = 256;
 constexpr int QK_BLOCKS_PER_SM = 8;  // at most: 256 threads each
 
-// One fp32 number, or two that arithmetic takes at once: bf16 rows, whose time is that of the instructions (gradient of 8192 tokens of 12 + 2
+// One fp32 number, or two that arithmetic takes at once: bf16 rows, where instructions count (gradient of 8192 tokens of 12 + 2
 // heads 34 -> 27 us; fp32 rows are bound by memory and lost 3 % with pairs, 114 -> 119 us for 16 x 2048 tokens of 2 x 10 heads).
 struct QkOne {
   float v;
