@@ -405,7 +405,7 @@ size_t ag_orthogonalise_scratch_bytes(int count, int rows, int cols, int precisi
 int ag_orthogonalise(ag_ctx* ctx, const void* const* g, void* const* out, int count, int rows, int cols,
                      const float* coefficients, int steps, float eps, int precision, int dtype, int out_dtype,
                      void* scratch, size_t scratch_bytes);
-/* How the calls above go about the first matrices of a list: *batch, how many of them share a launch; *form, what computes product 0 (X X^T),
+/* How ag_orthogonalise and ag_muon_step go about the first matrices of a list: *batch, how many of them share a launch; *form, what computes product 0 (X X^T),
  * 1 (its square) or 2 (the next X) of their steps, with either precision: one launch for everything, single CTAs, pairs of CTAs, or
  * clusters of CTAs that share a contraction.  A part of the list behind a whole number of batches may take another form. */
 enum { AG_NS_ONE_LAUNCH = 0, AG_NS_SINGLE = 1, AG_NS_PAIRS = 2, AG_NS_CLUSTERS = 3 };
